@@ -9,6 +9,7 @@
 #include "comm.cuh"
 #include "elementwise.cuh"
 #include "gemm_sm100.cuh"
+#include "token_loss.cuh"
 
 namespace {
 
@@ -481,6 +482,143 @@ void attn_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o
   check(ethb::attention_bwd(a, cur_stream()), "attention_bwd");
 }
 
+// ---- per-token vocabulary kernels --------------------------------------------------------------
+ethb::LogitsView logits_view(const Tensor& z, int64_t vocab_start, double temperature) {
+  need_cuda(z, "logits");
+  TORCH_CHECK(z.dim() == 2 && (z.stride(1) == 1 || z.size(1) == 1), "logits must be 2-D with unit inner stride");
+  TORCH_CHECK(z.size(1) >= 1 && z.size(1) < (int64_t{1} << 30), "vocabulary size out of range");
+  ethb::LogitsView a{};
+  a.z = z.data_ptr(); a.rows = z.size(0); a.ld = z.stride(0); a.vocab = static_cast<int>(z.size(1));
+  a.v0 = vocab_start;
+  a.dtype = dtype_code(z);
+  a.inv_temperature = static_cast<float>(1.0 / temperature);
+  return a;
+}
+// Contiguous tensor of `numel` elements of type `type` on the device of `like`; its data.
+template <typename T>
+T* flat(const Tensor& t, const Tensor& like, at::ScalarType type, int64_t numel, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.get_device() == like.get_device(), name, " must be on the device of the logits");
+  TORCH_CHECK(t.scalar_type() == type && t.is_contiguous() && t.numel() == numel, name, ": type, layout or size");
+  return numel == 0 ? nullptr : t.data_ptr<T>();
+}
+template <typename T>
+T* flat(const OptTensor& t, const Tensor& like, at::ScalarType type, int64_t numel, const char* name) {
+  return t.has_value() ? flat<T>(*t, like, type, numel, name) : nullptr;
+}
+ethb::TeacherView teacher_view(const Tensor& index, const Tensor& logit, const Tensor& like, int64_t rows) {
+  TORCH_CHECK(index.dim() == 2 && index.size(0) == rows && index.size(1) >= 1 &&
+                  index.size(1) <= ethb::kMaxTeacherEntries,
+              "teacher lists must be [rows, 1..", ethb::kMaxTeacherEntries, "]");
+  const int64_t n = rows * index.size(1);
+  return {flat<int64_t>(index, like, at::kLong, n, "teacher_index"),
+          flat<float>(logit, like, at::kFloat, n, "teacher_logit"), static_cast<int>(index.size(1))};
+}
+int64_t grad_pitch(const Tensor& dz, const Tensor& z) {
+  TORCH_CHECK(dz.is_cuda() && dz.get_device() == z.get_device() && dz.scalar_type() == z.scalar_type() &&
+                  dz.sizes() == z.sizes() && (dz.stride(1) == 1 || dz.size(1) == 1),
+              "gradient of the logits: device, type, shape or inner stride");
+  TORCH_CHECK(dz.size(0) <= 1 || dz.stride(0) >= dz.size(1), "gradient rows overlap");
+  return dz.stride(0);
+}
+ethb::TokenScoresOut scores_out(const Tensor& like, int64_t rows, int64_t k, const Tensor& logprob,
+                                const Tensor& entropy, const OptTensor& top_logprob, const OptTensor& top_index,
+                                const Tensor& stats) {
+  TORCH_CHECK(k == 0 || (top_logprob.has_value() && top_index.has_value()), "top_k outputs missing");
+  return {flat<float>(logprob, like, at::kFloat, rows, "logprob"), flat<float>(entropy, like, at::kFloat, rows, "entropy"),
+          flat<float>(top_logprob, like, at::kFloat, rows * k, "top_logprob"),
+          flat<int64_t>(top_index, like, at::kLong, rows * k, "top_index"),
+          flat<float>(stats, like, at::kFloat, rows * 2, "stats")};
+}
+void token_scores(const Tensor& z, const Tensor& tokens, int64_t top_k, double temperature, int64_t vocab_start,
+                  Tensor& logprob, Tensor& entropy, const OptTensor& top_logprob, const OptTensor& top_index,
+                  Tensor& stats) {
+  const auto a = logits_view(z, vocab_start, temperature);
+  c10::cuda::CUDAGuard guard(z.device());
+  check(ethb::token_scores(a, flat<int64_t>(tokens, z, at::kLong, a.rows, "tokens"), static_cast<int>(top_k),
+                           scores_out(z, a.rows, top_k, logprob, entropy, top_logprob, top_index, stats),
+                           cur_stream()), "token_scores");
+}
+void token_scores_partial(const Tensor& z, const Tensor& tokens, int64_t top_k, double temperature,
+                          int64_t vocab_start, Tensor& partial) {
+  const auto a = logits_view(z, vocab_start, temperature);
+  c10::cuda::CUDAGuard guard(z.device());
+  check(ethb::token_scores_partial(a, flat<int64_t>(tokens, z, at::kLong, a.rows, "tokens"), static_cast<int>(top_k),
+                                   flat<float>(partial, z, at::kFloat, a.rows * (4 + 2 * top_k), "partial"),
+                                   cur_stream()), "token_scores_partial");
+}
+void token_scores_combine(const Tensor& partials, const Tensor& tokens, int64_t top_k, double temperature,
+                          Tensor& logprob, Tensor& entropy, const OptTensor& top_logprob, const OptTensor& top_index,
+                          Tensor& stats) {
+  need_cuda(partials, "partials");
+  TORCH_CHECK(partials.dim() == 3 && partials.size(0) >= 1 && partials.size(2) == 4 + 2 * top_k, "partials shape");
+  const int64_t world = partials.size(0), rows = partials.size(1);
+  c10::cuda::CUDAGuard guard(partials.device());
+  check(ethb::token_scores_combine(flat<float>(partials, partials, at::kFloat, partials.numel(), "partials"),
+                                   static_cast<int>(world), rows,
+                                   flat<int64_t>(tokens, partials, at::kLong, rows, "tokens"),
+                                   static_cast<int>(top_k), static_cast<float>(1.0 / temperature),
+                                   scores_out(partials, rows, top_k, logprob, entropy, top_logprob, top_index, stats),
+                                   cur_stream()), "token_scores_combine");
+}
+void token_scores_bwd(const Tensor& z, const Tensor& tokens, const Tensor& stats, const Tensor& entropy,
+                      const OptTensor& top_index, int64_t top_k, double temperature, int64_t vocab_start,
+                      const OptTensor& g, const OptTensor& h, const OptTensor& u, Tensor& dz) {
+  const auto a = logits_view(z, vocab_start, temperature);
+  c10::cuda::CUDAGuard guard(z.device());
+  TORCH_CHECK(!u.has_value() || top_index.has_value(), "gradient of alternatives without their ids");
+  check(ethb::token_scores_bwd(a, flat<int64_t>(tokens, z, at::kLong, a.rows, "tokens"),
+                               flat<float>(stats, z, at::kFloat, 2 * a.rows, "stats"),
+                               flat<float>(entropy, z, at::kFloat, a.rows, "entropy"),
+                               flat<int64_t>(top_index, z, at::kLong, a.rows * top_k, "top_index"),
+                               static_cast<int>(top_k), flat<float>(g, z, at::kFloat, a.rows, "d_logprob"),
+                               flat<float>(h, z, at::kFloat, a.rows, "d_entropy"),
+                               flat<float>(u, z, at::kFloat, a.rows * top_k, "d_top_logprob"), dz.data_ptr(),
+                               grad_pitch(dz, z), cur_stream()), "token_scores_bwd");
+}
+void distill_fwd(const Tensor& z, const Tensor& index, const Tensor& logit, double temperature, int64_t vocab_start,
+                 Tensor& loss, Tensor& stats) {
+  const auto a = logits_view(z, vocab_start, temperature);
+  c10::cuda::CUDAGuard guard(z.device());
+  check(ethb::distill_fwd(a, teacher_view(index, logit, z, a.rows), flat<float>(loss, z, at::kFloat, a.rows, "loss"),
+                          flat<float>(stats, z, at::kFloat, 2 * a.rows, "stats"), cur_stream()), "distill_fwd");
+}
+void distill_partial(const Tensor& z, const Tensor& index, const Tensor& logit, double temperature,
+                     int64_t vocab_start, Tensor& partial) {
+  const auto a = logits_view(z, vocab_start, temperature);
+  c10::cuda::CUDAGuard guard(z.device());
+  check(ethb::distill_partial(a, teacher_view(index, logit, z, a.rows),
+                              flat<float>(partial, z, at::kFloat, 4 * a.rows, "partial"), cur_stream()),
+        "distill_partial");
+}
+void distill_combine(const Tensor& partials, const Tensor& index, const Tensor& logit, double temperature,
+                     Tensor& loss, Tensor& stats) {
+  need_cuda(partials, "partials");
+  TORCH_CHECK(partials.dim() == 3 && partials.size(0) >= 1 && partials.size(2) == 4, "partials shape");
+  const int64_t rows = partials.size(1);
+  c10::cuda::CUDAGuard guard(partials.device());
+  check(ethb::distill_combine(flat<float>(partials, partials, at::kFloat, partials.numel(), "partials"),
+                              static_cast<int>(partials.size(0)), rows, teacher_view(index, logit, partials, rows),
+                              static_cast<float>(1.0 / temperature), flat<float>(loss, partials, at::kFloat, rows, "loss"),
+                              flat<float>(stats, partials, at::kFloat, 2 * rows, "stats"), cur_stream()),
+        "distill_combine");
+}
+void distill_bwd(const Tensor& z, const Tensor& index, const Tensor& logit, const Tensor& stats, const Tensor& dloss,
+                 double temperature, int64_t vocab_start, Tensor& dz) {
+  const auto a = logits_view(z, vocab_start, temperature);
+  c10::cuda::CUDAGuard guard(z.device());
+  check(ethb::distill_bwd(a, teacher_view(index, logit, z, a.rows), flat<float>(stats, z, at::kFloat, 2 * a.rows, "stats"),
+                          flat<float>(dloss, z, at::kFloat, a.rows, "dloss"), dz.data_ptr(), grad_pitch(dz, z),
+                          cur_stream()), "distill_bwd");
+}
+void distill_step(const Tensor& z, const Tensor& index, const Tensor& logit, const Tensor& dloss, double temperature,
+                  int64_t vocab_start, Tensor& loss, Tensor& dz) {
+  const auto a = logits_view(z, vocab_start, temperature);
+  c10::cuda::CUDAGuard guard(z.device());
+  check(ethb::distill_step(a, teacher_view(index, logit, z, a.rows), flat<float>(dloss, z, at::kFloat, a.rows, "dloss"),
+                           flat<float>(loss, z, at::kFloat, a.rows, "loss"), dz.data_ptr(), grad_pitch(dz, z),
+                           cur_stream()), "distill_step");
+}
+
 // ---- peer memory -------------------------------------------------------------------------------
 ethb::PeerPtrs to_peers(const std::vector<int64_t>& ptrs) {
   TORCH_CHECK(ptrs.size() <= ethb::kMaxPeers, "too many peers");
@@ -638,6 +776,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("synthetic_batch", &synthetic_batch);
   m.def("attn_fwd", &attn_fwd);
   m.def("attn_bwd", &attn_bwd);
+  m.def("token_scores", &token_scores);
+  m.def("token_scores_partial", &token_scores_partial);
+  m.def("token_scores_combine", &token_scores_combine);
+  m.def("token_scores_bwd", &token_scores_bwd);
+  m.def("distill_fwd", &distill_fwd);
+  m.def("distill_partial", &distill_partial);
+  m.def("distill_combine", &distill_combine);
+  m.def("distill_bwd", &distill_bwd);
+  m.def("distill_step", &distill_step);
   m.def("launch_count", [] { return ethb::launch_count(); });
   m.def("set_gemm_variant", [](int v) { ethb::set_gemm_variant(v); });
   m.def("set_gemm_tail_split", [](int on) { ethb::set_gemm_tail_split(on); });

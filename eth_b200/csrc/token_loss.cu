@@ -1,0 +1,902 @@
+// Per-token kernels over the vocabulary: log-probabilities of given tokens with entropy and top
+// alternatives, and the loss against a teacher's top logits, forward and backward.
+//
+// All of them are bound by reading the logits [rows, vocab] (and writing their gradient). One CTA
+// owns one row; several CTAs per SM keep enough 16-byte loads in flight while others reduce.
+//
+//   x = z / T,  m = max z,  e_j = 2^((z_j - m) log2(e) / T),  L = sum e,  A = sum e_j log2 e_j
+//   log p_j = (z_j - m) / T - ln L,        entropy = ln L - ln2 * A / L
+//
+// The difference z - m is formed before it is scaled: a fused multiply-add of z * s - m * s would
+// overflow on masks of a type's lowest value and carry the rounding of m * s into every term.
+// All sums and statistics are fp32; 16-bit types are widened on load, a gradient is rounded once.
+#include "token_loss.cuh"
+
+#include "gemm_sm100.cuh"
+#include "sm100_common.cuh"
+
+#include <math_constants.h>
+#include <type_traits>
+
+namespace ethb {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+#define ETHB_DISPATCH_T(dtype, T, ...)                              \
+  do {                                                              \
+    if ((dtype) == kBF16) { using T = __nv_bfloat16; __VA_ARGS__; } \
+    else if ((dtype) == kF16) { using T = __half; __VA_ARGS__; }    \
+    else { using T = float; __VA_ARGS__; }                          \
+  } while (0)
+
+template <typename T> constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& u, float (&f)[kVec<T>]) {
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    constexpr int dt = std::is_same<T, __nv_bfloat16>::value ? kBF16 : kF16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = unpack2(w[i], dt);
+      f[2 * i] = v.x;
+      f[2 * i + 1] = v.y;
+    }
+  } else {
+    f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y);
+    f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 repack(const float (&f)[kVec<T>]) {
+  if constexpr (sizeof(T) == 2) {
+    constexpr int dt = std::is_same<T, __nv_bfloat16>::value ? kBF16 : kF16;
+    return make_uint4(pack2(f[0], f[1], dt), pack2(f[2], f[3], dt), pack2(f[4], f[5], dt), pack2(f[6], f[7], dt));
+  } else {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+}
+
+// A row as `head` single elements up to a 16-byte boundary, `nvec` 16-byte vectors, and a tail. Any
+// pitch and offset is taken; only the first and last few elements of a row go one by one.
+template <typename T> struct Row {
+  const T* p;
+  int head, nvec, n;
+  __device__ __forceinline__ Row(const T* row, int vocab) : p(row), n(vocab) {
+    const int off = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    head = min(off == 0 ? 0 : kVec<T> - off, vocab);
+    nvec = (vocab - head) / kVec<T>;
+  }
+  __device__ __forceinline__ int tail() const { return head + nvec * kVec<T>; }
+  __device__ __forceinline__ const uint4* vec() const { return reinterpret_cast<const uint4*>(p + head); }
+};
+
+// Order-preserving unsigned image of a value: larger value <=> larger key, NaN above everything,
+// -0 and +0 alike (they are ties, which go to the lower token id).
+// Integer steps only: float arithmetic here would flush subnormal logits.
+__device__ __forceinline__ uint32_t order_key(float v) {
+  uint32_t b = __float_as_uint(v);
+  if ((b & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
+  if (b == 0x80000000u) b = 0;
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// Running (maximum, sum of exponentials, sum of exponential * exponent). `mu` is what is subtracted:
+// the maximum, or 0 while only -inf has been seen (so that -inf - mu stays -inf and not NaN).
+template <bool kEntropy> struct Running {
+  float mx = -INFINITY, l = 0.f, a = 0.f;
+  __device__ __forceinline__ float mu() const { return mx == -INFINITY ? 0.f : mx; }
+  __device__ __forceinline__ void raise(float to, float s2) {   // to > mx
+    if (mx != -INFINITY) {
+      const float d = (mx - to) * s2, c = exp2f(d);
+      if (kEntropy) a = c == 0.f ? 0.f : c * (a + d * l);
+      l *= c;
+    }
+    mx = to;
+  }
+  // the scale that brings this sum to the maximum `to`; 0 for an empty one
+  __device__ __forceinline__ void rebase(float to, float s2) {
+    if (l == 0.f || to == mx) return;
+    const float d = (mu() - (to == -INFINITY ? 0.f : to)) * s2, c = exp2f(d);
+    if (kEntropy) a = c == 0.f ? 0.f : c * (a + d * l);
+    l *= c;
+  }
+  __device__ __forceinline__ void add(float z, float m, float s2) {
+    const float t = (z - m) * s2;
+    const float e = exp2f(t);
+    l += e;
+    if (kEntropy) a = fmaf(e, fmaxf(t, -1000.f), a);   // e is 0 far above -1000; -inf * 0 must not appear
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ float max_of(const uint4& u) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const __half2* h = reinterpret_cast<const __half2*>(&u);
+    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  } else {
+    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)),
+                 fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+  }
+}
+
+constexpr int kUnroll = 4;   // 16-byte loads in flight per thread
+
+// One thread's share of a row. Every maximum is taken over kUnroll vectors before their
+// exponentials, so the sums are rescaled only when a thread's maximum grows.
+template <typename T, bool kEntropy>
+__device__ __forceinline__ Running<kEntropy> scan_row(const Row<T>& r, float s2) {
+  Running<kEntropy> run;
+  auto one = [&](float z) {
+    if (z > run.mx) run.raise(z, s2);
+    run.add(z, run.mu(), s2);
+  };
+  const int tid = threadIdx.x, step = blockDim.x;
+  for (int i = tid; i < r.head; i += step) one(HalfTraits<T>::to_f(r.p[i]));
+  for (int i = r.tail() + tid; i < r.n; i += step) one(HalfTraits<T>::to_f(r.p[i]));
+  const uint4* v = r.vec();
+  int c = tid;
+  for (; c + (kUnroll - 1) * step < r.nvec; c += kUnroll * step) {
+    uint4 u[kUnroll];
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) u[k] = v[c + k * step];
+    float m = max_of<T>(u[0]);
+#pragma unroll
+    for (int k = 1; k < kUnroll; ++k) m = fmaxf(m, max_of<T>(u[k]));
+    if (m > run.mx) run.raise(m, s2);
+    const float mu = run.mu();
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) {
+      float f[kVec<T>];
+      unpack<T>(u[k], f);
+#pragma unroll
+      for (int j = 0; j < kVec<T>; ++j) run.add(f[j], mu, s2);
+    }
+  }
+  for (; c < r.nvec; c += step) {
+    const uint4 u = v[c];
+    const float m = max_of<T>(u);
+    if (m > run.mx) run.raise(m, s2);
+    const float mu = run.mu();
+    float f[kVec<T>];
+    unpack<T>(u, f);
+#pragma unroll
+    for (int j = 0; j < kVec<T>; ++j) run.add(f[j], mu, s2);
+  }
+  return run;
+}
+
+// The block's statistics, in every thread. `red` holds 3 x 32 floats.
+template <bool kEntropy>
+__device__ __forceinline__ Running<kEntropy> block_merge(Running<kEntropy> run, float s2, float* red) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  auto merge = [&](Running<kEntropy> x) {
+    const float m = warp_max(x.mx);
+    x.rebase(m, s2);
+    x.mx = m;
+    x.l = warp_sum(x.l);
+    if (kEntropy) x.a = warp_sum(x.a);
+    return x;
+  };
+  run = merge(run);
+  if (lane == 0) {
+    red[warp] = run.mx;
+    red[32 + warp] = run.l;
+    if (kEntropy) red[64 + warp] = run.a;
+  }
+  __syncthreads();
+  Running<kEntropy> x;
+  if (lane < nw) {
+    x.mx = red[lane];
+    x.l = red[32 + lane];
+    if (kEntropy) x.a = red[64 + lane];
+  }
+  return merge(x);
+}
+
+// ---------------------------------------------------------------------------------------------
+// top alternatives
+// ---------------------------------------------------------------------------------------------
+// Exact selection without keeping the row: the k-th largest of the threads' maxima is a lower bound
+// of the k-th largest element, and only threads whose own maximum reaches it can hold candidates.
+// Those few threads read their share again (it is still in L2); all others are done. The candidates
+// carry (key, ~token id), so ties go to the lowest id and the order in which they were found does
+// not matter. Where the bound is loose (a row of equal values, masked rows) and more than
+// kCandidates elements reach it, the exact k-th key and then the id up to which ties are taken are
+// found by bisection over their bits, with counts over the whole row.
+constexpr int kCandidates = 512;
+
+template <typename T, typename F>
+__device__ __forceinline__ void for_own(const Row<T>& r, F f) {   // f(value, local id) over a thread's share
+  const int tid = threadIdx.x, step = blockDim.x;
+  for (int i = tid; i < r.head; i += step) f(HalfTraits<T>::to_f(r.p[i]), i);
+  for (int i = r.tail() + tid; i < r.n; i += step) f(HalfTraits<T>::to_f(r.p[i]), i);
+  const uint4* v = r.vec();
+#pragma unroll 4
+  for (int c = tid; c < r.nvec; c += step) {
+    float x[kVec<T>];
+    unpack<T>(v[c], x);
+#pragma unroll
+    for (int j = 0; j < kVec<T>; ++j) f(x[j], r.head + c * kVec<T> + j);
+  }
+}
+
+struct SelectSmem {
+  unsigned long long cand[kCandidates];
+  unsigned long long best[kMaxTopAlternatives];
+  int count;
+  int sums[32];
+};
+
+__device__ __forceinline__ int block_count(int v, int* sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  v = __reduce_add_sync(0xffffffffu, v);
+  __syncthreads();
+  if (lane == 0) sums[warp] = v;
+  __syncthreads();
+  return __reduce_add_sync(0xffffffffu, lane < nw ? sums[lane] : 0);
+}
+
+// s.best[0..k) = the k largest (key << 32 | ~id), in falling order. Needs k <= blockDim.x, k <= r.n.
+template <typename T>
+__device__ void select_top(const Row<T>& r, int k, float thread_max, bool thread_nan, SelectSmem& s) {
+  const int tid = threadIdx.x;
+  uint32_t own = 0;                          // below the key of -inf: a thread without elements
+  const bool any = tid < r.head || r.tail() + tid < r.n || tid < r.nvec;
+  if (thread_nan || fabsf(thread_max) < 1.17549435e-38f) {
+    // NaN or +inf among this thread's elements, or a maximum so small that the float comparisons
+    // behind it flushed its competitors: take the true maximum
+    for_own(r, [&](float z, int) { own = max(own, order_key(z)); });
+  } else if (any) {
+    own = order_key(thread_max);
+  }
+  uint32_t bound = 0;
+  // 16-bit types widen exactly: their keys differ in the upper bits only (the lower 16 are all 0 for
+  // positive, all 1 for negative values), for fp16 in the upper 19
+  constexpr int kLow = std::is_same<T, __nv_bfloat16>::value ? 16 : 0;
+  for (int bit = 31; bit >= kLow; --bit) {
+    const uint32_t cand = bound | (1u << bit);
+    if (__syncthreads_count(own >= cand) >= k) bound = cand;
+  }
+  if (tid == 0) s.count = 0;
+  __syncthreads();
+  if (own >= bound && any) {
+    for_own(r, [&](float z, int id) {
+      const uint32_t key = order_key(z);
+      if (key >= bound) {
+        const int at = atomicAdd(&s.count, 1);
+        if (at < kCandidates) s.cand[at] = (static_cast<unsigned long long>(key) << 32) | (0xffffffffu - id);
+      }
+    });
+  }
+  __syncthreads();
+  int found = s.count;
+  if (found > kCandidates) {
+    uint32_t kth = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t cand = kth | (1u << bit);
+      int n = 0;
+      for_own(r, [&](float z, int) { n += order_key(z) >= cand; });
+      if (block_count(n, s.sums) >= k) kth = cand;
+    }
+    int above = 0;
+    for_own(r, [&](float z, int) { above += order_key(z) > kth; });
+    const int ties = k - block_count(above, s.sums);     // >= 1 elements equal to the k-th are taken
+    int upto = 0;                                         // the largest id with fewer than `ties` ties below it
+    for (int bit = 30; bit >= 0; --bit) {
+      const int cand = upto + (1 << bit);
+      if (cand > r.n) continue;
+      int n = 0;
+      for_own(r, [&](float z, int id) { n += order_key(z) == kth && id < cand; });
+      if (block_count(n, s.sums) < ties) upto = cand;
+    }
+    if (tid == 0) s.count = 0;
+    __syncthreads();
+    for_own(r, [&](float z, int id) {
+      const uint32_t key = order_key(z);
+      if (key > kth || (key == kth && id <= upto)) {
+        const int at = atomicAdd(&s.count, 1);
+        if (at < kCandidates) s.cand[at] = (static_cast<unsigned long long>(key) << 32) | (0xffffffffu - id);
+      }
+    });
+    __syncthreads();
+    found = min(s.count, kCandidates);
+  }
+  for (int i = tid; i < found; i += blockDim.x) {         // rank by counting: all candidates are distinct
+    const unsigned long long mine = s.cand[i];
+    int rank = 0;
+    for (int j = 0; j < found; ++j) rank += s.cand[j] > mine;
+    if (rank < k) s.best[rank] = mine;
+  }
+  __syncthreads();
+}
+
+// ---------------------------------------------------------------------------------------------
+// token log-probabilities, entropy, alternatives: forward
+// ---------------------------------------------------------------------------------------------
+template <typename T, bool kTop>
+__global__ void token_scores_kernel(const T* __restrict__ z, int64_t ld, int vocab, int64_t v0,
+                                    const int64_t* __restrict__ tokens, int top_k, float inv_t, TokenScoresOut out,
+                                    float* __restrict__ partial) {
+  __shared__ float red[96];
+  __shared__ SelectSmem sel;
+  const int64_t row = blockIdx.x;
+  const Row<T> r(z + row * ld, vocab);
+  const float s2 = inv_t * kLog2e;
+  const Running<true> own = scan_row<T, true>(r, s2);
+  const Running<true> all = block_merge<true>(own, s2, red);
+  const float mu = all.mu();
+  const float log_l = kLn2 * log2f(all.l);
+  const int width = 4 + 2 * top_k;
+  if (threadIdx.x == 0) {
+    const int64_t t = tokens[row], local = t - v0;
+    const bool here = t >= 0 && local >= 0 && local < vocab;
+    const float zt = here ? HalfTraits<T>::to_f(r.p[local]) : CUDART_NAN_F;
+    if (partial != nullptr) {
+      float* q = partial + row * width;
+      q[0] = all.mx; q[1] = all.l; q[2] = all.a; q[3] = zt;
+    } else {
+      out.logprob[row] = t < 0 ? 0.f : (zt - mu) * inv_t - log_l;
+      out.entropy[row] = log_l - kLn2 * (all.a / all.l);
+      out.stats[2 * row] = mu;
+      out.stats[2 * row + 1] = all.l;
+    }
+  }
+  if (kTop) {
+    select_top(r, top_k, own.mx, own.l != own.l, sel);
+    for (int i = threadIdx.x; i < top_k; i += blockDim.x) {
+      const int id = static_cast<int>(0xffffffffu - static_cast<uint32_t>(sel.best[i]));
+      const float zi = HalfTraits<T>::to_f(r.p[id]);
+      if (partial != nullptr) {
+        partial[row * width + 4 + i] = zi;
+        partial[row * width + 4 + top_k + i] = __int_as_float(static_cast<int>(id + v0));
+      } else {
+        out.top_logprob[row * top_k + i] = (zi - mu) * inv_t - log_l;
+        out.top_index[row * top_k + i] = id + v0;
+      }
+    }
+  }
+}
+
+// Merges the shards' parts of one row per warp. Every candidate is ranked by counting the better
+// ones among all shards' candidates, as in select_top.
+__global__ void token_scores_combine_kernel(const float* __restrict__ parts, int world, int64_t rows,
+                                            const int64_t* __restrict__ tokens, int top_k, float inv_t,
+                                            TokenScoresOut out) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int width = 4 + 2 * top_k;
+  const float s2 = inv_t * kLog2e;
+  float mx = -INFINITY;
+  for (int w = 0; w < world; ++w) mx = fmaxf(mx, parts[(w * rows + row) * width]);
+  Running<true> all;
+  all.mx = mx;
+  float zt = CUDART_NAN_F;
+  for (int w = 0; w < world; ++w) {
+    const float* q = parts + (w * rows + row) * width;
+    Running<true> x;
+    x.mx = q[0]; x.l = q[1]; x.a = q[2];
+    x.rebase(mx, s2);
+    all.l += x.l;
+    all.a += x.a;
+    if (q[3] == q[3]) zt = q[3];
+  }
+  const float mu = all.mu(), log_l = kLn2 * log2f(all.l);
+  if (lane == 0) {
+    out.logprob[row] = tokens[row] < 0 ? 0.f : (zt - mu) * inv_t - log_l;
+    out.entropy[row] = log_l - kLn2 * (all.a / all.l);
+    out.stats[2 * row] = mu;
+    out.stats[2 * row + 1] = all.l;
+  }
+  auto key = [&](int c) {
+    const float* q = parts + ((c / top_k) * rows + row) * width + 4 + c % top_k;
+    return (static_cast<unsigned long long>(order_key(q[0])) << 32) |
+           (0xffffffffu - static_cast<uint32_t>(__float_as_int(q[top_k])));
+  };
+  for (int c = lane; c < world * top_k; c += 32) {
+    const unsigned long long mine = key(c);
+    int rank = 0;
+    for (int o = 0; o < world * top_k; ++o) rank += key(o) > mine;
+    if (rank < top_k) {
+      const float* q = parts + ((c / top_k) * rows + row) * width + 4 + c % top_k;
+      out.top_logprob[row * top_k + rank] = (q[0] - mu) * inv_t - log_l;
+      out.top_index[row * top_k + rank] = __float_as_int(q[top_k]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// gradients: dz_j = p_j (A + B log p_j) + sum of the listed weights of j
+// ---------------------------------------------------------------------------------------------
+// The listed entries (a token, alternatives, a teacher's list) are few: their logits are read before
+// the dense pass, which may overwrite them, and the finished values are stored after it. The same id
+// may be listed several times; the first entry stores the sum of all, added in list order.
+struct Listed {
+  int id[kMaxTeacherEntries + 1];      // local token id, -1: not on this shard / unused
+  float w[kMaxTeacherEntries + 1];
+  float z[kMaxTeacherEntries + 1];
+};
+
+struct DenseTerm {
+  float mu, s2, inv_l, log2_l, a, b;   // a, b already hold the factor 1 / temperature
+  template <bool kLog> __device__ __forceinline__ float at(float z) const {
+    const float t = (z - mu) * s2, p = exp2f(t) * inv_l;
+    if constexpr (kLog) {
+      // b scales p log p; p is 0 far above -1000, where log p may be -inf
+      return p * fmaf(b, fmaxf(t - log2_l, -1000.f) * kLn2, a);
+    } else {
+      return p * a;
+    }
+  }
+};
+
+template <typename T, bool kLog>
+__device__ __forceinline__ void write_grad(const Row<T>& r, T* __restrict__ d, const DenseTerm& f, Listed& li, int n) {
+  const int tid = threadIdx.x, step = blockDim.x;
+  for (int i = tid; i < n; i += step)
+    if (li.id[i] >= 0) li.z[i] = HalfTraits<T>::to_f(r.p[li.id[i]]);
+  __syncthreads();
+  if (((reinterpret_cast<uintptr_t>(r.p) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0) {
+    for (int i = tid; i < r.head; i += step) d[i] = HalfTraits<T>::from_f(f.at<kLog>(HalfTraits<T>::to_f(r.p[i])));
+    for (int i = r.tail() + tid; i < r.n; i += step)
+      d[i] = HalfTraits<T>::from_f(f.at<kLog>(HalfTraits<T>::to_f(r.p[i])));
+    const uint4* v = r.vec();
+    uint4* o = reinterpret_cast<uint4*>(d + r.head);
+    int c = tid;
+    for (; c + (kUnroll - 1) * step < r.nvec; c += kUnroll * step) {
+      uint4 u[kUnroll];
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k) u[k] = v[c + k * step];
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k) {
+        float x[kVec<T>];
+        unpack<T>(u[k], x);
+#pragma unroll
+        for (int j = 0; j < kVec<T>; ++j) x[j] = f.at<kLog>(x[j]);
+        o[c + k * step] = repack<T>(x);
+      }
+    }
+    for (; c < r.nvec; c += step) {
+      float x[kVec<T>];
+      unpack<T>(v[c], x);
+#pragma unroll
+      for (int j = 0; j < kVec<T>; ++j) x[j] = f.at<kLog>(x[j]);
+      o[c] = repack<T>(x);
+    }
+  } else {   // rows of logits and gradient at different offsets from a 16-byte boundary
+    for (int i = tid; i < r.n; i += step) d[i] = HalfTraits<T>::from_f(f.at<kLog>(HalfTraits<T>::to_f(r.p[i])));
+  }
+  __syncthreads();
+  for (int i = tid; i < n; i += step) {
+    const int id = li.id[i];
+    if (id < 0) continue;
+    bool first = true;
+    for (int j = 0; j < i; ++j) first &= li.id[j] != id;
+    if (!first) continue;
+    float w = li.w[i];
+    for (int j = i + 1; j < n; ++j) w += li.id[j] == id ? li.w[j] : 0.f;
+    d[id] = HalfTraits<T>::from_f(f.at<kLog>(li.z[i]) + w);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void write_zero(T* __restrict__ d, int vocab) {
+  const Row<T> o(d, vocab);
+  const int tid = threadIdx.x, step = blockDim.x;
+  for (int i = tid; i < o.head; i += step) d[i] = HalfTraits<T>::from_f(0.f);
+  for (int i = o.tail() + tid; i < vocab; i += step) d[i] = HalfTraits<T>::from_f(0.f);
+  uint4* v = reinterpret_cast<uint4*>(d + o.head);
+  for (int c = tid; c < o.nvec; c += step) v[c] = make_uint4(0, 0, 0, 0);
+}
+
+template <typename T, bool kLog>
+__global__ void token_scores_bwd_kernel(const T* z, int64_t ld, int vocab, int64_t v0,
+                                        const int64_t* __restrict__ tokens, const float* __restrict__ stats,
+                                        const float* __restrict__ entropy, const int64_t* __restrict__ top_index,
+                                        int top_k, float inv_t, const float* __restrict__ g,
+                                        const float* __restrict__ h, const float* __restrict__ u, T* dz, int64_t ldd) {
+  __shared__ Listed li;
+  __shared__ float usum;
+  const int64_t row = blockIdx.x;
+  const Row<T> r(z + row * ld, vocab);
+  const int64_t t = tokens[row];
+  const float gr = g != nullptr && t >= 0 ? g[row] : 0.f;
+  const float hr = kLog ? h[row] : 0.f;
+  const int extra = u != nullptr ? top_k : 0;
+  if (threadIdx.x < 32) {
+    float sum = 0.f;
+    for (int i = threadIdx.x; i < extra; i += 32) {
+      const float w = u[row * top_k + i];
+      const int64_t id = top_index[row * top_k + i] - v0;
+      li.id[1 + i] = id >= 0 && id < vocab && w != 0.f ? static_cast<int>(id) : -1;
+      li.w[1 + i] = w * inv_t;
+      sum += w;
+    }
+    sum = warp_sum(sum);
+    if (threadIdx.x == 0) {
+      const int64_t id = t - v0;
+      li.id[0] = gr != 0.f && id >= 0 && id < vocab ? static_cast<int>(id) : -1;
+      li.w[0] = gr * inv_t;
+      usum = sum;
+    }
+  }
+  __syncthreads();
+  T* d = dz + row * ldd;
+  // a row that no gradient reaches (a masked token): its logits are not looked at
+  int live = gr != 0.f || hr != 0.f;
+  for (int i = 0; i < extra && !live; ++i) live = u[row * top_k + i] != 0.f;
+  if (!live) {
+    write_zero(d, vocab);
+    return;
+  }
+  DenseTerm f;
+  f.mu = stats[2 * row];
+  f.s2 = inv_t * kLog2e;
+  f.inv_l = 1.0f / stats[2 * row + 1];
+  f.log2_l = log2f(stats[2 * row + 1]);
+  f.a = -(gr + usum) * inv_t;
+  f.b = 0.f;
+  if (kLog) {
+    f.a -= hr * entropy[row] * inv_t;
+    f.b = -hr * inv_t;
+  }
+  write_grad<T, kLog>(r, d, f, li, 1 + extra);
+}
+
+// ---------------------------------------------------------------------------------------------
+// loss against a teacher's top logits
+// ---------------------------------------------------------------------------------------------
+// q = softmax of the listed teacher logits / T (entries at -inf have no weight; a row without any
+// entry has no loss), loss = sum_k q_k (log q_k - log p_{i_k}), dz_j = g / T (p_j sum q - sum_{i_k = j} q_k).
+struct TeacherRow {
+  float tmax, log_sum, mass;   // mass: sum of q (1, or 0 for an empty row)
+};
+__device__ __forceinline__ TeacherRow teacher_row(const TeacherView& t, int64_t row, int64_t v0, int vocab,
+                                                  float inv_t, Listed& li, float* red) {
+  const int lane = threadIdx.x & 31;
+  const float* tl = t.logit + row * t.k;
+  float mx = -INFINITY, sum = 0.f;
+  bool nan = false;
+  // every warp reduces the whole (short) list for itself
+  for (int i = lane; i < t.k; i += 32) {
+    mx = fmaxf(mx, tl[i]);
+    nan |= tl[i] != tl[i];
+  }
+  mx = warp_max(mx);
+  nan = __any_sync(0xffffffffu, nan);
+  TeacherRow out{mx, 0.f, 0.f};
+  if (mx == -INFINITY && !nan) {
+    for (int i = threadIdx.x; i < t.k; i += blockDim.x) {
+      li.id[i] = -1;
+      li.w[i] = 0.f;
+    }
+    __syncthreads();
+    return out;
+  }
+  for (int i = lane; i < t.k; i += 32) sum += exp2f((tl[i] - mx) * inv_t * kLog2e);
+  sum = warp_sum(sum);
+  if (nan) sum = CUDART_NAN_F;
+  const float inv = 1.0f / sum;
+  for (int i = threadIdx.x; i < t.k; i += blockDim.x) {
+    const float q = exp2f((tl[i] - mx) * inv_t * kLog2e) * inv;
+    const int64_t id = t.index[row * t.k + i] - v0;
+    li.w[i] = q;
+    li.id[i] = q != 0.f && id >= 0 && id < vocab ? static_cast<int>(id) : -1;
+  }
+  __syncthreads();
+  out.log_sum = kLn2 * log2f(sum);
+  out.mass = sum == sum ? 1.f : sum;
+  return out;
+}
+
+__device__ __forceinline__ float block_sum_f(float v, float* red) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  v = warp_sum(v);
+  __syncthreads();
+  if (lane == 0) red[warp] = v;
+  __syncthreads();
+  return warp_sum(lane < nw ? red[lane] : 0.f);
+}
+
+// loss of a row whose listed logits are all in this shard; NaN where a weighted entry is not
+template <typename T>
+__device__ __forceinline__ float listed_loss(const Row<T>& r, const TeacherView& t, int64_t row, const TeacherRow& tr,
+                                             float inv_t, float mu, float log_l, const Listed& li, float* red) {
+  float part = 0.f;
+  for (int i = threadIdx.x; i < t.k; i += blockDim.x) {
+    const float q = li.w[i];
+    if (q == 0.f) continue;
+    const float log_q = (t.logit[row * t.k + i] - tr.tmax) * inv_t - tr.log_sum;
+    const float zi = li.id[i] >= 0 ? HalfTraits<T>::to_f(r.p[li.id[i]]) : CUDART_NAN_F;
+    part += q * (log_q - ((zi - mu) * inv_t - log_l));
+  }
+  return block_sum_f(part, red);
+}
+
+template <typename T>
+__global__ void distill_fwd_kernel(const T* __restrict__ z, int64_t ld, int vocab, int64_t v0, TeacherView t,
+                                   float inv_t, float* __restrict__ loss, float* __restrict__ stats,
+                                   float* __restrict__ partial) {
+  __shared__ float red[96];
+  __shared__ Listed li;
+  const int64_t row = blockIdx.x;
+  const Row<T> r(z + row * ld, vocab);
+  const float s2 = inv_t * kLog2e;
+  const TeacherRow tr = teacher_row(t, row, v0, vocab, inv_t, li, red);
+  if (tr.mass == 0.f && partial == nullptr) {   // nothing listed: no loss, the logits are not looked at
+    if (threadIdx.x == 0) {
+      loss[row] = 0.f;
+      stats[2 * row] = 0.f;
+      stats[2 * row + 1] = 1.f;
+    }
+    return;
+  }
+  const Running<false> all = block_merge<false>(scan_row<T, false>(r, s2), s2, red);
+  const float mu = all.mu();
+  if (partial != nullptr) {
+    float found = 0.f, weight = 0.f;
+    for (int i = threadIdx.x; i < t.k; i += blockDim.x)
+      if (li.id[i] >= 0) {
+        found += li.w[i] * ((HalfTraits<T>::to_f(r.p[li.id[i]]) - mu) * inv_t);
+        weight += li.w[i];
+      }
+    found = block_sum_f(found, red);
+    weight = block_sum_f(weight, red);
+    if (threadIdx.x == 0) {
+      float* q = partial + row * 4;
+      q[0] = all.mx; q[1] = all.l; q[2] = found; q[3] = weight;
+    }
+    return;
+  }
+  const float l = listed_loss(r, t, row, tr, inv_t, mu, kLn2 * log2f(all.l), li, red);
+  if (threadIdx.x == 0) {
+    loss[row] = l;
+    stats[2 * row] = mu;
+    stats[2 * row + 1] = all.l;
+  }
+}
+
+__global__ void distill_combine_kernel(const float* __restrict__ parts, int world, int64_t rows, TeacherView t,
+                                       float inv_t, float* __restrict__ loss, float* __restrict__ stats) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const float s2 = inv_t * kLog2e;
+  float mx = -INFINITY;
+  for (int w = 0; w < world; ++w) mx = fmaxf(mx, parts[(w * rows + row) * 4]);
+  Running<false> all;
+  all.mx = mx;
+  const float mu = all.mu();
+  float found = 0.f, weight = 0.f;
+  for (int w = 0; w < world; ++w) {
+    const float* q = parts + (w * rows + row) * 4;
+    Running<false> x;
+    x.mx = q[0]; x.l = q[1];
+    if (q[3] != 0.f) found += q[2] + q[3] * ((x.mu() - mu) * inv_t);
+    weight += q[3];
+    x.rebase(mx, s2);
+    all.l += x.l;
+  }
+  const float* tl = t.logit + row * t.k;
+  float tmax = -INFINITY, sum = 0.f, self = 0.f;
+  bool nan = false;
+  for (int i = lane; i < t.k; i += 32) {
+    tmax = fmaxf(tmax, tl[i]);
+    nan |= tl[i] != tl[i];
+  }
+  tmax = warp_max(tmax);
+  nan = __any_sync(0xffffffffu, nan);
+  const bool empty = tmax == -INFINITY && !nan;
+  for (int i = lane; i < t.k; i += 32) sum += empty ? 0.f : exp2f((tl[i] - tmax) * inv_t * kLog2e);
+  sum = nan ? CUDART_NAN_F : warp_sum(sum);
+  const float log_sum = kLn2 * log2f(sum), inv = 1.0f / sum;
+  for (int i = lane; i < t.k && !empty; i += 32) {
+    const float x = (tl[i] - tmax) * inv_t, q = exp2f(x * kLog2e) * inv;
+    if (q != 0.f) self += q * (x - log_sum);
+  }
+  self = warp_sum(self);
+  if (lane == 0) {
+    // the weights found over all shards add up to 1 unless an entry lies outside the vocabulary
+    const bool whole = fabsf(weight - 1.f) < 1e-4f;
+    loss[row] = empty ? 0.f : whole ? self - found + kLn2 * log2f(all.l) : CUDART_NAN_F;
+    stats[2 * row] = empty ? 0.f : mu;
+    stats[2 * row + 1] = empty ? 1.f : all.l;
+  }
+}
+
+template <typename T>
+__global__ void distill_bwd_kernel(const T* z, int64_t ld, int vocab, int64_t v0, TeacherView t, float inv_t,
+                                   const float* __restrict__ stats, const float* __restrict__ dloss, T* dz,
+                                   int64_t ldd) {
+  __shared__ float red[96];
+  __shared__ Listed li;
+  const int64_t row = blockIdx.x;
+  const Row<T> r(z + row * ld, vocab);
+  T* d = dz + row * ldd;
+  const float g = dloss[row] * inv_t;
+  const TeacherRow tr = teacher_row(t, row, v0, vocab, inv_t, li, red);
+  if (tr.mass == 0.f || g == 0.f) {
+    write_zero(d, vocab);
+    return;
+  }
+  for (int i = threadIdx.x; i < t.k; i += blockDim.x) li.w[i] *= -g;
+  const DenseTerm f{stats[2 * row], inv_t * kLog2e, 1.0f / stats[2 * row + 1], 0.f, g * tr.mass, 0.f};
+  write_grad<T, false>(r, d, f, li, t.k);
+}
+
+// Loss and gradient of a row in one CTA: the second reading of the row comes out of L2, so DRAM sees
+// the logits once and the gradient once.
+template <typename T>
+__global__ void distill_step_kernel(const T* z, int64_t ld, int vocab, int64_t v0, TeacherView t, float inv_t,
+                                    const float* __restrict__ dloss, float* __restrict__ loss, T* dz, int64_t ldd) {
+  __shared__ float red[96];
+  __shared__ Listed li;
+  const int64_t row = blockIdx.x;
+  const Row<T> r(z + row * ld, vocab);
+  T* d = dz + row * ldd;
+  const float s2 = inv_t * kLog2e;
+  const float g = dloss[row] * inv_t;
+  const TeacherRow tr = teacher_row(t, row, v0, vocab, inv_t, li, red);
+  if (tr.mass == 0.f) {
+    if (threadIdx.x == 0) loss[row] = 0.f;
+    write_zero(d, vocab);
+    return;
+  }
+  const Running<false> all = block_merge<false>(scan_row<T, false>(r, s2), s2, red);
+  const float mu = all.mu();
+  const float l = listed_loss(r, t, row, tr, inv_t, mu, kLn2 * log2f(all.l), li, red);
+  if (threadIdx.x == 0) loss[row] = l;
+  if (g == 0.f) {
+    __syncthreads();
+    write_zero(d, vocab);
+    return;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < t.k; i += blockDim.x) li.w[i] *= -g;
+  const DenseTerm f{mu, s2, 1.0f / all.l, 0.f, g * tr.mass, 0.f};
+  write_grad<T, false>(r, d, f, li, t.k);
+}
+
+// Threads per row: with rows for every SM, 256 threads and up to eight rows per SM; a few rows get
+// a whole SM's worth of threads each, which shortens the row instead.
+int threads_for(int64_t rows, int vocab) {
+  if (rows <= 2 * 148 && vocab > 4096) return 1024;
+  return 256;
+}
+
+cudaError_t check_view(const LogitsView& a) {
+  ETHB_RETURN_IF(a.rows < 0 || a.vocab <= 0, cudaErrorInvalidValue, "token loss: empty vocabulary");
+  ETHB_RETURN_IF(a.rows > 0x7fffffffLL, cudaErrorInvalidValue, "token loss: too many rows for one grid");
+  ETHB_RETURN_IF(a.dtype != kF32 && a.dtype != kF16 && a.dtype != kBF16, cudaErrorInvalidValue, "token loss: dtype");
+  return cudaSuccess;
+}
+
+cudaError_t launch_scores(const LogitsView& a, const int64_t* tokens, int top_k, const TokenScoresOut& out,
+                          float* partial, cudaStream_t st) {
+  ETHB_TRY(check_view(a), "token_scores");
+  ETHB_RETURN_IF(top_k < 0 || top_k > kMaxTopAlternatives || top_k > a.vocab, cudaErrorInvalidValue, "top_k");
+  if (a.rows == 0) return cudaSuccess;
+  const int threads = threads_for(a.rows, a.vocab);
+  ETHB_DISPATCH_T(a.dtype, T, {
+    if (top_k > 0)
+      token_scores_kernel<T, true><<<static_cast<unsigned>(a.rows), threads, 0, st>>>(
+          static_cast<const T*>(a.z), a.ld, a.vocab, a.v0, tokens, top_k, a.inv_temperature, out, partial);
+    else
+      token_scores_kernel<T, false><<<static_cast<unsigned>(a.rows), threads, 0, st>>>(
+          static_cast<const T*>(a.z), a.ld, a.vocab, a.v0, tokens, top_k, a.inv_temperature, out, partial);
+  });
+  count_launch();
+  return cudaGetLastError();
+}
+
+cudaError_t launch_distill(const LogitsView& a, const TeacherView& t, float* loss, float* stats, float* partial,
+                           cudaStream_t st) {
+  ETHB_TRY(check_view(a), "distill");
+  ETHB_RETURN_IF(t.k < 1 || t.k > kMaxTeacherEntries, cudaErrorInvalidValue, "teacher entries");
+  if (a.rows == 0) return cudaSuccess;
+  ETHB_DISPATCH_T(a.dtype, T, {
+    distill_fwd_kernel<T><<<static_cast<unsigned>(a.rows), threads_for(a.rows, a.vocab), 0, st>>>(
+        static_cast<const T*>(a.z), a.ld, a.vocab, a.v0, t, a.inv_temperature, loss, stats, partial);
+  });
+  count_launch();
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t token_scores(const LogitsView& a, const int64_t* tokens, int top_k, const TokenScoresOut& out,
+                         cudaStream_t st) {
+  return launch_scores(a, tokens, top_k, out, nullptr, st);
+}
+cudaError_t token_scores_partial(const LogitsView& a, const int64_t* tokens, int top_k, float* partial,
+                                 cudaStream_t st) {
+  return launch_scores(a, tokens, top_k, TokenScoresOut{}, partial, st);
+}
+cudaError_t token_scores_combine(const float* partials, int world, int64_t rows, const int64_t* tokens, int top_k,
+                                 float inv_temperature, const TokenScoresOut& out, cudaStream_t st) {
+  if (rows == 0) return cudaSuccess;
+  token_scores_combine_kernel<<<static_cast<unsigned>((rows + 7) / 8), 256, 0, st>>>(partials, world, rows, tokens,
+                                                                                   top_k, inv_temperature, out);
+  count_launch();
+  return cudaGetLastError();
+}
+cudaError_t token_scores_bwd(const LogitsView& a, const int64_t* tokens, const float* stats, const float* entropy,
+                             const int64_t* top_index, int top_k, const float* g, const float* h, const float* u,
+                             void* dz, int64_t ldd, cudaStream_t st) {
+  ETHB_TRY(check_view(a), "token_scores_bwd");
+  ETHB_RETURN_IF(top_k < 0 || top_k > kMaxTopAlternatives, cudaErrorInvalidValue, "top_k");
+  if (a.rows == 0) return cudaSuccess;
+  const int threads = threads_for(a.rows, a.vocab);
+  ETHB_DISPATCH_T(a.dtype, T, {
+    if (h != nullptr)
+      token_scores_bwd_kernel<T, true><<<static_cast<unsigned>(a.rows), threads, 0, st>>>(
+          static_cast<const T*>(a.z), a.ld, a.vocab, a.v0, tokens, stats, entropy, top_index, top_k,
+          a.inv_temperature, g, h, u, static_cast<T*>(dz), ldd);
+    else
+      token_scores_bwd_kernel<T, false><<<static_cast<unsigned>(a.rows), threads, 0, st>>>(
+          static_cast<const T*>(a.z), a.ld, a.vocab, a.v0, tokens, stats, entropy, top_index, top_k,
+          a.inv_temperature, g, h, u, static_cast<T*>(dz), ldd);
+  });
+  count_launch();
+  return cudaGetLastError();
+}
+
+cudaError_t distill_fwd(const LogitsView& a, const TeacherView& t, float* loss, float* stats, cudaStream_t st) {
+  return launch_distill(a, t, loss, stats, nullptr, st);
+}
+cudaError_t distill_partial(const LogitsView& a, const TeacherView& t, float* partial, cudaStream_t st) {
+  return launch_distill(a, t, nullptr, nullptr, partial, st);
+}
+cudaError_t distill_combine(const float* partials, int world, int64_t rows, const TeacherView& t,
+                            float inv_temperature, float* loss, float* stats, cudaStream_t st) {
+  if (rows == 0) return cudaSuccess;
+  distill_combine_kernel<<<static_cast<unsigned>((rows + 7) / 8), 256, 0, st>>>(partials, world, rows, t,
+                                                                              inv_temperature, loss, stats);
+  count_launch();
+  return cudaGetLastError();
+}
+cudaError_t distill_bwd(const LogitsView& a, const TeacherView& t, const float* stats, const float* dloss, void* dz,
+                        int64_t ldd, cudaStream_t st) {
+  ETHB_TRY(check_view(a), "distill_bwd");
+  ETHB_RETURN_IF(t.k < 1 || t.k > kMaxTeacherEntries, cudaErrorInvalidValue, "teacher entries");
+  if (a.rows == 0) return cudaSuccess;
+  ETHB_DISPATCH_T(a.dtype, T, {
+    distill_bwd_kernel<T><<<static_cast<unsigned>(a.rows), threads_for(a.rows, a.vocab), 0, st>>>(
+        static_cast<const T*>(a.z), a.ld, a.vocab, a.v0, t, a.inv_temperature, stats, dloss, static_cast<T*>(dz), ldd);
+  });
+  count_launch();
+  return cudaGetLastError();
+}
+cudaError_t distill_step(const LogitsView& a, const TeacherView& t, const float* dloss, float* loss, void* dz,
+                         int64_t ldd, cudaStream_t st) {
+  ETHB_TRY(check_view(a), "distill_step");
+  ETHB_RETURN_IF(t.k < 1 || t.k > kMaxTeacherEntries, cudaErrorInvalidValue, "teacher entries");
+  if (a.rows == 0) return cudaSuccess;
+  ETHB_DISPATCH_T(a.dtype, T, {
+    distill_step_kernel<T><<<static_cast<unsigned>(a.rows), threads_for(a.rows, a.vocab), 0, st>>>(
+        static_cast<const T*>(a.z), a.ld, a.vocab, a.v0, t, a.inv_temperature, dloss, loss, static_cast<T*>(dz), ldd);
+  });
+  count_launch();
+  return cudaGetLastError();
+}
+
+}  // namespace ethb

@@ -458,3 +458,260 @@ def softmax_bwd(dy, y, scale, causal=True):
         return dx
     yf, dyf = y.float(), dy.float()
     return ((dyf - (dyf * yf).sum(-1, keepdim=True)) * yf * scale).to(y.dtype)
+
+
+# ---------------------------------------------------------------------------------- token log-probabilities
+MAX_TOP_ALTERNATIVES = 128    # top_k of token_scores_fwd
+MAX_TEACHER_ENTRIES = 512     # entries per row of a teacher's list
+
+
+def _wide(t):
+    """The type a CPU reference computes in: double stays double (gradient checks), the rest is fp32."""
+    return t if t.dtype == torch.float64 else t.float()
+
+
+def _check_logits(logits, temperature, what):
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError(f"{what}: logits must be [tokens, vocab], got {tuple(logits.shape)}")
+    kinds = (torch.float32, torch.float16, torch.bfloat16) + (() if logits.is_cuda else (torch.float64,))
+    if logits.dtype not in kinds:
+        raise ValueError(f"{what}: logits of type {logits.dtype} are not supported")
+    if not (math.isfinite(temperature) and temperature > 0):
+        raise ValueError(f"{what}: temperature must be positive and finite, got {temperature}")
+
+
+def _check_rows(t, logits, dtypes, shape, what):
+    """`t` as a contiguous tensor of the given shape beside the logits."""
+    if not isinstance(t, torch.Tensor) or t.device != logits.device or t.dtype not in dtypes or tuple(t.shape) != shape:
+        got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+        raise ValueError(f"{what} must be {' or '.join(str(d) for d in dtypes)} {shape} on {logits.device}, got {got}")
+    return t.contiguous()
+
+
+def _unit_rows(logits):
+    """Logits with unit inner stride and rows that do not overlap; any pitch is taken as it is."""
+    if logits.shape[1] > 1 and logits.stride(1) != 1 or logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]:
+        return logits.contiguous()
+    return logits
+
+
+def _grad_rows(logits):
+    """An uninitialised gradient whose rows sit at the same offsets from a 16-byte boundary as the
+    rows of `logits` (a slice of a padded vocabulary keeps vector accesses on both sides)."""
+    rows, vocab = logits.shape
+    per = 16 // logits.element_size()
+    lead = logits.data_ptr() % 16 // logits.element_size()
+    pitch = vocab + (logits.stride(0) - vocab) % per if rows > 1 else vocab
+    if lead == 0 and pitch == vocab:
+        return torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
+    flat = torch.empty(lead + rows * pitch, dtype=logits.dtype, device=logits.device)
+    return flat.as_strided((rows, vocab), (pitch, 1), lead)
+
+
+def token_scores_fwd(logits, tokens, top_k=0, temperature=1.0, vocab_start=0, gather_fn=None):
+    """Log-probability of `tokens` under softmax(logits / temperature), entropy of that distribution and
+    its `top_k` most likely tokens. Returns (logprob, entropy, top_logprob, top_index, stats); `stats`
+    [tokens, 2] (subtracted maximum, sum of exponentials) belongs to `token_scores_bwd`.
+
+    logits: [tokens, vocab_local] of a vocabulary shard that starts at `vocab_start`; `gather_fn` as in
+    `ce_fwd`. A negative token is none: its log-probability is 0 and has no gradient; one at or beyond
+    the whole vocabulary has NaN. Alternatives fall in log-probability, equal ones go by rising id."""
+    _check_logits(logits, temperature, "token_scores_fwd")
+    rows, vocab = logits.shape
+    if not 0 <= top_k <= min(MAX_TOP_ALTERNATIVES, vocab):
+        raise ValueError(f"top_k must be between 0 and {min(MAX_TOP_ALTERNATIVES, vocab)}, got {top_k}")
+    tokens = _check_rows(tokens, logits, (torch.int64,), (rows,), "tokens")
+    logits = _unit_rows(logits)
+    if native.use_native(logits):
+        def new(*shape, dtype=torch.float32):
+            return torch.empty(shape, dtype=dtype, device=logits.device)
+        logprob, entropy, stats = new(rows), new(rows), new(rows, 2)
+        top_logprob = new(rows, top_k) if top_k else None
+        top_index = new(rows, top_k, dtype=torch.int64) if top_k else None
+        if gather_fn is None:
+            native.lib().token_scores(logits, tokens, top_k, temperature, vocab_start, logprob, entropy, top_logprob,
+                                      top_index, stats)
+        else:
+            part = new(rows, 4 + 2 * top_k)
+            native.lib().token_scores_partial(logits, tokens, top_k, temperature, vocab_start, part)
+            native.lib().token_scores_combine(gather_fn(part).contiguous(), tokens, top_k, temperature, logprob,
+                                              entropy, top_logprob, top_index, stats)
+        return logprob, entropy, top_logprob, top_index, stats
+    z = _wide(logits)
+    mx = z.amax(1)
+    mu = torch.where(mx == -math.inf, 0.0, mx)
+    t = (z - mu[:, None]) / temperature
+    e = torch.exp(t)
+    local = tokens - vocab_start
+    here = (tokens >= 0) & (local >= 0) & (local < vocab)
+    zt = torch.where(here, z.gather(1, local.clamp(0, vocab - 1)[:, None])[:, 0], math.nan)
+    order = torch.sort(z, dim=1, descending=True, stable=True).indices[:, :top_k]
+    part = torch.cat([mx[:, None], e.sum(1, keepdim=True), torch.where(e > 0, e * t, e).sum(1, keepdim=True), zt[:, None],
+                      z.gather(1, order), (order + vocab_start).to(z.dtype)], 1)
+    parts = gather_fn(part) if gather_fn is not None else part.unsqueeze(0)
+    mx = parts[:, :, 0].amax(0)
+    mu = torch.where(mx == -math.inf, 0.0, mx)
+    d = torch.where(parts[:, :, 0] == -math.inf, 0.0, (parts[:, :, 0] - mu) / temperature)
+    c = torch.exp(d)
+    total = (c * parts[:, :, 1]).sum(0)
+    weighted = torch.where(c > 0, c * (parts[:, :, 2] + d * parts[:, :, 1]), 0.0).sum(0)
+    log_total = torch.log(total)
+    found = parts[:, :, 3]
+    zt = torch.where(found.isnan().all(0), math.nan, found.nan_to_num(nan=0.0, posinf=math.inf, neginf=-math.inf).sum(0))
+    logprob = torch.where(tokens < 0, 0.0, (zt - mu) / temperature - log_total)
+    entropy = log_total - weighted / total
+    top_logprob = top_index = None
+    if top_k:
+        value = parts[:, :, 4:4 + top_k].permute(1, 0, 2).flatten(1)
+        index = parts[:, :, 4 + top_k:].permute(1, 0, 2).flatten(1).long()
+        by_id = torch.argsort(index, 1)
+        value, index = value.gather(1, by_id), index.gather(1, by_id)
+        best = torch.sort(value, dim=1, descending=True, stable=True).indices[:, :top_k]
+        top_logprob = (value.gather(1, best) - mu[:, None]) / temperature - log_total[:, None]
+        top_index = index.gather(1, best)
+    return logprob, entropy, top_logprob, top_index, torch.stack([mu, total], 1)
+
+
+def token_scores_bwd(logits, tokens, stats, entropy, top_index, d_logprob=None, d_entropy=None, d_top=None,
+                     temperature=1.0, vocab_start=0):
+    """Gradient of the logits from the gradients of logprob [tokens], entropy [tokens] and top_logprob
+    [tokens, top_k] (any may be None). A row whose gradients are all 0 gets zeros, whatever its logits."""
+    logits = _unit_rows(logits)
+    rows, vocab = logits.shape
+    wide = (torch.float32,) if logits.is_cuda else (torch.float32, torch.float64)
+    top_k = 0 if top_index is None else top_index.shape[1]
+    grads = []
+    for t, shape, what in ((d_logprob, (rows,), "d_logprob"), (d_entropy, (rows,), "d_entropy"),
+                           (d_top, (rows, top_k), "d_top")):
+        grads.append(None if t is None else _check_rows(t, logits, wide, shape, what))
+    g, h, u = grads
+    if native.use_native(logits):
+        dz = _grad_rows(logits)
+        native.lib().token_scores_bwd(logits, tokens, stats, entropy, top_index, top_k, temperature, vocab_start, g, h, u,
+                                      dz)
+        return dz
+    z = _wide(logits)
+    logp = (z - stats[:, :1]) / temperature - torch.log(stats[:, 1:])
+    p = torch.exp(logp)
+    zero = z.new_zeros(rows)
+    g = zero if g is None else torch.where(tokens >= 0, g, 0.0).to(z.dtype)
+    h = zero if h is None else h.to(z.dtype)
+    total = g if u is None else g + u.sum(1).to(z.dtype)
+    dz = -p * total[:, None] - torch.where(p > 0, p * (logp + entropy[:, None]), 0.0) * h[:, None]
+    live = (g != 0) | (h != 0)
+    index, weight = tokens[:, None], g[:, None]
+    if u is not None:
+        live = live | (u != 0).any(1)
+        index, weight = torch.cat([index, top_index], 1), torch.cat([weight, u.to(z.dtype)], 1)
+    dz = torch.where(live[:, None], dz, 0.0)
+    return _add_listed(dz, index, weight, vocab_start).div_(temperature).to(logits.dtype)
+
+
+def _add_listed(dz, index, weight, vocab_start):
+    """dz[r, index[r, k] - vocab_start] += weight[r, k], entries of other shards left out."""
+    local = index - vocab_start
+    here = (index >= 0) & (local >= 0) & (local < dz.shape[1])
+    return dz.scatter_add_(1, local.clamp(0, dz.shape[1] - 1), torch.where(here, weight, 0.0))
+
+
+# ---------------------------------------------------------------------------------- distillation
+def _check_teacher(logits, index, logit):
+    rows = logits.shape[0]
+    if not isinstance(index, torch.Tensor) or index.dim() != 2 or not 1 <= index.shape[1] <= MAX_TEACHER_ENTRIES:
+        raise ValueError(f"teacher lists must be [tokens, 1..{MAX_TEACHER_ENTRIES}]")
+    shape = (rows, index.shape[1])
+    wide = (torch.float32,) if logits.is_cuda else (torch.float32, torch.float64)
+    return (_check_rows(index, logits, (torch.int64,), shape, "teacher_index"),
+            _check_rows(logit, logits, wide, shape, "teacher_logit"))
+
+
+def _teacher_ref(logits, logit, temperature):
+    """(q, log q, row has entries) of the listed teacher logits."""
+    t = logit.to(_wide(logits).dtype) / temperature
+    some = ~(t == -math.inf).all(1, keepdim=True)
+    log_q = torch.log_softmax(torch.where(some, t, 0.0), 1)
+    return torch.where(some, torch.exp(log_q), 0.0), log_q, some[:, 0]
+
+
+def distill_fwd(logits, teacher_index, teacher_logit, temperature=1.0, vocab_start=0, gather_fn=None):
+    """Per-token loss sum_k q_k (log q_k - log p[teacher_index_k]), q = softmax of the listed teacher
+    logits / temperature, p = softmax(logits / temperature) over the whole vocabulary. Returns (loss,
+    stats for `distill_bwd`). An entry at -inf is unused; a row without entries has loss 0; a used
+    entry outside the vocabulary makes the row's loss NaN. An id listed twice counts twice."""
+    _check_logits(logits, temperature, "distill_fwd")
+    index, logit = _check_teacher(logits, teacher_index, teacher_logit)
+    logits = _unit_rows(logits)
+    rows, vocab = logits.shape
+    if native.use_native(logits):
+        loss = torch.empty(rows, dtype=torch.float32, device=logits.device)
+        stats = torch.empty((rows, 2), dtype=torch.float32, device=logits.device)
+        if gather_fn is None:
+            native.lib().distill_fwd(logits, index, logit, temperature, vocab_start, loss, stats)
+        else:
+            part = torch.empty((rows, 4), dtype=torch.float32, device=logits.device)
+            native.lib().distill_partial(logits, index, logit, temperature, vocab_start, part)
+            native.lib().distill_combine(gather_fn(part).contiguous(), index, logit, temperature, loss, stats)
+        return loss, stats
+    z = _wide(logits)
+    q, log_q, some = _teacher_ref(logits, logit, temperature)
+    mx = z.amax(1)
+    mu = torch.where(mx == -math.inf, 0.0, mx)
+    local = index - vocab_start
+    here = (q != 0) & (local >= 0) & (local < vocab)
+    picked = (z.gather(1, local.clamp(0, vocab - 1)) - mu[:, None]) / temperature
+    part = torch.stack([mx, torch.exp((z - mu[:, None]) / temperature).sum(1), torch.where(here, q * picked, 0.0).sum(1),
+                        torch.where(here, q, 0.0).sum(1)], 1)
+    parts = gather_fn(part) if gather_fn is not None else part.unsqueeze(0)
+    top = parts[:, :, 0].amax(0)
+    mu = torch.where(top == -math.inf, 0.0, top)
+    d = (torch.where(parts[:, :, 0] == -math.inf, 0.0, parts[:, :, 0]) - mu) / temperature
+    total = torch.where(parts[:, :, 1] == 0, 0.0, torch.exp(d) * parts[:, :, 1]).sum(0)
+    found = torch.where(parts[:, :, 3] == 0, 0.0, parts[:, :, 2] + parts[:, :, 3] * d).sum(0)
+    whole = (parts[:, :, 3].sum(0) - 1).abs() < 1e-4
+    loss = torch.where(q != 0, q * log_q, 0.0).sum(1) - found + torch.log(total)
+    loss = torch.where(some, torch.where(whole, loss, math.nan), 0.0)
+    return loss, torch.stack([torch.where(some, mu, 0.0), torch.where(some, total, 1.0)], 1)
+
+
+def distill_bwd(logits, teacher_index, teacher_logit, stats, dloss, temperature=1.0, vocab_start=0):
+    """d loss / d logits scaled by dloss[row]; rows without entries or with dloss 0 get zeros."""
+    index, logit = _check_teacher(logits, teacher_index, teacher_logit)
+    logits = _unit_rows(logits)
+    wide = (torch.float32,) if logits.is_cuda else (torch.float32, torch.float64)
+    dloss = _check_rows(dloss, logits, wide, (logits.shape[0],), "dloss")
+    if native.use_native(logits):
+        dz = _grad_rows(logits)
+        native.lib().distill_bwd(logits, index, logit, stats, dloss, temperature, vocab_start, dz)
+        return dz
+    z = _wide(logits)
+    q, _, some = _teacher_ref(logits, logit, temperature)
+    g = torch.where(some, dloss.to(z.dtype), 0.0) / temperature
+    p = torch.exp((z - stats[:, :1]) / temperature) / stats[:, 1:]
+    dz = torch.where((g != 0)[:, None], p * g[:, None], 0.0)
+    return _add_listed(dz, index, -q * g[:, None], vocab_start).to(logits.dtype)
+
+
+def distill_step(logits, teacher_index, teacher_logit, dloss, temperature=1.0, out=None):
+    """(loss, d logits) of `distill_fwd` and `distill_bwd` in one pass over the logits, for a caller that
+    knows the gradient of every row's loss beforehand (the last pipeline stage does: loss scale over
+    token count). Whole vocabulary only. `out` takes the gradient; it may be `logits` itself."""
+    _check_logits(logits, temperature, "distill_step")
+    index, logit = _check_teacher(logits, teacher_index, teacher_logit)
+    wide = (torch.float32,) if logits.is_cuda else (torch.float32, torch.float64)
+    dloss = _check_rows(dloss, logits, wide, (logits.shape[0],), "dloss")
+    if out is not None:
+        if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device or \
+                (out.shape[1] > 1 and out.stride(1) != 1) or (out.shape[0] > 1 and out.stride(0) < out.shape[1]):
+            raise ValueError("distill_step: out must match the logits and have contiguous rows that do not overlap")
+        same = out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride()
+        if not same and out.untyped_storage().data_ptr() == logits.untyped_storage().data_ptr():
+            raise ValueError("distill_step: out may be the logits themselves or other memory, not an overlapping view")
+    x = _unit_rows(logits)
+    if native.use_native(x):
+        loss = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
+        dz = _grad_rows(x) if out is None else out
+        native.lib().distill_step(x, index, logit, dloss, temperature, 0, loss, dz)
+        return loss, dz
+    loss, stats = distill_fwd(x, index, logit, temperature)
+    dz = distill_bwd(x, index, logit, stats, dloss, temperature)
+    return loss, dz if out is None else out.copy_(dz)

@@ -1,0 +1,261 @@
+"""Vocabulary kernels (token log-probabilities with entropy and alternatives, distillation) against
+their definitions in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from eth_b200 import ops
+from eth_b200.ops import raw
+from helpers import oracle_tokens as oracle
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+#: rows, vocabulary, row pitch beyond the vocabulary, elements before the first row
+SHAPES = [(1, 1, 0, 0), (1, 50304, 0, 0), (3, 7, 0, 0), (5, 1000, 24, 0), (7, 1003, 5, 3), (40, 5003, 0, 1),
+          (300, 4099, 0, 0), (297, 50257, 47, 0), (2, 131071, 0, 0)]
+
+
+def _logits(rows, vocab, pad, lead, dtype, seed=0, scale=2.5):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    flat = torch.randn(lead + rows * (vocab + pad), generator=g, device=DEV).mul_(scale).to(dtype)
+    return flat[lead:].view(rows, vocab + pad)[:, :vocab], g
+
+
+def _teacher(rows, vocab, k, g):
+    index = torch.randint(vocab, (rows, k), generator=g, device=DEV)
+    logit = torch.randn(rows, k, generator=g, device=DEV)
+    used = (torch.arange(rows, device=DEV) * 5 % (2 * k + 1))[:, None]       # shorter lists, empty rows
+    return index, logit.masked_fill(torch.arange(k, device=DEV) >= used, -math.inf)
+
+
+def _close(got, want, tol):
+    """`tol` covers the statistics. A result far from 0 (a token masked with fp16's lowest value lies 65504
+    below the others) also carries the roundings of its last two fp32 steps, 2^-24 of itself each."""
+    return (((got - want).abs() <= tol + 2.0 ** -23 * want.abs()) | (got == want)).all()     # -inf equals -inf
+
+
+def _same_scores(r, logits, tokens, top_k, temperature):
+    lp, ent, top_lp, top_id, _ = oracle.scores(logits, tokens, top_k, temperature)
+    tol = oracle.statistic_tolerance(logits, temperature)
+    assert _close(r.logprob, lp, tol) and _close(r.entropy, ent, tol)
+    if top_k:
+        assert torch.equal(r.top_index, top_id) and _close(r.top_logprob, top_lp, tol[:, None])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("top_k", [0, 1, 20, 128])
+def test_token_logprobs_forward(dtype, shape, top_k):
+    rows, vocab = shape[:2]
+    logits, g = _logits(*shape, dtype)
+    top_k = min(top_k, vocab)
+    tokens = torch.randint(vocab, (rows,), generator=g, device=DEV)
+    for temperature in (1.0, 0.6):
+        _same_scores(ops.token_logprobs(logits, tokens, top_k, temperature), logits, tokens, top_k, temperature)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [130, 5003, 50304])
+@pytest.mark.parametrize("top_k", [3, 128])
+def test_ties_and_masks(dtype, vocab, top_k):
+    """Rows where the first bound on the k-th alternative is loose, empty or reached by everything."""
+    low = torch.finfo(dtype).min
+    z, g = _logits(12, vocab, 0, 0, dtype, seed=1)
+    z[0] = 0                                          # all equal
+    z[1] = low                                        # the type's lowest value everywhere
+    z[2] = -math.inf
+    z[2, vocab // 2:] = 1.0                           # many equal behind masked ones
+    z[3, 1:] = -math.inf                              # one token left
+    z[4] = z[4].round()                               # a handful of distinct values
+    z[5] = 0
+    z[5, ::2] = -0.0                                  # both zeros are one value
+    z[6, 2:] = low
+    z[7] = -torch.arange(vocab, device=DEV).to(dtype)
+    z[8] = torch.arange(vocab, device=DEV).to(dtype) / vocab
+    z[9] = torch.finfo(dtype).smallest_normal / 4     # subnormal, above, equal and below zero
+    z[9, ::3] *= -1
+    z[9, 5] *= 2
+    z[10, :] = 1.0
+    z[10, -top_k:] = 2.0
+    z[11, 17:33] = 30.0
+    tokens = torch.zeros(12, dtype=torch.long, device=DEV)
+    _same_scores(ops.token_logprobs(z, tokens, top_k), z, tokens, top_k, 1.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_undefined_rows_and_tokens(dtype):
+    z, g = _logits(7, 6000, 0, 0, dtype, seed=2)
+    z[0] = -math.inf
+    z[1, 77] = math.nan
+    z[2, 5001] = math.inf
+    z[3] = math.nan
+    tokens = torch.tensor([0, 1, 2, 3, -1, 6000, 1 << 40], device=DEV)
+    r = ops.token_logprobs(z, tokens, top_k=9)
+    assert r.logprob[:4].isnan().all() and r.entropy[:4].isnan().all()
+    assert r.logprob[4] == 0 and r.logprob[5:].isnan().all() and r.entropy[4:].isfinite().all()
+    order = torch.sort(z.double(), dim=1, descending=True, stable=True).indices[:, :9]   # NaN first, as torch sorts
+    assert torch.equal(r.top_index, order)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("which", ["logprob", "entropy", "top", "all"])
+def test_token_logprobs_backward(dtype, shape, which):
+    rows, vocab = shape[:2]
+    logits, g = _logits(*shape, dtype, seed=3)
+    logits.requires_grad_(True)
+    top_k = min(11, vocab)
+    tokens = torch.randint(-1, vocab, (rows,), generator=g, device=DEV)
+    r = ops.token_logprobs(logits, tokens, top_k=top_k, temperature=0.8)
+    outs = {"logprob": r[:1], "entropy": r[1:2], "top": r[2:3], "all": r[:3]}[which]
+    d = [torch.randn(x.shape, generator=g, device=DEV) for x in outs]
+    for x in d:
+        x[rows // 2] = 0                              # a row without any gradient
+    got, = torch.autograd.grad(outs, logits, d)
+    full = dict(zip({"logprob": "g", "entropy": "h", "top": "u", "all": "ghu"}[which], d))
+    want = oracle.scores_grad(logits, tokens, r.top_index, full.get("g"), full.get("h"), full.get("u"), 0.8)
+    # p is off by 2^-22 of itself and of its exponent (up to 60); p log p by the same of at most p |log p| <= 0.37
+    assert oracle.grad_error(got, want, sum(x.abs().reshape(rows, -1).sum(1) for x in d) * 2.0 ** -17) <= 1
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("k", [1, 32, 512])
+def test_distillation(dtype, shape, k):
+    rows, vocab = shape[:2]
+    logits, g = _logits(*shape, dtype, seed=4)
+    logits.requires_grad_(True)
+    index, logit = _teacher(rows, vocab, k, g)        # 512 entries over small vocabularies list ids many times
+    dloss = torch.randn(rows, generator=g, device=DEV)
+    dloss[rows // 2] = 0
+    for temperature in (1.0, 2.0):
+        loss = ops.topk_distillation_loss(logits, index, logit, temperature)
+        want_loss, want = oracle.distill(logits, index, logit, dloss, temperature)
+        assert ((loss - want_loss).abs() <= oracle.statistic_tolerance(logits, temperature)).all()
+        got, = torch.autograd.grad(loss, logits, dloss)
+        noise = dloss.abs() * 2.0 ** -17
+        assert oracle.grad_error(got, want, noise) <= 1
+        loss2, got2 = raw.distill_step(logits.detach(), index, logit, dloss, temperature)
+        assert ((loss2 - want_loss).abs() <= oracle.statistic_tolerance(logits, temperature)).all()
+        assert oracle.grad_error(got2, want, noise) <= 1
+    buf = torch.full((rows, vocab + 9), 7.0, dtype=dtype, device=DEV)
+    out = buf[:, :vocab]                              # another offset and pitch than the logits
+    loss3, _ = raw.distill_step(logits.detach(), index, logit, dloss, temperature, out=out)
+    assert torch.equal(out, got2) and torch.equal(loss3, loss2) and (buf[:, vocab:] == 7).all()
+    buf = torch.full((rows, vocab + 9), 7.0, dtype=dtype, device=DEV)
+    buf[:, :vocab] = logits.detach()
+    loss4, _ = raw.distill_step(buf[:, :vocab], index, logit, dloss, temperature, out=buf[:, :vocab])
+    assert oracle.grad_error(buf[:, :vocab].contiguous(), want, noise) <= 1 and (buf[:, vocab:] == 7).all()
+
+
+def test_unused_entries_and_strangers():
+    z, g = _logits(4, 3000, 0, 0, torch.bfloat16)
+    z.requires_grad_(True)
+    index = torch.tensor([[5, -9, 1 << 40], [2999, 2999, 2999], [7, 3000, 8], [1, 2, 3]], device=DEV)
+    logit = torch.tensor([[0.5, -math.inf, -math.inf], [0.0, 1.0, -1.0], [0.0, 0.0, 0.0],
+                          [math.nan, 0.0, 0.0]], device=DEV)
+    loss = ops.topk_distillation_loss(z, index, logit)
+    want, grad = oracle.distill(z[:2], index[:2], logit[:2], torch.ones(2, device=DEV), 1.0)
+    assert ((loss[:2] - want).abs() < 1e-5).all() and loss[2:].isnan().all()
+    got, = torch.autograd.grad(loss[:2].sum(), z)
+    assert oracle.grad_error(got[:2], grad, torch.full((2,), 2.0 ** -17, device=DEV)) <= 1 and (got[2:] == 0).all()
+
+
+@pytest.mark.parametrize("world", [2, 3])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_vocabulary_shards(dtype, world):
+    part, rows, k = 2051, 33, 40
+    logits, g = _logits(rows, part * world, 0, 0, dtype, seed=6)
+    logits[1, :part] = -math.inf
+    logits[2] = 0.5
+    tokens = torch.randint(part * world, (rows,), generator=g, device=DEV)
+    index, logit = _teacher(rows, part * world, 17, g)
+    shards = logits.split(part, 1)
+    sent = {"scores": [], "distill": []}
+    for w, z in enumerate(shards):
+        for name, op, args in (("scores", ops.token_logprobs, (tokens, k)),
+                               ("distill", ops.topk_distillation_loss, (index, logit))):
+            op(z, *args, 0.9, w * part, lambda x: (sent[name].append(x), x.unsqueeze(0))[1])
+    dloss = torch.randn(rows, generator=g, device=DEV)
+    want_loss, want = oracle.distill(logits, index, logit, dloss, 0.9)
+    _, _, _, top_id, _ = oracle.scores(logits, tokens, k, 0.9)
+    want_z = oracle.scores_grad(logits, tokens, top_id, dloss, dloss, None, 0.9)
+    for w in range(world):
+        z = shards[w].detach().requires_grad_(True)
+        r = ops.token_logprobs(z, tokens, k, 0.9, w * part, lambda x: torch.stack(sent["scores"]))
+        _same_scores(r, logits, tokens, k, 0.9)
+        loss = ops.topk_distillation_loss(z, index, logit, 0.9, w * part, lambda x: torch.stack(sent["distill"]))
+        assert _close(loss, want_loss, oracle.statistic_tolerance(logits, 0.9))     # row 1 may be infinitely far off
+        mine = slice(w * part, (w + 1) * part)
+        got, = torch.autograd.grad(loss, z, dloss)
+        assert oracle.grad_error(got, want[:, mine], dloss.abs() * 2.0 ** -17) <= 1
+        got, = torch.autograd.grad((r.logprob, r.entropy), z, (dloss, dloss))
+        assert oracle.grad_error(got, want_z[:, mine], dloss.abs() * 2.0 ** -16) <= 1
+
+
+def test_same_bits_every_time():
+    z, g = _logits(64, 50304, 0, 0, torch.bfloat16, seed=8)
+    tokens = torch.randint(50304, (64,), generator=g, device=DEV)
+    index, logit = _teacher(64, 50304, 100, g)
+    first = None
+    for _ in range(4):
+        zr = z.detach().requires_grad_(True)
+        r = ops.token_logprobs(zr, tokens, top_k=100)
+        gz, = torch.autograd.grad((r.logprob.sum() + r.top_logprob.sum(),), zr)
+        got = [*r, gz, *raw.distill_step(z, index, logit, r.logprob.detach())]
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
+
+
+def test_captured_and_on_another_stream():
+    z, g = _logits(33, 5000, 0, 0, torch.bfloat16, seed=9)
+    tokens = torch.randint(5000, (33,), generator=g, device=DEV)
+    index, logit = _teacher(33, 5000, 10, g)
+    dloss = torch.ones(33, device=DEV)
+    logits = z.clone()
+
+    def work():
+        return [*raw.token_scores_fwd(logits, tokens, 5)[:4], *raw.distill_step(logits, index, logit, dloss)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        eager = work()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work()
+    logits.copy_(z.flip(0))
+    graph.replay()
+    now = work()
+    assert all(torch.equal(a, b) for a, b in zip(out, now))
+    logits.copy_(z)
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(out, eager))
+
+
+def test_offsets_beyond_32_bits():
+    """3 rows, 2^30 elements apart, of one buffer: the last starts behind 2^31 elements."""
+    pitch = 1 << 30
+    flat = torch.empty(2 * pitch + 1024, dtype=torch.bfloat16, device=DEV)
+    z = flat.as_strided((3, 1000), (pitch, 1))
+    z.copy_(torch.randn(3, 1000, device=DEV))
+    tokens = torch.tensor([0, 999, 500], device=DEV)
+    _same_scores(ops.token_logprobs(z, tokens, 4), z.contiguous(), tokens, 4, 1.0)
+    index, logit = torch.tensor([[1, 2], [3, 4], [5, 6]], device=DEV), torch.zeros(3, 2, device=DEV)
+    want, grad = oracle.distill(z.contiguous(), index, logit, torch.ones(3, device=DEV), 1.0)
+    loss, _ = raw.distill_step(z, index, logit, torch.ones(3, device=DEV), out=z)
+    assert ((loss - want).abs() < 1e-5).all()
+    assert oracle.grad_error(z.contiguous(), grad, torch.full((3,), 2.0 ** -17, device=DEV)) <= 1
+
+
+def test_refusals_on_the_device():
+    z, t = torch.randn(3, 11, device=DEV), torch.zeros(3, dtype=torch.long, device=DEV)
+    index, logit = torch.zeros(3, 2, dtype=torch.long, device=DEV), torch.zeros(3, 2, device=DEV)
+    for bad in (lambda: ops.token_logprobs(z, t.cpu()), lambda: ops.token_logprobs(z.double(), t),
+                lambda: ops.topk_distillation_loss(z, index.cpu(), logit),
+                lambda: ops.topk_distillation_loss(z, index, logit.cpu()),
+                lambda: raw.distill_step(z, index, logit, torch.ones(3))):
+        with pytest.raises(ValueError):
+            bad()
