@@ -1,0 +1,1291 @@
+// Flash attention over packed documents for sm_100a: forward and backward on tcgen05 tensor cores with
+// TMEM accumulators, documents of any length one behind the other on one row axis, grouped heads.
+//
+// A host-built work list names (document start, length, tile) per unit of work, heaviest first; tiles
+// are aligned to their document, so no tile mixes documents and nothing of one document reaches
+// another. Where a tile runs over its document's end, its rows behind the end are cleared in shared
+// memory before they become summands of an MMA.
+//
+// Forward. One CTA owns two 128-row query tiles and streams the key/value tiles once for both:
+//   warp 0      TMA producer: Q (once), then K_j / V_j tiles into a ring of shared-memory stages.
+//   warp 1      MMA issuer:   S_t = Q_t K_j^T  (operands in shared memory, accumulator in TMEM),
+//               O_t += P_t V_j (P_t read from TMEM, V_j from shared memory as an MN-major operand).
+//   warps 2-5   softmax of query tile 0, warps 6-9 softmax of query tile 1: one thread per query
+//               row; online softmax in the exp2 domain, P written back to TMEM as packed 16-bit
+//               (aliasing the scores), the O accumulator rescaled only when the running maximum grew
+//               by more than 2^8 (exact after the final normalisation).
+// The two tiles are the same rows of two heads of a group where the group is even (both then meet the
+// same number of key tiles under the causal mask, and a document of up to 128 rows fills both), else
+// two consecutive tiles of one head.
+//
+// TMEM map (512 columns): S_0/P_0 [0,128)  S_1/P_1 [128,256)  O_0 [256,256+D)  O_1 [384,384+D).
+//
+// P and dS are rounded to the input type, as the tensor core takes both operands in one type; the
+// sums, the softmax statistics and all accumulators are fp32.
+#include "attention_packed_sm100.cuh"
+#include "gemm_sm100.cuh"
+#include "sm100_common.cuh"
+
+#include <atomic>
+#include <mutex>
+
+namespace ethb {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kTile = 128;
+constexpr float kRescaleThreshold = 8.0f;  // log2 units
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                              const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static EncodeFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* sym = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q) ==
+            cudaSuccess && q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeFn>(sym);
+  });
+  return fn;
+}
+
+// 3-D map over a [rows, heads, head_dim] view: dims {d, rows, heads}, box {64, 128, 1}. A tile may start
+// at any row; rows beyond the last read as 0.
+cudaError_t make_tmap_rhd(CUtensorMap* map, const void* base, int dtype, int d, int rows, int heads,
+                          const int64_t strides[2]) {
+  EncodeFn fn = encode_fn();
+  if (!fn) return cudaErrorNotSupported;
+  ensure_thread_context();
+  ETHB_RETURN_IF((reinterpret_cast<uintptr_t>(base) & 15) != 0 || strides[0] % 8 != 0 || strides[1] % 8 != 0,
+                 cudaErrorMisalignedAddress, "packed attention: base and strides must be multiples of 16 bytes");
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(rows),
+                              static_cast<cuuint64_t>(heads)};
+  const cuuint64_t gstr[2] = {static_cast<cuuint64_t>(strides[0]) * 2, static_cast<cuuint64_t>(strides[1]) * 2};
+  const cuuint32_t box[3] = {64, kTile, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(map, dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                        3, const_cast<void*>(base), dims, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  ETHB_RETURN_IF(r != CUDA_SUCCESS, cudaErrorInvalidValue, "cuTensorMapEncodeTiled (packed attention)");
+  return cudaSuccess;
+}
+
+// A wait whose outcome all lanes of the warp share, so that a timeout cannot split a warp (or, through
+// wg_and, a warpgroup) between leaving and going on to the next warp-wide or group-wide operation.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code));
+}
+
+__device__ __forceinline__ uint32_t pack_pair(float a, float b, int dtype) {
+  return pack2(a, b, dtype);
+}
+
+// Clears rows [first, 128) of a tile that a TMA load has written (kHalves blocks of 128 rows x 128
+// bytes; the swizzle permutes inside a row only) and makes that visible to the tensor core's reads.
+// Executed by one warp; the caller signals the tile afterwards.
+template <int kHalves>
+__device__ __forceinline__ void clear_tail(uint8_t* tile, int first, int lane) {
+#pragma unroll
+  for (int h = 0; h < kHalves; ++h)
+    for (int c = first * 8 + lane; c < kTile * 8; c += 32)
+      reinterpret_cast<uint4*>(tile + h * 16384)[c] = make_uint4(0, 0, 0, 0);
+  fence_proxy_async();
+}
+
+// Clears rows [first, rows) of a [rows, heads, D] 16-bit output: block `part` of `parts`.
+template <int D>
+__device__ __forceinline__ void clear_rows(void* base, int64_t row_stride, int64_t head_stride, int first, int rows, int heads,
+                                           int part, int parts) {
+  constexpr int kChunks = D / 8;
+  const int64_t total = static_cast<int64_t>(rows - first) * heads * kChunks;
+  for (int64_t i = static_cast<int64_t>(part) * blockDim.x + threadIdx.x; i < total;
+       i += static_cast<int64_t>(parts) * blockDim.x) {
+    const int c = static_cast<int>(i % kChunks);
+    const int64_t rh = i / kChunks;
+    uint16_t* at = reinterpret_cast<uint16_t*>(base) + (first + rh / heads) * row_stride + (rh % heads) * head_stride;
+    reinterpret_cast<uint4*>(at)[c] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+int sm_count() {
+  int dev = 0, n = 0;
+  cudaGetDevice(&dev);
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+  return n;
+}
+
+// The dynamic shared memory limit is a property of a kernel on a device; setting it again is harmless.
+template <typename K>
+cudaError_t allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
+// ==============================================================================================
+// forward
+// ==============================================================================================
+template <int D> struct FwdCfg {
+  static constexpr int kHalves = D / 64;
+  static constexpr int kQBytes = 2 * kHalves * 16384;       // two query tiles
+  // K and V tiles travel through one ring of equal slots in the order K_0 V_0 K_1 V_1 ...: a K
+  // slot is free again as soon as both score MMAs of its tile are done, a whole iteration before
+  // the V slot of the same tile, so five slots keep the loads a full iteration ahead of their use.
+  static constexpr int kSlotBytes = kHalves * 16384;
+  static constexpr int kSlots = (D == 128) ? 5 : 8;
+  static constexpr int kSmemBytes = kQBytes + kSlots * kSlotBytes + 1024 + 256;
+  static constexpr int kThreads = 320;
+};
+
+struct FwdBarriers {
+  uint64_t q_full;
+  uint64_t tail_full;     // the last V tile of a document has landed, rows behind its end not yet cleared
+  uint64_t kv_full[8];
+  uint64_t kv_empty[8];
+  uint64_t s_full[2];
+  uint64_t p_half[8];     // [tile * 4 + quarter]: 32 more P columns of a tile are written
+  uint64_t o_done[2];
+  uint32_t tmem_base;
+  uint32_t pad;
+};
+
+template <int D, int DT, bool kPair>
+__global__ void __launch_bounds__(320, 1)
+packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                const __grid_constant__ CUtensorMap tv, const PackedAttnArgs p) {
+  using C = FwdCfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sKV = smem + C::kQBytes;
+  FwdBarriers* bars = reinterpret_cast<FwdBarriers*>(sKV + C::kSlots * C::kSlotBytes);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  // 1-D grid, dispatched in index order: the work list is sorted heaviest first, every entry is taken
+  // by all its head units before the next one, so the last CTAs to start are the short ones
+  const int units = kPair ? p.heads / 2 : p.heads;
+  if (static_cast<int>(blockIdx.x) >= p.num_tiles * units) {
+    clear_rows<D>(p.o, p.o_strides[0], p.o_strides[1], p.used, p.rows, p.heads, blockIdx.x - p.num_tiles * units,
+                  gridDim.x - p.num_tiles * units);
+    return;
+  }
+  const PackedTile w = p.tiles[blockIdx.x / units];
+  const int unit = blockIdx.x % units;
+  const int group = p.heads / p.kv_heads;
+  const int head0 = kPair ? 2 * unit : unit;         // head of tile t: head0 + t when heads are paired
+  const int kv_head = head0 / group;
+  const int kv_tiles = (w.len + kTile - 1) / kTile;
+  int n_t[2], qt_t[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    qt_t[t] = kPair ? w.tile : 2 * w.tile + t;       // query tile inside the document
+    if (qt_t[t] * kTile >= w.len) n_t[t] = 0;
+    else n_t[t] = p.causal ? qt_t[t] + 1 : kv_tiles;
+  }
+  const int n = max(n_t[0], n_t[1]);
+  // keys of the last tile that lie behind the document's end (0: none): their V rows are cleared,
+  // since a probability of 0 times whatever stands there would still be NaN for an infinity
+  const int tail_rows = n == kv_tiles ? w.len - (kv_tiles - 1) * kTile : kTile;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&bars->q_full, 1);
+    mbar_init(&bars->tail_full, 1);
+    for (int s = 0; s < C::kSlots; ++s) {
+      mbar_init(&bars->kv_full[s], 1);
+      mbar_init(&bars->kv_empty[s], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&bars->s_full[t], 1);
+      for (int q = 0; q < 4; ++q) mbar_init(&bars->p_half[4 * t + q], 4);   // one arrival per softmax warp
+      mbar_init(&bars->o_done[t], 1);
+    }
+    fence_mbar_init();
+    prefetch_tmap(&tq);
+    prefetch_tmap(&tk);
+    prefetch_tmap(&tv);
+  }
+  if (warp == 1) tmem_alloc(&bars->tmem_base, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = bars->tmem_base;
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- producer
+    const bool cut = tail_rows < kTile;
+    if (elect_one()) {
+      mbar_expect_tx(&bars->q_full, C::kQBytes);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int h = 0; h < C::kHalves; ++h)
+          tma_load_3d(sQ + (t * C::kHalves + h) * 16384, &tq, &bars->q_full, h * 64, w.start + qt_t[t] * kTile,
+                      kPair ? head0 + t : head0);
+      int slot = 0;
+      uint32_t phase = 0;
+      for (int i = 0; i < 2 * n; ++i) {   // item 2j is K_j, item 2j + 1 is V_j
+        if (!mbar_wait(&bars->kv_empty[slot], phase ^ 1, p.status, kStatusTimeoutEmpty)) break;
+        uint8_t* dst = sKV + slot * C::kSlotBytes;
+        uint64_t* full = cut && i == 2 * n - 1 ? &bars->tail_full : &bars->kv_full[slot];
+        mbar_expect_tx(full, C::kSlotBytes);
+#pragma unroll
+        for (int h = 0; h < C::kHalves; ++h)
+          tma_load_3d(dst + h * 16384, (i & 1) ? &tv : &tk, full, h * 64, w.start + (i >> 1) * kTile, kv_head);
+        if (++slot == C::kSlots) { slot = 0; phase ^= 1; }
+      }
+    }
+    __syncwarp();
+    if (cut && warp_wait(&bars->tail_full, 0, p.status, kStatusTimeoutFull)) {
+      const int slot = (2 * n - 1) % C::kSlots;
+      clear_tail<C::kHalves>(sKV + slot * C::kSlotBytes, tail_rows, lane);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->kv_full[slot]);
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer
+    if (elect_one()) {
+      const int fmt = DT == kBF16 ? 1 : 0;
+      const uint32_t idesc_qk = make_idesc_f16(fmt, 0, 0, 128, 128);
+      const uint32_t idesc_pv = make_idesc_f16(fmt, 0, 1, 128, D);
+      bool ok = mbar_wait(&bars->q_full, 0, p.status, kStatusTimeoutFull);
+      // One thread issues every MMA, so the issue path is kept short: descriptors of the tile
+      // origins are built once, each MMA only adds a constant to them.
+      const uint64_t dq0 = make_smem_desc_sw128(smem_u32(sQ), 16, 1024);
+      const uint64_t dk0 = make_smem_desc_sw128(smem_u32(sKV), 16, 1024);
+      const uint64_t dv0 = make_smem_desc_sw128(smem_u32(sKV), 16384, 1024);
+      auto issue_qk = [&](int t, int slot) {
+        const uint64_t dq = desc_advance(dq0, t * C::kHalves * 16384);
+        const uint64_t dk = desc_advance(dk0, slot * C::kSlotBytes);
+#pragma unroll
+        for (int h = 0; h < C::kHalves; ++h)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tc_mma_f16(tmem_base + t * 128, desc_advance(dq, h * 16384 + k * 32),
+                       desc_advance(dk, h * 16384 + k * 32), idesc_qk, (h | k) != 0 ? 1u : 0u);
+        tc_commit(&bars->s_full[t]);
+      };
+      // O_t += P_t V_j in two halves of the key range: the first four MMAs start as soon as the
+      // softmax warps have written P columns 0-63, while they still compute columns 64-127.
+      auto issue_pv = [&](int t, int slot, int j) {
+        const uint64_t dv = desc_advance(dv0, slot * C::kSlotBytes);
+        bool got = true;
+#pragma unroll
+        for (int half = 0; half < 4 && got; ++half) {
+          got = mbar_wait(&bars->p_half[4 * t + half], j & 1, p.status, kStatusTimeoutTmemFull);
+          tc_fence_after();
+          if (!got) break;
+#pragma unroll
+          for (int k = half * 2; k < half * 2 + 2; ++k)
+            tc_mma_f16_ts(tmem_base + 256 + t * 128, tmem_base + t * 128 + k * 8,
+                          desc_advance(dv, k * 2048), idesc_pv, (j | k) != 0 ? 1u : 0u);
+        }
+        if (got) tc_commit(&bars->o_done[t]);
+        return got;
+      };
+      // ring position of item i (K_j is item 2j, V_j item 2j + 1)
+      auto wait_item = [&](int i) {
+        const bool got = mbar_wait(&bars->kv_full[i % C::kSlots], (i / C::kSlots) & 1, p.status, kStatusTimeoutFull);
+        tc_fence_after();
+        return got;
+      };
+      if (ok && n > 0) {
+        ok = wait_item(0);
+        if (ok) {
+          if (n_t[0] > 0) issue_qk(0, 0);
+          if (n_t[1] > 0) issue_qk(1, 0);
+          tc_commit(&bars->kv_empty[0]);
+        }
+      }
+      for (int j = 0; j < n && ok; ++j) {
+        const int vslot = (2 * j + 1) % C::kSlots, kslot = (2 * j + 2) % C::kSlots;
+        ok = wait_item(2 * j + 1);
+        if (!ok) break;
+        if (j < n_t[0]) {
+          ok = issue_pv(0, vslot, j);
+          if (!ok) break;
+        }
+        if (j + 1 < n) {
+          ok = wait_item(2 * j + 2);
+          if (!ok) break;
+        }
+        if (j + 1 < n_t[0]) issue_qk(0, kslot);
+        if (j < n_t[1]) {
+          ok = issue_pv(1, vslot, j);
+          if (!ok) break;
+        }
+        tc_commit(&bars->kv_empty[vslot]);
+        if (j + 1 < n_t[1]) issue_qk(1, kslot);
+        if (j + 1 < n) tc_commit(&bars->kv_empty[kslot]);
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax + epilogue
+    const int t = (warp - 2) >> 2;       // query tile of this warpgroup
+    const int quarter = warp & 3;        // TMEM lane quarter
+    const int r_local = quarter * 32 + lane;
+    const int qt = t == 0 ? qt_t[0] : qt_t[1];
+    const int q_local = qt * kTile + r_local;      // row inside the document
+    const int head = kPair ? head0 + t : head0;
+    const uint32_t lane_bits = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t s_addr = tmem_base + t * 128 + lane_bits;
+    const uint32_t o_addr = tmem_base + 256 + t * 128 + lane_bits;
+    const float sl2 = p.scale * kLog2e;
+    float m_run = -INFINITY, l_run = 0.f;
+    bool ok = true;
+    const int nt = t == 0 ? n_t[0] : n_t[1];
+    for (int j = 0; j < nt && ok; ++j) {
+      ok = warp_wait(&bars->s_full[t], j & 1, p.status, kStatusTimeoutTmemFull);
+      if (!ok) break;
+      tc_fence_after();
+      const bool diag = p.causal && (j == qt);
+      const bool tail = (j + 1) * kTile > w.len;
+      const int col_limit_tail = w.len - j * kTile;  // valid columns in a tail tile
+      // One TMEM read of the whole 128-column score row: the four loads are issued back to back
+      // and waited for once, so their latency overlaps.
+      uint32_t r[4][32];
+      __syncwarp();
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_addr + c * 32, r[c]);
+      tmem_ld_wait();
+      if (diag || tail) {   // rare: the diagonal tile of a causal row block, or a ragged last tile
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int col = c * 32 + i;
+            if ((diag && col > r_local) || (tail && col >= col_limit_tail)) r[c][i] = 0xff800000u;  // -inf
+          }
+      }
+      float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        mx0 = fmaxf(mx0, __uint_as_float(r[0][i]));
+        mx1 = fmaxf(mx1, __uint_as_float(r[1][i]));
+        mx2 = fmaxf(mx2, __uint_as_float(r[2][i]));
+        mx3 = fmaxf(mx3, __uint_as_float(r[3][i]));
+      }
+      const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
+      const float m_new = fmaxf(m_run, mx * sl2);
+      if (j == 0) {
+        m_run = m_new;
+      } else {
+        const bool need = m_new > m_run + kRescaleThreshold;
+        if (__any_sync(0xffffffffu, need)) {
+          const float m_upd = need ? m_new : m_run;
+          const float alpha = exp2f(m_run - m_upd);
+          l_run *= alpha;
+          m_run = m_upd;
+          // PV_{j-1} must have landed before O is touched
+          ok = warp_wait(&bars->o_done[t], (j - 1) & 1, p.status, kStatusTimeoutTmemFull);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o16[16];
+            tmem_ld_32x32b_x16(o_addr + c * 16, o16);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o16[i] = __float_as_uint(__uint_as_float(o16[i]) * alpha);
+            tmem_st_32x32b_x16(o_addr + c * 16, o16);
+          }
+          tmem_st_wait();
+        }
+      }
+      // P = exp2(s * scale_log2 - m), packed to 16 bit into the first 64 score columns
+      float ls0 = 0.f, ls1 = 0.f;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float p0 = exp2f(fmaf(__uint_as_float(r[c][2 * i]), sl2, -m_run));
+          const float p1 = exp2f(fmaf(__uint_as_float(r[c][2 * i + 1]), sl2, -m_run));
+          ls0 += p0;
+          ls1 += p1;
+          pk[i] = pack_pair(p0, p1, DT);
+        }
+        tmem_st_32x32b_x16(s_addr + c * 16, pk);
+        {   // a quarter of the key range is complete: hand it to the MMA warp
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->p_half[4 * t + c]);
+        }
+      }
+      const float lsum = ls0 + ls1;
+      l_run += lsum;
+    }
+    if (ok && nt > 0) {
+      ok = warp_wait(&bars->o_done[t], (nt - 1) & 1, p.status, kStatusTimeoutTmemFull);
+      tc_fence_after();
+    }
+    if (ok && nt > 0) {
+      const float inv_l = 1.0f / l_run;
+      const bool row_ok = q_local < w.len;
+      const int64_t q_row = static_cast<int64_t>(w.start) + q_local;
+      uint16_t* orow = reinterpret_cast<uint16_t*>(p.o) + q_row * p.o_strides[0] + head * p.o_strides[1];
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t r[32];
+        __syncwarp();
+        tmem_ld_32x32b_x32(o_addr + c * 32, r);
+        tmem_ld_wait();
+        if (row_ok) {
+          uint4* dst = reinterpret_cast<uint4*>(orow + c * 32);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint4 o;
+            o.x = pack_pair(__uint_as_float(r[q * 8 + 0]) * inv_l, __uint_as_float(r[q * 8 + 1]) * inv_l, DT);
+            o.y = pack_pair(__uint_as_float(r[q * 8 + 2]) * inv_l, __uint_as_float(r[q * 8 + 3]) * inv_l, DT);
+            o.z = pack_pair(__uint_as_float(r[q * 8 + 4]) * inv_l, __uint_as_float(r[q * 8 + 5]) * inv_l, DT);
+            o.w = pack_pair(__uint_as_float(r[q * 8 + 6]) * inv_l, __uint_as_float(r[q * 8 + 7]) * inv_l, DT);
+            dst[q] = o;
+          }
+        }
+      }
+      if (row_ok)
+        p.lse[static_cast<int64_t>(head) * p.rows + q_row] = (m_run + log2f(l_run)) * kLn2;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+template <int D, int DT, bool kPair>
+cudaError_t launch_fwd(const PackedAttnArgs& a, cudaStream_t st) {
+  using C = FwdCfg<D>;
+  CUtensorMap tq, tk, tv;
+  ETHB_TRY(make_tmap_rhd(&tq, a.q, a.dtype, D, a.rows, a.heads, a.q_strides), "packed forward: q");
+  ETHB_TRY(make_tmap_rhd(&tk, a.k, a.dtype, D, a.rows, a.kv_heads, a.k_strides), "packed forward: k");
+  ETHB_TRY(make_tmap_rhd(&tv, a.v, a.dtype, D, a.rows, a.kv_heads, a.v_strides), "packed forward: v");
+  static std::atomic<uint64_t> done{0};
+  ETHB_TRY(allow_smem(packed_fwd_kernel<D, DT, kPair>, C::kSmemBytes, done), "packed forward: shared memory");
+  const int units = kPair ? a.heads / 2 : a.heads;
+  // a few more CTAs clear the rows behind the last document
+  const int64_t spare = static_cast<int64_t>(a.rows - a.used) * a.heads * (D / 8);
+  const int clear = static_cast<int>(spare == 0 ? 0 : spare < 148 * 2560 ? (spare + 2559) / 2560 : 148);
+  const int64_t grid = static_cast<int64_t>(a.num_tiles) * units + clear;
+  ETHB_RETURN_IF(grid > 0x7fffffff, cudaErrorInvalidValue, "packed forward: too many tiles for one grid");
+  if (grid == 0) return cudaSuccess;
+  packed_fwd_kernel<D, DT, kPair><<<static_cast<unsigned>(grid), C::kThreads, C::kSmemBytes, st>>>(tq, tk, tv, a);
+  count_launch();
+  return cudaGetLastError();
+}
+
+// ==============================================================================================
+// backward
+// ==============================================================================================
+// dK / dV: one unit of work per (key tile, key/value head); it streams the query tiles that see the
+// tile, for every head of the group in turn, so the gradients of shared heads are summed in the
+// accumulators in a fixed order. dQ: one unit per (query tile, head). Both recompute the scores.
+//
+template <int D> struct BwdCfg {
+  static constexpr int kHalves = D / 64;
+  static constexpr int kTileBytes = kHalves * 16384;        // one 128-row tile
+  static constexpr int kResidentBytes = 2 * kTileBytes;
+  static constexpr int kStages = 2;
+  static constexpr int kStageBytes = 2 * kTileBytes;
+  static constexpr int kAuxBytes = 2 * 2 * 2 * 64 * 4;      // [wg][parity][lse|delta][64]
+  static constexpr int kSmemBytes = kResidentBytes + kStages * kStageBytes + kAuxBytes + 1024 + 256;
+  static constexpr int kThreads = 320;
+};
+
+struct BwdBarriers {
+  uint64_t res_full;
+  uint64_t tail_full;     // a streamed tile at a document's end has landed, rows behind the end not yet cleared
+  uint64_t st_full[2];
+  uint64_t st_empty[2];
+  uint64_t s_full[2];
+  uint64_t p_full[2];
+  uint64_t done;
+  uint64_t qdo_full;      // dQ kernel: the Q and dO rows of the tile sit in TMEM
+  uint64_t p_early[2];    // dQ kernel: the first 16 of each warpgroup's 32 dS columns are written
+  uint32_t tmem_base;
+  uint32_t pad;
+};
+
+// Barrier of a warpgroup that also tells all of it whether everybody is still `ok`.
+__device__ __forceinline__ bool wg_and(int wg, bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      "setp.ne.b32 p, %1, 0;\n"
+      "barrier.cta.red.and.pred q, %2, 128, p;\n"
+      "selp.u32 %0, 1, 0, q;\n"
+      "}\n"
+      : "=r"(all)
+      : "r"(static_cast<uint32_t>(ok)), "r"(wg + 1)
+      : "memory");
+  return all != 0;
+}
+
+// delta[h, row] = sum_d dO * O. A (row, head) vector of head_dim elements is covered by head_dim / 8
+// adjacent lanes with one 16-byte load each per tensor (head_dim is 64 or 128: 8 or 16 lanes); a
+// thread takes kDeltaRows of them, strided by the grid, and issues all their loads before any
+// arithmetic, so 2 * kDeltaRows requests are in flight per thread. The gradients of rows that belong
+// to no document are cleared here as well.
+constexpr int kDeltaRows = 4;
+template <int D>
+__global__ void __launch_bounds__(256) packed_delta_kernel(const PackedAttnArgs p) {
+  constexpr int lanes = D / 8;
+  constexpr int rows_per_block = 256 / lanes;
+  const int64_t total = static_cast<int64_t>(p.used) * p.heads;
+  const int sub = threadIdx.x / lanes, vec = threadIdx.x % lanes;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * rows_per_block;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * rows_per_block + sub;
+  uint4 ov[kDeltaRows], gv[kDeltaRows];
+#pragma unroll
+  for (int u = 0; u < kDeltaRows; ++u) {
+    const int64_t i = row0 + u * stride;
+    if (i < total) {
+      const int h = static_cast<int>(i % p.heads);
+      const int64_t s = i / p.heads;
+      ov[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.o) + s * p.o_strides[0] +
+                                              h * p.o_strides[1] + vec * 8);
+      gv[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.d_o) + s * p.do_strides[0] +
+                                              h * p.do_strides[1] + vec * 8);
+    } else {
+      ov[u] = make_uint4(0, 0, 0, 0);
+      gv[u] = make_uint4(0, 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kDeltaRows; ++u) {
+    const uint32_t ow[4] = {ov[u].x, ov[u].y, ov[u].z, ov[u].w}, gw[4] = {gv[u].x, gv[u].y, gv[u].z, gv[u].w};
+    float acc = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 a = unpack2(ow[e], p.dtype), d = unpack2(gw[e], p.dtype);
+      acc += a.x * d.x + a.y * d.y;
+    }
+#pragma unroll
+    for (int off = lanes >> 1; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
+    const int64_t i = row0 + u * stride;
+    if (vec == 0 && i < total) p.delta[(i % p.heads) * p.rows + i / p.heads] = acc;
+  }
+  if (p.used < p.rows) {
+    clear_rows<D>(p.dq, p.dq_strides[0], p.dq_strides[1], p.used, p.rows, p.heads, blockIdx.x, gridDim.x);
+    clear_rows<D>(p.dk, p.dk_strides[0], p.dk_strides[1], p.used, p.rows, p.kv_heads, blockIdx.x, gridDim.x);
+    clear_rows<D>(p.dv, p.dv_strides[0], p.dv_strides[1], p.used, p.rows, p.kv_heads, blockIdx.x, gridDim.x);
+  }
+}
+
+// ---- dK / dV: persistent CTAs over (key/value tile, key/value head) ------------------------------
+// One CTA per SM walks a static list of tiles, heaviest first (under the causal mask key tile j
+// meets q_tiles - j query tiles of each head), handed out round by round in alternating CTA order.
+// TMEM, the barriers and the tensor-map prefetch are set up once per CTA instead of once per tile;
+// barrier parities therefore run on counters that persist across tiles (`it`: tiles done by this
+// CTA, `sbase`: query tiles streamed so far). No CTA-wide barrier
+// separates the tiles: the loads and first score MMAs of the next tile overlap the accumulator stores
+// of the current one.
+template <int D, int DT>
+__global__ void __launch_bounds__(320, 1)
+packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                     const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tdo,
+                     const PackedAttnArgs p) {
+  using C = BwdCfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint8_t* sK = smem;
+  uint8_t* sV = smem + C::kTileBytes;
+  uint8_t* sStage = smem + C::kResidentBytes;  // stage: [Q tile | dO tile]
+  float* sAux = reinterpret_cast<float*>(sStage + C::kStages * C::kStageBytes);
+  BwdBarriers* bars = reinterpret_cast<BwdBarriers*>(reinterpret_cast<uint8_t*>(sAux) + C::kAuxBytes);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = p.heads / p.kv_heads;
+  const int total_tiles = p.num_k_tiles * p.kv_heads;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&bars->res_full, 1);
+    mbar_init(&bars->tail_full, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars->st_full[s], 1);
+      mbar_init(&bars->st_empty[s], 1);
+      mbar_init(&bars->s_full[s], 1);
+      mbar_init(&bars->p_full[s], 8);      // both softmax warpgroups work on every sub-tile, one arrival per warp
+    }
+    mbar_init(&bars->done, 1);
+    fence_mbar_init();
+    prefetch_tmap(&tq); prefetch_tmap(&tk); prefetch_tmap(&tv); prefetch_tmap(&tdo);
+  }
+  if (warp == 1) tmem_alloc(&bars->tmem_base, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = bars->tmem_base;
+  int p_stage = 0;           // producer: ring position of the next query-tile stage (persists across tiles)
+  uint32_t p_phase = 0;
+  int sbase = 0;             // query tiles streamed by this CTA before the current tile
+  uint32_t cuts = 0;         // producer: tiles at a document's end so far
+
+  // Round r hands out tiles [r * grid, (r + 1) * grid), heaviest first, in alternating direction
+  // (CTA 0 gets the heaviest tile of an even round and the lightest of an odd one), so the tile
+  // weights of a CTA add up to nearly the same total everywhere; `it` counts the tiles this CTA
+  // has processed (barrier parities run on it).
+  for (int round = 0, it = 0; round * static_cast<int>(gridDim.x) < total_tiles; ++round) {
+  const int tile = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+  if (tile >= total_tiles) continue;             // only in the last round
+  const PackedTile w = p.k_tiles[tile / p.kv_heads];
+  const int kv_head = tile % p.kv_heads;
+  const int j = w.tile;                          // key/value tile inside the document
+  const int q_tiles = (w.len + kTile - 1) / kTile;
+  const int i0 = p.causal ? j : 0;
+  const int nd = q_tiles - i0;                   // query tiles of the document that see these keys
+  const int nq = nd * group;                     // streamed: all of them for every head of the group
+  const int tail_rows = w.len - (q_tiles - 1) * kTile;   // rows of the document's last tile
+  const int U = 2 * nq;
+  if (warp == 0) {
+    // the resident K / V buffers are free once every MMA of the previous tile has completed; the
+    // loads of this tile then run while the other warps still store the previous accumulators
+    const bool free_kv = it == 0 || warp_wait(&bars->done, (it - 1) & 1, p.status, kStatusTimeoutTmemFull);
+    if (free_kv && elect_one()) {
+      mbar_expect_tx(&bars->res_full, C::kResidentBytes);
+#pragma unroll
+      for (int h = 0; h < C::kHalves; ++h) {
+        tma_load_3d(sK + h * 16384, &tk, &bars->res_full, h * 64, w.start + j * kTile, kv_head);
+        tma_load_3d(sV + h * 16384, &tv, &bars->res_full, h * 64, w.start + j * kTile, kv_head);
+      }
+    }
+    int stage = p_stage;
+    uint32_t phase = p_phase;
+    for (int t = 0, i = i0, head = kv_head * group; t < nq && free_kv; ++t) {
+      if (!warp_wait(&bars->st_empty[stage], phase ^ 1, p.status, kStatusTimeoutEmpty)) break;
+      uint8_t* sq = sStage + stage * C::kStageBytes;
+      uint8_t* sdo = sq + C::kTileBytes;
+      const bool cut = i == q_tiles - 1 && tail_rows < kTile;
+      __syncwarp();
+      if (elect_one()) {
+        uint64_t* full = cut ? &bars->tail_full : &bars->st_full[stage];
+        mbar_expect_tx(full, C::kStageBytes);
+#pragma unroll
+        for (int h = 0; h < C::kHalves; ++h) {
+          tma_load_3d(sq + h * 16384, &tq, full, h * 64, w.start + i * kTile, head);
+          tma_load_3d(sdo + h * 16384, &tdo, full, h * 64, w.start + i * kTile, head);
+        }
+      }
+      __syncwarp();
+      if (cut) {   // rows behind the document's end are summands of dK and dV: 0 times them must be 0
+        if (!warp_wait(&bars->tail_full, cuts & 1, p.status, kStatusTimeoutFull)) break;
+        ++cuts;
+        clear_tail<C::kHalves>(sq, tail_rows, lane);
+        clear_tail<C::kHalves>(sdo, tail_rows, lane);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->st_full[stage]);
+      }
+      if (++stage == 2) { stage = 0; phase ^= 1; }
+      if (++i == q_tiles) { i = i0; ++head; }
+    }
+    // every lane tracks the ring position, whichever lane is elected next time
+    p_phase ^= static_cast<uint32_t>(((p_stage + nq) >> 1) & 1);
+    p_stage = (p_stage + nq) & 1;
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const int fmt = DT == kBF16 ? 1 : 0;
+      const uint32_t idesc_s = make_idesc_f16(fmt, 0, 0, 128, 64);
+      const uint32_t idesc_acc = make_idesc_f16(fmt, 0, 1, 128, D);
+      // One thread issues every MMA and the score MMAs are short (N = 64), so the issue path must
+      // stay short too: tile-origin descriptors are built once, each MMA adds a constant.
+      const uint64_t dK0 = make_smem_desc_sw128(smem_u32(sK), 16, 1024);
+      const uint64_t dV0 = make_smem_desc_sw128(smem_u32(sV), 16, 1024);
+      const uint64_t dQk0 = make_smem_desc_sw128(smem_u32(sStage), 16, 1024);          // K-major view
+      const uint64_t dQm0 = make_smem_desc_sw128(smem_u32(sStage), 16384, 1024);       // MN-major view
+      auto issue_sdp = [&](int u) {
+        const int stage = (sbase + (u >> 1)) & 1, sub = u & 1, b = u & 1;
+        const uint64_t dQ = desc_advance(dQk0, stage * C::kStageBytes + sub * 8192);
+        const uint64_t dDO = desc_advance(dQ, C::kTileBytes);
+#pragma unroll
+        for (int h = 0; h < C::kHalves; ++h)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tc_mma_f16(tmem_base + b * 128, desc_advance(dK0, h * 16384 + k * 32),
+                       desc_advance(dQ, h * 16384 + k * 32), idesc_s, (h | k) != 0 ? 1u : 0u);
+#pragma unroll
+        for (int h = 0; h < C::kHalves; ++h)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tc_mma_f16(tmem_base + b * 128 + 64, desc_advance(dV0, h * 16384 + k * 32),
+                       desc_advance(dDO, h * 16384 + k * 32), idesc_s, (h | k) != 0 ? 1u : 0u);
+        tc_commit(&bars->s_full[b]);
+      };
+      bool ok = mbar_wait(&bars->res_full, it & 1, p.status, kStatusTimeoutFull);
+      if (ok && U > 0) {
+        ok = mbar_wait(&bars->st_full[sbase & 1], (sbase >> 1) & 1, p.status, kStatusTimeoutFull);
+        tc_fence_after();
+        if (ok) { issue_sdp(0); issue_sdp(1); }
+      }
+      for (int u = 0; u < U && ok; ++u) {
+        const int b = u & 1, stage = (sbase + (u >> 1)) & 1, sub = u & 1;
+        ok = mbar_wait(&bars->p_full[b], (sbase + (u >> 1)) & 1, p.status, kStatusTimeoutTmemFull);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t dQ = desc_advance(dQm0, stage * C::kStageBytes + sub * 8192);
+        const uint64_t dDO = desc_advance(dQ, C::kTileBytes);
+        // queries 0-31 of P / dS sit at columns [0, 16) of their buffer, queries 32-63 at [32, 48)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)   // dV += P^T dO
+          tc_mma_f16_ts(tmem_base + 256, tmem_base + b * 128 + (k >> 1) * 32 + (k & 1) * 8,
+                        desc_advance(dDO, k * 2048), idesc_acc, (u | k) != 0 ? 1u : 0u);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)   // dK += dS^T Q
+          tc_mma_f16_ts(tmem_base + 384, tmem_base + b * 128 + 64 + (k >> 1) * 32 + (k & 1) * 8,
+                        desc_advance(dQ, k * 2048), idesc_acc, (u | k) != 0 ? 1u : 0u);
+        if (sub == 1) tc_commit(&bars->st_empty[stage]);
+        if (u + 2 < U) {
+          const int u2 = u + 2;
+          if ((u2 & 1) == 0) {
+            const int sq = sbase + (u2 >> 1);
+            ok = mbar_wait(&bars->st_full[sq & 1], (sq >> 1) & 1, p.status, kStatusTimeoutFull);
+            if (!ok) break;
+            tc_fence_after();
+          }
+          issue_sdp(u2);
+        }
+      }
+      tc_commit(&bars->done);
+    }
+  } else {
+    const int wg = (warp - 2) >> 2;      // sub-tile parity handled by this warpgroup
+    const int quarter = warp & 3;
+    const int r_local = quarter * 32 + lane;     // key/value row inside the tile
+    const int wg_tid = threadIdx.x - 64 - wg * 128;
+    const uint32_t lane_bits = static_cast<uint32_t>(quarter * 32) << 16;
+    const float sl2 = p.scale * kLog2e;
+    bool ok = true;
+    // Both warpgroups work on every 64-query sub-tile, each on 32 of its columns (see the dQ kernel),
+    // so the softmax of a sub-tile takes half as long and hides under the score MMAs of the other
+    // buffer; each warpgroup overwrites only columns it has read itself. The lse / delta values of a
+    // query tile are staged once per tile and warpgroup (its 2 x 32 columns), one tile ahead: the
+    // global loads for tile t + 1 are issued before tile t is processed and parked in shared memory
+    // after it, so their latency is never waited for.
+    const int a_sub = (wg_tid >> 5) & 1, a_col = wg_tid & 31;
+    // streamed tile t is query tile i0 + t % nd of head kv_head * group + t / nd
+    auto aux_load = [&](int i, int head, float& lse, float& delta) {
+      const int qi = i * kTile + a_sub * 64 + wg * 32 + a_col;
+      const bool in = qi < w.len;
+      const int64_t at = static_cast<int64_t>(head) * p.rows + w.start + qi;
+      lse = in ? p.lse[at] * kLog2e : INFINITY;
+      delta = in ? p.delta[at] : 0.f;
+    };
+    auto aux_slot = [&](int t) { return sAux + ((wg * 2 + (t & 1)) * 2) * 64; };   // [lse 2 x 32 | delta 2 x 32]
+    if (wg_tid < 64 && nq > 0) {
+      float lse, delta;
+      aux_load(i0, kv_head * group, lse, delta);
+      aux_slot(0)[wg_tid] = lse;
+      aux_slot(0)[64 + wg_tid] = delta;
+    }
+    int i = i0, head = kv_head * group;
+    for (int t = 0; t < nq; ++t) {
+      const int i_next = i + 1 == q_tiles ? i0 : i + 1, head_next = i + 1 == q_tiles ? head + 1 : head;
+      ok = wg_and(wg, ok);             // tile t's values are staged; everyone has left tile t - 1
+      if (!ok) break;
+      float next_lse = INFINITY, next_delta = 0.f;
+      if (wg_tid < 64 && t + 1 < nq) {
+        aux_load(i_next, head_next, next_lse, next_delta);
+      }
+      const bool diag = p.causal && (i == j);
+#pragma unroll 1
+      for (int sub = 0; sub < 2 && ok; ++sub) {
+        const float* a_lse = aux_slot(t) + sub * 32;
+        const float* a_del = a_lse + 64;
+        const uint32_t s_addr = tmem_base + sub * 128 + wg * 32 + lane_bits;
+        const uint32_t dp_addr = s_addr + 64;
+        ok = warp_wait(&bars->s_full[sub], (sbase + t) & 1, p.status, kStatusTimeoutTmemFull);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t rs[32], rd[32];
+        __syncwarp();
+        tmem_ld_32x32b_x32(s_addr, rs);
+        tmem_ld_32x32b_x32(dp_addr, rd);
+        tmem_ld_wait();
+        uint32_t pk[16], dk[16];
+        // lse / delta come as 16-byte broadcast loads (four query columns each); only the tile on
+        // the diagonal pays for the causal mask
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+          const float4 l4 = *reinterpret_cast<const float4*>(a_lse + 4 * y);
+          const float4 e4 = *reinterpret_cast<const float4*>(a_del + 4 * y);
+          const float lv[4] = {l4.x, l4.y, l4.z, l4.w}, ev[4] = {e4.x, e4.y, e4.z, e4.w};
+          float pv[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) pv[c] = exp2f(fmaf(__uint_as_float(rs[4 * y + c]), sl2, -lv[c]));
+          if (diag) {
+            const int ql = sub * 64 + wg * 32 + 4 * y;     // query row inside the 128-row tile
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              if (r_local > ql + c) pv[c] = 0.f;
+          }
+          float dv[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) dv[c] = pv[c] * (__uint_as_float(rd[4 * y + c]) - ev[c]);
+          pk[2 * y] = pack_pair(pv[0], pv[1], DT);
+          pk[2 * y + 1] = pack_pair(pv[2], pv[3], DT);
+          dk[2 * y] = pack_pair(dv[0], dv[1], DT);
+          dk[2 * y + 1] = pack_pair(dv[2], dv[3], DT);
+        }
+        tmem_st_32x32b_x16(s_addr, pk);
+        tmem_st_32x32b_x16(dp_addr, dk);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->p_full[sub]);   // one arrival per warp
+      }
+      if (wg_tid < 64 && t + 1 < nq) {
+        aux_slot(t + 1)[wg_tid] = next_lse;
+        aux_slot(t + 1)[64 + wg_tid] = next_delta;
+      }
+      i = i_next;
+      head = head_next;
+    }
+    // epilogue: warpgroup 0 stores dV, warpgroup 1 stores dK * scale
+    if (ok) ok = warp_wait(&bars->done, it & 1, p.status, kStatusTimeoutTmemFull);
+    if (ok && U > 0) {
+      tc_fence_after();
+      const int kv_row = j * kTile + r_local;
+      const bool row_ok = kv_row < w.len;
+      const int64_t* st = wg == 0 ? p.dv_strides : p.dk_strides;
+      uint16_t* orow = reinterpret_cast<uint16_t*>(wg == 0 ? p.dv : p.dk) +
+                       (static_cast<int64_t>(w.start) + kv_row) * st[0] + kv_head * st[1];
+      const float mul = wg == 0 ? 1.0f : p.scale;
+      const uint32_t acc_addr = tmem_base + 256 + wg * 128 + lane_bits;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t r[32];
+        __syncwarp();
+        tmem_ld_32x32b_x32(acc_addr + c * 32, r);
+        tmem_ld_wait();
+        if (row_ok) {
+          uint4* dst = reinterpret_cast<uint4*>(orow + c * 32);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint4 o;
+            o.x = pack_pair(__uint_as_float(r[q * 8 + 0]) * mul, __uint_as_float(r[q * 8 + 1]) * mul, DT);
+            o.y = pack_pair(__uint_as_float(r[q * 8 + 2]) * mul, __uint_as_float(r[q * 8 + 3]) * mul, DT);
+            o.z = pack_pair(__uint_as_float(r[q * 8 + 4]) * mul, __uint_as_float(r[q * 8 + 5]) * mul, DT);
+            o.w = pack_pair(__uint_as_float(r[q * 8 + 6]) * mul, __uint_as_float(r[q * 8 + 7]) * mul, DT);
+            dst[q] = o;
+          }
+        }
+      }
+    }
+  }
+  // End of tile, without a CTA-wide barrier: the roles meet again only through the mbarriers. The
+  // producer waits for `done` before it refills K / V; the first dV / dK MMAs of the next tile
+  // (which overwrite the accumulators) wait for that tile's first P, and a softmax warp writes that
+  // only after it has stored its part of these accumulators.
+  sbase += nq;
+  ++it;
+  // a wait gave up: stop. A warpgroup decides together, its barrier needs all of it.
+  const bool go = p.status == nullptr || *reinterpret_cast<volatile int*>(p.status) == 0;
+  if (!(warp < 2 ? __all_sync(0xffffffffu, go) : wg_and((warp - 2) >> 2, go))) break;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// ---- dQ: persistent CTAs over (query tile, head) -------------------------------------------------
+// Like the dK / dV kernel: one CTA per SM, tiles heaviest first (query tile i meets i + 1 key tiles
+// under the causal mask) handed out round by round in alternating CTA order, TMEM and barriers set
+// up once, parities on counters that persist across tiles (`it`, `sbase`), and no CTA-wide barrier
+// between tiles: the Q / dO loads and first score MMAs of the next tile overlap the dQ store.
+template <int D, int DT>
+__global__ void __launch_bounds__(320, 1)
+packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                   const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tdo,
+                   const PackedAttnArgs p) {
+  using C = BwdCfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sDO = smem + C::kTileBytes;
+  uint8_t* sStage = smem + C::kResidentBytes;  // stage: [K tile | V tile]
+  BwdBarriers* bars = reinterpret_cast<BwdBarriers*>(sStage + C::kStages * C::kStageBytes + C::kAuxBytes);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = p.heads / p.kv_heads;
+  const int total_tiles = p.num_q_tiles * p.heads;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&bars->res_full, 1);
+    mbar_init(&bars->tail_full, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars->st_full[s], 1);
+      mbar_init(&bars->st_empty[s], 1);
+      mbar_init(&bars->s_full[s], 1);
+      mbar_init(&bars->p_full[s], 8);      // both softmax warpgroups work on every sub-tile, one arrival per warp
+      mbar_init(&bars->p_early[s], 8);
+    }
+    mbar_init(&bars->done, 1);
+    mbar_init(&bars->qdo_full, 8);         // one arrival per softmax warp
+    fence_mbar_init();
+    prefetch_tmap(&tq); prefetch_tmap(&tk); prefetch_tmap(&tv); prefetch_tmap(&tdo);
+  }
+  if (warp == 1) tmem_alloc(&bars->tmem_base, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = bars->tmem_base;
+  int p_stage = 0;           // producer: ring position of the next key/value stage (persists across tiles)
+  uint32_t p_phase = 0;
+  int sbase = 0;             // key/value tiles streamed by this CTA before the current tile
+  uint32_t cuts = 0;         // producer: tiles at a document's end so far
+
+  for (int round = 0, it = 0; round * static_cast<int>(gridDim.x) < total_tiles; ++round) {
+  const int tile = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+  if (tile >= total_tiles) continue;             // only in the last round
+  const PackedTile w = p.q_tiles[tile / p.heads];
+  const int head = tile % p.heads, kv_head = head / group;
+  const int i = w.tile;                          // query tile inside the document
+  const int kv_tiles = (w.len + kTile - 1) / kTile;
+  const int nkv = p.causal ? i + 1 : kv_tiles;
+  const int tail_rows = w.len - (kv_tiles - 1) * kTile;   // rows of the document's last tile
+  const int U = 2 * nkv;
+  if (warp == 0) {
+    // Q / dO are free once every MMA of the previous tile has completed
+    const bool free_q = it == 0 || warp_wait(&bars->done, (it - 1) & 1, p.status, kStatusTimeoutTmemFull);
+    if (free_q && elect_one()) {
+      mbar_expect_tx(&bars->res_full, C::kResidentBytes);
+#pragma unroll
+      for (int h = 0; h < C::kHalves; ++h) {
+        tma_load_3d(sQ + h * 16384, &tq, &bars->res_full, h * 64, w.start + i * kTile, head);
+        tma_load_3d(sDO + h * 16384, &tdo, &bars->res_full, h * 64, w.start + i * kTile, head);
+      }
+    }
+    int stage = p_stage;
+    uint32_t phase = p_phase;
+    for (int t = 0; t < nkv && free_q; ++t) {
+      if (!warp_wait(&bars->st_empty[stage], phase ^ 1, p.status, kStatusTimeoutEmpty)) break;
+      uint8_t* sk = sStage + stage * C::kStageBytes;
+      uint8_t* sv = sk + C::kTileBytes;
+      const bool cut = t == kv_tiles - 1 && tail_rows < kTile;
+      __syncwarp();
+      if (elect_one()) {
+        uint64_t* full = cut ? &bars->tail_full : &bars->st_full[stage];
+        mbar_expect_tx(full, C::kStageBytes);
+#pragma unroll
+        for (int h = 0; h < C::kHalves; ++h) {
+          tma_load_3d(sk + h * 16384, &tk, full, h * 64, w.start + t * kTile, kv_head);
+          tma_load_3d(sv + h * 16384, &tv, full, h * 64, w.start + t * kTile, kv_head);
+        }
+      }
+      __syncwarp();
+      if (cut) {   // keys behind the document's end are summands of dQ: 0 times them must be 0
+        if (!warp_wait(&bars->tail_full, cuts & 1, p.status, kStatusTimeoutFull)) break;
+        ++cuts;
+        clear_tail<C::kHalves>(sk, tail_rows, lane);
+        clear_tail<C::kHalves>(sv, tail_rows, lane);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->st_full[stage]);
+      }
+      if (++stage == 2) { stage = 0; phase ^= 1; }
+    }
+    // every lane tracks the ring position, whichever lane is elected next time
+    p_phase ^= static_cast<uint32_t>(((p_stage + nkv) >> 1) & 1);
+    p_stage = (p_stage + nkv) & 1;
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const int fmt = DT == kBF16 ? 1 : 0;
+      const uint32_t idesc_s = make_idesc_f16(fmt, 0, 0, 128, 64);
+      const uint32_t idesc_acc = make_idesc_f16(fmt, 0, 1, 128, D);
+      // short issue path: tile-origin descriptors once, constants added per MMA
+      const uint64_t dKk0 = make_smem_desc_sw128(smem_u32(sStage), 16, 1024);          // K-major view
+      const uint64_t dKm0 = make_smem_desc_sw128(smem_u32(sStage), 16384, 1024);       // MN-major view
+      // Q and dO are A operands read from TMEM (columns [384, 448) and [448, 512), staged there by
+      // the softmax warps): a score MMA then reads only its 2 KB B operand from shared memory, where
+      // with both operands in shared memory the N = 64 MMAs ran into the 128 B/clk of the SM.
+      auto issue_sdp = [&](int u) {
+        const int stage = (sbase + (u >> 1)) & 1, sub = u & 1, b = u & 1;
+        const uint64_t dK = desc_advance(dKk0, stage * C::kStageBytes + sub * 8192);
+        const uint64_t dV = desc_advance(dK, C::kTileBytes);
+#pragma unroll
+        for (int h = 0; h < C::kHalves; ++h)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tc_mma_f16_ts(tmem_base + b * 128, tmem_base + 384 + (h * 4 + k) * 8,
+                          desc_advance(dK, h * 16384 + k * 32), idesc_s, (h | k) != 0 ? 1u : 0u);
+#pragma unroll
+        for (int h = 0; h < C::kHalves; ++h)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tc_mma_f16_ts(tmem_base + b * 128 + 64, tmem_base + 448 + (h * 4 + k) * 8,
+                          desc_advance(dV, h * 16384 + k * 32), idesc_s, (h | k) != 0 ? 1u : 0u);
+        tc_commit(&bars->s_full[b]);
+      };
+      bool ok = mbar_wait(&bars->qdo_full, it & 1, p.status, kStatusTimeoutFull);
+      if (ok && U > 0) {
+        ok = mbar_wait(&bars->st_full[sbase & 1], (sbase >> 1) & 1, p.status, kStatusTimeoutFull);
+        tc_fence_after();
+        if (ok) { issue_sdp(0); issue_sdp(1); }
+      }
+      for (int u = 0; u < U && ok; ++u) {
+        const int b = u & 1, stage = (sbase + (u >> 1)) & 1, sub = u & 1;
+        // dQ += dS K; keys 0-31 of dS sit at columns [0, 16), keys 32-63 at [32, 48). The first 16
+        // keys of each warpgroup (k-steps 0 and 2) are handed over before the other 16 (1 and 3).
+        const uint64_t dK = desc_advance(dKm0, stage * C::kStageBytes + sub * 8192);
+        ok = mbar_wait(&bars->p_early[b], (sbase + (u >> 1)) & 1, p.status, kStatusTimeoutTmemFull);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < 4; k += 2)
+          tc_mma_f16_ts(tmem_base + 256, tmem_base + b * 128 + 64 + (k >> 1) * 32 + (k & 1) * 8,
+                        desc_advance(dK, k * 2048), idesc_acc, (u | k) != 0 ? 1u : 0u);
+        ok = mbar_wait(&bars->p_full[b], (sbase + (u >> 1)) & 1, p.status, kStatusTimeoutTmemFull);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int k = 1; k < 4; k += 2)
+          tc_mma_f16_ts(tmem_base + 256, tmem_base + b * 128 + 64 + (k >> 1) * 32 + (k & 1) * 8,
+                        desc_advance(dK, k * 2048), idesc_acc, 1u);
+        if (sub == 1) tc_commit(&bars->st_empty[stage]);
+        if (u + 2 < U) {
+          const int u2 = u + 2;
+          if ((u2 & 1) == 0) {
+            const int sq = sbase + (u2 >> 1);
+            ok = mbar_wait(&bars->st_full[sq & 1], (sq >> 1) & 1, p.status, kStatusTimeoutFull);
+            if (!ok) break;
+            tc_fence_after();
+          }
+          issue_sdp(u2);
+        }
+      }
+      tc_commit(&bars->done);
+    }
+  } else {
+    const int wg = (warp - 2) >> 2;
+    const int quarter = warp & 3;
+    const int r_local = quarter * 32 + lane;     // query row inside the tile
+    const int q_local = i * kTile + r_local;     // row inside the document
+    const bool row_ok = q_local < w.len;
+    const int64_t q_row = static_cast<int64_t>(w.start) + q_local;
+    const uint32_t lane_bits = static_cast<uint32_t>(quarter * 32) << 16;
+    const float sl2 = p.scale * kLog2e;
+    const int64_t at = static_cast<int64_t>(head) * p.rows + q_row;
+    const float lse2 = row_ok ? p.lse[at] * kLog2e : INFINITY;
+    const float delta = row_ok ? p.delta[at] : 0.f;
+    bool ok = true;
+    // Stage the tile's rows as TMEM operands: warpgroup 0 copies the Q rows, warpgroup 1 the dO rows,
+    // one thread per row, out of the 128-byte-swizzled tiles the TMA wrote (16-byte chunk c of row r
+    // sits at chunk c ^ (r & 7)); element d of a row lands in TMEM column d / 2 of the operand.
+    ok = warp_wait(&bars->res_full, it & 1, p.status, kStatusTimeoutFull);
+    if (ok) {
+      const uint8_t* src = (wg == 0 ? sQ : sDO) + r_local * 128;
+      const uint32_t dst = tmem_base + 384 + wg * 64 + lane_bits;
+      __syncwarp();
+#pragma unroll
+      for (int h = 0; h < C::kHalves; ++h)
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          uint32_t v[16];
+#pragma unroll
+          for (int c4 = 0; c4 < 4; ++c4) {
+            const int c = g * 4 + c4;
+            const uint4 x = *reinterpret_cast<const uint4*>(src + h * 16384 + ((c ^ (r_local & 7)) << 4));
+            v[c4 * 4 + 0] = x.x; v[c4 * 4 + 1] = x.y; v[c4 * 4 + 2] = x.z; v[c4 * 4 + 3] = x.w;
+          }
+          tmem_st_32x32b_x16(dst + h * 32 + g * 16, v);
+        }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->qdo_full);
+    }
+    // Both warpgroups work on every 64-key sub-tile, each on 32 of its columns: the time from
+    // "scores ready" to "dS ready" halves, so it fits under the score MMAs of the other buffer and
+    // the tensor core seldom waits for it. A warpgroup writes its 16-bit dS over the first half of
+    // the dP columns it has just read (its own input), never over the other warpgroup's.
+    for (int u = 0; u < U && ok; ++u) {
+      const int t = u >> 1, sub = u & 1;
+      const uint32_t s_addr = tmem_base + sub * 128 + wg * 32 + lane_bits;
+      const uint32_t dp_addr = s_addr + 64;
+      ok = warp_wait(&bars->s_full[sub], (sbase + t) & 1, p.status, kStatusTimeoutTmemFull);
+      if (!ok) break;
+      tc_fence_after();
+      const bool diag = p.causal && (t == i);
+      const int kv0 = t * kTile + sub * 64 + wg * 32;   // first key index of this warpgroup's columns
+      const bool ragged = kv0 + 32 > w.len;
+      uint32_t rs[32], rd[32];
+      __syncwarp();
+      tmem_ld_32x32b_x32(s_addr, rs);
+      tmem_ld_32x32b_x32(dp_addr, rd);
+      tmem_ld_wait();
+      uint32_t dk[16];
+      const float neg_lse = -lse2;
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {   // 16 keys at a time, handed over as soon as they are written
+        if (!(diag || ragged)) {   // the common case carries no mask
+#pragma unroll
+          for (int x = part * 8; x < part * 8 + 8; ++x) {
+            const float p0 = exp2f(fmaf(__uint_as_float(rs[2 * x]), sl2, neg_lse));
+            const float p1 = exp2f(fmaf(__uint_as_float(rs[2 * x + 1]), sl2, neg_lse));
+            dk[x] = pack_pair(p0 * (__uint_as_float(rd[2 * x]) - delta), p1 * (__uint_as_float(rd[2 * x + 1]) - delta),
+                              DT);
+          }
+        } else {
+#pragma unroll
+          for (int x = part * 8; x < part * 8 + 8; ++x) {
+            const int col = 2 * x;
+            const int kl = sub * 64 + wg * 32 + col;      // key row inside the 128-row tile
+            float p0 = exp2f(fmaf(__uint_as_float(rs[2 * x]), sl2, neg_lse));
+            float p1 = exp2f(fmaf(__uint_as_float(rs[2 * x + 1]), sl2, neg_lse));
+            if ((diag && kl > r_local) || (ragged && kv0 + col >= w.len)) p0 = 0.f;
+            if ((diag && kl + 1 > r_local) || (ragged && kv0 + col + 1 >= w.len)) p1 = 0.f;
+            dk[x] = pack_pair(p0 * (__uint_as_float(rd[2 * x]) - delta), p1 * (__uint_as_float(rd[2 * x + 1]) - delta),
+                              DT);
+          }
+        }
+        if (part == 0) {
+          tmem_st_32x32b_x8(dp_addr, dk);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->p_early[sub]);
+        }
+      }
+      tmem_st_32x32b_x8(dp_addr + 8, dk + 8);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->p_full[sub]);   // one arrival per warp
+    }
+    if (ok) ok = warp_wait(&bars->done, it & 1, p.status, kStatusTimeoutTmemFull);
+    if (ok && U > 0) {
+      tc_fence_after();
+      // each warpgroup stores half of the head dimension
+      uint16_t* orow = reinterpret_cast<uint16_t*>(p.dq) + q_row * p.dq_strides[0] + head * p.dq_strides[1];
+      const uint32_t acc_addr = tmem_base + 256 + lane_bits;
+#pragma unroll 1
+      for (int c = wg * (D / 64); c < (wg + 1) * (D / 64); ++c) {
+        uint32_t r[32];
+        __syncwarp();
+        tmem_ld_32x32b_x32(acc_addr + c * 32, r);
+        tmem_ld_wait();
+        if (row_ok) {
+          uint4* dst = reinterpret_cast<uint4*>(orow + c * 32);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint4 o;
+            o.x = pack_pair(__uint_as_float(r[q * 8 + 0]) * p.scale, __uint_as_float(r[q * 8 + 1]) * p.scale, DT);
+            o.y = pack_pair(__uint_as_float(r[q * 8 + 2]) * p.scale, __uint_as_float(r[q * 8 + 3]) * p.scale, DT);
+            o.z = pack_pair(__uint_as_float(r[q * 8 + 4]) * p.scale, __uint_as_float(r[q * 8 + 5]) * p.scale, DT);
+            o.w = pack_pair(__uint_as_float(r[q * 8 + 6]) * p.scale, __uint_as_float(r[q * 8 + 7]) * p.scale, DT);
+            dst[q] = o;
+          }
+        }
+      }
+    }
+  }
+  // End of tile, without a CTA-wide barrier: the producer waits for `done` before it reloads Q / dO;
+  // the first dQ MMAs of the next tile (which overwrite the accumulator) wait for that tile's first
+  // dS, and a softmax warp writes that only after it has stored its part of this accumulator.
+  sbase += nkv;
+  ++it;
+  if (!__all_sync(0xffffffffu, p.status == nullptr || *reinterpret_cast<volatile int*>(p.status) == 0)) break;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+template <int D, int DT>
+cudaError_t launch_bwd(const PackedAttnArgs& a, cudaStream_t st) {
+  using C = BwdCfg<D>;
+  CUtensorMap tq, tk, tv, tdo;
+  ETHB_TRY(make_tmap_rhd(&tq, a.q, a.dtype, D, a.rows, a.heads, a.q_strides), "packed backward: q");
+  ETHB_TRY(make_tmap_rhd(&tk, a.k, a.dtype, D, a.rows, a.kv_heads, a.k_strides), "packed backward: k");
+  ETHB_TRY(make_tmap_rhd(&tv, a.v, a.dtype, D, a.rows, a.kv_heads, a.v_strides), "packed backward: v");
+  ETHB_TRY(make_tmap_rhd(&tdo, a.d_o, a.dtype, D, a.rows, a.heads, a.do_strides), "packed backward: dO");
+  static std::atomic<uint64_t> done_kv{0}, done_q{0};
+  ETHB_TRY(allow_smem(packed_bwd_dkdv_kernel<D, DT>, C::kSmemBytes, done_kv), "packed backward: shared memory");
+  ETHB_TRY(allow_smem(packed_bwd_dq_kernel<D, DT>, C::kSmemBytes, done_q), "packed backward: shared memory");
+  const int64_t k_work = static_cast<int64_t>(a.num_k_tiles) * a.kv_heads;
+  const int64_t q_work = static_cast<int64_t>(a.num_q_tiles) * a.heads;
+  ETHB_RETURN_IF(k_work > 0x3fffffff || q_work > 0x3fffffff, cudaErrorInvalidValue, "packed backward: too many tiles");
+  const int sms = sm_count();
+  const int64_t vectors = static_cast<int64_t>(a.rows) * a.heads;
+  constexpr int per_block = 256 / (D / 8) * kDeltaRows;
+  packed_delta_kernel<D><<<static_cast<unsigned>((vectors + per_block - 1) / per_block), 256, 0, st>>>(a);
+  count_launch();
+  if (a.used > 0) {
+    packed_bwd_dkdv_kernel<D, DT><<<static_cast<unsigned>(k_work < sms ? k_work : sms), C::kThreads, C::kSmemBytes,
+                                    st>>>(tq, tk, tv, tdo, a);
+    packed_bwd_dq_kernel<D, DT><<<static_cast<unsigned>(q_work < sms ? q_work : sms), C::kThreads, C::kSmemBytes,
+                                  st>>>(tq, tk, tv, tdo, a);
+    count_launch(2);
+  }
+  return cudaGetLastError();
+}
+
+cudaError_t check_common(const PackedAttnArgs& a) {
+  ETHB_RETURN_IF(a.dtype != kF16 && a.dtype != kBF16, cudaErrorInvalidValue, "packed attention: fp16 or bf16 only");
+  ETHB_RETURN_IF(a.head_dim != 64 && a.head_dim != 128, cudaErrorInvalidValue, "packed attention: head_dim 64 or 128");
+  ETHB_RETURN_IF(a.heads < 1 || a.kv_heads < 1 || a.heads % a.kv_heads != 0, cudaErrorInvalidValue,
+                 "packed attention: heads must be a multiple of kv_heads");
+  ETHB_RETURN_IF(a.used < 0 || a.used > a.rows || a.rows > 0x7fffff00, cudaErrorInvalidValue, "packed attention: rows");
+  return cudaSuccess;
+}
+cudaError_t check_out(const void* base, const int64_t strides[2]) {
+  ETHB_RETURN_IF((reinterpret_cast<uintptr_t>(base) & 15) != 0 || strides[0] % 8 != 0 || strides[1] % 8 != 0,
+                 cudaErrorMisalignedAddress, "packed attention: outputs must be 16-byte aligned");
+  return cudaSuccess;
+}
+
+template <int D, int DT>
+cudaError_t launch_fwd_for(const PackedAttnArgs& a, cudaStream_t st) {
+  return attention_packed_pairs_heads(a.heads, a.kv_heads) ? launch_fwd<D, DT, true>(a, st)
+                                                           : launch_fwd<D, DT, false>(a, st);
+}
+
+}  // namespace
+
+bool attention_packed_pairs_heads(int heads, int kv_heads) { return (heads / kv_heads) % 2 == 0; }
+
+cudaError_t attention_packed_fwd(const PackedAttnArgs& a, cudaStream_t st) {
+  ETHB_TRY(check_common(a), "packed forward");
+  ETHB_TRY(check_out(a.o, a.o_strides), "packed forward: out");
+  if (a.rows == 0) return cudaSuccess;
+  const bool bf = a.dtype == kBF16;
+  if (a.head_dim == 128) return bf ? launch_fwd_for<128, kBF16>(a, st) : launch_fwd_for<128, kF16>(a, st);
+  return bf ? launch_fwd_for<64, kBF16>(a, st) : launch_fwd_for<64, kF16>(a, st);
+}
+
+cudaError_t attention_packed_bwd(const PackedAttnArgs& a, cudaStream_t st) {
+  ETHB_TRY(check_common(a), "packed backward");
+  ETHB_TRY(check_out(a.o, a.o_strides), "packed backward: out");
+  ETHB_TRY(check_out(a.dq, a.dq_strides), "packed backward: dq");
+  ETHB_TRY(check_out(a.dk, a.dk_strides), "packed backward: dk");
+  ETHB_TRY(check_out(a.dv, a.dv_strides), "packed backward: dv");
+  if (a.rows == 0) return cudaSuccess;
+  const bool bf = a.dtype == kBF16;
+  if (a.head_dim == 128) return bf ? launch_bwd<128, kBF16>(a, st) : launch_bwd<128, kF16>(a, st);
+  return bf ? launch_bwd<64, kBF16>(a, st) : launch_bwd<64, kF16>(a, st);
+}
+
+}  // namespace ethb

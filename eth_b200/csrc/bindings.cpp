@@ -5,6 +5,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include "attention_packed_sm100.cuh"
 #include "attention_sm100.cuh"
 #include "comm.cuh"
 #include "elementwise.cuh"
@@ -482,6 +483,79 @@ void attn_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o
   check(ethb::attention_bwd(a, cur_stream()), "attention_bwd");
 }
 
+// ---- attention over packed documents -----------------------------------------------------------
+// Element strides of (row, head); a dimension of size 1 has no stride of its own and gets one that a
+// tensor map takes.
+void rhd_strides(const Tensor& t, int64_t rows, int64_t heads, int64_t dim, const Tensor& like, const char* name,
+                 int64_t out[2]) {
+  TORCH_CHECK(t.is_cuda() && t.get_device() == like.get_device() && t.scalar_type() == like.scalar_type(), name,
+              ": device or type differs from q");
+  TORCH_CHECK(t.dim() == 3 && t.size(0) == rows && t.size(1) == heads && t.size(2) == dim && t.stride(2) == 1, name,
+              ": expected [", rows, ", ", heads, ", ", dim, "] with contiguous head_dim");
+  out[1] = heads == 1 ? dim : t.stride(1);
+  out[0] = rows == 1 ? dim * heads : t.stride(0);
+  TORCH_CHECK(out[0] > 0 && out[1] > 0, name, ": expanded dimensions are not supported");
+}
+// Work list on the device: int32 [n, 4] rows (start, len, tile, 0) as ops.PackedLayout builds them.
+const ethb::PackedTile* tile_list(const Tensor& t, const Tensor& like, int& n) {
+  TORCH_CHECK(t.is_cuda() && t.get_device() == like.get_device() && t.scalar_type() == at::kInt && t.dim() == 2 &&
+                  t.size(1) == 4 && t.is_contiguous(), "work list: int32 [n, 4] on the device of q");
+  n = static_cast<int>(t.size(0));
+  return reinterpret_cast<const ethb::PackedTile*>(t.data_ptr());
+}
+ethb::PackedAttnArgs packed_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o,
+                                 const Tensor& lse, int64_t used, double scale, bool causal,
+                                 const OptTensor& status) {
+  need_cuda(q, "q");
+  TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && v.dim() == 3, "q, k, v must be [rows, heads, head_dim]");
+  ethb::PackedAttnArgs a{};
+  const int64_t rows = q.size(0), d = q.size(2);
+  TORCH_CHECK(rows < 0x7fffff00, "too many rows");
+  a.rows = static_cast<int>(rows); a.used = static_cast<int>(used);
+  a.heads = static_cast<int>(q.size(1)); a.kv_heads = static_cast<int>(k.size(1)); a.head_dim = static_cast<int>(d);
+  a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr(); a.o = const_cast<void*>(o.data_ptr());
+  rhd_strides(q, rows, a.heads, d, q, "q", a.q_strides);
+  rhd_strides(k, rows, a.kv_heads, d, q, "k", a.k_strides);
+  rhd_strides(v, rows, a.kv_heads, d, q, "v", a.v_strides);
+  rhd_strides(o, rows, a.heads, d, q, "out", a.o_strides);
+  TORCH_CHECK(lse.is_cuda() && lse.get_device() == q.get_device() && lse.scalar_type() == at::kFloat &&
+                  lse.is_contiguous() && lse.numel() == a.heads * rows, "lse: fp32 [heads, rows]");
+  a.lse = const_cast<float*>(lse.data_ptr<float>());
+  a.scale = static_cast<float>(scale);
+  a.causal = causal;
+  a.dtype = dtype_code(q);
+  a.status = status.has_value() ? status->data_ptr<int>() : nullptr;
+  return a;
+}
+bool attn_packed_pairs_heads(int64_t heads, int64_t kv_heads) {
+  TORCH_CHECK(kv_heads > 0 && heads > 0);
+  return ethb::attention_packed_pairs_heads(static_cast<int>(heads), static_cast<int>(kv_heads));
+}
+void attn_packed_fwd(const Tensor& q, const Tensor& k, const Tensor& v, Tensor& o, Tensor& lse, const Tensor& tiles,
+                     int64_t used, double scale, bool causal, const OptTensor& status) {
+  c10::cuda::CUDAGuard guard(q.device());
+  auto a = packed_args(q, k, v, o, lse, used, scale, causal, status);
+  a.tiles = tile_list(tiles, q, a.num_tiles);
+  check(ethb::attention_packed_fwd(a, cur_stream()), "attention_packed_fwd");
+}
+void attn_packed_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& d_o,
+                     const Tensor& lse, Tensor& dq, Tensor& dk, Tensor& dv, Tensor& delta, const Tensor& q_tiles,
+                     const Tensor& k_tiles, int64_t used, double scale, bool causal, const OptTensor& status) {
+  c10::cuda::CUDAGuard guard(q.device());
+  auto a = packed_args(q, k, v, o, lse, used, scale, causal, status);
+  rhd_strides(d_o, a.rows, a.heads, a.head_dim, q, "d_out", a.do_strides);
+  rhd_strides(dq, a.rows, a.heads, a.head_dim, q, "dq", a.dq_strides);
+  rhd_strides(dk, a.rows, a.kv_heads, a.head_dim, q, "dk", a.dk_strides);
+  rhd_strides(dv, a.rows, a.kv_heads, a.head_dim, q, "dv", a.dv_strides);
+  TORCH_CHECK(delta.is_cuda() && delta.get_device() == q.get_device() && delta.scalar_type() == at::kFloat &&
+                  delta.is_contiguous() && delta.numel() == lse.numel(), "delta: fp32 [heads, rows]");
+  a.d_o = d_o.data_ptr(); a.dq = dq.data_ptr(); a.dk = dk.data_ptr(); a.dv = dv.data_ptr();
+  a.delta = delta.data_ptr<float>();
+  a.q_tiles = tile_list(q_tiles, q, a.num_q_tiles);
+  a.k_tiles = tile_list(k_tiles, q, a.num_k_tiles);
+  check(ethb::attention_packed_bwd(a, cur_stream()), "attention_packed_bwd");
+}
+
 // ---- per-token vocabulary kernels --------------------------------------------------------------
 ethb::LogitsView logits_view(const Tensor& z, int64_t vocab_start, double temperature) {
   need_cuda(z, "logits");
@@ -776,6 +850,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("synthetic_batch", &synthetic_batch);
   m.def("attn_fwd", &attn_fwd);
   m.def("attn_bwd", &attn_bwd);
+  m.def("attn_packed_pairs_heads", &attn_packed_pairs_heads);
+  m.def("attn_packed_fwd", &attn_packed_fwd);
+  m.def("attn_packed_bwd", &attn_packed_bwd);
   m.def("token_scores", &token_scores);
   m.def("token_scores_partial", &token_scores_partial);
   m.def("token_scores_combine", &token_scores_combine);

@@ -373,6 +373,105 @@ def attention_bwd(d_out, qkv, out, lse, batch, seq, heads, head_dim, scale=None,
     return torch.stack([gq, gk, gv], 3).to(qkv.dtype).reshape(qkv.shape)
 
 
+# ---------------------------------------------------------------------------------- attention over packed documents
+def attention_packed_fwd(q, k, v, layout, scale=None, causal=True):
+    """Attention inside each document of `layout` (a `PackedLayout`). q: [total, heads, head_dim], k / v:
+    [total, kv_heads, head_dim] (head h reads key/value head h // (heads / kv_heads)). Returns (out like
+    q, contiguous; lse [heads, total]). Rows behind the last document are 0 in `out`."""
+    scale = _check_packed(q, k, v, layout, scale)
+    if native.use_native(q):
+        q, k, v = _addressable(q), _addressable(k), _addressable(v)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
+        pairs = native.lib().attn_packed_pairs_heads(q.shape[1], k.shape[1])
+        native.lib().attn_packed_fwd(q, k, v, out, lse, layout.forward_tiles(causal, pairs), layout.used, scale,
+                                     bool(causal), native.status(q.device))
+        return out, lse
+    out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.zeros((q.shape[1], q.shape[0]), dtype=_wide(q).dtype, device=q.device)
+    for start, n in layout.documents():
+        rows = slice(start, start + n)
+        o, l = _document_ref(*(_wide(t[rows]) for t in (q, k, v)), scale, causal)
+        out[rows], lse[:, rows] = o.to(q.dtype), l
+    return out, lse
+
+
+def attention_packed_bwd(d_out, q, k, v, out, lse, layout, scale=None, causal=True):
+    """(dq, dk, dv), contiguous; gradients of a shared key/value head are summed over its group."""
+    scale = _check_packed(q, k, v, layout, scale)
+    if d_out.shape != q.shape or d_out.dtype != q.dtype or d_out.device != q.device:
+        raise ValueError("attention_packed_bwd: d_out must match q")
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    if native.use_native(q):
+        q, k, v, d_out = _addressable(q), _addressable(k), _addressable(v), _addressable(d_out)
+        delta = torch.empty_like(lse)
+        native.lib().attn_packed_bwd(q, k, v, out, d_out, lse, dq, dk, dv, delta, layout.query_tiles(causal),
+                                     layout.key_tiles(causal), layout.used, scale, bool(causal),
+                                     native.status(q.device))
+        return dq, dk, dv
+    for g in (dq, dk, dv):
+        g.zero_()
+    group = q.shape[1] // k.shape[1]
+    for start, n in layout.documents():
+        rows = slice(start, start + n)
+        qf, kf, vf, do = (_wide(t[rows]).transpose(0, 1) for t in (q, k, v, d_out))
+        kf, vf = kf.repeat_interleave(group, 0), vf.repeat_interleave(group, 0)
+        p = _scores_ref(qf, kf, scale, causal).sub_(lse[:, rows, None]).exp_()
+        dp = do @ vf.transpose(1, 2)
+        ds = p * (dp - (p * dp).sum(-1, keepdim=True)) * scale
+        dq[rows] = (ds @ kf).transpose(0, 1).to(q.dtype)
+        for dst, x in ((dk, ds.transpose(1, 2) @ qf), (dv, p.transpose(1, 2) @ do)):
+            dst[rows] = x.unflatten(0, (-1, group)).sum(1).transpose(0, 1).to(q.dtype)
+    return dq, dk, dv
+
+
+def _check_packed(q, k, v, layout, scale):
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        raise ValueError(f"packed attention: q [total, heads, dim], k and v [total, kv_heads, dim]; got "
+                         f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if k.shape[1] < 1 or q.shape[1] < 1 or q.shape[1] % k.shape[1]:
+        raise ValueError(f"packed attention: {q.shape[1]} heads cannot share {k.shape[1]} key/value heads evenly")
+    if not (q.dtype == k.dtype == v.dtype and q.device == k.device == v.device):
+        raise ValueError("packed attention: q, k and v must agree in type and device")
+    if q.is_cuda and (q.dtype not in (torch.float16, torch.bfloat16) or q.shape[2] not in (64, 128)):
+        raise ValueError(f"packed attention: fp16 / bf16 with head_dim 64 or 128 only, got {q.dtype}, {q.shape[2]}")
+    if not q.dtype.is_floating_point:
+        raise ValueError(f"packed attention: floating point only, got {q.dtype}")
+    if layout.total != q.shape[0]:
+        raise ValueError(f"packed attention: layout of {layout.total} rows, tensors of {q.shape[0]}")
+    if q.is_cuda and layout.device != q.device:
+        raise ValueError(f"packed attention: layout on {layout.device}, tensors on {q.device}")
+    scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
+    if not (math.isfinite(scale) and scale > 0):
+        raise ValueError(f"packed attention: scale must be positive and finite, got {scale}")
+    return scale
+
+
+def _addressable(t):
+    """`t` itself where a tensor map can describe it (16-byte aligned, strides of 16 bytes), else a copy."""
+    ok = t.data_ptr() % 16 == 0 and (t.stride(2) == 1 or t.shape[2] == 1)
+    for d in (0, 1):
+        ok = ok and (t.shape[d] <= 1 or (t.stride(d) > 0 and t.stride(d) % 8 == 0))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _scores_ref(q, k, scale, causal):
+    s = (q @ k.transpose(1, 2)) * scale
+    if causal:
+        n = s.shape[-1]
+        s = s.masked_fill(torch.ones(n, n, dtype=torch.bool, device=s.device).triu(1), -math.inf)
+    return s
+
+
+def _document_ref(q, k, v, scale, causal):
+    """(out, lse) of one document: q [n, heads, d], k / v [n, kv_heads, d], in the type they come in."""
+    group = q.shape[1] // k.shape[1]
+    qh, kh, vh = q.transpose(0, 1), *(t.transpose(0, 1).repeat_interleave(group, 0) for t in (k, v))
+    s = _scores_ref(qh, kh, scale, causal)
+    lse = torch.logsumexp(s, -1)
+    return (torch.exp(s - lse[..., None]) @ vh).transpose(0, 1), lse
+
+
 # ---------------------------------------------------------------------------------- unfused attention (13-op manifest)
 def bmm_heads(a, b, out, *, a_mn=False, b_mn=False, alpha=1.0, accumulate=False):
     """out[i, j] = alpha * a[i, j] x b[i, j]^T (+ out[i, j]) over two leading batch dims
