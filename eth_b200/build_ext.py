@@ -4,7 +4,8 @@ The reference JIT-compiles its four CUDA extensions and the dataset helper at st
 sm_70/sm_80 (eth/runtime/megatron/fused_kernels/__init__.py:30-95,
 eth/runtime/megatron/data/Makefile). Here everything is compiled ahead of time by plain
 `nvcc` / `g++` commands: kernel sources (`csrc/*.cu`) carry no PyTorch headers and build in
-seconds; one `bindings.cpp` exposes them to Python through pybind11 + ATen.
+seconds; `bindings.cpp` and `packed_ops.cpp` (ops with a C++ autograd node) expose them to Python
+through pybind11 + ATen.
 
 Usage: `python -m eth_b200.build_ext [--force] [--verbose]`.
 """
@@ -63,7 +64,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     BUILD.mkdir(exist_ok=True)
     headers = sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h"))
     cu_sources = sorted(CSRC.glob("*.cu"))
-    cpp_sources = [CSRC / "bindings.cpp"]
+    cpp_sources = [CSRC / "bindings.cpp", CSRC / "packed_ops.cpp"]
     stamp_file = BUILD / "stamp.json"
     stamps = {}
     if stamp_file.exists() and not force:

@@ -5,12 +5,10 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
-#include "attention_packed_sm100.cuh"
 #include "attention_sm100.cuh"
 #include "comm.cuh"
 #include "elementwise.cuh"
 #include "gemm_sm100.cuh"
-#include "token_loss.cuh"
 
 namespace {
 
@@ -483,216 +481,6 @@ void attn_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o
   check(ethb::attention_bwd(a, cur_stream()), "attention_bwd");
 }
 
-// ---- attention over packed documents -----------------------------------------------------------
-// Element strides of (row, head); a dimension of size 1 has no stride of its own and gets one that a
-// tensor map takes.
-void rhd_strides(const Tensor& t, int64_t rows, int64_t heads, int64_t dim, const Tensor& like, const char* name,
-                 int64_t out[2]) {
-  TORCH_CHECK(t.is_cuda() && t.get_device() == like.get_device() && t.scalar_type() == like.scalar_type(), name,
-              ": device or type differs from q");
-  TORCH_CHECK(t.dim() == 3 && t.size(0) == rows && t.size(1) == heads && t.size(2) == dim && t.stride(2) == 1, name,
-              ": expected [", rows, ", ", heads, ", ", dim, "] with contiguous head_dim");
-  out[1] = heads == 1 ? dim : t.stride(1);
-  out[0] = rows == 1 ? dim * heads : t.stride(0);
-  TORCH_CHECK(out[0] > 0 && out[1] > 0, name, ": expanded dimensions are not supported");
-}
-// Work list on the device: int32 [n, 4] rows (start, len, tile, 0) as ops.PackedLayout builds them.
-const ethb::PackedTile* tile_list(const Tensor& t, const Tensor& like, int& n) {
-  TORCH_CHECK(t.is_cuda() && t.get_device() == like.get_device() && t.scalar_type() == at::kInt && t.dim() == 2 &&
-                  t.size(1) == 4 && t.is_contiguous(), "work list: int32 [n, 4] on the device of q");
-  n = static_cast<int>(t.size(0));
-  return reinterpret_cast<const ethb::PackedTile*>(t.data_ptr());
-}
-ethb::PackedAttnArgs packed_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o,
-                                 const Tensor& lse, int64_t used, double scale, bool causal,
-                                 const OptTensor& status) {
-  need_cuda(q, "q");
-  TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && v.dim() == 3, "q, k, v must be [rows, heads, head_dim]");
-  ethb::PackedAttnArgs a{};
-  const int64_t rows = q.size(0), d = q.size(2);
-  TORCH_CHECK(rows < 0x7fffff00, "too many rows");
-  a.rows = static_cast<int>(rows); a.used = static_cast<int>(used);
-  a.heads = static_cast<int>(q.size(1)); a.kv_heads = static_cast<int>(k.size(1)); a.head_dim = static_cast<int>(d);
-  a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr(); a.o = const_cast<void*>(o.data_ptr());
-  rhd_strides(q, rows, a.heads, d, q, "q", a.q_strides);
-  rhd_strides(k, rows, a.kv_heads, d, q, "k", a.k_strides);
-  rhd_strides(v, rows, a.kv_heads, d, q, "v", a.v_strides);
-  rhd_strides(o, rows, a.heads, d, q, "out", a.o_strides);
-  TORCH_CHECK(lse.is_cuda() && lse.get_device() == q.get_device() && lse.scalar_type() == at::kFloat &&
-                  lse.is_contiguous() && lse.numel() == a.heads * rows, "lse: fp32 [heads, rows]");
-  a.lse = const_cast<float*>(lse.data_ptr<float>());
-  a.scale = static_cast<float>(scale);
-  a.causal = causal;
-  a.dtype = dtype_code(q);
-  a.status = status.has_value() ? status->data_ptr<int>() : nullptr;
-  return a;
-}
-bool attn_packed_pairs_heads(int64_t heads, int64_t kv_heads) {
-  TORCH_CHECK(kv_heads > 0 && heads > 0);
-  return ethb::attention_packed_pairs_heads(static_cast<int>(heads), static_cast<int>(kv_heads));
-}
-void attn_packed_fwd(const Tensor& q, const Tensor& k, const Tensor& v, Tensor& o, Tensor& lse, const Tensor& tiles,
-                     int64_t used, double scale, bool causal, const OptTensor& status) {
-  c10::cuda::CUDAGuard guard(q.device());
-  auto a = packed_args(q, k, v, o, lse, used, scale, causal, status);
-  a.tiles = tile_list(tiles, q, a.num_tiles);
-  check(ethb::attention_packed_fwd(a, cur_stream()), "attention_packed_fwd");
-}
-void attn_packed_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& d_o,
-                     const Tensor& lse, Tensor& dq, Tensor& dk, Tensor& dv, Tensor& delta, const Tensor& q_tiles,
-                     const Tensor& k_tiles, int64_t used, double scale, bool causal, const OptTensor& status) {
-  c10::cuda::CUDAGuard guard(q.device());
-  auto a = packed_args(q, k, v, o, lse, used, scale, causal, status);
-  rhd_strides(d_o, a.rows, a.heads, a.head_dim, q, "d_out", a.do_strides);
-  rhd_strides(dq, a.rows, a.heads, a.head_dim, q, "dq", a.dq_strides);
-  rhd_strides(dk, a.rows, a.kv_heads, a.head_dim, q, "dk", a.dk_strides);
-  rhd_strides(dv, a.rows, a.kv_heads, a.head_dim, q, "dv", a.dv_strides);
-  TORCH_CHECK(delta.is_cuda() && delta.get_device() == q.get_device() && delta.scalar_type() == at::kFloat &&
-                  delta.is_contiguous() && delta.numel() == lse.numel(), "delta: fp32 [heads, rows]");
-  a.d_o = d_o.data_ptr(); a.dq = dq.data_ptr(); a.dk = dk.data_ptr(); a.dv = dv.data_ptr();
-  a.delta = delta.data_ptr<float>();
-  a.q_tiles = tile_list(q_tiles, q, a.num_q_tiles);
-  a.k_tiles = tile_list(k_tiles, q, a.num_k_tiles);
-  check(ethb::attention_packed_bwd(a, cur_stream()), "attention_packed_bwd");
-}
-
-// ---- per-token vocabulary kernels --------------------------------------------------------------
-ethb::LogitsView logits_view(const Tensor& z, int64_t vocab_start, double temperature) {
-  need_cuda(z, "logits");
-  TORCH_CHECK(z.dim() == 2 && (z.stride(1) == 1 || z.size(1) == 1), "logits must be 2-D with unit inner stride");
-  TORCH_CHECK(z.size(1) >= 1 && z.size(1) < (int64_t{1} << 30), "vocabulary size out of range");
-  ethb::LogitsView a{};
-  a.z = z.data_ptr(); a.rows = z.size(0); a.ld = z.stride(0); a.vocab = static_cast<int>(z.size(1));
-  a.v0 = vocab_start;
-  a.dtype = dtype_code(z);
-  a.inv_temperature = static_cast<float>(1.0 / temperature);
-  return a;
-}
-// Contiguous tensor of `numel` elements of type `type` on the device of `like`; its data.
-template <typename T>
-T* flat(const Tensor& t, const Tensor& like, at::ScalarType type, int64_t numel, const char* name) {
-  TORCH_CHECK(t.is_cuda() && t.get_device() == like.get_device(), name, " must be on the device of the logits");
-  TORCH_CHECK(t.scalar_type() == type && t.is_contiguous() && t.numel() == numel, name, ": type, layout or size");
-  return numel == 0 ? nullptr : t.data_ptr<T>();
-}
-template <typename T>
-T* flat(const OptTensor& t, const Tensor& like, at::ScalarType type, int64_t numel, const char* name) {
-  return t.has_value() ? flat<T>(*t, like, type, numel, name) : nullptr;
-}
-ethb::TeacherView teacher_view(const Tensor& index, const Tensor& logit, const Tensor& like, int64_t rows) {
-  TORCH_CHECK(index.dim() == 2 && index.size(0) == rows && index.size(1) >= 1 &&
-                  index.size(1) <= ethb::kMaxTeacherEntries,
-              "teacher lists must be [rows, 1..", ethb::kMaxTeacherEntries, "]");
-  const int64_t n = rows * index.size(1);
-  return {flat<int64_t>(index, like, at::kLong, n, "teacher_index"),
-          flat<float>(logit, like, at::kFloat, n, "teacher_logit"), static_cast<int>(index.size(1))};
-}
-int64_t grad_pitch(const Tensor& dz, const Tensor& z) {
-  TORCH_CHECK(dz.is_cuda() && dz.get_device() == z.get_device() && dz.scalar_type() == z.scalar_type() &&
-                  dz.sizes() == z.sizes() && (dz.stride(1) == 1 || dz.size(1) == 1),
-              "gradient of the logits: device, type, shape or inner stride");
-  TORCH_CHECK(dz.size(0) <= 1 || dz.stride(0) >= dz.size(1), "gradient rows overlap");
-  return dz.stride(0);
-}
-ethb::TokenScoresOut scores_out(const Tensor& like, int64_t rows, int64_t k, const Tensor& logprob,
-                                const Tensor& entropy, const OptTensor& top_logprob, const OptTensor& top_index,
-                                const Tensor& stats) {
-  TORCH_CHECK(k == 0 || (top_logprob.has_value() && top_index.has_value()), "top_k outputs missing");
-  return {flat<float>(logprob, like, at::kFloat, rows, "logprob"), flat<float>(entropy, like, at::kFloat, rows, "entropy"),
-          flat<float>(top_logprob, like, at::kFloat, rows * k, "top_logprob"),
-          flat<int64_t>(top_index, like, at::kLong, rows * k, "top_index"),
-          flat<float>(stats, like, at::kFloat, rows * 2, "stats")};
-}
-void token_scores(const Tensor& z, const Tensor& tokens, int64_t top_k, double temperature, int64_t vocab_start,
-                  Tensor& logprob, Tensor& entropy, const OptTensor& top_logprob, const OptTensor& top_index,
-                  Tensor& stats) {
-  const auto a = logits_view(z, vocab_start, temperature);
-  c10::cuda::CUDAGuard guard(z.device());
-  check(ethb::token_scores(a, flat<int64_t>(tokens, z, at::kLong, a.rows, "tokens"), static_cast<int>(top_k),
-                           scores_out(z, a.rows, top_k, logprob, entropy, top_logprob, top_index, stats),
-                           cur_stream()), "token_scores");
-}
-void token_scores_partial(const Tensor& z, const Tensor& tokens, int64_t top_k, double temperature,
-                          int64_t vocab_start, Tensor& partial) {
-  const auto a = logits_view(z, vocab_start, temperature);
-  c10::cuda::CUDAGuard guard(z.device());
-  check(ethb::token_scores_partial(a, flat<int64_t>(tokens, z, at::kLong, a.rows, "tokens"), static_cast<int>(top_k),
-                                   flat<float>(partial, z, at::kFloat, a.rows * (4 + 2 * top_k), "partial"),
-                                   cur_stream()), "token_scores_partial");
-}
-void token_scores_combine(const Tensor& partials, const Tensor& tokens, int64_t top_k, double temperature,
-                          Tensor& logprob, Tensor& entropy, const OptTensor& top_logprob, const OptTensor& top_index,
-                          Tensor& stats) {
-  need_cuda(partials, "partials");
-  TORCH_CHECK(partials.dim() == 3 && partials.size(0) >= 1 && partials.size(2) == 4 + 2 * top_k, "partials shape");
-  const int64_t world = partials.size(0), rows = partials.size(1);
-  c10::cuda::CUDAGuard guard(partials.device());
-  check(ethb::token_scores_combine(flat<float>(partials, partials, at::kFloat, partials.numel(), "partials"),
-                                   static_cast<int>(world), rows,
-                                   flat<int64_t>(tokens, partials, at::kLong, rows, "tokens"),
-                                   static_cast<int>(top_k), static_cast<float>(1.0 / temperature),
-                                   scores_out(partials, rows, top_k, logprob, entropy, top_logprob, top_index, stats),
-                                   cur_stream()), "token_scores_combine");
-}
-void token_scores_bwd(const Tensor& z, const Tensor& tokens, const Tensor& stats, const Tensor& entropy,
-                      const OptTensor& top_index, int64_t top_k, double temperature, int64_t vocab_start,
-                      const OptTensor& g, const OptTensor& h, const OptTensor& u, Tensor& dz) {
-  const auto a = logits_view(z, vocab_start, temperature);
-  c10::cuda::CUDAGuard guard(z.device());
-  TORCH_CHECK(!u.has_value() || top_index.has_value(), "gradient of alternatives without their ids");
-  check(ethb::token_scores_bwd(a, flat<int64_t>(tokens, z, at::kLong, a.rows, "tokens"),
-                               flat<float>(stats, z, at::kFloat, 2 * a.rows, "stats"),
-                               flat<float>(entropy, z, at::kFloat, a.rows, "entropy"),
-                               flat<int64_t>(top_index, z, at::kLong, a.rows * top_k, "top_index"),
-                               static_cast<int>(top_k), flat<float>(g, z, at::kFloat, a.rows, "d_logprob"),
-                               flat<float>(h, z, at::kFloat, a.rows, "d_entropy"),
-                               flat<float>(u, z, at::kFloat, a.rows * top_k, "d_top_logprob"), dz.data_ptr(),
-                               grad_pitch(dz, z), cur_stream()), "token_scores_bwd");
-}
-void distill_fwd(const Tensor& z, const Tensor& index, const Tensor& logit, double temperature, int64_t vocab_start,
-                 Tensor& loss, Tensor& stats) {
-  const auto a = logits_view(z, vocab_start, temperature);
-  c10::cuda::CUDAGuard guard(z.device());
-  check(ethb::distill_fwd(a, teacher_view(index, logit, z, a.rows), flat<float>(loss, z, at::kFloat, a.rows, "loss"),
-                          flat<float>(stats, z, at::kFloat, 2 * a.rows, "stats"), cur_stream()), "distill_fwd");
-}
-void distill_partial(const Tensor& z, const Tensor& index, const Tensor& logit, double temperature,
-                     int64_t vocab_start, Tensor& partial) {
-  const auto a = logits_view(z, vocab_start, temperature);
-  c10::cuda::CUDAGuard guard(z.device());
-  check(ethb::distill_partial(a, teacher_view(index, logit, z, a.rows),
-                              flat<float>(partial, z, at::kFloat, 4 * a.rows, "partial"), cur_stream()),
-        "distill_partial");
-}
-void distill_combine(const Tensor& partials, const Tensor& index, const Tensor& logit, double temperature,
-                     Tensor& loss, Tensor& stats) {
-  need_cuda(partials, "partials");
-  TORCH_CHECK(partials.dim() == 3 && partials.size(0) >= 1 && partials.size(2) == 4, "partials shape");
-  const int64_t rows = partials.size(1);
-  c10::cuda::CUDAGuard guard(partials.device());
-  check(ethb::distill_combine(flat<float>(partials, partials, at::kFloat, partials.numel(), "partials"),
-                              static_cast<int>(partials.size(0)), rows, teacher_view(index, logit, partials, rows),
-                              static_cast<float>(1.0 / temperature), flat<float>(loss, partials, at::kFloat, rows, "loss"),
-                              flat<float>(stats, partials, at::kFloat, 2 * rows, "stats"), cur_stream()),
-        "distill_combine");
-}
-void distill_bwd(const Tensor& z, const Tensor& index, const Tensor& logit, const Tensor& stats, const Tensor& dloss,
-                 double temperature, int64_t vocab_start, Tensor& dz) {
-  const auto a = logits_view(z, vocab_start, temperature);
-  c10::cuda::CUDAGuard guard(z.device());
-  check(ethb::distill_bwd(a, teacher_view(index, logit, z, a.rows), flat<float>(stats, z, at::kFloat, 2 * a.rows, "stats"),
-                          flat<float>(dloss, z, at::kFloat, a.rows, "dloss"), dz.data_ptr(), grad_pitch(dz, z),
-                          cur_stream()), "distill_bwd");
-}
-void distill_step(const Tensor& z, const Tensor& index, const Tensor& logit, const Tensor& dloss, double temperature,
-                  int64_t vocab_start, Tensor& loss, Tensor& dz) {
-  const auto a = logits_view(z, vocab_start, temperature);
-  c10::cuda::CUDAGuard guard(z.device());
-  check(ethb::distill_step(a, teacher_view(index, logit, z, a.rows), flat<float>(dloss, z, at::kFloat, a.rows, "dloss"),
-                           flat<float>(loss, z, at::kFloat, a.rows, "loss"), dz.data_ptr(), grad_pitch(dz, z),
-                           cur_stream()), "distill_step");
-}
-
 // ---- peer memory -------------------------------------------------------------------------------
 ethb::PeerPtrs to_peers(const std::vector<int64_t>& ptrs) {
   TORCH_CHECK(ptrs.size() <= ethb::kMaxPeers, "too many peers");
@@ -809,7 +597,10 @@ void flags_wait(const std::vector<int64_t>& ptrs, int64_t value, int64_t limit_s
 
 }  // namespace
 
+namespace ethb { void bind_packed_ops(pybind11::module_& m); }   // packed_ops.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  ethb::bind_packed_ops(m);
   m.def("gemm", &gemm, py::arg("a"), py::arg("a_mn"), py::arg("b"), py::arg("b_mn"), py::arg("d"), py::arg("bias"),
         py::arg("aux"), py::arg("aux_mode"), py::arg("d2"), py::arg("accumulate"), py::arg("alpha"), py::arg("status"),
         py::arg("sm_count"), py::arg("drop_p") = 0.0, py::arg("drop_seed") = 0, py::arg("drop_offset") = 0);
@@ -850,18 +641,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("synthetic_batch", &synthetic_batch);
   m.def("attn_fwd", &attn_fwd);
   m.def("attn_bwd", &attn_bwd);
-  m.def("attn_packed_pairs_heads", &attn_packed_pairs_heads);
-  m.def("attn_packed_fwd", &attn_packed_fwd);
-  m.def("attn_packed_bwd", &attn_packed_bwd);
-  m.def("token_scores", &token_scores);
-  m.def("token_scores_partial", &token_scores_partial);
-  m.def("token_scores_combine", &token_scores_combine);
-  m.def("token_scores_bwd", &token_scores_bwd);
-  m.def("distill_fwd", &distill_fwd);
-  m.def("distill_partial", &distill_partial);
-  m.def("distill_combine", &distill_combine);
-  m.def("distill_bwd", &distill_bwd);
-  m.def("distill_step", &distill_step);
   m.def("launch_count", [] { return ethb::launch_count(); });
   m.def("set_gemm_variant", [](int v) { ethb::set_gemm_variant(v); });
   m.def("set_gemm_tail_split", [](int on) { ethb::set_gemm_tail_split(on); });

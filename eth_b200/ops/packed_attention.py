@@ -8,8 +8,9 @@ from __future__ import annotations
 
 import numpy as np
 import torch
+from torch.autograd.function import once_differentiable
 
-from . import raw
+from . import native, raw
 
 _TILE = 128     # rows of a query or key tile of the kernels (csrc/attention_packed_sm100.cu)
 
@@ -41,15 +42,17 @@ class PackedLayout:
         self.device = torch.device(device)
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
-        self._tables = None
+        self._lists = None
         if self.device.type == "cuda":
             parts = list(self._work_lists(lengths))
             host = torch.from_numpy(np.concatenate([x for _, x in parts]))
             flat = host.to(self.device)
-            self._tables, at = {}, 0
+            tables, at = {}, 0
             for name, x in parts:
-                self._tables[name] = flat[at:at + len(x)]
+                tables[name] = flat[at:at + len(x)]
                 at += len(x)
+            self._lists = {True: (tables["causal128"], tables["causal256"], tables["keys128"]),
+                           False: (tables["full128"], tables["full256"], tables["full128"])}
 
     def documents(self):
         """(first row, rows) of every document that has tokens."""
@@ -76,19 +79,11 @@ class PackedLayout:
             for name, weight in orders.items():
                 yield f"{name}{rows}", table[np.argsort(weight, kind="stable")]
 
-    def _table(self, name):
-        if self._tables is None:
+    def work_lists(self, causal):
+        """The kernels' device tables for one mask: 128-row tiles, 256-row blocks, key tiles."""
+        if self._lists is None:
             raise ValueError(f"PackedLayout on {self.device} has no work lists for CUDA tensors")
-        return self._tables[name]
-
-    def forward_tiles(self, causal, pairs_heads):
-        return self._table(("causal" if causal else "full") + str(_TILE if pairs_heads else 2 * _TILE))
-
-    def query_tiles(self, causal):
-        return self._table(("causal" if causal else "full") + str(_TILE))
-
-    def key_tiles(self, causal):
-        return self._table(("keys" if causal else "full") + str(_TILE))
+        return self._lists[bool(causal)]
 
 
 class _PackedAttnFn(torch.autograd.Function):
@@ -100,6 +95,7 @@ class _PackedAttnFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_out):
         q, k, v, out, lse = ctx.saved_tensors
         dq, dk, dv = raw.attention_packed_bwd(d_out, q, k, v, out, lse, ctx.layout, ctx.scale, ctx.causal)
@@ -115,4 +111,8 @@ def flash_attention_packed(q, k, v, layout, scale=None, causal=True):
     read in place, what a tensor map cannot address is copied. A document attends to itself only: what
     stands in other documents or behind the last one, infinities and NaN included, does not reach it.
     `scale` defaults to 1 / sqrt(head_dim)."""
+    if native.use_native(q):     # the autograd node is native too
+        return native.lib().flash_attention_packed(q, k, v, *layout.work_lists(causal), layout.used, layout.total,
+                                                   scale, bool(causal),
+                                                   native.status(q.device))
     return _PackedAttnFn.apply(q, k, v, layout, scale, bool(causal))

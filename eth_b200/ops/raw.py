@@ -378,15 +378,11 @@ def attention_packed_fwd(q, k, v, layout, scale=None, causal=True):
     """Attention inside each document of `layout` (a `PackedLayout`). q: [total, heads, head_dim], k / v:
     [total, kv_heads, head_dim] (head h reads key/value head h // (heads / kv_heads)). Returns (out like
     q, contiguous; lse [heads, total]). Rows behind the last document are 0 in `out`."""
-    scale = _check_packed(q, k, v, layout, scale)
     if native.use_native(q):
-        q, k, v = _addressable(q), _addressable(k), _addressable(v)
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
-        pairs = native.lib().attn_packed_pairs_heads(q.shape[1], k.shape[1])
-        native.lib().attn_packed_fwd(q, k, v, out, lse, layout.forward_tiles(causal, pairs), layout.used, scale,
-                                     bool(causal), native.status(q.device))
-        return out, lse
+        return native.lib().attention_packed_fwd(q, k, v, *layout.work_lists(causal), layout.used, layout.total,
+                                                 scale, bool(causal),
+                                                 native.status(q.device))
+    scale = _check_packed(q, k, v, layout, scale)
     out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.zeros((q.shape[1], q.shape[0]), dtype=_wide(q).dtype, device=q.device)
     for start, n in layout.documents():
@@ -398,17 +394,14 @@ def attention_packed_fwd(q, k, v, layout, scale=None, causal=True):
 
 def attention_packed_bwd(d_out, q, k, v, out, lse, layout, scale=None, causal=True):
     """(dq, dk, dv), contiguous; gradients of a shared key/value head are summed over its group."""
+    if native.use_native(q):
+        return native.lib().attention_packed_bwd(d_out, q, k, v, out, lse, *layout.work_lists(causal), layout.used,
+                                                 layout.total, scale,
+                                                 bool(causal), native.status(q.device))
     scale = _check_packed(q, k, v, layout, scale)
     if d_out.shape != q.shape or d_out.dtype != q.dtype or d_out.device != q.device:
         raise ValueError("attention_packed_bwd: d_out must match q")
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    if native.use_native(q):
-        q, k, v, d_out = _addressable(q), _addressable(k), _addressable(v), _addressable(d_out)
-        delta = torch.empty_like(lse)
-        native.lib().attn_packed_bwd(q, k, v, out, d_out, lse, dq, dk, dv, delta, layout.query_tiles(causal),
-                                     layout.key_tiles(causal), layout.used, scale, bool(causal),
-                                     native.status(q.device))
-        return dq, dk, dv
     for g in (dq, dk, dv):
         g.zero_()
     group = q.shape[1] // k.shape[1]
@@ -426,6 +419,7 @@ def attention_packed_bwd(d_out, q, k, v, out, lse, layout, scale=None, causal=Tr
 
 
 def _check_packed(q, k, v, layout, scale):
+    """Refusals of the CPU path; csrc/packed_ops.cpp makes them for CUDA tensors."""
     if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
         raise ValueError(f"packed attention: q [total, heads, dim], k and v [total, kv_heads, dim]; got "
                          f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
@@ -433,26 +427,14 @@ def _check_packed(q, k, v, layout, scale):
         raise ValueError(f"packed attention: {q.shape[1]} heads cannot share {k.shape[1]} key/value heads evenly")
     if not (q.dtype == k.dtype == v.dtype and q.device == k.device == v.device):
         raise ValueError("packed attention: q, k and v must agree in type and device")
-    if q.is_cuda and (q.dtype not in (torch.float16, torch.bfloat16) or q.shape[2] not in (64, 128)):
-        raise ValueError(f"packed attention: fp16 / bf16 with head_dim 64 or 128 only, got {q.dtype}, {q.shape[2]}")
     if not q.dtype.is_floating_point:
         raise ValueError(f"packed attention: floating point only, got {q.dtype}")
     if layout.total != q.shape[0]:
         raise ValueError(f"packed attention: layout of {layout.total} rows, tensors of {q.shape[0]}")
-    if q.is_cuda and layout.device != q.device:
-        raise ValueError(f"packed attention: layout on {layout.device}, tensors on {q.device}")
     scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
     if not (math.isfinite(scale) and scale > 0):
         raise ValueError(f"packed attention: scale must be positive and finite, got {scale}")
     return scale
-
-
-def _addressable(t):
-    """`t` itself where a tensor map can describe it (16-byte aligned, strides of 16 bytes), else a copy."""
-    ok = t.data_ptr() % 16 == 0 and (t.stride(2) == 1 or t.shape[2] == 1)
-    for d in (0, 1):
-        ok = ok and (t.shape[d] <= 1 or (t.stride(d) > 0 and t.stride(d) % 8 == 0))
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
 def _scores_ref(q, k, scale, causal):
@@ -570,10 +552,10 @@ def _wide(t):
 
 
 def _check_logits(logits, temperature, what):
+    """Refusals of the CPU path; csrc/packed_ops.cpp makes them for CUDA tensors."""
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"{what}: logits must be [tokens, vocab], got {tuple(logits.shape)}")
-    kinds = (torch.float32, torch.float16, torch.bfloat16) + (() if logits.is_cuda else (torch.float64,))
-    if logits.dtype not in kinds:
+    if logits.dtype not in (torch.float32, torch.float16, torch.bfloat16, torch.float64):
         raise ValueError(f"{what}: logits of type {logits.dtype} are not supported")
     if not (math.isfinite(temperature) and temperature > 0):
         raise ValueError(f"{what}: temperature must be positive and finite, got {temperature}")
@@ -587,26 +569,6 @@ def _check_rows(t, logits, dtypes, shape, what):
     return t.contiguous()
 
 
-def _unit_rows(logits):
-    """Logits with unit inner stride and rows that do not overlap; any pitch is taken as it is."""
-    if logits.shape[1] > 1 and logits.stride(1) != 1 or logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]:
-        return logits.contiguous()
-    return logits
-
-
-def _grad_rows(logits):
-    """An uninitialised gradient whose rows sit at the same offsets from a 16-byte boundary as the
-    rows of `logits` (a slice of a padded vocabulary keeps vector accesses on both sides)."""
-    rows, vocab = logits.shape
-    per = 16 // logits.element_size()
-    lead = logits.data_ptr() % 16 // logits.element_size()
-    pitch = vocab + (logits.stride(0) - vocab) % per if rows > 1 else vocab
-    if lead == 0 and pitch == vocab:
-        return torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
-    flat = torch.empty(lead + rows * pitch, dtype=logits.dtype, device=logits.device)
-    return flat.as_strided((rows, vocab), (pitch, 1), lead)
-
-
 def token_scores_fwd(logits, tokens, top_k=0, temperature=1.0, vocab_start=0, gather_fn=None):
     """Log-probability of `tokens` under softmax(logits / temperature), entropy of that distribution and
     its `top_k` most likely tokens. Returns (logprob, entropy, top_logprob, top_index, stats); `stats`
@@ -615,27 +577,16 @@ def token_scores_fwd(logits, tokens, top_k=0, temperature=1.0, vocab_start=0, ga
     logits: [tokens, vocab_local] of a vocabulary shard that starts at `vocab_start`; `gather_fn` as in
     `ce_fwd`. A negative token is none: its log-probability is 0 and has no gradient; one at or beyond
     the whole vocabulary has NaN. Alternatives fall in log-probability, equal ones go by rising id."""
+    if native.use_native(logits):
+        if gather_fn is None:
+            return native.lib().token_scores_fwd(logits, tokens, top_k, temperature, vocab_start)
+        part = native.lib().token_scores_partial(logits, tokens, top_k, temperature, vocab_start)
+        return native.lib().token_scores_combine(gather_fn(part).contiguous(), tokens, top_k, temperature)
     _check_logits(logits, temperature, "token_scores_fwd")
     rows, vocab = logits.shape
     if not 0 <= top_k <= min(MAX_TOP_ALTERNATIVES, vocab):
         raise ValueError(f"top_k must be between 0 and {min(MAX_TOP_ALTERNATIVES, vocab)}, got {top_k}")
     tokens = _check_rows(tokens, logits, (torch.int64,), (rows,), "tokens")
-    logits = _unit_rows(logits)
-    if native.use_native(logits):
-        def new(*shape, dtype=torch.float32):
-            return torch.empty(shape, dtype=dtype, device=logits.device)
-        logprob, entropy, stats = new(rows), new(rows), new(rows, 2)
-        top_logprob = new(rows, top_k) if top_k else None
-        top_index = new(rows, top_k, dtype=torch.int64) if top_k else None
-        if gather_fn is None:
-            native.lib().token_scores(logits, tokens, top_k, temperature, vocab_start, logprob, entropy, top_logprob,
-                                      top_index, stats)
-        else:
-            part = new(rows, 4 + 2 * top_k)
-            native.lib().token_scores_partial(logits, tokens, top_k, temperature, vocab_start, part)
-            native.lib().token_scores_combine(gather_fn(part).contiguous(), tokens, top_k, temperature, logprob,
-                                              entropy, top_logprob, top_index, stats)
-        return logprob, entropy, top_logprob, top_index, stats
     z = _wide(logits)
     mx = z.amax(1)
     mu = torch.where(mx == -math.inf, 0.0, mx)
@@ -675,20 +626,17 @@ def token_scores_bwd(logits, tokens, stats, entropy, top_index, d_logprob=None, 
                      temperature=1.0, vocab_start=0):
     """Gradient of the logits from the gradients of logprob [tokens], entropy [tokens] and top_logprob
     [tokens, top_k] (any may be None). A row whose gradients are all 0 gets zeros, whatever its logits."""
-    logits = _unit_rows(logits)
+    if native.use_native(logits):
+        return native.lib().token_scores_bwd(logits, tokens, stats, entropy, top_index, d_logprob, d_entropy, d_top,
+                                             temperature, vocab_start)
     rows, vocab = logits.shape
-    wide = (torch.float32,) if logits.is_cuda else (torch.float32, torch.float64)
+    wide = (torch.float32, torch.float64)
     top_k = 0 if top_index is None else top_index.shape[1]
     grads = []
     for t, shape, what in ((d_logprob, (rows,), "d_logprob"), (d_entropy, (rows,), "d_entropy"),
                            (d_top, (rows, top_k), "d_top")):
         grads.append(None if t is None else _check_rows(t, logits, wide, shape, what))
     g, h, u = grads
-    if native.use_native(logits):
-        dz = _grad_rows(logits)
-        native.lib().token_scores_bwd(logits, tokens, stats, entropy, top_index, top_k, temperature, vocab_start, g, h, u,
-                                      dz)
-        return dz
     z = _wide(logits)
     logp = (z - stats[:, :1]) / temperature - torch.log(stats[:, 1:])
     p = torch.exp(logp)
@@ -719,9 +667,8 @@ def _check_teacher(logits, index, logit):
     if not isinstance(index, torch.Tensor) or index.dim() != 2 or not 1 <= index.shape[1] <= MAX_TEACHER_ENTRIES:
         raise ValueError(f"teacher lists must be [tokens, 1..{MAX_TEACHER_ENTRIES}]")
     shape = (rows, index.shape[1])
-    wide = (torch.float32,) if logits.is_cuda else (torch.float32, torch.float64)
     return (_check_rows(index, logits, (torch.int64,), shape, "teacher_index"),
-            _check_rows(logit, logits, wide, shape, "teacher_logit"))
+            _check_rows(logit, logits, (torch.float32, torch.float64), shape, "teacher_logit"))
 
 
 def _teacher_ref(logits, logit, temperature):
@@ -737,20 +684,14 @@ def distill_fwd(logits, teacher_index, teacher_logit, temperature=1.0, vocab_sta
     logits / temperature, p = softmax(logits / temperature) over the whole vocabulary. Returns (loss,
     stats for `distill_bwd`). An entry at -inf is unused; a row without entries has loss 0; a used
     entry outside the vocabulary makes the row's loss NaN. An id listed twice counts twice."""
+    if native.use_native(logits):
+        if gather_fn is None:
+            return native.lib().distill_fwd(logits, teacher_index, teacher_logit, temperature, vocab_start)
+        part = native.lib().distill_partial(logits, teacher_index, teacher_logit, temperature, vocab_start)
+        return native.lib().distill_combine(gather_fn(part).contiguous(), teacher_index, teacher_logit, temperature)
     _check_logits(logits, temperature, "distill_fwd")
     index, logit = _check_teacher(logits, teacher_index, teacher_logit)
-    logits = _unit_rows(logits)
-    rows, vocab = logits.shape
-    if native.use_native(logits):
-        loss = torch.empty(rows, dtype=torch.float32, device=logits.device)
-        stats = torch.empty((rows, 2), dtype=torch.float32, device=logits.device)
-        if gather_fn is None:
-            native.lib().distill_fwd(logits, index, logit, temperature, vocab_start, loss, stats)
-        else:
-            part = torch.empty((rows, 4), dtype=torch.float32, device=logits.device)
-            native.lib().distill_partial(logits, index, logit, temperature, vocab_start, part)
-            native.lib().distill_combine(gather_fn(part).contiguous(), index, logit, temperature, loss, stats)
-        return loss, stats
+    vocab = logits.shape[1]
     z = _wide(logits)
     q, log_q, some = _teacher_ref(logits, logit, temperature)
     mx = z.amax(1)
@@ -774,14 +715,10 @@ def distill_fwd(logits, teacher_index, teacher_logit, temperature=1.0, vocab_sta
 
 def distill_bwd(logits, teacher_index, teacher_logit, stats, dloss, temperature=1.0, vocab_start=0):
     """d loss / d logits scaled by dloss[row]; rows without entries or with dloss 0 get zeros."""
-    index, logit = _check_teacher(logits, teacher_index, teacher_logit)
-    logits = _unit_rows(logits)
-    wide = (torch.float32,) if logits.is_cuda else (torch.float32, torch.float64)
-    dloss = _check_rows(dloss, logits, wide, (logits.shape[0],), "dloss")
     if native.use_native(logits):
-        dz = _grad_rows(logits)
-        native.lib().distill_bwd(logits, index, logit, stats, dloss, temperature, vocab_start, dz)
-        return dz
+        return native.lib().distill_bwd(logits, teacher_index, teacher_logit, stats, dloss, temperature, vocab_start)
+    index, logit = _check_teacher(logits, teacher_index, teacher_logit)
+    dloss = _check_rows(dloss, logits, (torch.float32, torch.float64), (logits.shape[0],), "dloss")
     z = _wide(logits)
     q, _, some = _teacher_ref(logits, logit, temperature)
     g = torch.where(some, dloss.to(z.dtype), 0.0) / temperature
@@ -794,10 +731,9 @@ def distill_step(logits, teacher_index, teacher_logit, dloss, temperature=1.0, o
     """(loss, d logits) of `distill_fwd` and `distill_bwd` in one pass over the logits, for a caller that
     knows the gradient of every row's loss beforehand (the last pipeline stage does: loss scale over
     token count). Whole vocabulary only. `out` takes the gradient; it may be `logits` itself."""
+    if native.use_native(logits):
+        return native.lib().distill_step(logits, teacher_index, teacher_logit, dloss, temperature, out)
     _check_logits(logits, temperature, "distill_step")
-    index, logit = _check_teacher(logits, teacher_index, teacher_logit)
-    wide = (torch.float32,) if logits.is_cuda else (torch.float32, torch.float64)
-    dloss = _check_rows(dloss, logits, wide, (logits.shape[0],), "dloss")
     if out is not None:
         if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device or \
                 (out.shape[1] > 1 and out.stride(1) != 1) or (out.shape[0] > 1 and out.stride(0) < out.shape[1]):
@@ -805,12 +741,6 @@ def distill_step(logits, teacher_index, teacher_logit, dloss, temperature=1.0, o
         same = out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride()
         if not same and out.untyped_storage().data_ptr() == logits.untyped_storage().data_ptr():
             raise ValueError("distill_step: out may be the logits themselves or other memory, not an overlapping view")
-    x = _unit_rows(logits)
-    if native.use_native(x):
-        loss = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
-        dz = _grad_rows(x) if out is None else out
-        native.lib().distill_step(x, index, logit, dloss, temperature, 0, loss, dz)
-        return loss, dz
-    loss, stats = distill_fwd(x, index, logit, temperature)
-    dz = distill_bwd(x, index, logit, stats, dloss, temperature)
+    loss, stats = distill_fwd(logits, teacher_index, teacher_logit, temperature)
+    dz = distill_bwd(logits, teacher_index, teacher_logit, stats, dloss, temperature)
     return loss, dz if out is None else out.copy_(dz)

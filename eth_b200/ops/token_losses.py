@@ -10,8 +10,9 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
-from . import raw
+from . import native, raw
 
 
 class TokenScores(NamedTuple):
@@ -34,6 +35,7 @@ class _TokenScoresFn(torch.autograd.Function):
         return logprob, entropy, top_logprob, top_index
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_logprob, d_entropy, d_top, _):
         logits, tokens, stats, entropy, top_index = ctx.saved_tensors
         dz = raw.token_scores_bwd(logits, tokens, stats, entropy, top_index, d_logprob, d_entropy, d_top,
@@ -50,6 +52,9 @@ def token_logprobs(logits, tokens, top_k=0, temperature=1.0, vocab_start=0, gath
     128) adds the most likely tokens, equal ones by rising id. `vocab_start` and `gather_fn` as in
     `vocab_parallel_cross_entropy` (`gather_fn` returns the `[tp, tokens, n]` stack of a `[tokens, n]`
     tensor over the tensor-parallel group)."""
+    if gather_fn is None and native.use_native(logits):     # the autograd node is native too
+        r = native.lib().token_logprobs(logits, tokens, top_k, temperature, vocab_start)
+        return TokenScores(*r) if top_k else TokenScores(*r, None, None)
     return TokenScores(*_TokenScoresFn.apply(logits, tokens, int(top_k), float(temperature), int(vocab_start), gather_fn))
 
 
@@ -62,6 +67,7 @@ class _DistillFn(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dloss):
         logits, index, logit, stats = ctx.saved_tensors
         dz = raw.distill_bwd(logits, index, logit, stats, dloss, ctx.temperature, ctx.vocab_start)
@@ -77,4 +83,6 @@ def topk_distillation_loss(logits, teacher_index, teacher_logit, temperature=1.0
     softmax at the same temperature: loss = sum_k q_k (log q_k - log p_k). The customary factor
     temperature**2 is left to the caller. A row without entries has loss 0 and no gradient. No gradient
     flows to the teacher. `vocab_start` / `gather_fn`: see `token_logprobs`."""
+    if gather_fn is None and native.use_native(logits):
+        return native.lib().topk_distillation_loss(logits, teacher_index, teacher_logit, temperature, vocab_start)
     return _DistillFn.apply(logits, teacher_index, teacher_logit, float(temperature), int(vocab_start), gather_fn)

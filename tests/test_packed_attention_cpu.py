@@ -81,7 +81,7 @@ def test_refusals():
                 lambda: ops.flash_attention_packed(q, k, v, layout, scale=0.0),
                 lambda: ops.flash_attention_packed(q, k, v, layout, scale=-1.0),
                 lambda: ops.flash_attention_packed(q, k, v, layout, scale=math.inf),
-                lambda: layout.query_tiles(True),
+                lambda: layout.work_lists(True),
                 lambda: raw.attention_packed_bwd(q[:, :2], q, k, v, q, None, layout)):
         with pytest.raises(ValueError):
             bad()

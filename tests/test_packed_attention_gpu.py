@@ -157,14 +157,31 @@ def test_no_documents():
     assert _check([], *empty, True)[0].shape == (0, 4, 64)
 
 
+def test_no_second_derivative():
+    q, k, v, do = (t.contiguous().requires_grad_(True) for t in _inputs([5], 4, 2, 64, torch.bfloat16))
+    out = ops.flash_attention_packed(q, k, v, ops.PackedLayout([5], device=DEV))
+    with pytest.raises(RuntimeError, match="differentiated"):
+        torch.autograd.grad(out, q, do, create_graph=True)
+
+
 def test_refusals_on_the_device():
     q, k, v, _ = _inputs([5], 4, 2, 64, torch.bfloat16)
     layout = ops.PackedLayout([5], device=DEV)
     for bad in (lambda: ops.flash_attention_packed(q, k, v, ops.PackedLayout([5])),
                 lambda: ops.flash_attention_packed(q.float(), k.float(), v.float(), layout),
                 lambda: ops.flash_attention_packed(q[..., :32], k[..., :32], v[..., :32], layout),
-                lambda: ops.flash_attention_packed(q, k, v.cpu(), layout)):
-        with pytest.raises(ValueError):
+                lambda: ops.flash_attention_packed(q, k, v.cpu(), layout),
+                lambda: ops.flash_attention_packed(q, k[:, :1], v, layout),
+                lambda: ops.flash_attention_packed(q[:, :3], k, v, layout),
+                lambda: ops.flash_attention_packed(q[:, :0], k, v, layout),
+                lambda: ops.flash_attention_packed(q[0], k, v, layout),
+                lambda: ops.flash_attention_packed(q[..., :0], k[..., :0], v[..., :0], layout),
+                lambda: ops.flash_attention_packed(q, k, v, ops.PackedLayout([4], device=DEV)),
+                lambda: ops.flash_attention_packed(q, k, v, layout, scale=0.0),
+                lambda: ops.flash_attention_packed(q, k, v, layout, scale=math.nan),
+                lambda: raw.attention_packed_bwd(q[:, :2], q, k, v, q, None, layout),
+                lambda: raw.attention_packed_bwd(q[:, :2], q, k, v, q, torch.zeros(4, 5, device=DEV), layout)):
+        with pytest.raises((ValueError, TypeError)):
             bad()
 
 

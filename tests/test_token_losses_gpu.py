@@ -256,6 +256,21 @@ def test_refusals_on_the_device():
     for bad in (lambda: ops.token_logprobs(z, t.cpu()), lambda: ops.token_logprobs(z.double(), t),
                 lambda: ops.topk_distillation_loss(z, index.cpu(), logit),
                 lambda: ops.topk_distillation_loss(z, index, logit.cpu()),
-                lambda: raw.distill_step(z, index, logit, torch.ones(3))):
+                lambda: raw.distill_step(z, index, logit, torch.ones(3)),
+                lambda: ops.token_logprobs(z[0], t), lambda: ops.token_logprobs(z.int(), t),
+                lambda: ops.token_logprobs(z, t.int()), lambda: ops.token_logprobs(z, t[:2]),
+                lambda: ops.token_logprobs(z, t, top_k=12), lambda: ops.token_logprobs(z, t, top_k=-1),
+                lambda: ops.token_logprobs(torch.randn(3, 500, device=DEV), t, top_k=129),
+                lambda: ops.token_logprobs(z, t, temperature=0.0), lambda: ops.token_logprobs(z, t, temperature=math.nan),
+                lambda: ops.token_logprobs(z[:, :0], t),
+                lambda: ops.token_logprobs(z, t, 2, 1.0, 0, lambda x: x),
+                lambda: ops.topk_distillation_loss(z, index, logit[:, :1]),
+                lambda: ops.topk_distillation_loss(z, index.int(), logit),
+                lambda: ops.topk_distillation_loss(z, index, logit.half()),
+                lambda: ops.topk_distillation_loss(z, index[:, :0], logit[:, :0]),
+                lambda: ops.topk_distillation_loss(z, index.new_zeros(3, 513), logit.new_zeros(3, 513)),
+                lambda: raw.distill_step(z, index, logit, torch.ones(2, device=DEV)),
+                lambda: raw.distill_step(z, index, logit, torch.ones(3, device=DEV), out=z.half()),
+                lambda: raw.distill_step(z[:, :10], index, logit, torch.ones(3, device=DEV), out=z[:, 1:])):
         with pytest.raises(ValueError):
             bad()
