@@ -94,6 +94,40 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
+// Two fp32 lanes per instruction: the kernels below issue four to five instructions per logit, and
+// these pairs are what keeps that below the time DRAM needs.
+struct Pair {
+  unsigned long long v;
+};
+__device__ __forceinline__ Pair pair(float x, float y) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void split(Pair p, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p.v));
+}
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ Pair exp2_pair(Pair t) {
+  float x, y;
+  split(t, x, y);
+  return pair(exp2f(x), exp2f(y));
+}
+
 // Running (maximum, sum of exponentials, sum of exponential * exponent). `mu` is what is subtracted:
 // the maximum, or 0 while only -inf has been seen (so that -inf - mu stays -inf and not NaN).
 template <bool kEntropy> struct Running {
@@ -120,21 +154,83 @@ template <bool kEntropy> struct Running {
     l += e;
     if (kEntropy) a = fmaf(e, fmaxf(t, -1000.f), a);   // e is 0 far above -1000; -inf * 0 must not appear
   }
+  // N vectors of one thread at once. The sum of e * t goes without the clamp of add(); where a masked
+  // (-inf) logit has made it NaN, the group's share of it is taken again with it.
+  template <typename T, int N>
+  __device__ __forceinline__ void add_group(const uint4 (&u)[N], float s2);
 };
 
-template <typename T>
+template <typename T, bool kNan = false>
 __device__ __forceinline__ float max_of(const uint4& u) {
   if constexpr (std::is_same<T, __nv_bfloat16>::value) {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
-    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-    return fmaxf(__low2float(m), __high2float(m));
+    const __nv_bfloat162 m = kNan ? __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]))
+                                  : __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    const __nv_bfloat16 r = kNan ? __hmax_nan(__low2bfloat16(m), __high2bfloat16(m))
+                                 : __hmax(__low2bfloat16(m), __high2bfloat16(m));
+    return __bfloat162float(r);
   } else if constexpr (std::is_same<T, __half>::value) {
     const __half2* h = reinterpret_cast<const __half2*>(&u);
-    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-    return fmaxf(__low2float(m), __high2float(m));
+    const __half2 m = kNan ? __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]))
+                           : __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    const __half r = kNan ? __hmax_nan(__low2half(m), __high2half(m)) : __hmax(__low2half(m), __high2half(m));
+    return __half2float(r);
   } else {
-    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)),
-                 fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+    const float m = fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)),
+                          fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+    static_assert(!kNan, "fp32 elements are looked at one by one where NaN counts");
+    return m;
+  }
+}
+
+// A vector as pairs of fp32.
+template <typename T>
+__device__ __forceinline__ void unpack_pairs(const uint4& u, Pair (&p)[kVec<T> / 2]) {
+  float f[kVec<T>];
+  unpack<T>(u, f);
+#pragma unroll
+  for (int i = 0; i < kVec<T> / 2; ++i) p[i] = pair(f[2 * i], f[2 * i + 1]);
+}
+
+template <bool kEntropy>
+template <typename T, int N>
+__device__ __forceinline__ void Running<kEntropy>::add_group(const uint4 (&u)[N], float s2) {
+  float m = max_of<T>(u[0]);
+#pragma unroll
+  for (int k = 1; k < N; ++k) m = fmaxf(m, max_of<T>(u[k]));
+  if (m > mx) raise(m, s2);
+  const Pair neg = pair(-mu(), -mu()), scale = pair(s2, s2);
+  Pair lsum = pair(0.f, 0.f), asum = lsum;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    Pair z[kVec<T> / 2];
+    unpack_pairs<T>(u[k], z);
+#pragma unroll
+    for (int j = 0; j < kVec<T> / 2; ++j) {
+      const Pair t = (z[j] + neg) * scale, e = exp2_pair(t);
+      lsum = lsum + e;
+      if (kEntropy) asum = fma2(e, t, asum);
+    }
+  }
+  float x, y;
+  split(lsum, x, y);
+  l += x + y;
+  if (kEntropy) {
+    split(asum, x, y);
+    float part = x + y;
+    if (part != part) {
+      Running<true> again;
+      const float base = mu();
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        float f[kVec<T>];
+        unpack<T>(u[k], f);
+#pragma unroll
+        for (int j = 0; j < kVec<T>; ++j) again.add(f[j], base, s2);
+      }
+      part = again.a;
+    }
+    a += part;
   }
 }
 
@@ -158,28 +254,11 @@ __device__ __forceinline__ Running<kEntropy> scan_row(const Row<T>& r, float s2)
     uint4 u[kUnroll];
 #pragma unroll
     for (int k = 0; k < kUnroll; ++k) u[k] = v[c + k * step];
-    float m = max_of<T>(u[0]);
-#pragma unroll
-    for (int k = 1; k < kUnroll; ++k) m = fmaxf(m, max_of<T>(u[k]));
-    if (m > run.mx) run.raise(m, s2);
-    const float mu = run.mu();
-#pragma unroll
-    for (int k = 0; k < kUnroll; ++k) {
-      float f[kVec<T>];
-      unpack<T>(u[k], f);
-#pragma unroll
-      for (int j = 0; j < kVec<T>; ++j) run.add(f[j], mu, s2);
-    }
+    run.template add_group<T>(u, s2);
   }
   for (; c < r.nvec; c += step) {
-    const uint4 u = v[c];
-    const float m = max_of<T>(u);
-    if (m > run.mx) run.raise(m, s2);
-    const float mu = run.mu();
-    float f[kVec<T>];
-    unpack<T>(u, f);
-#pragma unroll
-    for (int j = 0; j < kVec<T>; ++j) run.add(f[j], mu, s2);
+    const uint4 u[1] = {v[c]};
+    run.template add_group<T>(u, s2);
   }
   return run;
 }
@@ -217,8 +296,7 @@ __device__ __forceinline__ Running<kEntropy> block_merge(Running<kEntropy> run, 
 // ---------------------------------------------------------------------------------------------
 // Exact selection without keeping the row: the k-th largest of the threads' maxima is a lower bound
 // of the k-th largest element, and only threads whose own maximum reaches it can hold candidates.
-// Those few threads read their share again (it is still in L2); all others are done. The candidates
-// carry (key, ~token id), so ties go to the lowest id and the order in which they were found does
+// The block reads the shares of those few threads again (they are still in L2). The candidates carry (key, ~token id), so ties go to the lowest id and the order in which they were found does
 // not matter. Where the bound is loose (a row of equal values, masked rows) and more than
 // kCandidates elements reach it, the exact k-th key and then the id up to which ties are taken are
 // found by bisection over their bits, with counts over the whole row.
@@ -242,7 +320,8 @@ __device__ __forceinline__ void for_own(const Row<T>& r, F f) {   // f(value, lo
 struct SelectSmem {
   unsigned long long cand[kCandidates];
   unsigned long long best[kMaxTopAlternatives];
-  int count;
+  short owner[1024];
+  int count, owners;
   int sums[32];
 };
 
@@ -271,25 +350,41 @@ __device__ void select_top(const Row<T>& r, int k, float thread_max, bool thread
   uint32_t bound = 0;
   // 16-bit types widen exactly: their keys differ in the upper bits only (the lower 16 are all 0 for
   // positive, all 1 for negative values), for fp16 in the upper 19
-  constexpr int kLow = std::is_same<T, __nv_bfloat16>::value ? 16 : 0;
+  constexpr int kLow = std::is_same<T, __nv_bfloat16>::value ? 16 : std::is_same<T, __half>::value ? 13 : 0;
   for (int bit = 31; bit >= kLow; --bit) {
     const uint32_t cand = bound | (1u << bit);
     if (__syncthreads_count(own >= cand) >= k) bound = cand;
   }
-  if (tid == 0) s.count = 0;
+  if (tid == 0) s.count = s.owners = 0;
   __syncthreads();
+  auto take = [&](float z, int id) {
+    const uint32_t key = order_key(z);
+    if (key >= bound) {
+      const int at = atomicAdd(&s.count, 1);
+      if (at < kCandidates) s.cand[at] = (static_cast<unsigned long long>(key) << 32) | (0xffffffffu - id);
+    }
+  };
   if (own >= bound && any) {
-    for_own(r, [&](float z, int id) {
-      const uint32_t key = order_key(z);
-      if (key >= bound) {
-        const int at = atomicAdd(&s.count, 1);
-        if (at < kCandidates) s.cand[at] = (static_cast<unsigned long long>(key) << 32) | (0xffffffffu - id);
-      }
-    });
+    s.owner[atomicAdd(&s.owners, 1)] = static_cast<short>(tid);
+    if (tid < r.head) take(HalfTraits<T>::to_f(r.p[tid]), tid);
+    if (r.tail() + tid < r.n) take(HalfTraits<T>::to_f(r.p[r.tail() + tid]), r.tail() + tid);
+  }
+  __syncthreads();
+  // the block reads the owners' vectors together
+  const int step = blockDim.x, per = (r.nvec + step - 1) / step, items = s.owners * per;
+  for (int i = tid; i < items; i += step) {
+    const int c = s.owner[i / per] + (i % per) * step;
+    if (c >= r.nvec) continue;
+    const uint4 u = r.vec()[c];
+    if (sizeof(T) == 2 && order_key(max_of<T, sizeof(T) == 2>(u)) < bound) continue;   // (an fp32 maximum may flush)
+    float x[kVec<T>];
+    unpack<T>(u, x);
+#pragma unroll
+    for (int j = 0; j < kVec<T>; ++j) take(x[j], r.head + c * kVec<T> + j);
   }
   __syncthreads();
   int found = s.count;
-  if (found > kCandidates) {
+  if (found > kCandidates || found < k) {   // (fewer than k cannot be; the exact way needs no such argument)
     uint32_t kth = 0;
     for (int bit = 31; bit >= 0; --bit) {
       const uint32_t cand = kth | (1u << bit);
@@ -437,15 +532,68 @@ struct Listed {
 };
 
 struct DenseTerm {
-  float mu, s2, inv_l, log2_l, a, b;   // a, b already hold the factor 1 / temperature
+  float mu, s2;
+  float a, b;       // value = 2^t (a + b t), t = (z - mu) s2; 1 / L, ln L, ln 2 and 1 / temperature are in a and b
+  float low;        // kLog: logits are raised to this before (2^t is 0 there all the same), -inf if not possible
+
+  // p (A + B log p) with p = 2^t / l
+  __device__ __forceinline__ static DenseTerm of(float mu, float l, float s2, float A, float B) {
+    DenseTerm f;
+    f.mu = mu;
+    f.s2 = s2;
+    const float inv = 1.0f / l;
+    f.a = (B == 0.f ? A : A - B * (kLn2 * log2f(l))) * inv;
+    f.b = B * kLn2 * inv;
+    // 2^t is 0 in fp32 below t = -150: a floor under the masked logits that lies below that keeps t
+    // finite, as 0 * -inf would be NaN. -60000 is one for fp16 and every ordinary row.
+    f.low = (mu + 60000.f) * s2 > 200.f ? -60000.f : -INFINITY;
+    return f;
+  }
   template <bool kLog> __device__ __forceinline__ float at(float z) const {
-    const float t = (z - mu) * s2, p = exp2f(t) * inv_l;
+    const float t = (z - mu) * s2, e = exp2f(t);
+    return kLog ? e * fmaf(b, fmaxf(t, -1000.f), a) : e * a;
+  }
+  // all logits of a vector that are at least `low`
+  template <bool kLog> __device__ __forceinline__ Pair at(Pair z) const {
+    const Pair t = (z + pair(-mu, -mu)) * pair(s2, s2), e = exp2_pair(t);
+    return kLog ? e * fma2(pair(b, b), t, pair(a, a)) : e * pair(a, a);
+  }
+  template <typename T, bool kLog> __device__ __forceinline__ uint4 at(uint4 u) const {
     if constexpr (kLog) {
-      // b scales p log p; p is 0 far above -1000, where log p may be -inf
-      return p * fmaf(b, fmaxf(t - log2_l, -1000.f) * kLn2, a);
-    } else {
-      return p * a;
+      if (low == -INFINITY) {
+        float x[kVec<T>];
+        unpack<T>(u, x);
+#pragma unroll
+        for (int j = 0; j < kVec<T>; ++j) x[j] = at<true>(x[j]);
+        return repack<T>(x);
+      }
+      u = raise<T>(u, low);
     }
+    Pair z[kVec<T> / 2];
+    unpack_pairs<T>(u, z);
+    float x[kVec<T>];
+#pragma unroll
+    for (int j = 0; j < kVec<T> / 2; ++j) split(at<kLog>(z[j]), x[2 * j], x[2 * j + 1]);
+    return repack<T>(x);
+  }
+  template <typename T> __device__ __forceinline__ static uint4 raise(uint4 u, float low) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
+      const __nv_bfloat162 f = __float2bfloat162_rn(low);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[i] = __hmax2(h[i], f);
+    } else if constexpr (std::is_same<T, __half>::value) {
+      __half2* h = reinterpret_cast<__half2*>(&u);
+      const __half2 f = __float2half2_rn(low);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[i] = __hmax2(h[i], f);
+    } else {
+      u.x = __float_as_uint(fmaxf(__uint_as_float(u.x), low));
+      u.y = __float_as_uint(fmaxf(__uint_as_float(u.y), low));
+      u.z = __float_as_uint(fmaxf(__uint_as_float(u.z), low));
+      u.w = __float_as_uint(fmaxf(__uint_as_float(u.w), low));
+    }
+    return u;
   }
 };
 
@@ -456,9 +604,9 @@ __device__ __forceinline__ void write_grad(const Row<T>& r, T* __restrict__ d, c
     if (li.id[i] >= 0) li.z[i] = HalfTraits<T>::to_f(r.p[li.id[i]]);
   __syncthreads();
   if (((reinterpret_cast<uintptr_t>(r.p) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0) {
-    for (int i = tid; i < r.head; i += step) d[i] = HalfTraits<T>::from_f(f.at<kLog>(HalfTraits<T>::to_f(r.p[i])));
+    for (int i = tid; i < r.head; i += step) d[i] = HalfTraits<T>::from_f(f.template at<kLog>(HalfTraits<T>::to_f(r.p[i])));
     for (int i = r.tail() + tid; i < r.n; i += step)
-      d[i] = HalfTraits<T>::from_f(f.at<kLog>(HalfTraits<T>::to_f(r.p[i])));
+      d[i] = HalfTraits<T>::from_f(f.template at<kLog>(HalfTraits<T>::to_f(r.p[i])));
     const uint4* v = r.vec();
     uint4* o = reinterpret_cast<uint4*>(d + r.head);
     int c = tid;
@@ -467,23 +615,11 @@ __device__ __forceinline__ void write_grad(const Row<T>& r, T* __restrict__ d, c
 #pragma unroll
       for (int k = 0; k < kUnroll; ++k) u[k] = v[c + k * step];
 #pragma unroll
-      for (int k = 0; k < kUnroll; ++k) {
-        float x[kVec<T>];
-        unpack<T>(u[k], x);
-#pragma unroll
-        for (int j = 0; j < kVec<T>; ++j) x[j] = f.at<kLog>(x[j]);
-        o[c + k * step] = repack<T>(x);
-      }
+      for (int k = 0; k < kUnroll; ++k) o[c + k * step] = f.template at<T, kLog>(u[k]);
     }
-    for (; c < r.nvec; c += step) {
-      float x[kVec<T>];
-      unpack<T>(v[c], x);
-#pragma unroll
-      for (int j = 0; j < kVec<T>; ++j) x[j] = f.at<kLog>(x[j]);
-      o[c] = repack<T>(x);
-    }
+    for (; c < r.nvec; c += step) o[c] = f.template at<T, kLog>(v[c]);
   } else {   // rows of logits and gradient at different offsets from a 16-byte boundary
-    for (int i = tid; i < r.n; i += step) d[i] = HalfTraits<T>::from_f(f.at<kLog>(HalfTraits<T>::to_f(r.p[i])));
+    for (int i = tid; i < r.n; i += step) d[i] = HalfTraits<T>::from_f(f.template at<kLog>(HalfTraits<T>::to_f(r.p[i])));
   }
   __syncthreads();
   for (int i = tid; i < n; i += step) {
@@ -494,7 +630,7 @@ __device__ __forceinline__ void write_grad(const Row<T>& r, T* __restrict__ d, c
     if (!first) continue;
     float w = li.w[i];
     for (int j = i + 1; j < n; ++j) w += li.id[j] == id ? li.w[j] : 0.f;
-    d[id] = HalfTraits<T>::from_f(f.at<kLog>(li.z[i]) + w);
+    d[id] = HalfTraits<T>::from_f(f.template at<kLog>(li.z[i]) + w);
   }
 }
 
@@ -548,17 +684,8 @@ __global__ void token_scores_bwd_kernel(const T* z, int64_t ld, int vocab, int64
     write_zero(d, vocab);
     return;
   }
-  DenseTerm f;
-  f.mu = stats[2 * row];
-  f.s2 = inv_t * kLog2e;
-  f.inv_l = 1.0f / stats[2 * row + 1];
-  f.log2_l = log2f(stats[2 * row + 1]);
-  f.a = -(gr + usum) * inv_t;
-  f.b = 0.f;
-  if (kLog) {
-    f.a -= hr * entropy[row] * inv_t;
-    f.b = -hr * inv_t;
-  }
+  const float A = -(gr + usum + (kLog ? hr * entropy[row] : 0.f)) * inv_t;
+  const DenseTerm f = DenseTerm::of(stats[2 * row], stats[2 * row + 1], inv_t * kLog2e, A, kLog ? -hr * inv_t : 0.f);
   write_grad<T, kLog>(r, d, f, li, 1 + extra);
 }
 
@@ -739,7 +866,7 @@ __global__ void distill_bwd_kernel(const T* z, int64_t ld, int vocab, int64_t v0
     return;
   }
   for (int i = threadIdx.x; i < t.k; i += blockDim.x) li.w[i] *= -g;
-  const DenseTerm f{stats[2 * row], inv_t * kLog2e, 1.0f / stats[2 * row + 1], 0.f, g * tr.mass, 0.f};
+  const DenseTerm f = DenseTerm::of(stats[2 * row], stats[2 * row + 1], inv_t * kLog2e, g * tr.mass, 0.f);
   write_grad<T, false>(r, d, f, li, t.k);
 }
 
@@ -772,7 +899,7 @@ __global__ void distill_step_kernel(const T* z, int64_t ld, int vocab, int64_t v
   }
   __syncthreads();
   for (int i = threadIdx.x; i < t.k; i += blockDim.x) li.w[i] *= -g;
-  const DenseTerm f{mu, s2, 1.0f / all.l, 0.f, g * tr.mass, 0.f};
+  const DenseTerm f = DenseTerm::of(mu, all.l, s2, g * tr.mass, 0.f);
   write_grad<T, false>(r, d, f, li, t.k);
 }
 
