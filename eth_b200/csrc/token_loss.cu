@@ -128,6 +128,38 @@ __device__ __forceinline__ Pair exp2_pair(Pair t) {
   return pair(exp2f(x), exp2f(y));
 }
 
+// A masked (-inf) logit has 2^t = 0 and t = -inf, whose product would be NaN. Where a sum or gradient
+// needs 2^t * t, logits below kFloor are raised to it, which leaves 2^t at 0 (it is 0 in fp32 below
+// t = -150) and t finite. Rows that lie so low themselves, or a temperature so high, that this does
+// not hold take a clamp per element instead.
+constexpr float kFloor = -60000.f;   // exact enough in every type, fp16 included
+__device__ __forceinline__ bool has_floor(float mu, float s2) { return (mu - kFloor) * s2 > 200.f; }
+__device__ __forceinline__ uint32_t max_nan(uint32_t x, float low) {
+  uint32_t r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(__float_as_uint(low)));
+  return r;
+}
+template <typename T>   // NaN stays
+__device__ __forceinline__ uint4 at_least(uint4 u, float low) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
+    const __nv_bfloat162 f = __float2bfloat162_rn(low);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __hmax2_nan(h[i], f);
+  } else if constexpr (std::is_same<T, __half>::value) {
+    __half2* h = reinterpret_cast<__half2*>(&u);
+    const __half2 f = __float2half2_rn(low);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __hmax2_nan(h[i], f);
+  } else {
+    u.x = max_nan(u.x, low);
+    u.y = max_nan(u.y, low);
+    u.z = max_nan(u.z, low);
+    u.w = max_nan(u.w, low);
+  }
+  return u;
+}
+
 // Running (maximum, sum of exponentials, sum of exponential * exponent). `mu` is what is subtracted:
 // the maximum, or 0 while only -inf has been seen (so that -inf - mu stays -inf and not NaN).
 template <bool kEntropy> struct Running {
@@ -154,8 +186,7 @@ template <bool kEntropy> struct Running {
     l += e;
     if (kEntropy) a = fmaf(e, fmaxf(t, -1000.f), a);   // e is 0 far above -1000; -inf * 0 must not appear
   }
-  // N vectors of one thread at once. The sum of e * t goes without the clamp of add(); where a masked
-  // (-inf) logit has made it NaN, the group's share of it is taken again with it.
+  // N vectors of one thread at once.
   template <typename T, int N>
   __device__ __forceinline__ void add_group(const uint4 (&u)[N], float s2);
 };
@@ -192,6 +223,16 @@ __device__ __forceinline__ void unpack_pairs(const uint4& u, Pair (&p)[kVec<T> /
   for (int i = 0; i < kVec<T> / 2; ++i) p[i] = pair(f[2 * i], f[2 * i + 1]);
 }
 
+template <typename T>
+__device__ __noinline__ Running<true> add_clamped(Running<true> run, uint4 u, float s2) {
+  float f[kVec<T>];
+  unpack<T>(u, f);
+  const float mu = run.mu();
+#pragma unroll
+  for (int j = 0; j < kVec<T>; ++j) run.add(f[j], mu, s2);
+  return run;
+}
+
 template <bool kEntropy>
 template <typename T, int N>
 __device__ __forceinline__ void Running<kEntropy>::add_group(const uint4 (&u)[N], float s2) {
@@ -199,12 +240,20 @@ __device__ __forceinline__ void Running<kEntropy>::add_group(const uint4 (&u)[N]
 #pragma unroll
   for (int k = 1; k < N; ++k) m = fmaxf(m, max_of<T>(u[k]));
   if (m > mx) raise(m, s2);
-  const Pair neg = pair(-mu(), -mu()), scale = pair(s2, s2);
+  const float base = mu();
+  if constexpr (kEntropy) {
+    if (!has_floor(base, s2)) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) *this = add_clamped<T>(*this, u[k], s2);
+      return;
+    }
+  }
+  const Pair neg = pair(-base, -base), scale = pair(s2, s2);
   Pair lsum = pair(0.f, 0.f), asum = lsum;
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     Pair z[kVec<T> / 2];
-    unpack_pairs<T>(u[k], z);
+    unpack_pairs<T>(kEntropy ? at_least<T>(u[k], kFloor) : u[k], z);
 #pragma unroll
     for (int j = 0; j < kVec<T> / 2; ++j) {
       const Pair t = (z[j] + neg) * scale, e = exp2_pair(t);
@@ -217,20 +266,7 @@ __device__ __forceinline__ void Running<kEntropy>::add_group(const uint4 (&u)[N]
   l += x + y;
   if (kEntropy) {
     split(asum, x, y);
-    float part = x + y;
-    if (part != part) {
-      Running<true> again;
-      const float base = mu();
-#pragma unroll
-      for (int k = 0; k < N; ++k) {
-        float f[kVec<T>];
-        unpack<T>(u[k], f);
-#pragma unroll
-        for (int j = 0; j < kVec<T>; ++j) again.add(f[j], base, s2);
-      }
-      part = again.a;
-    }
-    a += part;
+    a += x + y;
   }
 }
 
@@ -256,10 +292,16 @@ __device__ __forceinline__ Running<kEntropy> scan_row(const Row<T>& r, float s2)
     for (int k = 0; k < kUnroll; ++k) u[k] = v[c + k * step];
     run.template add_group<T>(u, s2);
   }
-  for (; c < r.nvec; c += step) {
-    const uint4 u[1] = {v[c]};
-    run.template add_group<T>(u, s2);
-  }
+  uint4 u[kUnroll];   // the rest: all loads first, too
+#pragma unroll
+  for (int k = 0; k < kUnroll; ++k)
+    if (c + k * step < r.nvec) u[k] = v[c + k * step];
+#pragma unroll
+  for (int k = 0; k < kUnroll; ++k)
+    if (c + k * step < r.nvec) {
+      const uint4 one_vec[1] = {u[k]};
+      run.template add_group<T>(one_vec, s2);
+    }
   return run;
 }
 
@@ -267,28 +309,29 @@ __device__ __forceinline__ Running<kEntropy> scan_row(const Row<T>& r, float s2)
 template <bool kEntropy>
 __device__ __forceinline__ Running<kEntropy> block_merge(Running<kEntropy> run, float s2, float* red) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  auto merge = [&](Running<kEntropy> x) {
-    const float m = warp_max(x.mx);
-    x.rebase(m, s2);
-    x.mx = m;
-    x.l = warp_sum(x.l);
-    if (kEntropy) x.a = warp_sum(x.a);
-    return x;
-  };
-  run = merge(run);
+  const float m = warp_max(run.mx);
+  run.rebase(m, s2);
+  run.mx = m;
+  run.l = warp_sum(run.l);
+  if (kEntropy) run.a = warp_sum(run.a);
   if (lane == 0) {
     red[warp] = run.mx;
     red[32 + warp] = run.l;
     if (kEntropy) red[64 + warp] = run.a;
   }
   __syncthreads();
-  Running<kEntropy> x;
-  if (lane < nw) {
-    x.mx = red[lane];
-    x.l = red[32 + lane];
-    if (kEntropy) x.a = red[64 + lane];
+  Running<kEntropy> all;
+  for (int w = 0; w < nw; ++w) all.mx = fmaxf(all.mx, red[w]);
+  for (int w = 0; w < nw; ++w) {   // the same order in every thread: the same bits
+    Running<kEntropy> x;
+    x.mx = red[w];
+    x.l = red[32 + w];
+    if (kEntropy) x.a = red[64 + w];
+    x.rebase(all.mx, s2);
+    all.l += x.l;
+    if (kEntropy) all.a += x.a;
   }
-  return merge(x);
+  return all;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -317,10 +360,10 @@ __device__ __forceinline__ void for_own(const Row<T>& r, F f) {   // f(value, lo
   }
 }
 
-struct SelectSmem {
+template <int kThreads> struct SelectSmem {
   unsigned long long cand[kCandidates];
   unsigned long long best[kMaxTopAlternatives];
-  short owner[1024];
+  short owner[kThreads];
   int count, owners;
   int sums[32];
 };
@@ -335,8 +378,8 @@ __device__ __forceinline__ int block_count(int v, int* sums) {
 }
 
 // s.best[0..k) = the k largest (key << 32 | ~id), in falling order. Needs k <= blockDim.x, k <= r.n.
-template <typename T>
-__device__ void select_top(const Row<T>& r, int k, float thread_max, bool thread_nan, SelectSmem& s) {
+template <typename T, int kThreads>
+__device__ void select_top(const Row<T>& r, int k, float thread_max, bool thread_nan, SelectSmem<kThreads>& s) {
   const int tid = threadIdx.x;
   uint32_t own = 0;                          // below the key of -inf: a thread without elements
   const bool any = tid < r.head || r.tail() + tid < r.n || tid < r.nvec;
@@ -427,22 +470,27 @@ __device__ void select_top(const Row<T>& r, int k, float thread_max, bool thread
 // ---------------------------------------------------------------------------------------------
 // token log-probabilities, entropy, alternatives: forward
 // ---------------------------------------------------------------------------------------------
-template <typename T, bool kTop>
-__global__ void token_scores_kernel(const T* __restrict__ z, int64_t ld, int vocab, int64_t v0,
-                                    const int64_t* __restrict__ tokens, int top_k, float inv_t, TokenScoresOut out,
-                                    float* __restrict__ partial) {
+// Bound by reading the logits. Rows are many and each CTA waits at its end (merge, selection), so small
+// CTAs of 128 threads keep most of an SM's warps loading; fewer registers than 50 would spill, more
+// leave too few warps. 8192 x 50304 bf16 without alternatives: 134 us = 6.1 TB/s with 10 CTAs of 128
+// threads per SM, 139 with 6 of 256, 155 with 3 of 512.
+template <typename T, bool kTop, int kThreads, int kPerSm>
+__global__ void __launch_bounds__(kThreads, kPerSm)
+token_scores_kernel(const T* __restrict__ z, int64_t ld, int vocab, int64_t v0, const int64_t* __restrict__ tokens,
+                    int top_k, float inv_t, TokenScoresOut out, float* __restrict__ partial) {
   __shared__ float red[96];
-  __shared__ SelectSmem sel;
+  __shared__ SelectSmem<kThreads> sel;
   const int64_t row = blockIdx.x;
   const Row<T> r(z + row * ld, vocab);
   const float s2 = inv_t * kLog2e;
+  const int64_t t = threadIdx.x == 0 ? tokens[row] : -1;   // on its way while the row is read
   const Running<true> own = scan_row<T, true>(r, s2);
   const Running<true> all = block_merge<true>(own, s2, red);
   const float mu = all.mu();
   const float log_l = kLn2 * log2f(all.l);
   const int width = 4 + 2 * top_k;
   if (threadIdx.x == 0) {
-    const int64_t t = tokens[row], local = t - v0;
+    const int64_t local = t - v0;
     const bool here = t >= 0 && local >= 0 && local < vocab;
     const float zt = here ? HalfTraits<T>::to_f(r.p[local]) : CUDART_NAN_F;
     if (partial != nullptr) {
@@ -534,7 +582,7 @@ struct Listed {
 struct DenseTerm {
   float mu, s2;
   float a, b;       // value = 2^t (a + b t), t = (z - mu) s2; 1 / L, ln L, ln 2 and 1 / temperature are in a and b
-  float low;        // kLog: logits are raised to this before (2^t is 0 there all the same), -inf if not possible
+  bool floor;       // kLog: masked logits may be raised to kFloor, see has_floor
 
   // p (A + B log p) with p = 2^t / l
   __device__ __forceinline__ static DenseTerm of(float mu, float l, float s2, float A, float B) {
@@ -544,30 +592,28 @@ struct DenseTerm {
     const float inv = 1.0f / l;
     f.a = (B == 0.f ? A : A - B * (kLn2 * log2f(l))) * inv;
     f.b = B * kLn2 * inv;
-    // 2^t is 0 in fp32 below t = -150: a floor under the masked logits that lies below that keeps t
-    // finite, as 0 * -inf would be NaN. -60000 is one for fp16 and every ordinary row.
-    f.low = (mu + 60000.f) * s2 > 200.f ? -60000.f : -INFINITY;
+    f.floor = has_floor(mu, s2);
     return f;
   }
   template <bool kLog> __device__ __forceinline__ float at(float z) const {
     const float t = (z - mu) * s2, e = exp2f(t);
     return kLog ? e * fmaf(b, fmaxf(t, -1000.f), a) : e * a;
   }
-  // all logits of a vector that are at least `low`
+  // logits that are not -inf
   template <bool kLog> __device__ __forceinline__ Pair at(Pair z) const {
     const Pair t = (z + pair(-mu, -mu)) * pair(s2, s2), e = exp2_pair(t);
     return kLog ? e * fma2(pair(b, b), t, pair(a, a)) : e * pair(a, a);
   }
   template <typename T, bool kLog> __device__ __forceinline__ uint4 at(uint4 u) const {
     if constexpr (kLog) {
-      if (low == -INFINITY) {
+      if (!floor) {
         float x[kVec<T>];
         unpack<T>(u, x);
 #pragma unroll
         for (int j = 0; j < kVec<T>; ++j) x[j] = at<true>(x[j]);
         return repack<T>(x);
       }
-      u = raise<T>(u, low);
+      u = at_least<T>(u, kFloor);
     }
     Pair z[kVec<T> / 2];
     unpack_pairs<T>(u, z);
@@ -576,50 +622,33 @@ struct DenseTerm {
     for (int j = 0; j < kVec<T> / 2; ++j) split(at<kLog>(z[j]), x[2 * j], x[2 * j + 1]);
     return repack<T>(x);
   }
-  template <typename T> __device__ __forceinline__ static uint4 raise(uint4 u, float low) {
-    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-      __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
-      const __nv_bfloat162 f = __float2bfloat162_rn(low);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) h[i] = __hmax2(h[i], f);
-    } else if constexpr (std::is_same<T, __half>::value) {
-      __half2* h = reinterpret_cast<__half2*>(&u);
-      const __half2 f = __float2half2_rn(low);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) h[i] = __hmax2(h[i], f);
-    } else {
-      u.x = __float_as_uint(fmaxf(__uint_as_float(u.x), low));
-      u.y = __float_as_uint(fmaxf(__uint_as_float(u.y), low));
-      u.z = __float_as_uint(fmaxf(__uint_as_float(u.z), low));
-      u.w = __float_as_uint(fmaxf(__uint_as_float(u.w), low));
-    }
-    return u;
-  }
 };
 
-template <typename T, bool kLog>
-__device__ __forceinline__ void write_grad(const Row<T>& r, T* __restrict__ d, const DenseTerm& f, Listed& li, int n) {
+// The whole gradient of a row. The list's logits have been staged before (li.z), behind a barrier.
+// kLast: the row's logits are read for the last time.
+template <typename T, bool kLog, bool kLast>
+__device__ __forceinline__ void write_grad(const Row<T>& r, T* __restrict__ d, const DenseTerm& f, const Listed& li,
+                                           int n) {
   const int tid = threadIdx.x, step = blockDim.x;
-  for (int i = tid; i < n; i += step)
-    if (li.id[i] >= 0) li.z[i] = HalfTraits<T>::to_f(r.p[li.id[i]]);
-  __syncthreads();
   if (((reinterpret_cast<uintptr_t>(r.p) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0) {
-    for (int i = tid; i < r.head; i += step) d[i] = HalfTraits<T>::from_f(f.template at<kLog>(HalfTraits<T>::to_f(r.p[i])));
+    for (int i = tid; i < r.head; i += step)
+      d[i] = HalfTraits<T>::from_f(f.template at<kLog>(HalfTraits<T>::to_f(r.p[i])));
     for (int i = r.tail() + tid; i < r.n; i += step)
       d[i] = HalfTraits<T>::from_f(f.template at<kLog>(HalfTraits<T>::to_f(r.p[i])));
     const uint4* v = r.vec();
     uint4* o = reinterpret_cast<uint4*>(d + r.head);
-    int c = tid;
-    for (; c + (kUnroll - 1) * step < r.nvec; c += kUnroll * step) {
+    for (int c = tid; c < r.nvec; c += kUnroll * step) {
       uint4 u[kUnroll];
 #pragma unroll
-      for (int k = 0; k < kUnroll; ++k) u[k] = v[c + k * step];
+      for (int k = 0; k < kUnroll; ++k)
+        if (c + k * step < r.nvec) u[k] = kLast ? __ldcs(v + c + k * step) : v[c + k * step];
 #pragma unroll
-      for (int k = 0; k < kUnroll; ++k) o[c + k * step] = f.template at<T, kLog>(u[k]);
+      for (int k = 0; k < kUnroll; ++k)
+        if (c + k * step < r.nvec) __stcs(o + c + k * step, f.template at<T, kLog>(u[k]));
     }
-    for (; c < r.nvec; c += step) o[c] = f.template at<T, kLog>(v[c]);
   } else {   // rows of logits and gradient at different offsets from a 16-byte boundary
-    for (int i = tid; i < r.n; i += step) d[i] = HalfTraits<T>::from_f(f.template at<kLog>(HalfTraits<T>::to_f(r.p[i])));
+    for (int i = tid; i < r.n; i += step)
+      d[i] = HalfTraits<T>::from_f(f.template at<kLog>(HalfTraits<T>::to_f(r.p[i])));
   }
   __syncthreads();
   for (int i = tid; i < n; i += step) {
@@ -663,15 +692,19 @@ __global__ void token_scores_bwd_kernel(const T* z, int64_t ld, int vocab, int64
     for (int i = threadIdx.x; i < extra; i += 32) {
       const float w = u[row * top_k + i];
       const int64_t id = top_index[row * top_k + i] - v0;
-      li.id[1 + i] = id >= 0 && id < vocab && w != 0.f ? static_cast<int>(id) : -1;
+      const bool here = id >= 0 && id < vocab && w != 0.f;
+      li.id[1 + i] = here ? static_cast<int>(id) : -1;
       li.w[1 + i] = w * inv_t;
+      li.z[1 + i] = here ? HalfTraits<T>::to_f(r.p[id]) : 0.f;
       sum += w;
     }
     sum = warp_sum(sum);
     if (threadIdx.x == 0) {
       const int64_t id = t - v0;
-      li.id[0] = gr != 0.f && id >= 0 && id < vocab ? static_cast<int>(id) : -1;
+      const bool here = gr != 0.f && id >= 0 && id < vocab;
+      li.id[0] = here ? static_cast<int>(id) : -1;
       li.w[0] = gr * inv_t;
+      li.z[0] = here ? HalfTraits<T>::to_f(r.p[id]) : 0.f;
       usum = sum;
     }
   }
@@ -686,7 +719,7 @@ __global__ void token_scores_bwd_kernel(const T* z, int64_t ld, int vocab, int64
   }
   const float A = -(gr + usum + (kLog ? hr * entropy[row] : 0.f)) * inv_t;
   const DenseTerm f = DenseTerm::of(stats[2 * row], stats[2 * row + 1], inv_t * kLog2e, A, kLog ? -hr * inv_t : 0.f);
-  write_grad<T, kLog>(r, d, f, li, 1 + extra);
+  write_grad<T, kLog, false>(r, d, f, li, 1 + extra);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -697,108 +730,109 @@ __global__ void token_scores_bwd_kernel(const T* z, int64_t ld, int vocab, int64
 struct TeacherRow {
   float tmax, log_sum, mass;   // mass: sum of q (1, or 0 for an empty row)
 };
-__device__ __forceinline__ TeacherRow teacher_row(const TeacherView& t, int64_t row, int64_t v0, int vocab,
-                                                  float inv_t, Listed& li, float* red) {
+
+// A thread's first entry, requested before the row is read so that it is there afterwards.
+struct FirstEntry {
+  float logit;
+  int64_t id;
+  __device__ __forceinline__ FirstEntry(const TeacherView& t, int64_t row) : logit(0.f), id(-1) {
+    if (static_cast<int>(threadIdx.x) < t.k) {
+      logit = t.logit[row * t.k + threadIdx.x];
+      id = t.index[row * t.k + threadIdx.x];
+    }
+  }
+};
+
+// The row's list in shared memory: local ids (-1: not on this shard), teacher logits (later replaced
+// by their weights) and, where asked for, the student's logits. Followed by a barrier of the caller.
+template <typename T>
+__device__ __forceinline__ void stage_list(const TeacherView& t, int64_t row, const FirstEntry& first, const Row<T>& r,
+                                           int64_t v0, Listed& li) {
+  for (int i = threadIdx.x; i < t.k; i += blockDim.x) {
+    const bool mine = i == static_cast<int>(threadIdx.x);
+    const float logit = mine ? first.logit : t.logit[row * t.k + i];
+    const int64_t id = (mine ? first.id : t.index[row * t.k + i]) - v0;
+    const bool here = logit != -INFINITY && id >= 0 && id < r.n;
+    li.w[i] = logit;
+    li.id[i] = here ? static_cast<int>(id) : -1;
+    li.z[i] = here ? HalfTraits<T>::to_f(r.p[id]) : CUDART_NAN_F;
+  }
+}
+
+// The teacher's side of a staged row; every warp works it out for itself.
+__device__ __forceinline__ TeacherRow teacher_row(const Listed& li, int k, float inv_t) {
   const int lane = threadIdx.x & 31;
-  const float* tl = t.logit + row * t.k;
   float mx = -INFINITY, sum = 0.f;
   bool nan = false;
-  // every warp reduces the whole (short) list for itself
-  for (int i = lane; i < t.k; i += 32) {
-    mx = fmaxf(mx, tl[i]);
-    nan |= tl[i] != tl[i];
+  for (int i = lane; i < k; i += 32) {
+    mx = fmaxf(mx, li.w[i]);
+    nan |= li.w[i] != li.w[i];
   }
   mx = warp_max(mx);
   nan = __any_sync(0xffffffffu, nan);
-  TeacherRow out{mx, 0.f, 0.f};
-  if (mx == -INFINITY && !nan) {
-    for (int i = threadIdx.x; i < t.k; i += blockDim.x) {
-      li.id[i] = -1;
-      li.w[i] = 0.f;
-    }
-    __syncthreads();
-    return out;
-  }
-  for (int i = lane; i < t.k; i += 32) sum += exp2f((tl[i] - mx) * inv_t * kLog2e);
-  sum = warp_sum(sum);
-  if (nan) sum = CUDART_NAN_F;
-  const float inv = 1.0f / sum;
-  for (int i = threadIdx.x; i < t.k; i += blockDim.x) {
-    const float q = exp2f((tl[i] - mx) * inv_t * kLog2e) * inv;
-    const int64_t id = t.index[row * t.k + i] - v0;
-    li.w[i] = q;
-    li.id[i] = q != 0.f && id >= 0 && id < vocab ? static_cast<int>(id) : -1;
-  }
-  __syncthreads();
-  out.log_sum = kLn2 * log2f(sum);
-  out.mass = sum == sum ? 1.f : sum;
-  return out;
+  if (mx == -INFINITY && !nan) return {mx, 0.f, 0.f};
+  for (int i = lane; i < k; i += 32) sum += exp2f((li.w[i] - mx) * inv_t * kLog2e);
+  sum = nan ? CUDART_NAN_F : warp_sum(sum);
+  return {mx, kLn2 * log2f(sum), sum == sum ? 1.f : sum};
+}
+// log q of a listed teacher logit
+__device__ __forceinline__ float log_weight(const TeacherRow& t, float logit, float inv_t) {
+  return (logit - t.tmax) * inv_t - t.log_sum;
 }
 
-__device__ __forceinline__ float block_sum_f(float v, float* red) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  v = warp_sum(v);
-  __syncthreads();
-  if (lane == 0) red[warp] = v;
-  __syncthreads();
-  return warp_sum(lane < nw ? red[lane] : 0.f);
-}
-
-// loss of a row whose listed logits are all in this shard; NaN where a weighted entry is not
-template <typename T>
-__device__ __forceinline__ float listed_loss(const Row<T>& r, const TeacherView& t, int64_t row, const TeacherRow& tr,
-                                             float inv_t, float mu, float log_l, const Listed& li, float* red) {
+// One warp: the loss of a staged row whose listed logits are all on this shard; NaN where an entry with
+// weight is not, 0 where there are no entries.
+__device__ __forceinline__ float listed_loss(const Listed& li, int k, const TeacherRow& tr, float inv_t, float mu,
+                                             float log_l) {
   float part = 0.f;
-  for (int i = threadIdx.x; i < t.k; i += blockDim.x) {
-    const float q = li.w[i];
-    if (q == 0.f) continue;
-    const float log_q = (t.logit[row * t.k + i] - tr.tmax) * inv_t - tr.log_sum;
-    const float zi = li.id[i] >= 0 ? HalfTraits<T>::to_f(r.p[li.id[i]]) : CUDART_NAN_F;
-    part += q * (log_q - ((zi - mu) * inv_t - log_l));
+  if (tr.mass == 0.f) return 0.f;
+  for (int i = threadIdx.x & 31; i < k; i += 32) {
+    const float log_q = log_weight(tr, li.w[i], inv_t), q = exp2f(log_q * kLog2e);
+    if (q != 0.f) part += q * (log_q - ((li.z[i] - mu) * inv_t - log_l));
   }
-  return block_sum_f(part, red);
+  return warp_sum(part);
 }
 
-template <typename T>
-__global__ void distill_fwd_kernel(const T* __restrict__ z, int64_t ld, int vocab, int64_t v0, TeacherView t,
-                                   float inv_t, float* __restrict__ loss, float* __restrict__ stats,
-                                   float* __restrict__ partial) {
+// Same shape as token_scores_kernel, without the entropy (8192 x 50304 bf16: 6.6 TB/s).
+template <typename T, int kThreads, int kPerSm>
+__global__ void __launch_bounds__(kThreads, kPerSm)
+distill_fwd_kernel(const T* __restrict__ z, int64_t ld, int vocab, int64_t v0, TeacherView t, float inv_t,
+                   float* __restrict__ loss, float* __restrict__ stats, float* __restrict__ partial) {
   __shared__ float red[96];
   __shared__ Listed li;
   const int64_t row = blockIdx.x;
   const Row<T> r(z + row * ld, vocab);
   const float s2 = inv_t * kLog2e;
-  const TeacherRow tr = teacher_row(t, row, v0, vocab, inv_t, li, red);
-  if (tr.mass == 0.f && partial == nullptr) {   // nothing listed: no loss, the logits are not looked at
-    if (threadIdx.x == 0) {
-      loss[row] = 0.f;
-      stats[2 * row] = 0.f;
-      stats[2 * row + 1] = 1.f;
-    }
-    return;
-  }
-  const Running<false> all = block_merge<false>(scan_row<T, false>(r, s2), s2, red);
+  const FirstEntry first(t, row);
+  const Running<false> own = scan_row<T, false>(r, s2);
+  stage_list(t, row, first, r, v0, li);
+  const Running<false> all = block_merge<false>(own, s2, red);   // its barrier publishes the list, too
+  if (threadIdx.x >= 32) return;
   const float mu = all.mu();
+  const TeacherRow tr = teacher_row(li, t.k, inv_t);
   if (partial != nullptr) {
     float found = 0.f, weight = 0.f;
-    for (int i = threadIdx.x; i < t.k; i += blockDim.x)
-      if (li.id[i] >= 0) {
-        found += li.w[i] * ((HalfTraits<T>::to_f(r.p[li.id[i]]) - mu) * inv_t);
-        weight += li.w[i];
+    for (int i = threadIdx.x; i < t.k && tr.mass != 0.f; i += 32) {
+      const float q = exp2f(log_weight(tr, li.w[i], inv_t) * kLog2e);
+      if (li.id[i] >= 0 && q != 0.f) {
+        found += q * ((li.z[i] - mu) * inv_t);
+        weight += q;
       }
-    found = block_sum_f(found, red);
-    weight = block_sum_f(weight, red);
+    }
+    found = warp_sum(found);
+    weight = warp_sum(weight);
     if (threadIdx.x == 0) {
       float* q = partial + row * 4;
       q[0] = all.mx; q[1] = all.l; q[2] = found; q[3] = weight;
     }
     return;
   }
-  const float l = listed_loss(r, t, row, tr, inv_t, mu, kLn2 * log2f(all.l), li, red);
+  const float l = listed_loss(li, t.k, tr, inv_t, mu, kLn2 * log2f(all.l));
   if (threadIdx.x == 0) {
+    const bool empty = tr.mass == 0.f;   // nothing listed: no loss, whatever the logits
     loss[row] = l;
-    stats[2 * row] = mu;
-    stats[2 * row + 1] = all.l;
+    stats[2 * row] = empty ? 0.f : mu;
+    stats[2 * row + 1] = empty ? 1.f : all.l;
   }
 }
 
@@ -850,65 +884,77 @@ __global__ void distill_combine_kernel(const float* __restrict__ parts, int worl
   }
 }
 
+// Turns the staged teacher logits into the gradient's listed weights -g q.
+__device__ __forceinline__ void weigh_list(Listed& li, int k, const TeacherRow& tr, float inv_t, float g) {
+  __syncthreads();   // every warp has its teacher_row
+  for (int i = threadIdx.x; i < k; i += blockDim.x) {
+    const float w = -g * exp2f(log_weight(tr, li.w[i], inv_t) * kLog2e);
+    li.w[i] = w;
+    if (w == 0.f) li.id[i] = -1;
+  }
+  __syncthreads();
+}
+
 template <typename T>
 __global__ void distill_bwd_kernel(const T* z, int64_t ld, int vocab, int64_t v0, TeacherView t, float inv_t,
                                    const float* __restrict__ stats, const float* __restrict__ dloss, T* dz,
                                    int64_t ldd) {
-  __shared__ float red[96];
   __shared__ Listed li;
   const int64_t row = blockIdx.x;
   const Row<T> r(z + row * ld, vocab);
   T* d = dz + row * ldd;
   const float g = dloss[row] * inv_t;
-  const TeacherRow tr = teacher_row(t, row, v0, vocab, inv_t, li, red);
+  stage_list(t, row, FirstEntry(t, row), r, v0, li);
+  __syncthreads();
+  const TeacherRow tr = teacher_row(li, t.k, inv_t);
   if (tr.mass == 0.f || g == 0.f) {
     write_zero(d, vocab);
     return;
   }
-  for (int i = threadIdx.x; i < t.k; i += blockDim.x) li.w[i] *= -g;
+  weigh_list(li, t.k, tr, inv_t, g);
   const DenseTerm f = DenseTerm::of(stats[2 * row], stats[2 * row + 1], inv_t * kLog2e, g * tr.mass, 0.f);
-  write_grad<T, false>(r, d, f, li, t.k);
+  write_grad<T, false, false>(r, d, f, li, t.k);
 }
 
 // Loss and gradient of a row in one CTA: the second reading of the row comes out of L2, so DRAM sees
-// the logits once and the gradient once.
-template <typename T>
-__global__ void distill_step_kernel(const T* z, int64_t ld, int vocab, int64_t v0, TeacherView t, float inv_t,
-                                    const float* __restrict__ dloss, float* __restrict__ loss, T* dz, int64_t ldd) {
+// the logits once and the gradient once. That needs the rows in flight to stay in L2 beside the
+// gradients being written: the second reading and the stores are marked as not needed again, and long
+// rows run fewer at a time (launch_step). 8192 x 50304 bf16: 268 us = 6.1 TB/s with 4 CTAs of 384
+// threads per SM (334 without the marks); 361 with 6 of 256; with the row kept in shared memory
+// instead of read again, 327 at best, as two rows per SM leave too little in flight.
+template <typename T, int kThreads, int kPerSm>
+__global__ void __launch_bounds__(kThreads, kPerSm)
+distill_step_kernel(const T* z, int64_t ld, int vocab, int64_t v0, TeacherView t, float inv_t,
+                    const float* __restrict__ dloss, float* __restrict__ loss, T* dz, int64_t ldd) {
   __shared__ float red[96];
   __shared__ Listed li;
   const int64_t row = blockIdx.x;
   const Row<T> r(z + row * ld, vocab);
   T* d = dz + row * ldd;
   const float s2 = inv_t * kLog2e;
+  const FirstEntry first(t, row);
   const float g = dloss[row] * inv_t;
-  const TeacherRow tr = teacher_row(t, row, v0, vocab, inv_t, li, red);
-  if (tr.mass == 0.f) {
-    if (threadIdx.x == 0) loss[row] = 0.f;
-    write_zero(d, vocab);
-    return;
-  }
-  const Running<false> all = block_merge<false>(scan_row<T, false>(r, s2), s2, red);
+  const Running<false> own = scan_row<T, false>(r, s2);
+  stage_list(t, row, first, r, v0, li);
+  const Running<false> all = block_merge<false>(own, s2, red);
   const float mu = all.mu();
-  const float l = listed_loss(r, t, row, tr, inv_t, mu, kLn2 * log2f(all.l), li, red);
-  if (threadIdx.x == 0) loss[row] = l;
-  if (g == 0.f) {
-    __syncthreads();
+  const TeacherRow tr = teacher_row(li, t.k, inv_t);
+  if (threadIdx.x < 32) {
+    const float l = listed_loss(li, t.k, tr, inv_t, mu, kLn2 * log2f(all.l));
+    if (threadIdx.x == 0) loss[row] = l;
+  }
+  if (tr.mass == 0.f || g == 0.f) {
     write_zero(d, vocab);
     return;
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < t.k; i += blockDim.x) li.w[i] *= -g;
+  weigh_list(li, t.k, tr, inv_t, g);
   const DenseTerm f = DenseTerm::of(mu, all.l, s2, g * tr.mass, 0.f);
-  write_grad<T, false>(r, d, f, li, t.k);
+  write_grad<T, false, true>(r, d, f, li, t.k);
 }
 
-// Threads per row: with rows for every SM, 256 threads and up to eight rows per SM; a few rows get
-// a whole SM's worth of threads each, which shortens the row instead.
-int threads_for(int64_t rows, int vocab) {
-  if (rows <= 2 * 148 && vocab > 4096) return 1024;
-  return 256;
-}
+// Fewer rows than two per SM: a whole SM's worth of threads for each shortens the single row.
+bool few_rows(int64_t rows, int vocab) { return rows <= 2 * 148 && vocab > 4096; }
+int threads_for(int64_t rows, int vocab) { return few_rows(rows, vocab) ? 1024 : 256; }
 
 cudaError_t check_view(const LogitsView& a) {
   ETHB_RETURN_IF(a.rows < 0 || a.vocab <= 0, cudaErrorInvalidValue, "token loss: empty vocabulary");
@@ -917,20 +963,28 @@ cudaError_t check_view(const LogitsView& a) {
   return cudaSuccess;
 }
 
+// With 128 threads the bound on the k-th alternative (the k-th largest of as many maxima) is loose for k
+// near 128: about 620 elements would reach it. 256 threads leave about 180.
+template <typename T>
+void launch_scores_for(const LogitsView& a, const int64_t* tokens, int top_k, const TokenScoresOut& out, float* partial,
+                       cudaStream_t st) {
+  const auto go = [&](auto* kernel, int threads) {
+    kernel<<<static_cast<unsigned>(a.rows), threads, 0, st>>>(static_cast<const T*>(a.z), a.ld, a.vocab, a.v0, tokens,
+                                                              top_k, a.inv_temperature, out, partial);
+  };
+  if (few_rows(a.rows, a.vocab))
+    top_k > 0 ? go(token_scores_kernel<T, true, 1024, 1>, 1024) : go(token_scores_kernel<T, false, 1024, 1>, 1024);
+  else if (top_k > 64)
+    go(token_scores_kernel<T, true, 256, 5>, 256);
+  else
+    top_k > 0 ? go(token_scores_kernel<T, true, 128, 10>, 128) : go(token_scores_kernel<T, false, 128, 10>, 128);
+}
 cudaError_t launch_scores(const LogitsView& a, const int64_t* tokens, int top_k, const TokenScoresOut& out,
                           float* partial, cudaStream_t st) {
   ETHB_TRY(check_view(a), "token_scores");
   ETHB_RETURN_IF(top_k < 0 || top_k > kMaxTopAlternatives || top_k > a.vocab, cudaErrorInvalidValue, "top_k");
   if (a.rows == 0) return cudaSuccess;
-  const int threads = threads_for(a.rows, a.vocab);
-  ETHB_DISPATCH_T(a.dtype, T, {
-    if (top_k > 0)
-      token_scores_kernel<T, true><<<static_cast<unsigned>(a.rows), threads, 0, st>>>(
-          static_cast<const T*>(a.z), a.ld, a.vocab, a.v0, tokens, top_k, a.inv_temperature, out, partial);
-    else
-      token_scores_kernel<T, false><<<static_cast<unsigned>(a.rows), threads, 0, st>>>(
-          static_cast<const T*>(a.z), a.ld, a.vocab, a.v0, tokens, top_k, a.inv_temperature, out, partial);
-  });
+  ETHB_DISPATCH_T(a.dtype, T, launch_scores_for<T>(a, tokens, top_k, out, partial, st));
   count_launch();
   return cudaGetLastError();
 }
@@ -941,11 +995,27 @@ cudaError_t launch_distill(const LogitsView& a, const TeacherView& t, float* los
   ETHB_RETURN_IF(t.k < 1 || t.k > kMaxTeacherEntries, cudaErrorInvalidValue, "teacher entries");
   if (a.rows == 0) return cudaSuccess;
   ETHB_DISPATCH_T(a.dtype, T, {
-    distill_fwd_kernel<T><<<static_cast<unsigned>(a.rows), threads_for(a.rows, a.vocab), 0, st>>>(
-        static_cast<const T*>(a.z), a.ld, a.vocab, a.v0, t, a.inv_temperature, loss, stats, partial);
+    const auto go = [&](auto* kernel, int threads) {
+      kernel<<<static_cast<unsigned>(a.rows), threads, 0, st>>>(static_cast<const T*>(a.z), a.ld, a.vocab, a.v0, t,
+                                                                a.inv_temperature, loss, stats, partial);
+    };
+    few_rows(a.rows, a.vocab) ? go(distill_fwd_kernel<T, 1024, 1>, 1024) : go(distill_fwd_kernel<T, 128, 12>, 128);
   });
   count_launch();
   return cudaGetLastError();
+}
+
+// Rows in flight take SMs x rows per SM x row bytes of L2 (126 MB, which also passes the gradients on).
+template <typename T>
+void launch_step(const LogitsView& a, const TeacherView& t, const float* dloss, float* loss, T* dz, int64_t ldd,
+                 cudaStream_t st) {
+  const auto go = [&](auto* kernel, int threads) {
+    kernel<<<static_cast<unsigned>(a.rows), threads, 0, st>>>(static_cast<const T*>(a.z), a.ld, a.vocab, a.v0, t,
+                                                              a.inv_temperature, dloss, loss, dz, ldd);
+  };
+  const int64_t row_bytes = static_cast<int64_t>(a.vocab) * sizeof(T);
+  if (few_rows(a.rows, a.vocab) || row_bytes > 200 << 10) go(distill_step_kernel<T, 1024, 2>, 1024);
+  else go(distill_step_kernel<T, 384, 4>, 384);
 }
 
 }  // namespace
@@ -1019,8 +1089,7 @@ cudaError_t distill_step(const LogitsView& a, const TeacherView& t, const float*
   ETHB_RETURN_IF(t.k < 1 || t.k > kMaxTeacherEntries, cudaErrorInvalidValue, "teacher entries");
   if (a.rows == 0) return cudaSuccess;
   ETHB_DISPATCH_T(a.dtype, T, {
-    distill_step_kernel<T><<<static_cast<unsigned>(a.rows), threads_for(a.rows, a.vocab), 0, st>>>(
-        static_cast<const T*>(a.z), a.ld, a.vocab, a.v0, t, a.inv_temperature, dloss, loss, static_cast<T*>(dz), ldd);
+    launch_step<T>(a, t, dloss, loss, static_cast<T*>(dz), ldd, st);
   });
   count_launch();
   return cudaGetLastError();
