@@ -186,9 +186,9 @@ template <bool kEntropy> struct Running {
     l += e;
     if (kEntropy) a = fmaf(e, fmaxf(t, -1000.f), a);   // e is 0 far above -1000; -inf * 0 must not appear
   }
-  // N vectors of one thread at once.
+  // N vectors of one thread at once; returns their maximum.
   template <typename T, int N>
-  __device__ __forceinline__ void add_group(const uint4 (&u)[N], float s2);
+  __device__ __forceinline__ float add_group(const uint4 (&u)[N], float s2);
 };
 
 template <typename T, bool kNan = false>
@@ -235,7 +235,7 @@ __device__ __noinline__ Running<true> add_clamped(Running<true> run, uint4 u, fl
 
 template <bool kEntropy>
 template <typename T, int N>
-__device__ __forceinline__ void Running<kEntropy>::add_group(const uint4 (&u)[N], float s2) {
+__device__ __forceinline__ float Running<kEntropy>::add_group(const uint4 (&u)[N], float s2) {
   float m = max_of<T>(u[0]);
 #pragma unroll
   for (int k = 1; k < N; ++k) m = fmaxf(m, max_of<T>(u[k]));
@@ -245,7 +245,7 @@ __device__ __forceinline__ void Running<kEntropy>::add_group(const uint4 (&u)[N]
     if (!has_floor(base, s2)) {
 #pragma unroll
       for (int k = 0; k < N; ++k) *this = add_clamped<T>(*this, u[k], s2);
-      return;
+      return m;
     }
   }
   const Pair neg = pair(-base, -base), scale = pair(s2, s2);
@@ -268,14 +268,39 @@ __device__ __forceinline__ void Running<kEntropy>::add_group(const uint4 (&u)[N]
     split(asum, x, y);
     a += x + y;
   }
+  return m;
 }
 
-constexpr int kUnroll = 4;   // 16-byte loads in flight per thread
+// The maxima of a thread's segments (runs of `length` groups of kGroup vectors), for select_top: at most
+// kSegments, at max[segment * blockDim.x + threadIdx.x].
+constexpr int kSegments = 8;
+struct NoSegments {
+  __device__ __forceinline__ void add(float) {}
+  __device__ __forceinline__ void close() {}
+};
+struct Segments {
+  float* max;
+  int length, done = 0, segment = 0;
+  float m = -INFINITY;
+  __device__ __forceinline__ Segments(float* smem, int nvec, int group)
+      : max(smem), length((nvec + group * kSegments * blockDim.x - 1) / (group * kSegments * blockDim.x)) {}
+  __device__ __forceinline__ void add(float group_max) {
+    m = fmaxf(m, group_max);
+    if (++done == length) close();
+  }
+  __device__ __forceinline__ void close() {
+    if (done == 0) return;
+    max[segment++ * blockDim.x + threadIdx.x] = m;
+    m = -INFINITY;
+    done = 0;
+  }
+};
 
-// One thread's share of a row. Every maximum is taken over kUnroll vectors before their
-// exponentials, so the sums are rescaled only when a thread's maximum grows.
-template <typename T, bool kEntropy>
-__device__ __forceinline__ Running<kEntropy> scan_row(const Row<T>& r, float s2) {
+// One thread's share of a row, kGroup 16-byte loads at a time: every maximum is taken over a group
+// before its exponentials, so the sums are rescaled only when the thread's maximum grows. `first` runs
+// once, when the first group is through: what it loads is on its way while the rest of the row is read.
+template <typename T, bool kEntropy, int kGroup, typename Seg, typename First>
+__device__ __forceinline__ Running<kEntropy> scan_row(const Row<T>& r, float s2, Seg& seg, First first) {
   Running<kEntropy> run;
   auto one = [&](float z) {
     if (z > run.mx) run.raise(z, s2);
@@ -286,22 +311,27 @@ __device__ __forceinline__ Running<kEntropy> scan_row(const Row<T>& r, float s2)
   for (int i = r.tail() + tid; i < r.n; i += step) one(HalfTraits<T>::to_f(r.p[i]));
   const uint4* v = r.vec();
   int c = tid;
-  for (; c + (kUnroll - 1) * step < r.nvec; c += kUnroll * step) {
-    uint4 u[kUnroll];
+  for (; c + (kGroup - 1) * step < r.nvec; c += kGroup * step) {
+    uint4 u[kGroup];
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) u[k] = v[c + k * step];
-    run.template add_group<T>(u, s2);
+    for (int k = 0; k < kGroup; ++k) u[k] = v[c + k * step];
+    seg.add(run.template add_group<T>(u, s2));
+    if (c < step) first();
   }
-  uint4 u[kUnroll];   // the rest: all loads first, too
+  uint4 u[kGroup];   // the rest: all its loads first, too
 #pragma unroll
-  for (int k = 0; k < kUnroll; ++k)
+  for (int k = 0; k < kGroup; ++k)
     if (c + k * step < r.nvec) u[k] = v[c + k * step];
+  if (c < step) first();
+  float m = -INFINITY;
 #pragma unroll
-  for (int k = 0; k < kUnroll; ++k)
+  for (int k = 0; k < kGroup; ++k)
     if (c + k * step < r.nvec) {
-      const uint4 one_vec[1] = {u[k]};
-      run.template add_group<T>(one_vec, s2);
+      const uint4 single[1] = {u[k]};
+      m = fmaxf(m, run.template add_group<T>(single, s2));
     }
+  seg.add(m);
+  seg.close();
   return run;
 }
 
@@ -338,8 +368,9 @@ __device__ __forceinline__ Running<kEntropy> block_merge(Running<kEntropy> run, 
 // top alternatives
 // ---------------------------------------------------------------------------------------------
 // Exact selection without keeping the row: the k-th largest of the threads' maxima is a lower bound
-// of the k-th largest element, and only threads whose own maximum reaches it can hold candidates.
-// The block reads the shares of those few threads again (they are still in L2). The candidates carry (key, ~token id), so ties go to the lowest id and the order in which they were found does
+// of the k-th largest element, and only segments whose own maximum reaches it can hold candidates.
+// The block reads those few segments again (they are still in L2). The candidates carry
+// (key, ~token id), so ties go to the lowest id and the order in which they were found does
 // not matter. Where the bound is loose (a row of equal values, masked rows) and more than
 // kCandidates elements reach it, the exact k-th key and then the id up to which ties are taken are
 // found by bisection over their bits, with counts over the whole row.
@@ -360,10 +391,16 @@ __device__ __forceinline__ void for_own(const Row<T>& r, F f) {   // f(value, lo
   }
 }
 
+// the value of a key (of NaN: some NaN)
+__device__ __forceinline__ float value_of(uint32_t key) {
+  return __uint_as_float((key & 0x80000000u) ? key ^ 0x80000000u : ~key);
+}
+
 template <int kThreads> struct SelectSmem {
+  float segment_max[kThreads * kSegments];
   unsigned long long cand[kCandidates];
   unsigned long long best[kMaxTopAlternatives];
-  short owner[kThreads];
+  unsigned short owner[kThreads * kSegments];   // segments with candidates: segment * threads + thread
   int count, owners;
   int sums[32];
 };
@@ -378,12 +415,15 @@ __device__ __forceinline__ int block_count(int v, int* sums) {
 }
 
 // s.best[0..k) = the k largest (key << 32 | ~id), in falling order. Needs k <= blockDim.x, k <= r.n.
-template <typename T, int kThreads>
-__device__ void select_top(const Row<T>& r, int k, float thread_max, bool thread_nan, SelectSmem<kThreads>& s) {
+template <typename T, int kGroup, int kThreads>
+__device__ void select_top(const Row<T>& r, int k, float thread_max, bool thread_nan, const Segments& seg,
+                           SelectSmem<kThreads>& s) {
   const int tid = threadIdx.x;
   uint32_t own = 0;                          // below the key of -inf: a thread without elements
   const bool any = tid < r.head || r.tail() + tid < r.n || tid < r.nvec;
-  if (thread_nan || fabsf(thread_max) < 1.17549435e-38f) {
+  constexpr float kTiny = 1.17549435e-38f;   // below it float comparisons flush
+  const bool unsure = thread_nan || fabsf(thread_max) < kTiny;
+  if (unsure) {
     // NaN or +inf among this thread's elements, or a maximum so small that the float comparisons
     // behind it flushed its competitors: take the true maximum
     for_own(r, [&](float z, int) { own = max(own, order_key(z)); });
@@ -408,22 +448,39 @@ __device__ void select_top(const Row<T>& r, int k, float thread_max, bool thread
     }
   };
   if (own >= bound && any) {
-    s.owner[atomicAdd(&s.owners, 1)] = static_cast<short>(tid);
-    if (tid < r.head) take(HalfTraits<T>::to_f(r.p[tid]), tid);
-    if (r.tail() + tid < r.n) take(HalfTraits<T>::to_f(r.p[r.tail() + tid]), r.tail() + tid);
+    const bool all = unsure || fabsf(value_of(bound)) < kTiny;
+    for (int g = 0; g < seg.segment; ++g)
+      if (all || order_key(seg.max[g * kThreads + tid]) >= bound)
+        s.owner[atomicAdd(&s.owners, 1)] = static_cast<unsigned short>(g * kThreads + tid);
+    for (int i = tid; i < r.head; i += kThreads) take(HalfTraits<T>::to_f(r.p[i]), i);
+    for (int i = r.tail() + tid; i < r.n; i += kThreads) take(HalfTraits<T>::to_f(r.p[i]), i);
   }
   __syncthreads();
-  // the block reads the owners' vectors together
-  const int step = blockDim.x, per = (r.nvec + step - 1) / step, items = s.owners * per;
-  for (int i = tid; i < items; i += step) {
-    const int c = s.owner[i / per] + (i % per) * step;
-    if (c >= r.nvec) continue;
-    const uint4 u = r.vec()[c];
-    if (sizeof(T) == 2 && order_key(max_of<T, sizeof(T) == 2>(u)) < bound) continue;   // (an fp32 maximum may flush)
-    float x[kVec<T>];
-    unpack<T>(u, x);
+  // the block reads the segments' vectors together, four loads at a time
+  const int per = seg.length * kGroup, items = s.owners * per;
+  for (int i0 = tid; i0 < items; i0 += 4 * kThreads) {
+    uint4 u[4];
+    int at[4];
 #pragma unroll
-    for (int j = 0; j < kVec<T>; ++j) take(x[j], r.head + c * kVec<T> + j);
+    for (int q = 0; q < 4; ++q) {
+      const int i = i0 + q * kThreads;
+      at[q] = -1;
+      if (i < items) {
+        const int own_seg = s.owner[i / per];
+        const int c = (own_seg / kThreads * per + i % per) * kThreads + own_seg % kThreads;
+        if (c < r.nvec) at[q] = c;
+      }
+      if (at[q] >= 0) u[q] = r.vec()[at[q]];
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (at[q] < 0) continue;
+      if (sizeof(T) == 2 && order_key(max_of<T, sizeof(T) == 2>(u[q])) < bound) continue;   // (fp32 maxima flush)
+      float x[kVec<T>];
+      unpack<T>(u[q], x);
+#pragma unroll
+      for (int j = 0; j < kVec<T>; ++j) take(x[j], r.head + at[q] * kVec<T> + j);
+    }
   }
   __syncthreads();
   int found = s.count;
@@ -467,13 +524,16 @@ __device__ void select_top(const Row<T>& r, int k, float thread_max, bool thread
   __syncthreads();
 }
 
+constexpr int kScanGroup = 8;   // loads in flight per thread of the kernels that read a row once
+
 // ---------------------------------------------------------------------------------------------
 // token log-probabilities, entropy, alternatives: forward
 // ---------------------------------------------------------------------------------------------
-// Bound by reading the logits. Rows are many and each CTA waits at its end (merge, selection), so small
-// CTAs of 128 threads keep most of an SM's warps loading; fewer registers than 50 would spill, more
-// leave too few warps. 8192 x 50304 bf16 without alternatives: 134 us = 6.1 TB/s with 10 CTAs of 128
-// threads per SM, 139 with 6 of 256, 155 with 3 of 512.
+// Bound by reading the logits. Each CTA waits at its end (merge, selection), so many small CTAs keep
+// most of an SM loading, with eight loads in flight per thread so that a few of them suffice when the
+// last rows run out. Without the entropy, GB/s for 128 threads x 8 per SM, 256 x 4, 512 x 2 and 1024 x 1:
+// 8192 x 50304 bf16 6590, 6230, 4715, 2452; 2048 x 128000 5928, 6055, 5556, 3933; 250 x 50304 fp32
+// 3816, 4203, 3920, 2938.
 template <typename T, bool kTop, int kThreads, int kPerSm>
 __global__ void __launch_bounds__(kThreads, kPerSm)
 token_scores_kernel(const T* __restrict__ z, int64_t ld, int vocab, int64_t v0, const int64_t* __restrict__ tokens,
@@ -483,16 +543,24 @@ token_scores_kernel(const T* __restrict__ z, int64_t ld, int vocab, int64_t v0, 
   const int64_t row = blockIdx.x;
   const Row<T> r(z + row * ld, vocab);
   const float s2 = inv_t * kLog2e;
-  const int64_t t = threadIdx.x == 0 ? tokens[row] : -1;   // on its way while the row is read
-  const Running<true> own = scan_row<T, true>(r, s2);
+  using Seg = std::conditional_t<kTop, Segments, NoSegments>;
+  Seg seg = [&] {
+    if constexpr (kTop) return Segments(sel.segment_max, r.nvec, kScanGroup);
+    else return NoSegments{};
+  }();
+  int64_t t = -1;
+  float zt = CUDART_NAN_F;
+  const Running<true> own = scan_row<T, true, kScanGroup>(r, s2, seg, [&] {
+    if (threadIdx.x != 0) return;
+    t = tokens[row];
+    const int64_t local = t - v0;
+    if (t >= 0 && local >= 0 && local < vocab) zt = HalfTraits<T>::to_f(r.p[local]);
+  });
   const Running<true> all = block_merge<true>(own, s2, red);
   const float mu = all.mu();
   const float log_l = kLn2 * log2f(all.l);
   const int width = 4 + 2 * top_k;
   if (threadIdx.x == 0) {
-    const int64_t local = t - v0;
-    const bool here = t >= 0 && local >= 0 && local < vocab;
-    const float zt = here ? HalfTraits<T>::to_f(r.p[local]) : CUDART_NAN_F;
     if (partial != nullptr) {
       float* q = partial + row * width;
       q[0] = all.mx; q[1] = all.l; q[2] = all.a; q[3] = zt;
@@ -503,11 +571,11 @@ token_scores_kernel(const T* __restrict__ z, int64_t ld, int vocab, int64_t v0, 
       out.stats[2 * row + 1] = all.l;
     }
   }
-  if (kTop) {
-    select_top(r, top_k, own.mx, own.l != own.l, sel);
+  if constexpr (kTop) {
+    select_top<T, kScanGroup>(r, top_k, own.mx, own.l != own.l, seg, sel);
     for (int i = threadIdx.x; i < top_k; i += blockDim.x) {
       const int id = static_cast<int>(0xffffffffu - static_cast<uint32_t>(sel.best[i]));
-      const float zi = HalfTraits<T>::to_f(r.p[id]);
+      const float zi = value_of(static_cast<uint32_t>(sel.best[i] >> 32));
       if (partial != nullptr) {
         partial[row * width + 4 + i] = zi;
         partial[row * width + 4 + top_k + i] = __int_as_float(static_cast<int>(id + v0));
@@ -624,11 +692,14 @@ struct DenseTerm {
   }
 };
 
+constexpr int kUnroll = 4;   // loads in flight per thread of the kernels that also write a row
+
 // The whole gradient of a row. The list's logits have been staged before (li.z), behind a barrier.
 // kLast: the row's logits are read for the last time.
-template <typename T, bool kLog, bool kLast>
+// weight(i): what entry i adds.
+template <typename T, bool kLog, bool kLast, typename Weight>
 __device__ __forceinline__ void write_grad(const Row<T>& r, T* __restrict__ d, const DenseTerm& f, const Listed& li,
-                                           int n) {
+                                           int n, Weight weight) {
   const int tid = threadIdx.x, step = blockDim.x;
   if (((reinterpret_cast<uintptr_t>(r.p) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0) {
     for (int i = tid; i < r.head; i += step)
@@ -657,8 +728,9 @@ __device__ __forceinline__ void write_grad(const Row<T>& r, T* __restrict__ d, c
     bool first = true;
     for (int j = 0; j < i; ++j) first &= li.id[j] != id;
     if (!first) continue;
-    float w = li.w[i];
-    for (int j = i + 1; j < n; ++j) w += li.id[j] == id ? li.w[j] : 0.f;
+    float w = weight(i);
+    for (int j = i + 1; j < n; ++j)
+      if (li.id[j] == id) w += weight(j);
     d[id] = HalfTraits<T>::from_f(f.template at<kLog>(li.z[i]) + w);
   }
 }
@@ -719,7 +791,7 @@ __global__ void token_scores_bwd_kernel(const T* z, int64_t ld, int vocab, int64
   }
   const float A = -(gr + usum + (kLog ? hr * entropy[row] : 0.f)) * inv_t;
   const DenseTerm f = DenseTerm::of(stats[2 * row], stats[2 * row + 1], inv_t * kLog2e, A, kLog ? -hr * inv_t : 0.f);
-  write_grad<T, kLog, false>(r, d, f, li, 1 + extra);
+  write_grad<T, kLog, false>(r, d, f, li, 1 + extra, [&](int i) { return li.w[i]; });
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -731,27 +803,14 @@ struct TeacherRow {
   float tmax, log_sum, mass;   // mass: sum of q (1, or 0 for an empty row)
 };
 
-// A thread's first entry, requested before the row is read so that it is there afterwards.
-struct FirstEntry {
-  float logit;
-  int64_t id;
-  __device__ __forceinline__ FirstEntry(const TeacherView& t, int64_t row) : logit(0.f), id(-1) {
-    if (static_cast<int>(threadIdx.x) < t.k) {
-      logit = t.logit[row * t.k + threadIdx.x];
-      id = t.index[row * t.k + threadIdx.x];
-    }
-  }
-};
-
-// The row's list in shared memory: local ids (-1: not on this shard), teacher logits (later replaced
-// by their weights) and, where asked for, the student's logits. Followed by a barrier of the caller.
+// The row's list in shared memory: local ids (-1: not on this shard or unused), teacher logits, student
+// logits. Staged while the row is read (scan_row's `first`), so only the few warps that hold entries wait
+// for the two dependent loads, the others read on; a barrier follows.
 template <typename T>
-__device__ __forceinline__ void stage_list(const TeacherView& t, int64_t row, const FirstEntry& first, const Row<T>& r,
-                                           int64_t v0, Listed& li) {
+__device__ __forceinline__ void stage_list(const TeacherView& t, int64_t row, const Row<T>& r, int64_t v0, Listed& li) {
   for (int i = threadIdx.x; i < t.k; i += blockDim.x) {
-    const bool mine = i == static_cast<int>(threadIdx.x);
-    const float logit = mine ? first.logit : t.logit[row * t.k + i];
-    const int64_t id = (mine ? first.id : t.index[row * t.k + i]) - v0;
+    const float logit = t.logit[row * t.k + i];
+    const int64_t id = t.index[row * t.k + i] - v0;
     const bool here = logit != -INFINITY && id >= 0 && id < r.n;
     li.w[i] = logit;
     li.id[i] = here ? static_cast<int>(id) : -1;
@@ -803,9 +862,8 @@ distill_fwd_kernel(const T* __restrict__ z, int64_t ld, int vocab, int64_t v0, T
   const int64_t row = blockIdx.x;
   const Row<T> r(z + row * ld, vocab);
   const float s2 = inv_t * kLog2e;
-  const FirstEntry first(t, row);
-  const Running<false> own = scan_row<T, false>(r, s2);
-  stage_list(t, row, first, r, v0, li);
+  NoSegments none;
+  const Running<false> own = scan_row<T, false, kScanGroup>(r, s2, none, [&] { stage_list(t, row, r, v0, li); });
   const Running<false> all = block_merge<false>(own, s2, red);   // its barrier publishes the list, too
   if (threadIdx.x >= 32) return;
   const float mu = all.mu();
@@ -884,15 +942,9 @@ __global__ void distill_combine_kernel(const float* __restrict__ parts, int worl
   }
 }
 
-// Turns the staged teacher logits into the gradient's listed weights -g q.
-__device__ __forceinline__ void weigh_list(Listed& li, int k, const TeacherRow& tr, float inv_t, float g) {
-  __syncthreads();   // every warp has its teacher_row
-  for (int i = threadIdx.x; i < k; i += blockDim.x) {
-    const float w = -g * exp2f(log_weight(tr, li.w[i], inv_t) * kLog2e);
-    li.w[i] = w;
-    if (w == 0.f) li.id[i] = -1;
-  }
-  __syncthreads();
+// what entry i of a list adds to its token's gradient
+__device__ __forceinline__ float listed_grad(const Listed& li, const TeacherRow& tr, float inv_t, float g, int i) {
+  return -g * exp2f(log_weight(tr, li.w[i], inv_t) * kLog2e);
 }
 
 template <typename T>
@@ -904,24 +956,23 @@ __global__ void distill_bwd_kernel(const T* z, int64_t ld, int vocab, int64_t v0
   const Row<T> r(z + row * ld, vocab);
   T* d = dz + row * ldd;
   const float g = dloss[row] * inv_t;
-  stage_list(t, row, FirstEntry(t, row), r, v0, li);
+  stage_list(t, row, r, v0, li);
   __syncthreads();
   const TeacherRow tr = teacher_row(li, t.k, inv_t);
   if (tr.mass == 0.f || g == 0.f) {
     write_zero(d, vocab);
     return;
   }
-  weigh_list(li, t.k, tr, inv_t, g);
   const DenseTerm f = DenseTerm::of(stats[2 * row], stats[2 * row + 1], inv_t * kLog2e, g * tr.mass, 0.f);
-  write_grad<T, false, false>(r, d, f, li, t.k);
+  write_grad<T, false, false>(r, d, f, li, t.k, [&](int i) { return listed_grad(li, tr, inv_t, g, i); });
 }
 
 // Loss and gradient of a row in one CTA: the second reading of the row comes out of L2, so DRAM sees
 // the logits once and the gradient once. That needs the rows in flight to stay in L2 beside the
 // gradients being written: the second reading and the stores are marked as not needed again, and long
-// rows run fewer at a time (launch_step). 8192 x 50304 bf16: 268 us = 6.1 TB/s with 4 CTAs of 384
-// threads per SM (334 without the marks); 361 with 6 of 256; with the row kept in shared memory
-// instead of read again, 327 at best, as two rows per SM leave too little in flight.
+// rows run fewer at a time (launch_step). Without the marks a burst of 8192 x 50304 bf16 takes 334 us in
+// place of 268; with the row kept in shared memory instead of read again 327, as two rows per SM leave
+// too little in flight.
 template <typename T, int kThreads, int kPerSm>
 __global__ void __launch_bounds__(kThreads, kPerSm)
 distill_step_kernel(const T* z, int64_t ld, int vocab, int64_t v0, TeacherView t, float inv_t,
@@ -932,29 +983,27 @@ distill_step_kernel(const T* z, int64_t ld, int vocab, int64_t v0, TeacherView t
   const Row<T> r(z + row * ld, vocab);
   T* d = dz + row * ldd;
   const float s2 = inv_t * kLog2e;
-  const FirstEntry first(t, row);
   const float g = dloss[row] * inv_t;
-  const Running<false> own = scan_row<T, false>(r, s2);
-  stage_list(t, row, first, r, v0, li);
+  NoSegments none;
+  const Running<false> own = scan_row<T, false, kUnroll>(r, s2, none, [&] { stage_list(t, row, r, v0, li); });
   const Running<false> all = block_merge<false>(own, s2, red);
   const float mu = all.mu();
   const TeacherRow tr = teacher_row(li, t.k, inv_t);
+  if (tr.mass == 0.f || g == 0.f) {
+    write_zero(d, vocab);
+  } else {
+    const DenseTerm f = DenseTerm::of(mu, all.l, s2, g * tr.mass, 0.f);
+    write_grad<T, false, true>(r, d, f, li, t.k, [&](int i) { return listed_grad(li, tr, inv_t, g, i); });
+  }
   if (threadIdx.x < 32) {
     const float l = listed_loss(li, t.k, tr, inv_t, mu, kLn2 * log2f(all.l));
     if (threadIdx.x == 0) loss[row] = l;
   }
-  if (tr.mass == 0.f || g == 0.f) {
-    write_zero(d, vocab);
-    return;
-  }
-  weigh_list(li, t.k, tr, inv_t, g);
-  const DenseTerm f = DenseTerm::of(mu, all.l, s2, g * tr.mass, 0.f);
-  write_grad<T, false, true>(r, d, f, li, t.k);
 }
 
-// Fewer rows than two per SM: a whole SM's worth of threads for each shortens the single row.
-bool few_rows(int64_t rows, int vocab) { return rows <= 2 * 148 && vocab > 4096; }
-int threads_for(int64_t rows, int vocab) { return few_rows(rows, vocab) ? 1024 : 256; }
+// Below a row per SM, more threads shorten the single row.
+bool few_rows(int64_t rows, int vocab) { return rows < 148 && vocab > 4096; }
+int threads_for(int64_t rows, int vocab) { return few_rows(rows, vocab) ? 512 : 256; }
 
 cudaError_t check_view(const LogitsView& a) {
   ETHB_RETURN_IF(a.rows < 0 || a.vocab <= 0, cudaErrorInvalidValue, "token loss: empty vocabulary");
@@ -973,11 +1022,11 @@ void launch_scores_for(const LogitsView& a, const int64_t* tokens, int top_k, co
                                                               top_k, a.inv_temperature, out, partial);
   };
   if (few_rows(a.rows, a.vocab))
-    top_k > 0 ? go(token_scores_kernel<T, true, 1024, 1>, 1024) : go(token_scores_kernel<T, false, 1024, 1>, 1024);
+    top_k > 0 ? go(token_scores_kernel<T, true, 512, 2>, 512) : go(token_scores_kernel<T, false, 512, 2>, 512);
   else if (top_k > 64)
-    go(token_scores_kernel<T, true, 256, 5>, 256);
+    go(token_scores_kernel<T, true, 256, 4>, 256);
   else
-    top_k > 0 ? go(token_scores_kernel<T, true, 128, 10>, 128) : go(token_scores_kernel<T, false, 128, 10>, 128);
+    top_k > 0 ? go(token_scores_kernel<T, true, 128, 8>, 128) : go(token_scores_kernel<T, false, 128, 8>, 128);
 }
 cudaError_t launch_scores(const LogitsView& a, const int64_t* tokens, int top_k, const TokenScoresOut& out,
                           float* partial, cudaStream_t st) {
@@ -999,13 +1048,15 @@ cudaError_t launch_distill(const LogitsView& a, const TeacherView& t, float* los
       kernel<<<static_cast<unsigned>(a.rows), threads, 0, st>>>(static_cast<const T*>(a.z), a.ld, a.vocab, a.v0, t,
                                                                 a.inv_temperature, loss, stats, partial);
     };
-    few_rows(a.rows, a.vocab) ? go(distill_fwd_kernel<T, 1024, 1>, 1024) : go(distill_fwd_kernel<T, 128, 12>, 128);
+    few_rows(a.rows, a.vocab) ? go(distill_fwd_kernel<T, 512, 2>, 512) : go(distill_fwd_kernel<T, 128, 8>, 128);
   });
   count_launch();
   return cudaGetLastError();
 }
 
-// Rows in flight take SMs x rows per SM x row bytes of L2 (126 MB, which also passes the gradients on).
+// Rows in flight take SMs x rows per SM x row bytes of L2 (126 MB, which also passes the gradients on):
+// four a SM up to 150 KB (89 MB), two beyond. Back to back at the power limit, with 4 x 320, 2 x 512, 3 x
+// 512, 1 x 1024 threads: 8192 x 50304 bf16 343, 393, 388, - us; 2048 x 128000 245, 225, 243, 278 us.
 template <typename T>
 void launch_step(const LogitsView& a, const TeacherView& t, const float* dloss, float* loss, T* dz, int64_t ldd,
                  cudaStream_t st) {
@@ -1014,8 +1065,8 @@ void launch_step(const LogitsView& a, const TeacherView& t, const float* dloss, 
                                                               a.inv_temperature, dloss, loss, dz, ldd);
   };
   const int64_t row_bytes = static_cast<int64_t>(a.vocab) * sizeof(T);
-  if (few_rows(a.rows, a.vocab) || row_bytes > 200 << 10) go(distill_step_kernel<T, 1024, 2>, 1024);
-  else go(distill_step_kernel<T, 384, 4>, 384);
+  if (few_rows(a.rows, a.vocab) || row_bytes > 150 << 10) go(distill_step_kernel<T, 512, 2>, 512);
+  else go(distill_step_kernel<T, 320, 4>, 320);
 }
 
 }  // namespace
