@@ -497,30 +497,145 @@ cudaError_t launch_fwd(const PackedAttnArgs& a, cudaStream_t st) {
 // tile, for every head of the group in turn, so the gradients of shared heads are summed in the
 // accumulators in a fixed order. dQ: one unit per (query tile, head). Both recompute the scores.
 //
+// Both kernels keep two 128-row tiles resident and stream pairs of tiles through a ring of five 32 KB
+// slots; score and gradient tiles are 128 x 128, one buffer each:
+//   S [0,128)   dP [128,256)   accumulators from column 256 on.
+// Each of the two softmax warpgroups works on 64 of the 128 columns, one thread per row. Its 16-bit P
+// (dS) goes over the first half of the S (dP) columns that it has read itself. With one buffer each,
+// what overlaps is the two halves of an iteration: while the exponentials of S are taken the tensor
+// core works on the dP side, and the other way round. (64-column tiles with two buffers of S and dP,
+// as in attention_sm100.cu, need 1.25 times the shared-memory reads per MMA and leave the tensor core
+// waiting for the softmax of a buffer: dK / dV 133 -> DKDV_US us, dQ 107 -> DQ_US us at 8192 rows of nine documents,
+// 16 heads of 128.)
 template <int D> struct BwdCfg {
   static constexpr int kHalves = D / 64;
   static constexpr int kTileBytes = kHalves * 16384;        // one 128-row tile
-  static constexpr int kResidentBytes = 2 * kTileBytes;
-  static constexpr int kStages = 2;
-  static constexpr int kStageBytes = 2 * kTileBytes;
-  static constexpr int kAuxBytes = 2 * 2 * 2 * 64 * 4;      // [wg][parity][lse|delta][64]
-  static constexpr int kSmemBytes = kResidentBytes + kStages * kStageBytes + kAuxBytes + 1024 + 256;
+  static constexpr int kSlots = 5;
+  // [lse | delta of two query tiles, 2 KB][barriers, 1 KB][two resident tiles][ring]: with D = 128 all
+  // 227 KB that a block may have, so the tiles rely on the 1024-byte alignment of dynamic shared memory
+  static constexpr int kFrontBytes = 3072;
+  static constexpr int kSmemBytes = kFrontBytes + (2 + kSlots) * kTileBytes;
   static constexpr int kThreads = 320;
 };
 
 struct BwdBarriers {
   uint64_t res_full;
-  uint64_t tail_full;     // a streamed tile at a document's end has landed, rows behind the end not yet cleared
-  uint64_t st_full[2];
-  uint64_t st_empty[2];
-  uint64_t s_full[2];
-  uint64_t p_full[2];
+  uint64_t tail_full;     // both streamed tiles at a document's end have landed, rows behind the end not yet cleared
+  uint64_t full[5];
+  uint64_t empty[5];
+  uint64_t s_full;        // S of an iteration is complete
+  uint64_t dp_full;       // dP of an iteration is complete
+  uint64_t s_read;        // dK / dV: P is written; dQ: S has been read
+  uint64_t ds_half;       // dQ: the first 32 of each warpgroup's 64 dS columns are written
+  uint64_t ds_full;       // dS is written
   uint64_t done;
-  uint64_t qdo_full;      // dQ kernel: the Q and dO rows of the tile sit in TMEM
-  uint64_t p_early[2];    // dQ kernel: the first 16 of each warpgroup's 32 dS columns are written
+  uint64_t qdo_full;      // dQ: the Q and dO rows of the tile sit in TMEM
   uint32_t tmem_base;
-  uint32_t pad;
 };
+
+// Position in the ring of slots.
+struct RingPos {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void advance(int by) {   // by < 5
+    slot += by;
+    if (slot >= 5) { slot -= 5; phase ^= 1; }
+  }
+  __device__ __forceinline__ RingPos next(int by) const {
+    RingPos r = *this;
+    r.advance(by);
+    return r;
+  }
+};
+
+// Barriers, TMEM and tensor maps of a backward CTA; false if shared memory is not laid out as assumed.
+__device__ __forceinline__ bool bwd_setup(uint8_t* smem, BwdBarriers* bars, int warp, const CUtensorMap& tq,
+                                          const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo,
+                                          int* status) {
+  if ((smem_u32(smem) & 1023) != 0) {
+    if (threadIdx.x == 0 && status != nullptr) atomicCAS(status, 0, kStatusBadArgument);
+    return false;
+  }
+  if (threadIdx.x == 0) {
+    mbar_init(&bars->res_full, 1);
+    mbar_init(&bars->tail_full, 2);
+    for (int s = 0; s < 5; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], 1);
+    }
+    mbar_init(&bars->s_full, 1);
+    mbar_init(&bars->dp_full, 1);
+    mbar_init(&bars->s_read, 8);      // one arrival per softmax warp
+    mbar_init(&bars->ds_half, 8);
+    mbar_init(&bars->ds_full, 8);
+    mbar_init(&bars->done, 1);
+    mbar_init(&bars->qdo_full, 8);
+    fence_mbar_init();
+    prefetch_tmap(&tq); prefetch_tmap(&tk); prefetch_tmap(&tv); prefetch_tmap(&tdo);
+  }
+  if (warp == 1) tmem_alloc(&bars->tmem_base, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  return true;
+}
+
+// Producer warp: streams tile `row` of two tensors (heads ha, hb) through the next two slots. With
+// tail_rows < 128 the tile ends its document: the rows behind are summands of the accumulators and are
+// cleared before the slots are handed on, as 0 times what stands there may be NaN.
+template <int D>
+__device__ __forceinline__ bool stream_pair(BwdBarriers* bars, uint8_t* ring, RingPos& pos, uint32_t& cuts,
+                                            const CUtensorMap* ma, const CUtensorMap* mb, int row, int head,
+                                            int tail_rows, int lane, int* status) {
+  using C = BwdCfg<D>;
+  const bool cut = tail_rows < kTile;
+  const int first = pos.slot;
+#pragma unroll
+  for (int a = 0; a < 2; ++a) {
+    if (!warp_wait(&bars->empty[pos.slot], pos.phase ^ 1, status, kStatusTimeoutEmpty)) return false;
+    if (elect_one()) {
+      uint64_t* full = cut ? &bars->tail_full : &bars->full[pos.slot];
+      mbar_expect_tx(full, C::kTileBytes);
+#pragma unroll
+      for (int h = 0; h < C::kHalves; ++h)
+        tma_load_3d(ring + pos.slot * C::kTileBytes + h * 16384, a == 0 ? ma : mb, full, h * 64, row, head);
+    }
+    __syncwarp();
+    pos.advance(1);
+  }
+  if (cut) {
+    const int second = first == 4 ? 0 : first + 1;
+    if (!warp_wait(&bars->tail_full, cuts & 1, status, kStatusTimeoutFull)) return false;
+    ++cuts;
+    clear_tail<C::kHalves>(ring + first * C::kTileBytes, tail_rows, lane);
+    clear_tail<C::kHalves>(ring + second * C::kTileBytes, tail_rows, lane);
+    __syncwarp();
+    if (lane == 0) {
+      mbar_arrive(&bars->full[first]);
+      mbar_arrive(&bars->full[second]);
+    }
+  }
+  return true;
+}
+
+// 32 fp32 accumulator columns of one row -> 64 bytes of a 16-bit output row.
+template <int DT>
+__device__ __forceinline__ void store_columns(uint32_t acc, uint16_t* dst, float mul, bool row_ok) {
+  uint32_t r[32];
+  __syncwarp();
+  tmem_ld_32x32b_x32(acc, r);
+  tmem_ld_wait();
+  if (!row_ok) return;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint4 o;
+    o.x = pack_pair(__uint_as_float(r[q * 8 + 0]) * mul, __uint_as_float(r[q * 8 + 1]) * mul, DT);
+    o.y = pack_pair(__uint_as_float(r[q * 8 + 2]) * mul, __uint_as_float(r[q * 8 + 3]) * mul, DT);
+    o.z = pack_pair(__uint_as_float(r[q * 8 + 4]) * mul, __uint_as_float(r[q * 8 + 5]) * mul, DT);
+    o.w = pack_pair(__uint_as_float(r[q * 8 + 6]) * mul, __uint_as_float(r[q * 8 + 7]) * mul, DT);
+    reinterpret_cast<uint4*>(dst)[q] = o;
+  }
+}
 
 // Barrier of a warpgroup that also tells all of it whether everybody is still `ok`.
 __device__ __forceinline__ bool wg_and(int wg, bool ok) {
@@ -536,6 +651,12 @@ __device__ __forceinline__ bool wg_and(int wg, bool ok) {
       : "r"(static_cast<uint32_t>(ok)), "r"(wg + 1)
       : "memory");
   return all != 0;
+}
+
+// A wait gave up somewhere: stop after this tile. A warpgroup decides together, its barrier needs all of it.
+__device__ __forceinline__ bool go_on(int warp, const int* status) {
+  const bool go = status == nullptr || *reinterpret_cast<const volatile int*>(status) == 0;
+  return warp < 2 ? __all_sync(0xffffffffu, go) : wg_and((warp - 2) >> 2, go);
 }
 
 // delta[h, row] = sum_d dO * O. A (row, head) vector of head_dim elements is covered by head_dim / 8
@@ -591,313 +712,266 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const PackedAttnArgs 
 
 // ---- dK / dV: persistent CTAs over (key/value tile, key/value head) ------------------------------
 // One CTA per SM walks a static list of tiles, heaviest first (under the causal mask key tile j
-// meets q_tiles - j query tiles of each head), handed out round by round in alternating CTA order.
-// TMEM, the barriers and the tensor-map prefetch are set up once per CTA instead of once per tile;
-// barrier parities therefore run on counters that persist across tiles (`it`: tiles done by this
-// CTA, `sbase`: query tiles streamed so far). No CTA-wide barrier
-// separates the tiles: the loads and first score MMAs of the next tile overlap the accumulator stores
-// of the current one.
+// meets tiles - j query tiles of each head), handed out round by round in alternating CTA order.
+// TMEM, the barriers and the tensor-map prefetch are set up once per CTA; barrier parities therefore
+// run on counters that persist across tiles (`it`: tiles done by this CTA, `g`: query tiles streamed).
+// No CTA-wide barrier separates the tiles: the loads and first score MMAs of the next tile overlap the
+// accumulator stores of the current one.
+//
+// S^T = K Q^T and dP^T = V dO^T, so P^T and dS^T are A operands of dV += P^T dO and dK += dS^T Q.
+// The tensor core's order is  dV(i) S(i+1) | dK(i) dP(i+1):  the first pair needs P(i), the second dS(i).
 template <int D, int DT>
 __global__ void __launch_bounds__(320, 1)
 packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                     const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tdo,
-                     const PackedAttnArgs p) {
+                       const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tdo,
+                       const PackedAttnArgs p) {
   using C = BwdCfg<D>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                             ~static_cast<uintptr_t>(1023));
-  uint8_t* sK = smem;
-  uint8_t* sV = smem + C::kTileBytes;
-  uint8_t* sStage = smem + C::kResidentBytes;  // stage: [Q tile | dO tile]
-  float* sAux = reinterpret_cast<float*>(sStage + C::kStages * C::kStageBytes);
-  BwdBarriers* bars = reinterpret_cast<BwdBarriers*>(reinterpret_cast<uint8_t*>(sAux) + C::kAuxBytes);
+  extern __shared__ uint8_t smem[];
+  float* sAux = reinterpret_cast<float*>(smem);
+  BwdBarriers* bars = reinterpret_cast<BwdBarriers*>(smem + 2048);
+  uint8_t* sK = smem + C::kFrontBytes;
+  uint8_t* sV = sK + C::kTileBytes;
+  uint8_t* sRing = sV + C::kTileBytes;          // Q_0 dO_0 Q_1 dO_1 ...
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = p.heads / p.kv_heads;
   const int total_tiles = p.num_k_tiles * p.kv_heads;
-
-  if (threadIdx.x == 0) {
-    mbar_init(&bars->res_full, 1);
-    mbar_init(&bars->tail_full, 1);
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&bars->st_full[s], 1);
-      mbar_init(&bars->st_empty[s], 1);
-      mbar_init(&bars->s_full[s], 1);
-      mbar_init(&bars->p_full[s], 8);      // both softmax warpgroups work on every sub-tile, one arrival per warp
-    }
-    mbar_init(&bars->done, 1);
-    fence_mbar_init();
-    prefetch_tmap(&tq); prefetch_tmap(&tk); prefetch_tmap(&tv); prefetch_tmap(&tdo);
-  }
-  if (warp == 1) tmem_alloc(&bars->tmem_base, 512);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
+  if (!bwd_setup(smem, bars, warp, tq, tk, tv, tdo, p.status)) return;
   const uint32_t tmem_base = bars->tmem_base;
-  int p_stage = 0;           // producer: ring position of the next query-tile stage (persists across tiles)
-  uint32_t p_phase = 0;
-  int sbase = 0;             // query tiles streamed by this CTA before the current tile
-  uint32_t cuts = 0;         // producer: tiles at a document's end so far
+  RingPos pos;               // producer and MMA issuer: slot of the next Q tile
+  uint32_t cuts = 0;         // producer: tile pairs at a document's end so far
+  int g = 0;                 // query tiles streamed by this CTA before the current tile
 
-  // Round r hands out tiles [r * grid, (r + 1) * grid), heaviest first, in alternating direction
-  // (CTA 0 gets the heaviest tile of an even round and the lightest of an odd one), so the tile
-  // weights of a CTA add up to nearly the same total everywhere; `it` counts the tiles this CTA
-  // has processed (barrier parities run on it).
   for (int round = 0, it = 0; round * static_cast<int>(gridDim.x) < total_tiles; ++round) {
-  const int tile = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-  if (tile >= total_tiles) continue;             // only in the last round
-  const PackedTile w = p.k_tiles[tile / p.kv_heads];
-  const int kv_head = tile % p.kv_heads;
-  const int j = w.tile;                          // key/value tile inside the document
-  const int q_tiles = (w.len + kTile - 1) / kTile;
-  const int i0 = p.causal ? j : 0;
-  const int nd = q_tiles - i0;                   // query tiles of the document that see these keys
-  const int nq = nd * group;                     // streamed: all of them for every head of the group
-  const int tail_rows = w.len - (q_tiles - 1) * kTile;   // rows of the document's last tile
-  const int U = 2 * nq;
-  if (warp == 0) {
-    // the resident K / V buffers are free once every MMA of the previous tile has completed; the
-    // loads of this tile then run while the other warps still store the previous accumulators
-    const bool free_kv = it == 0 || warp_wait(&bars->done, (it - 1) & 1, p.status, kStatusTimeoutTmemFull);
-    if (free_kv && elect_one()) {
-      mbar_expect_tx(&bars->res_full, C::kResidentBytes);
-#pragma unroll
-      for (int h = 0; h < C::kHalves; ++h) {
-        tma_load_3d(sK + h * 16384, &tk, &bars->res_full, h * 64, w.start + j * kTile, kv_head);
-        tma_load_3d(sV + h * 16384, &tv, &bars->res_full, h * 64, w.start + j * kTile, kv_head);
-      }
-    }
-    int stage = p_stage;
-    uint32_t phase = p_phase;
-    for (int t = 0, i = i0, head = kv_head * group; t < nq && free_kv; ++t) {
-      if (!warp_wait(&bars->st_empty[stage], phase ^ 1, p.status, kStatusTimeoutEmpty)) break;
-      uint8_t* sq = sStage + stage * C::kStageBytes;
-      uint8_t* sdo = sq + C::kTileBytes;
-      const bool cut = i == q_tiles - 1 && tail_rows < kTile;
-      __syncwarp();
-      if (elect_one()) {
-        uint64_t* full = cut ? &bars->tail_full : &bars->st_full[stage];
-        mbar_expect_tx(full, C::kStageBytes);
+    const int tile = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+    if (tile >= total_tiles) continue;             // only in the last round
+    const PackedTile w = p.k_tiles[tile / p.kv_heads];
+    const int kv_head = tile % p.kv_heads;
+    const int j = w.tile;                          // key/value tile inside the document
+    const int q_tiles = (w.len + kTile - 1) / kTile;
+    const int i0 = p.causal ? j : 0;
+    const int nd = q_tiles - i0;                   // query tiles of the document that see these keys
+    const int nq = nd * group;                     // streamed: all of them for every head of the group
+    const int last_rows = w.len - (q_tiles - 1) * kTile;   // rows of the document's last tile
+    if (warp == 0) {
+      // the resident K / V buffers are free once every MMA of the previous tile has completed; the
+      // loads of this tile then run while the other warps still store the previous accumulators
+      bool ok = it == 0 || warp_wait(&bars->done, (it - 1) & 1, p.status, kStatusTimeoutTmemFull);
+      if (ok && elect_one()) {
+        mbar_expect_tx(&bars->res_full, 2 * C::kTileBytes);
 #pragma unroll
         for (int h = 0; h < C::kHalves; ++h) {
-          tma_load_3d(sq + h * 16384, &tq, full, h * 64, w.start + i * kTile, head);
-          tma_load_3d(sdo + h * 16384, &tdo, full, h * 64, w.start + i * kTile, head);
+          tma_load_3d(sK + h * 16384, &tk, &bars->res_full, h * 64, w.start + j * kTile, kv_head);
+          tma_load_3d(sV + h * 16384, &tv, &bars->res_full, h * 64, w.start + j * kTile, kv_head);
         }
       }
       __syncwarp();
-      if (cut) {   // rows behind the document's end are summands of dK and dV: 0 times them must be 0
-        if (!warp_wait(&bars->tail_full, cuts & 1, p.status, kStatusTimeoutFull)) break;
-        ++cuts;
-        clear_tail<C::kHalves>(sq, tail_rows, lane);
-        clear_tail<C::kHalves>(sdo, tail_rows, lane);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->st_full[stage]);
+      for (int t = 0, i = i0, head = kv_head * group; t < nq && ok; ++t) {
+        ok = stream_pair<D>(bars, sRing, pos, cuts, &tq, &tdo, w.start + i * kTile, head,
+                            i == q_tiles - 1 ? last_rows : kTile, lane, p.status);
+        if (++i == q_tiles) { i = i0; ++head; }
       }
-      if (++stage == 2) { stage = 0; phase ^= 1; }
-      if (++i == q_tiles) { i = i0; ++head; }
-    }
-    // every lane tracks the ring position, whichever lane is elected next time
-    p_phase ^= static_cast<uint32_t>(((p_stage + nq) >> 1) & 1);
-    p_stage = (p_stage + nq) & 1;
-  } else if (warp == 1) {
-    if (elect_one()) {
-      const int fmt = DT == kBF16 ? 1 : 0;
-      const uint32_t idesc_s = make_idesc_f16(fmt, 0, 0, 128, 64);
-      const uint32_t idesc_acc = make_idesc_f16(fmt, 0, 1, 128, D);
-      // One thread issues every MMA and the score MMAs are short (N = 64), so the issue path must
-      // stay short too: tile-origin descriptors are built once, each MMA adds a constant.
-      const uint64_t dK0 = make_smem_desc_sw128(smem_u32(sK), 16, 1024);
-      const uint64_t dV0 = make_smem_desc_sw128(smem_u32(sV), 16, 1024);
-      const uint64_t dQk0 = make_smem_desc_sw128(smem_u32(sStage), 16, 1024);          // K-major view
-      const uint64_t dQm0 = make_smem_desc_sw128(smem_u32(sStage), 16384, 1024);       // MN-major view
-      auto issue_sdp = [&](int u) {
-        const int stage = (sbase + (u >> 1)) & 1, sub = u & 1, b = u & 1;
-        const uint64_t dQ = desc_advance(dQk0, stage * C::kStageBytes + sub * 8192);
-        const uint64_t dDO = desc_advance(dQ, C::kTileBytes);
+    } else if (warp == 1) {
+      if (elect_one()) {
+        const int fmt = DT == kBF16 ? 1 : 0;
+        const uint32_t idesc_s = make_idesc_f16(fmt, 0, 0, 128, 128);
+        const uint32_t idesc_acc = make_idesc_f16(fmt, 0, 1, 128, D);
+        // One thread issues every MMA, so the issue path is kept short: descriptors of the tile
+        // origins are built once, each MMA only adds a constant to them.
+        const uint64_t dK0 = make_smem_desc_sw128(smem_u32(sK), 16, 1024);
+        const uint64_t dV0 = make_smem_desc_sw128(smem_u32(sV), 16, 1024);
+        const uint64_t dRk = make_smem_desc_sw128(smem_u32(sRing), 16, 1024);          // K-major view
+        const uint64_t dRm = make_smem_desc_sw128(smem_u32(sRing), 16384, 1024);       // MN-major view
+        auto issue_scores = [&](uint64_t a0, int slot, uint32_t tmem, uint64_t* full) {
+          const uint64_t b0 = desc_advance(dRk, slot * C::kTileBytes);
 #pragma unroll
-        for (int h = 0; h < C::kHalves; ++h)
+          for (int h = 0; h < C::kHalves; ++h)
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            tc_mma_f16(tmem_base + b * 128, desc_advance(dK0, h * 16384 + k * 32),
-                       desc_advance(dQ, h * 16384 + k * 32), idesc_s, (h | k) != 0 ? 1u : 0u);
+            for (int k = 0; k < 4; ++k)
+              tc_mma_f16(tmem_base + tmem, desc_advance(a0, h * 16384 + k * 32),
+                         desc_advance(b0, h * 16384 + k * 32), idesc_s, (h | k) != 0 ? 1u : 0u);
+          tc_commit(full);
+        };
+        // queries 0-63 of P / dS sit at columns [0, 32) of their buffer, queries 64-127 at [64, 96)
+        auto issue_acc = [&](uint32_t acc, uint32_t a, int slot, bool first) {
+          const uint64_t b0 = desc_advance(dRm, slot * C::kTileBytes);
 #pragma unroll
-        for (int h = 0; h < C::kHalves; ++h)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            tc_mma_f16(tmem_base + b * 128 + 64, desc_advance(dV0, h * 16384 + k * 32),
-                       desc_advance(dDO, h * 16384 + k * 32), idesc_s, (h | k) != 0 ? 1u : 0u);
-        tc_commit(&bars->s_full[b]);
-      };
-      bool ok = mbar_wait(&bars->res_full, it & 1, p.status, kStatusTimeoutFull);
-      if (ok && U > 0) {
-        ok = mbar_wait(&bars->st_full[sbase & 1], (sbase >> 1) & 1, p.status, kStatusTimeoutFull);
-        tc_fence_after();
-        if (ok) { issue_sdp(0); issue_sdp(1); }
-      }
-      for (int u = 0; u < U && ok; ++u) {
-        const int b = u & 1, stage = (sbase + (u >> 1)) & 1, sub = u & 1;
-        ok = mbar_wait(&bars->p_full[b], (sbase + (u >> 1)) & 1, p.status, kStatusTimeoutTmemFull);
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t dQ = desc_advance(dQm0, stage * C::kStageBytes + sub * 8192);
-        const uint64_t dDO = desc_advance(dQ, C::kTileBytes);
-        // queries 0-31 of P / dS sit at columns [0, 16) of their buffer, queries 32-63 at [32, 48)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)   // dV += P^T dO
-          tc_mma_f16_ts(tmem_base + 256, tmem_base + b * 128 + (k >> 1) * 32 + (k & 1) * 8,
-                        desc_advance(dDO, k * 2048), idesc_acc, (u | k) != 0 ? 1u : 0u);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)   // dK += dS^T Q
-          tc_mma_f16_ts(tmem_base + 384, tmem_base + b * 128 + 64 + (k >> 1) * 32 + (k & 1) * 8,
-                        desc_advance(dQ, k * 2048), idesc_acc, (u | k) != 0 ? 1u : 0u);
-        if (sub == 1) tc_commit(&bars->st_empty[stage]);
-        if (u + 2 < U) {
-          const int u2 = u + 2;
-          if ((u2 & 1) == 0) {
-            const int sq = sbase + (u2 >> 1);
-            ok = mbar_wait(&bars->st_full[sq & 1], (sq >> 1) & 1, p.status, kStatusTimeoutFull);
+          for (int k = 0; k < 8; ++k)
+            tc_mma_f16_ts(tmem_base + acc, tmem_base + a + (k >> 2) * 64 + (k & 3) * 8, desc_advance(b0, k * 2048),
+                          idesc_acc, first && k == 0 ? 0u : 1u);
+          tc_commit(&bars->empty[slot]);
+        };
+        auto wait_full = [&](const RingPos& at) {
+          const bool got = mbar_wait(&bars->full[at.slot], at.phase, p.status, kStatusTimeoutFull);
+          tc_fence_after();
+          return got;
+        };
+        auto wait_softmax = [&](uint64_t* bar, int iter) {
+          const bool got = mbar_wait(bar, iter & 1, p.status, kStatusTimeoutTmemFull);
+          tc_fence_after();
+          return got;
+        };
+        RingPos at = pos;
+        bool ok = mbar_wait(&bars->res_full, it & 1, p.status, kStatusTimeoutFull) && wait_full(at);
+        if (ok) {
+          issue_scores(dK0, at.slot, 0, &bars->s_full);
+          ok = wait_full(at.next(1));
+          if (ok) issue_scores(dV0, at.next(1).slot, 128, &bars->dp_full);
+        }
+        for (int t = 0; t < nq && ok; ++t) {
+          const RingPos qi = at, doi = at.next(1), qn = at.next(2), don = at.next(3);
+          ok = wait_softmax(&bars->s_read, g + t);
+          if (!ok) break;
+          issue_acc(256, 0, doi.slot, t == 0);                     // dV += P^T dO
+          if (t + 1 < nq) {
+            ok = wait_full(qn);
             if (!ok) break;
-            tc_fence_after();
+            issue_scores(dK0, qn.slot, 0, &bars->s_full);
           }
-          issue_sdp(u2);
+          ok = wait_softmax(&bars->ds_full, g + t);
+          if (!ok) break;
+          issue_acc(384, 128, qi.slot, t == 0);                    // dK += dS^T Q
+          if (t + 1 < nq) {
+            ok = wait_full(don);
+            if (!ok) break;
+            issue_scores(dV0, don.slot, 128, &bars->dp_full);
+          }
+          at = qn;
         }
+        tc_commit(&bars->done);
       }
-      tc_commit(&bars->done);
-    }
-  } else {
-    const int wg = (warp - 2) >> 2;      // sub-tile parity handled by this warpgroup
-    const int quarter = warp & 3;
-    const int r_local = quarter * 32 + lane;     // key/value row inside the tile
-    const int wg_tid = threadIdx.x - 64 - wg * 128;
-    const uint32_t lane_bits = static_cast<uint32_t>(quarter * 32) << 16;
-    const float sl2 = p.scale * kLog2e;
-    bool ok = true;
-    // Both warpgroups work on every 64-query sub-tile, each on 32 of its columns (see the dQ kernel),
-    // so the softmax of a sub-tile takes half as long and hides under the score MMAs of the other
-    // buffer; each warpgroup overwrites only columns it has read itself. The lse / delta values of a
-    // query tile are staged once per tile and warpgroup (its 2 x 32 columns), one tile ahead: the
-    // global loads for tile t + 1 are issued before tile t is processed and parked in shared memory
-    // after it, so their latency is never waited for.
-    const int a_sub = (wg_tid >> 5) & 1, a_col = wg_tid & 31;
-    // streamed tile t is query tile i0 + t % nd of head kv_head * group + t / nd
-    auto aux_load = [&](int i, int head, float& lse, float& delta) {
-      const int qi = i * kTile + a_sub * 64 + wg * 32 + a_col;
-      const bool in = qi < w.len;
-      const int64_t at = static_cast<int64_t>(head) * p.rows + w.start + qi;
-      lse = in ? p.lse[at] * kLog2e : INFINITY;
-      delta = in ? p.delta[at] : 0.f;
-    };
-    auto aux_slot = [&](int t) { return sAux + ((wg * 2 + (t & 1)) * 2) * 64; };   // [lse 2 x 32 | delta 2 x 32]
-    if (wg_tid < 64 && nq > 0) {
-      float lse, delta;
-      aux_load(i0, kv_head * group, lse, delta);
-      aux_slot(0)[wg_tid] = lse;
-      aux_slot(0)[64 + wg_tid] = delta;
-    }
-    int i = i0, head = kv_head * group;
-    for (int t = 0; t < nq; ++t) {
-      const int i_next = i + 1 == q_tiles ? i0 : i + 1, head_next = i + 1 == q_tiles ? head + 1 : head;
-      ok = wg_and(wg, ok);             // tile t's values are staged; everyone has left tile t - 1
-      if (!ok) break;
-      float next_lse = INFINITY, next_delta = 0.f;
-      if (wg_tid < 64 && t + 1 < nq) {
-        aux_load(i_next, head_next, next_lse, next_delta);
+      __syncwarp();
+      // every lane tracks the ring position, whichever lane is elected next time
+      const int items = 2 * nq;
+      pos.phase ^= static_cast<uint32_t>(((pos.slot + items) / 5) & 1);
+      pos.slot = (pos.slot + items) % 5;
+    } else {
+      const int wg = (warp - 2) >> 2;      // columns [64 wg, 64 wg + 64) of every tile
+      const int quarter = warp & 3;
+      const int r_local = quarter * 32 + lane;     // key/value row inside the tile
+      const int wg_tid = threadIdx.x - 64 - wg * 128;
+      const uint32_t lane_bits = static_cast<uint32_t>(quarter * 32) << 16;
+      const uint32_t s_addr = tmem_base + wg * 64 + lane_bits, dp_addr = s_addr + 128;
+      const float sl2 = p.scale * kLog2e;
+      bool ok = true;
+      // lse / delta of this warpgroup's 64 queries, staged one query tile ahead: the global loads for
+      // tile t + 1 are issued before tile t is processed and parked in shared memory after it, so their
+      // latency is never waited for. Streamed tile t is query tile i0 + t % nd of head
+      // kv_head * group + t / nd.
+      auto aux_load = [&](int i, int head, float& lse, float& delta) {
+        const int qi = i * kTile + wg * 64 + wg_tid;
+        const bool in = qi < w.len;
+        const int64_t at = static_cast<int64_t>(head) * p.rows + w.start + qi;
+        lse = in ? p.lse[at] * kLog2e : INFINITY;
+        delta = in ? p.delta[at] : 0.f;
+      };
+      auto aux_slot = [&](int t) { return sAux + ((wg * 2 + (t & 1)) * 2) * 64; };   // [lse 64 | delta 64]
+      if (wg_tid < 64) {
+        float lse, delta;
+        aux_load(i0, kv_head * group, lse, delta);
+        aux_slot(0)[wg_tid] = lse;
+        aux_slot(0)[64 + wg_tid] = delta;
       }
-      const bool diag = p.causal && (i == j);
-#pragma unroll 1
-      for (int sub = 0; sub < 2 && ok; ++sub) {
-        const float* a_lse = aux_slot(t) + sub * 32;
-        const float* a_del = a_lse + 64;
-        const uint32_t s_addr = tmem_base + sub * 128 + wg * 32 + lane_bits;
-        const uint32_t dp_addr = s_addr + 64;
-        ok = warp_wait(&bars->s_full[sub], (sbase + t) & 1, p.status, kStatusTimeoutTmemFull);
+      int i = i0, head = kv_head * group;
+      for (int t = 0; t < nq; ++t) {
+        const int i_next = i + 1 == q_tiles ? i0 : i + 1, head_next = i + 1 == q_tiles ? head + 1 : head;
+        ok = wg_and(wg, ok);             // tile t's values are staged; everyone has left tile t - 1
         if (!ok) break;
+        float next_lse = INFINITY, next_delta = 0.f;
+        if (wg_tid < 64 && t + 1 < nq) aux_load(i_next, head_next, next_lse, next_delta);
+        const bool diag = p.causal && (i == j);
+        const float* a_lse = aux_slot(t);
+        const float* a_del = a_lse + 64;
+        float pv[64];
+        ok = warp_wait(&bars->s_full, (g + t) & 1, p.status, kStatusTimeoutTmemFull);
+        if (!ok) continue;
         tc_fence_after();
-        uint32_t rs[32], rd[32];
-        __syncwarp();
-        tmem_ld_32x32b_x32(s_addr, rs);
-        tmem_ld_32x32b_x32(dp_addr, rd);
-        tmem_ld_wait();
-        uint32_t pk[16], dk[16];
-        // lse / delta come as 16-byte broadcast loads (four query columns each); only the tile on
-        // the diagonal pays for the causal mask
+        {
+          uint32_t rs[2][32];
+          tmem_ld_32x32b_x32(s_addr, rs[0]);
+          tmem_ld_32x32b_x32(s_addr + 32, rs[1]);
+          tmem_ld_wait();
+          // lse comes as 16-byte broadcast loads (four query columns each); only the tile on the
+          // diagonal pays for the causal mask
 #pragma unroll
-        for (int y = 0; y < 8; ++y) {
-          const float4 l4 = *reinterpret_cast<const float4*>(a_lse + 4 * y);
-          const float4 e4 = *reinterpret_cast<const float4*>(a_del + 4 * y);
-          const float lv[4] = {l4.x, l4.y, l4.z, l4.w}, ev[4] = {e4.x, e4.y, e4.z, e4.w};
-          float pv[4];
+          for (int y = 0; y < 16; ++y) {
+            const float4 l4 = *reinterpret_cast<const float4*>(a_lse + 4 * y);
+            const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
 #pragma unroll
-          for (int c = 0; c < 4; ++c) pv[c] = exp2f(fmaf(__uint_as_float(rs[4 * y + c]), sl2, -lv[c]));
-          if (diag) {
-            const int ql = sub * 64 + wg * 32 + 4 * y;     // query row inside the 128-row tile
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              if (r_local > ql + c) pv[c] = 0.f;
+            for (int c = 0; c < 4; ++c) {
+              const int e = 4 * y + c;
+              pv[e] = exp2f(fmaf(__uint_as_float(rs[e >> 5][e & 31]), sl2, -lv[c]));
+            }
           }
-          float dv[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) dv[c] = pv[c] * (__uint_as_float(rd[4 * y + c]) - ev[c]);
-          pk[2 * y] = pack_pair(pv[0], pv[1], DT);
-          pk[2 * y + 1] = pack_pair(pv[2], pv[3], DT);
-          dk[2 * y] = pack_pair(dv[0], dv[1], DT);
-          dk[2 * y + 1] = pack_pair(dv[2], dv[3], DT);
         }
-        tmem_st_32x32b_x16(s_addr, pk);
-        tmem_st_32x32b_x16(dp_addr, dk);
+        if (diag) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            if (r_local > wg * 64 + e) pv[e] = 0.f;
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int x = 0; x < 16; ++x) pk[x] = pack_pair(pv[half * 32 + 2 * x], pv[half * 32 + 2 * x + 1], DT);
+          tmem_st_32x32b_x16(s_addr + half * 16, pk);
+        }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->p_full[sub]);   // one arrival per warp
-      }
-      if (wg_tid < 64 && t + 1 < nq) {
-        aux_slot(t + 1)[wg_tid] = next_lse;
-        aux_slot(t + 1)[64 + wg_tid] = next_delta;
-      }
-      i = i_next;
-      head = head_next;
-    }
-    // epilogue: warpgroup 0 stores dV, warpgroup 1 stores dK * scale
-    if (ok) ok = warp_wait(&bars->done, it & 1, p.status, kStatusTimeoutTmemFull);
-    if (ok && U > 0) {
-      tc_fence_after();
-      const int kv_row = j * kTile + r_local;
-      const bool row_ok = kv_row < w.len;
-      const int64_t* st = wg == 0 ? p.dv_strides : p.dk_strides;
-      uint16_t* orow = reinterpret_cast<uint16_t*>(wg == 0 ? p.dv : p.dk) +
-                       (static_cast<int64_t>(w.start) + kv_row) * st[0] + kv_head * st[1];
-      const float mul = wg == 0 ? 1.0f : p.scale;
-      const uint32_t acc_addr = tmem_base + 256 + wg * 128 + lane_bits;
-#pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t r[32];
-        __syncwarp();
-        tmem_ld_32x32b_x32(acc_addr + c * 32, r);
-        tmem_ld_wait();
-        if (row_ok) {
-          uint4* dst = reinterpret_cast<uint4*>(orow + c * 32);
+        if (lane == 0) mbar_arrive(&bars->s_read);
+        ok = warp_wait(&bars->dp_full, (g + t) & 1, p.status, kStatusTimeoutTmemFull);
+        if (!ok) continue;
+        tc_fence_after();
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint4 o;
-            o.x = pack_pair(__uint_as_float(r[q * 8 + 0]) * mul, __uint_as_float(r[q * 8 + 1]) * mul, DT);
-            o.y = pack_pair(__uint_as_float(r[q * 8 + 2]) * mul, __uint_as_float(r[q * 8 + 3]) * mul, DT);
-            o.z = pack_pair(__uint_as_float(r[q * 8 + 4]) * mul, __uint_as_float(r[q * 8 + 5]) * mul, DT);
-            o.w = pack_pair(__uint_as_float(r[q * 8 + 6]) * mul, __uint_as_float(r[q * 8 + 7]) * mul, DT);
-            dst[q] = o;
+        for (int half = 0; half < 2; ++half) {
+          uint32_t rd[32], dk[16];
+          tmem_ld_32x32b_x32(dp_addr + half * 32, rd);
+          tmem_ld_wait();
+#pragma unroll
+          for (int y = 0; y < 8; ++y) {
+            const float4 e4 = *reinterpret_cast<const float4*>(a_del + half * 32 + 4 * y);
+            const float ev[4] = {e4.x, e4.y, e4.z, e4.w};
+            float dv[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) dv[c] = pv[half * 32 + 4 * y + c] * (__uint_as_float(rd[4 * y + c]) - ev[c]);
+            dk[2 * y] = pack_pair(dv[0], dv[1], DT);
+            dk[2 * y + 1] = pack_pair(dv[2], dv[3], DT);
           }
+          tmem_st_32x32b_x16(dp_addr + half * 16, dk);
         }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->ds_full);
+        if (wg_tid < 64 && t + 1 < nq) {
+          aux_slot(t + 1)[wg_tid] = next_lse;
+          aux_slot(t + 1)[64 + wg_tid] = next_delta;
+        }
+        i = i_next;
+        head = head_next;
+      }
+      // epilogue: warpgroup 0 stores dV, warpgroup 1 stores dK * scale
+      if (ok) ok = warp_wait(&bars->done, it & 1, p.status, kStatusTimeoutTmemFull);
+      if (ok) {
+        tc_fence_after();
+        const int kv_row = j * kTile + r_local;
+        const int64_t* st = wg == 0 ? p.dv_strides : p.dk_strides;
+        uint16_t* orow = reinterpret_cast<uint16_t*>(wg == 0 ? p.dv : p.dk) +
+                         (static_cast<int64_t>(w.start) + kv_row) * st[0] + kv_head * st[1];
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c)
+          store_columns<DT>(tmem_base + 256 + wg * 128 + lane_bits + c * 32, orow + c * 32, wg == 0 ? 1.0f : p.scale,
+                            kv_row < w.len);
       }
     }
-  }
-  // End of tile, without a CTA-wide barrier: the roles meet again only through the mbarriers. The
-  // producer waits for `done` before it refills K / V; the first dV / dK MMAs of the next tile
-  // (which overwrite the accumulators) wait for that tile's first P, and a softmax warp writes that
-  // only after it has stored its part of these accumulators.
-  sbase += nq;
-  ++it;
-  // a wait gave up: stop. A warpgroup decides together, its barrier needs all of it.
-  const bool go = p.status == nullptr || *reinterpret_cast<volatile int*>(p.status) == 0;
-  if (!(warp < 2 ? __all_sync(0xffffffffu, go) : wg_and((warp - 2) >> 2, go))) break;
+    // End of tile, without a CTA-wide barrier: the roles meet again only through the mbarriers. The
+    // producer waits for `done` before it refills K / V; the first dV / dK MMAs of the next tile
+    // (which overwrite the accumulators) wait for that tile's first P, and a softmax warp writes that
+    // only after it has stored its part of these accumulators.
+    g += nq;
+    ++it;
+    if (!go_on(warp, p.status)) break;
   }
   tc_fence_before();
   __syncthreads();
@@ -910,301 +984,235 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
 // ---- dQ: persistent CTAs over (query tile, head) -------------------------------------------------
 // Like the dK / dV kernel: one CTA per SM, tiles heaviest first (query tile i meets i + 1 key tiles
 // under the causal mask) handed out round by round in alternating CTA order, TMEM and barriers set
-// up once, parities on counters that persist across tiles (`it`, `sbase`), and no CTA-wide barrier
+// up once, parities on counters that persist across tiles (`it`, `g`), and no CTA-wide barrier
 // between tiles: the Q / dO loads and first score MMAs of the next tile overlap the dQ store.
+//
+// S = Q K^T and dP = dO V^T read Q and dO as A operands from TMEM (columns [384, 448) and [448, 512)),
+// where the softmax warps put them once per tile: an MMA then fetches only its B operand from shared
+// memory. P stays in registers; only dS is written back. The tensor core's order is
+// S(i+1) | dQ(i) dP(i+1):  S(i+1) needs S(i) read, the others dS(i).
 template <int D, int DT>
 __global__ void __launch_bounds__(320, 1)
 packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                   const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tdo,
-                   const PackedAttnArgs p) {
+                     const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tdo,
+                     const PackedAttnArgs p) {
   using C = BwdCfg<D>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                             ~static_cast<uintptr_t>(1023));
-  uint8_t* sQ = smem;
-  uint8_t* sDO = smem + C::kTileBytes;
-  uint8_t* sStage = smem + C::kResidentBytes;  // stage: [K tile | V tile]
-  BwdBarriers* bars = reinterpret_cast<BwdBarriers*>(sStage + C::kStages * C::kStageBytes + C::kAuxBytes);
+  extern __shared__ uint8_t smem[];
+  BwdBarriers* bars = reinterpret_cast<BwdBarriers*>(smem + 2048);
+  uint8_t* sQ = smem + C::kFrontBytes;
+  uint8_t* sDO = sQ + C::kTileBytes;
+  uint8_t* sRing = sDO + C::kTileBytes;         // K_0 V_0 K_1 V_1 ...
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = p.heads / p.kv_heads;
   const int total_tiles = p.num_q_tiles * p.heads;
-
-  if (threadIdx.x == 0) {
-    mbar_init(&bars->res_full, 1);
-    mbar_init(&bars->tail_full, 1);
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&bars->st_full[s], 1);
-      mbar_init(&bars->st_empty[s], 1);
-      mbar_init(&bars->s_full[s], 1);
-      mbar_init(&bars->p_full[s], 8);      // both softmax warpgroups work on every sub-tile, one arrival per warp
-      mbar_init(&bars->p_early[s], 8);
-    }
-    mbar_init(&bars->done, 1);
-    mbar_init(&bars->qdo_full, 8);         // one arrival per softmax warp
-    fence_mbar_init();
-    prefetch_tmap(&tq); prefetch_tmap(&tk); prefetch_tmap(&tv); prefetch_tmap(&tdo);
-  }
-  if (warp == 1) tmem_alloc(&bars->tmem_base, 512);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
+  if (!bwd_setup(smem, bars, warp, tq, tk, tv, tdo, p.status)) return;
   const uint32_t tmem_base = bars->tmem_base;
-  int p_stage = 0;           // producer: ring position of the next key/value stage (persists across tiles)
-  uint32_t p_phase = 0;
-  int sbase = 0;             // key/value tiles streamed by this CTA before the current tile
-  uint32_t cuts = 0;         // producer: tiles at a document's end so far
+  RingPos pos;               // producer and MMA issuer: slot of the next K tile
+  uint32_t cuts = 0;         // producer: tile pairs at a document's end so far
+  int g = 0;                 // key/value tiles streamed by this CTA before the current tile
 
   for (int round = 0, it = 0; round * static_cast<int>(gridDim.x) < total_tiles; ++round) {
-  const int tile = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-  if (tile >= total_tiles) continue;             // only in the last round
-  const PackedTile w = p.q_tiles[tile / p.heads];
-  const int head = tile % p.heads, kv_head = head / group;
-  const int i = w.tile;                          // query tile inside the document
-  const int kv_tiles = (w.len + kTile - 1) / kTile;
-  const int nkv = p.causal ? i + 1 : kv_tiles;
-  const int tail_rows = w.len - (kv_tiles - 1) * kTile;   // rows of the document's last tile
-  const int U = 2 * nkv;
-  if (warp == 0) {
-    // Q / dO are free once every MMA of the previous tile has completed
-    const bool free_q = it == 0 || warp_wait(&bars->done, (it - 1) & 1, p.status, kStatusTimeoutTmemFull);
-    if (free_q && elect_one()) {
-      mbar_expect_tx(&bars->res_full, C::kResidentBytes);
-#pragma unroll
-      for (int h = 0; h < C::kHalves; ++h) {
-        tma_load_3d(sQ + h * 16384, &tq, &bars->res_full, h * 64, w.start + i * kTile, head);
-        tma_load_3d(sDO + h * 16384, &tdo, &bars->res_full, h * 64, w.start + i * kTile, head);
-      }
-    }
-    int stage = p_stage;
-    uint32_t phase = p_phase;
-    for (int t = 0; t < nkv && free_q; ++t) {
-      if (!warp_wait(&bars->st_empty[stage], phase ^ 1, p.status, kStatusTimeoutEmpty)) break;
-      uint8_t* sk = sStage + stage * C::kStageBytes;
-      uint8_t* sv = sk + C::kTileBytes;
-      const bool cut = t == kv_tiles - 1 && tail_rows < kTile;
-      __syncwarp();
-      if (elect_one()) {
-        uint64_t* full = cut ? &bars->tail_full : &bars->st_full[stage];
-        mbar_expect_tx(full, C::kStageBytes);
+    const int tile = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+    if (tile >= total_tiles) continue;             // only in the last round
+    const PackedTile w = p.q_tiles[tile / p.heads];
+    const int head = tile % p.heads, kv_head = head / group;
+    const int i = w.tile;                          // query tile inside the document
+    const int kv_tiles = (w.len + kTile - 1) / kTile;
+    const int n = p.causal ? i + 1 : kv_tiles;
+    const int last_rows = w.len - (kv_tiles - 1) * kTile;   // rows of the document's last tile
+    if (warp == 0) {
+      // Q / dO are free once every MMA of the previous tile has completed
+      bool ok = it == 0 || warp_wait(&bars->done, (it - 1) & 1, p.status, kStatusTimeoutTmemFull);
+      if (ok && elect_one()) {
+        mbar_expect_tx(&bars->res_full, 2 * C::kTileBytes);
 #pragma unroll
         for (int h = 0; h < C::kHalves; ++h) {
-          tma_load_3d(sk + h * 16384, &tk, full, h * 64, w.start + t * kTile, kv_head);
-          tma_load_3d(sv + h * 16384, &tv, full, h * 64, w.start + t * kTile, kv_head);
+          tma_load_3d(sQ + h * 16384, &tq, &bars->res_full, h * 64, w.start + i * kTile, head);
+          tma_load_3d(sDO + h * 16384, &tdo, &bars->res_full, h * 64, w.start + i * kTile, head);
         }
       }
       __syncwarp();
-      if (cut) {   // keys behind the document's end are summands of dQ: 0 times them must be 0
-        if (!warp_wait(&bars->tail_full, cuts & 1, p.status, kStatusTimeoutFull)) break;
-        ++cuts;
-        clear_tail<C::kHalves>(sk, tail_rows, lane);
-        clear_tail<C::kHalves>(sv, tail_rows, lane);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->st_full[stage]);
-      }
-      if (++stage == 2) { stage = 0; phase ^= 1; }
-    }
-    // every lane tracks the ring position, whichever lane is elected next time
-    p_phase ^= static_cast<uint32_t>(((p_stage + nkv) >> 1) & 1);
-    p_stage = (p_stage + nkv) & 1;
-  } else if (warp == 1) {
-    if (elect_one()) {
-      const int fmt = DT == kBF16 ? 1 : 0;
-      const uint32_t idesc_s = make_idesc_f16(fmt, 0, 0, 128, 64);
-      const uint32_t idesc_acc = make_idesc_f16(fmt, 0, 1, 128, D);
-      // short issue path: tile-origin descriptors once, constants added per MMA
-      const uint64_t dKk0 = make_smem_desc_sw128(smem_u32(sStage), 16, 1024);          // K-major view
-      const uint64_t dKm0 = make_smem_desc_sw128(smem_u32(sStage), 16384, 1024);       // MN-major view
-      // Q and dO are A operands read from TMEM (columns [384, 448) and [448, 512), staged there by
-      // the softmax warps): a score MMA then reads only its 2 KB B operand from shared memory, where
-      // with both operands in shared memory the N = 64 MMAs ran into the 128 B/clk of the SM.
-      auto issue_sdp = [&](int u) {
-        const int stage = (sbase + (u >> 1)) & 1, sub = u & 1, b = u & 1;
-        const uint64_t dK = desc_advance(dKk0, stage * C::kStageBytes + sub * 8192);
-        const uint64_t dV = desc_advance(dK, C::kTileBytes);
+      for (int t = 0; t < n && ok; ++t)
+        ok = stream_pair<D>(bars, sRing, pos, cuts, &tk, &tv, w.start + t * kTile, kv_head,
+                            t == kv_tiles - 1 ? last_rows : kTile, lane, p.status);
+    } else if (warp == 1) {
+      if (elect_one()) {
+        const int fmt = DT == kBF16 ? 1 : 0;
+        const uint32_t idesc_s = make_idesc_f16(fmt, 0, 0, 128, 128);
+        const uint32_t idesc_acc = make_idesc_f16(fmt, 0, 1, 128, D);
+        // short issue path: tile-origin descriptors once, constants added per MMA
+        const uint64_t dRk = make_smem_desc_sw128(smem_u32(sRing), 16, 1024);          // K-major view
+        const uint64_t dRm = make_smem_desc_sw128(smem_u32(sRing), 16384, 1024);       // MN-major view
+        auto issue_scores = [&](uint32_t a, int slot, uint32_t tmem, uint64_t* full) {
+          const uint64_t b0 = desc_advance(dRk, slot * C::kTileBytes);
 #pragma unroll
-        for (int h = 0; h < C::kHalves; ++h)
+          for (int h = 0; h < C::kHalves; ++h)
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            tc_mma_f16_ts(tmem_base + b * 128, tmem_base + 384 + (h * 4 + k) * 8,
-                          desc_advance(dK, h * 16384 + k * 32), idesc_s, (h | k) != 0 ? 1u : 0u);
+            for (int k = 0; k < 4; ++k)
+              tc_mma_f16_ts(tmem_base + tmem, tmem_base + a + (h * 4 + k) * 8, desc_advance(b0, h * 16384 + k * 32),
+                            idesc_s, (h | k) != 0 ? 1u : 0u);
+          tc_commit(full);
+        };
+        // keys 0-63 of dS sit at columns [0, 32) of the dP buffer, keys 64-127 at [64, 96); the first 32
+        // keys of each warpgroup (k-steps 0 1 4 5) are handed over before the others (2 3 6 7)
+        auto issue_acc = [&](int slot, int half, bool first) {
+          const uint64_t b0 = desc_advance(dRm, slot * C::kTileBytes);
 #pragma unroll
-        for (int h = 0; h < C::kHalves; ++h)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            tc_mma_f16_ts(tmem_base + b * 128 + 64, tmem_base + 448 + (h * 4 + k) * 8,
-                          desc_advance(dV, h * 16384 + k * 32), idesc_s, (h | k) != 0 ? 1u : 0u);
-        tc_commit(&bars->s_full[b]);
-      };
-      bool ok = mbar_wait(&bars->qdo_full, it & 1, p.status, kStatusTimeoutFull);
-      if (ok && U > 0) {
-        ok = mbar_wait(&bars->st_full[sbase & 1], (sbase >> 1) & 1, p.status, kStatusTimeoutFull);
-        tc_fence_after();
-        if (ok) { issue_sdp(0); issue_sdp(1); }
-      }
-      for (int u = 0; u < U && ok; ++u) {
-        const int b = u & 1, stage = (sbase + (u >> 1)) & 1, sub = u & 1;
-        // dQ += dS K; keys 0-31 of dS sit at columns [0, 16), keys 32-63 at [32, 48). The first 16
-        // keys of each warpgroup (k-steps 0 and 2) are handed over before the other 16 (1 and 3).
-        const uint64_t dK = desc_advance(dKm0, stage * C::kStageBytes + sub * 8192);
-        ok = mbar_wait(&bars->p_early[b], (sbase + (u >> 1)) & 1, p.status, kStatusTimeoutTmemFull);
-        if (!ok) break;
-        tc_fence_after();
-#pragma unroll
-        for (int k = 0; k < 4; k += 2)
-          tc_mma_f16_ts(tmem_base + 256, tmem_base + b * 128 + 64 + (k >> 1) * 32 + (k & 1) * 8,
-                        desc_advance(dK, k * 2048), idesc_acc, (u | k) != 0 ? 1u : 0u);
-        ok = mbar_wait(&bars->p_full[b], (sbase + (u >> 1)) & 1, p.status, kStatusTimeoutTmemFull);
-        if (!ok) break;
-        tc_fence_after();
-#pragma unroll
-        for (int k = 1; k < 4; k += 2)
-          tc_mma_f16_ts(tmem_base + 256, tmem_base + b * 128 + 64 + (k >> 1) * 32 + (k & 1) * 8,
-                        desc_advance(dK, k * 2048), idesc_acc, 1u);
-        if (sub == 1) tc_commit(&bars->st_empty[stage]);
-        if (u + 2 < U) {
-          const int u2 = u + 2;
-          if ((u2 & 1) == 0) {
-            const int sq = sbase + (u2 >> 1);
-            ok = mbar_wait(&bars->st_full[sq & 1], (sq >> 1) & 1, p.status, kStatusTimeoutFull);
+          for (int q = 0; q < 4; ++q) {
+            const int k = (q >> 1) * 4 + half * 2 + (q & 1);
+            tc_mma_f16_ts(tmem_base + 256, tmem_base + 128 + (k >> 2) * 64 + (k & 3) * 8, desc_advance(b0, k * 2048),
+                          idesc_acc, first && half == 0 && q == 0 ? 0u : 1u);
+          }
+        };
+        auto wait_full = [&](const RingPos& at) {
+          const bool got = mbar_wait(&bars->full[at.slot], at.phase, p.status, kStatusTimeoutFull);
+          tc_fence_after();
+          return got;
+        };
+        auto wait_softmax = [&](uint64_t* bar, int iter) {
+          const bool got = mbar_wait(bar, iter & 1, p.status, kStatusTimeoutTmemFull);
+          tc_fence_after();
+          return got;
+        };
+        RingPos at = pos;
+        bool ok = mbar_wait(&bars->qdo_full, it & 1, p.status, kStatusTimeoutFull) && wait_full(at);
+        if (ok) {
+          tc_fence_after();
+          issue_scores(384, at.slot, 0, &bars->s_full);
+          ok = wait_full(at.next(1));
+          if (ok) {
+            issue_scores(448, at.next(1).slot, 128, &bars->dp_full);
+            tc_commit(&bars->empty[at.next(1).slot]);
+          }
+        }
+        for (int t = 0; t < n && ok; ++t) {
+          const RingPos kn = at.next(2), vn = at.next(3);
+          if (t + 1 < n) {
+            ok = wait_full(kn) && wait_softmax(&bars->s_read, g + t);
             if (!ok) break;
-            tc_fence_after();
+            issue_scores(384, kn.slot, 0, &bars->s_full);
           }
-          issue_sdp(u2);
+          ok = wait_softmax(&bars->ds_half, g + t);
+          if (!ok) break;
+          issue_acc(at.slot, 0, t == 0);                            // dQ += dS K
+          ok = wait_softmax(&bars->ds_full, g + t);
+          if (!ok) break;
+          issue_acc(at.slot, 1, t == 0);
+          tc_commit(&bars->empty[at.slot]);
+          if (t + 1 < n) {
+            ok = wait_full(vn);
+            if (!ok) break;
+            issue_scores(448, vn.slot, 128, &bars->dp_full);
+            tc_commit(&bars->empty[vn.slot]);
+          }
+          at = kn;
         }
+        tc_commit(&bars->done);
       }
-      tc_commit(&bars->done);
-    }
-  } else {
-    const int wg = (warp - 2) >> 2;
-    const int quarter = warp & 3;
-    const int r_local = quarter * 32 + lane;     // query row inside the tile
-    const int q_local = i * kTile + r_local;     // row inside the document
-    const bool row_ok = q_local < w.len;
-    const int64_t q_row = static_cast<int64_t>(w.start) + q_local;
-    const uint32_t lane_bits = static_cast<uint32_t>(quarter * 32) << 16;
-    const float sl2 = p.scale * kLog2e;
-    const int64_t at = static_cast<int64_t>(head) * p.rows + q_row;
-    const float lse2 = row_ok ? p.lse[at] * kLog2e : INFINITY;
-    const float delta = row_ok ? p.delta[at] : 0.f;
-    bool ok = true;
-    // Stage the tile's rows as TMEM operands: warpgroup 0 copies the Q rows, warpgroup 1 the dO rows,
-    // one thread per row, out of the 128-byte-swizzled tiles the TMA wrote (16-byte chunk c of row r
-    // sits at chunk c ^ (r & 7)); element d of a row lands in TMEM column d / 2 of the operand.
-    ok = warp_wait(&bars->res_full, it & 1, p.status, kStatusTimeoutFull);
-    if (ok) {
-      const uint8_t* src = (wg == 0 ? sQ : sDO) + r_local * 128;
-      const uint32_t dst = tmem_base + 384 + wg * 64 + lane_bits;
       __syncwarp();
+      // every lane tracks the ring position, whichever lane is elected next time
+      const int items = 2 * n;
+      pos.phase ^= static_cast<uint32_t>(((pos.slot + items) / 5) & 1);
+      pos.slot = (pos.slot + items) % 5;
+    } else {
+      const int wg = (warp - 2) >> 2;      // columns [64 wg, 64 wg + 64) of every tile
+      const int quarter = warp & 3;
+      const int r_local = quarter * 32 + lane;     // query row inside the tile
+      const int q_local = i * kTile + r_local;     // row inside the document
+      const bool row_ok = q_local < w.len;
+      const int64_t q_row = static_cast<int64_t>(w.start) + q_local;
+      const uint32_t lane_bits = static_cast<uint32_t>(quarter * 32) << 16;
+      const uint32_t s_addr = tmem_base + wg * 64 + lane_bits, dp_addr = s_addr + 128;
+      const float sl2 = p.scale * kLog2e;
+      const int64_t at = static_cast<int64_t>(head) * p.rows + q_row;
+      const float neg_lse = row_ok ? -p.lse[at] * kLog2e : -INFINITY;
+      const float delta = row_ok ? p.delta[at] : 0.f;
+      // Stage the tile's rows as TMEM operands: warpgroup 0 copies the Q rows, warpgroup 1 the dO rows,
+      // one thread per row, out of the 128-byte-swizzled tiles the TMA wrote (16-byte chunk c of row r
+      // sits at chunk c ^ (r & 7)); element d of a row lands in TMEM column d / 2 of the operand.
+      bool ok = warp_wait(&bars->res_full, it & 1, p.status, kStatusTimeoutFull);
+      if (ok) {
+        const uint8_t* src = (wg == 0 ? sQ : sDO) + r_local * 128;
+        const uint32_t dst = tmem_base + 384 + wg * 64 + lane_bits;
 #pragma unroll
-      for (int h = 0; h < C::kHalves; ++h)
+        for (int h = 0; h < C::kHalves; ++h)
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          uint32_t v[16];
+          for (int gq = 0; gq < 2; ++gq) {
+            uint32_t v[16];
 #pragma unroll
-          for (int c4 = 0; c4 < 4; ++c4) {
-            const int c = g * 4 + c4;
-            const uint4 x = *reinterpret_cast<const uint4*>(src + h * 16384 + ((c ^ (r_local & 7)) << 4));
-            v[c4 * 4 + 0] = x.x; v[c4 * 4 + 1] = x.y; v[c4 * 4 + 2] = x.z; v[c4 * 4 + 3] = x.w;
+            for (int c4 = 0; c4 < 4; ++c4) {
+              const int c = gq * 4 + c4;
+              const uint4 x = *reinterpret_cast<const uint4*>(src + h * 16384 + ((c ^ (r_local & 7)) << 4));
+              v[c4 * 4 + 0] = x.x; v[c4 * 4 + 1] = x.y; v[c4 * 4 + 2] = x.z; v[c4 * 4 + 3] = x.w;
+            }
+            tmem_st_32x32b_x16(dst + h * 32 + gq * 16, v);
           }
-          tmem_st_32x32b_x16(dst + h * 32 + g * 16, v);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->qdo_full);
+      }
+      for (int t = 0; t < n && ok; ++t) {
+        ok = warp_wait(&bars->s_full, (g + t) & 1, p.status, kStatusTimeoutTmemFull);
+        if (!ok) break;
+        tc_fence_after();
+        const int kv0 = t * kTile + wg * 64;              // first key of this warpgroup's columns
+        const bool masked = (p.causal && t == i) || kv0 + 64 > w.len;
+        float pv[64];
+        {
+          uint32_t rs[2][32];
+          tmem_ld_32x32b_x32(s_addr, rs[0]);
+          tmem_ld_32x32b_x32(s_addr + 32, rs[1]);
+          tmem_ld_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->s_read);
+#pragma unroll
+          for (int e = 0; e < 64; ++e) pv[e] = exp2f(fmaf(__uint_as_float(rs[e >> 5][e & 31]), sl2, neg_lse));
         }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->qdo_full);
-    }
-    // Both warpgroups work on every 64-key sub-tile, each on 32 of its columns: the time from
-    // "scores ready" to "dS ready" halves, so it fits under the score MMAs of the other buffer and
-    // the tensor core seldom waits for it. A warpgroup writes its 16-bit dS over the first half of
-    // the dP columns it has just read (its own input), never over the other warpgroup's.
-    for (int u = 0; u < U && ok; ++u) {
-      const int t = u >> 1, sub = u & 1;
-      const uint32_t s_addr = tmem_base + sub * 128 + wg * 32 + lane_bits;
-      const uint32_t dp_addr = s_addr + 64;
-      ok = warp_wait(&bars->s_full[sub], (sbase + t) & 1, p.status, kStatusTimeoutTmemFull);
-      if (!ok) break;
-      tc_fence_after();
-      const bool diag = p.causal && (t == i);
-      const int kv0 = t * kTile + sub * 64 + wg * 32;   // first key index of this warpgroup's columns
-      const bool ragged = kv0 + 32 > w.len;
-      uint32_t rs[32], rd[32];
-      __syncwarp();
-      tmem_ld_32x32b_x32(s_addr, rs);
-      tmem_ld_32x32b_x32(dp_addr, rd);
-      tmem_ld_wait();
-      uint32_t dk[16];
-      const float neg_lse = -lse2;
+        if (masked) {   // the common case carries no mask
+          // keys this row sees: up to itself on the diagonal tile, up to the document's end on the last
+          const int seen = min(p.causal && t == i ? q_local + 1 : w.len, w.len) - kv0;
 #pragma unroll
-      for (int part = 0; part < 2; ++part) {   // 16 keys at a time, handed over as soon as they are written
-        if (!(diag || ragged)) {   // the common case carries no mask
-#pragma unroll
-          for (int x = part * 8; x < part * 8 + 8; ++x) {
-            const float p0 = exp2f(fmaf(__uint_as_float(rs[2 * x]), sl2, neg_lse));
-            const float p1 = exp2f(fmaf(__uint_as_float(rs[2 * x + 1]), sl2, neg_lse));
-            dk[x] = pack_pair(p0 * (__uint_as_float(rd[2 * x]) - delta), p1 * (__uint_as_float(rd[2 * x + 1]) - delta),
-                              DT);
-          }
-        } else {
-#pragma unroll
-          for (int x = part * 8; x < part * 8 + 8; ++x) {
-            const int col = 2 * x;
-            const int kl = sub * 64 + wg * 32 + col;      // key row inside the 128-row tile
-            float p0 = exp2f(fmaf(__uint_as_float(rs[2 * x]), sl2, neg_lse));
-            float p1 = exp2f(fmaf(__uint_as_float(rs[2 * x + 1]), sl2, neg_lse));
-            if ((diag && kl > r_local) || (ragged && kv0 + col >= w.len)) p0 = 0.f;
-            if ((diag && kl + 1 > r_local) || (ragged && kv0 + col + 1 >= w.len)) p1 = 0.f;
-            dk[x] = pack_pair(p0 * (__uint_as_float(rd[2 * x]) - delta), p1 * (__uint_as_float(rd[2 * x + 1]) - delta),
-                              DT);
-          }
+          for (int e = 0; e < 64; ++e)
+            if (e >= seen) pv[e] = 0.f;
         }
-        if (part == 0) {
-          tmem_st_32x32b_x8(dp_addr, dk);
+        ok = warp_wait(&bars->dp_full, (g + t) & 1, p.status, kStatusTimeoutTmemFull);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t rd[32], dk[16];
+          tmem_ld_32x32b_x32(dp_addr + half * 32, rd);
+          tmem_ld_wait();
+#pragma unroll
+          for (int x = 0; x < 16; ++x)
+            dk[x] = pack_pair(pv[half * 32 + 2 * x] * (__uint_as_float(rd[2 * x]) - delta),
+                              pv[half * 32 + 2 * x + 1] * (__uint_as_float(rd[2 * x + 1]) - delta), DT);
+          tmem_st_32x32b_x16(dp_addr + half * 16, dk);
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->p_early[sub]);
+          if (lane == 0) mbar_arrive(half == 0 ? &bars->ds_half : &bars->ds_full);
         }
       }
-      tmem_st_32x32b_x8(dp_addr + 8, dk + 8);
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->p_full[sub]);   // one arrival per warp
-    }
-    if (ok) ok = warp_wait(&bars->done, it & 1, p.status, kStatusTimeoutTmemFull);
-    if (ok && U > 0) {
-      tc_fence_after();
-      // each warpgroup stores half of the head dimension
-      uint16_t* orow = reinterpret_cast<uint16_t*>(p.dq) + q_row * p.dq_strides[0] + head * p.dq_strides[1];
-      const uint32_t acc_addr = tmem_base + 256 + lane_bits;
+      if (ok) ok = warp_wait(&bars->done, it & 1, p.status, kStatusTimeoutTmemFull);
+      if (ok) {
+        tc_fence_after();
+        // each warpgroup stores half of the head dimension
+        uint16_t* orow = reinterpret_cast<uint16_t*>(p.dq) + q_row * p.dq_strides[0] + head * p.dq_strides[1];
 #pragma unroll 1
-      for (int c = wg * (D / 64); c < (wg + 1) * (D / 64); ++c) {
-        uint32_t r[32];
-        __syncwarp();
-        tmem_ld_32x32b_x32(acc_addr + c * 32, r);
-        tmem_ld_wait();
-        if (row_ok) {
-          uint4* dst = reinterpret_cast<uint4*>(orow + c * 32);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint4 o;
-            o.x = pack_pair(__uint_as_float(r[q * 8 + 0]) * p.scale, __uint_as_float(r[q * 8 + 1]) * p.scale, DT);
-            o.y = pack_pair(__uint_as_float(r[q * 8 + 2]) * p.scale, __uint_as_float(r[q * 8 + 3]) * p.scale, DT);
-            o.z = pack_pair(__uint_as_float(r[q * 8 + 4]) * p.scale, __uint_as_float(r[q * 8 + 5]) * p.scale, DT);
-            o.w = pack_pair(__uint_as_float(r[q * 8 + 6]) * p.scale, __uint_as_float(r[q * 8 + 7]) * p.scale, DT);
-            dst[q] = o;
-          }
-        }
+        for (int c = wg * (D / 64); c < (wg + 1) * (D / 64); ++c)
+          store_columns<DT>(tmem_base + 256 + lane_bits + c * 32, orow + c * 32, p.scale, row_ok);
       }
     }
-  }
-  // End of tile, without a CTA-wide barrier: the producer waits for `done` before it reloads Q / dO;
-  // the first dQ MMAs of the next tile (which overwrite the accumulator) wait for that tile's first
-  // dS, and a softmax warp writes that only after it has stored its part of this accumulator.
-  sbase += nkv;
-  ++it;
-  if (!__all_sync(0xffffffffu, p.status == nullptr || *reinterpret_cast<volatile int*>(p.status) == 0)) break;
+    // End of tile, without a CTA-wide barrier: the producer waits for `done` before it reloads Q / dO;
+    // the first dQ MMAs of the next tile (which overwrite the accumulator) wait for that tile's first
+    // dS, and a softmax warp writes that only after it has stored its part of this accumulator.
+    g += n;
+    ++it;
+    if (!go_on(warp, p.status)) break;
   }
   tc_fence_before();
   __syncthreads();
