@@ -530,6 +530,9 @@ struct BwdBarriers {
   uint64_t ds_full;       // dS is written
   uint64_t done;
   uint64_t qdo_full;      // dQ: the Q and dO rows of the tile sit in TMEM
+  uint64_t unit_full[2];  // the next unit of work is known
+  uint64_t unit_empty[2];
+  int unit[2];
   uint32_t tmem_base;
 };
 
@@ -570,6 +573,10 @@ __device__ __forceinline__ bool bwd_setup(uint8_t* smem, BwdBarriers* bars, int 
     mbar_init(&bars->ds_full, 8);
     mbar_init(&bars->done, 1);
     mbar_init(&bars->qdo_full, 8);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars->unit_full[s], 1);
+      mbar_init(&bars->unit_empty[s], 9);   // every warp but the producer's
+    }
     fence_mbar_init();
     prefetch_tmap(&tq); prefetch_tmap(&tk); prefetch_tmap(&tv); prefetch_tmap(&tdo);
   }
@@ -578,6 +585,34 @@ __device__ __forceinline__ bool bwd_setup(uint8_t* smem, BwdBarriers* bars, int 
   __syncthreads();
   tc_fence_after();
   return true;
+}
+
+// The unit of work that this CTA takes as its `it`-th, -1 when there is none left. Units are sorted
+// heaviest first and taken from a common counter, so CTAs with short units take more of them: which CTA
+// works on a unit depends on timing, its result does not. The producer warp asks (its loads run ahead,
+// so the answer is there before the others need it) and passes the number on.
+__device__ __forceinline__ int next_unit(BwdBarriers* bars, int it, int units, int* counter, int warp, int lane,
+                                         int* status) {
+  const int b = it & 1;
+  const uint32_t phase = static_cast<uint32_t>(it >> 1) & 1;
+  int unit = -1;
+  if (warp == 0) {
+    if (lane == 0) unit = it == 0 ? static_cast<int>(blockIdx.x) : static_cast<int>(gridDim.x) + atomicAdd(counter, 1);
+    unit = __shfl_sync(0xffffffffu, unit, 0);
+    if (unit >= units) unit = -1;
+    if (!warp_wait(&bars->unit_empty[b], phase ^ 1, status, kStatusTimeoutEmpty)) unit = -1;
+    if (lane == 0) {
+      bars->unit[b] = unit;
+      mbar_arrive(&bars->unit_full[b]);
+    }
+    __syncwarp();
+    return unit;
+  }
+  if (!warp_wait(&bars->unit_full[b], phase, status, kStatusTimeoutFull)) return -1;
+  unit = *reinterpret_cast<volatile int*>(&bars->unit[b]);
+  __syncwarp();
+  if (lane == 0) mbar_arrive(&bars->unit_empty[b]);
+  return unit;
 }
 
 // Producer warp: streams tile `row` of two tensors (heads ha, hb) through the next two slots. With
@@ -653,6 +688,9 @@ __device__ __forceinline__ bool wg_and(int wg, bool ok) {
   return all != 0;
 }
 
+// The smallest value of a warpgroup: all of it has the same unit of work, or, after a timeout, none.
+__device__ __forceinline__ int wg_min(int wg, int v) { return wg_and(wg, v >= 0) ? v : -1; }
+
 // A wait gave up somewhere: stop after this tile. A warpgroup decides together, its barrier needs all of it.
 __device__ __forceinline__ bool go_on(int warp, const int* status) {
   const bool go = status == nullptr || *reinterpret_cast<const volatile int*>(status) == 0;
@@ -703,6 +741,7 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const PackedAttnArgs 
     const int64_t i = row0 + u * stride;
     if (vec == 0 && i < total) p.delta[(i % p.heads) * p.rows + i / p.heads] = acc;
   }
+  if (blockIdx.x == 0 && threadIdx.x < 2) p.counters[threadIdx.x] = 0;   // of the two kernels that follow
   if (p.used < p.rows) {
     clear_rows<D>(p.dq, p.dq_strides[0], p.dq_strides[1], p.used, p.rows, p.heads, blockIdx.x, gridDim.x);
     clear_rows<D>(p.dk, p.dk_strides[0], p.dk_strides[1], p.used, p.rows, p.kv_heads, blockIdx.x, gridDim.x);
@@ -710,9 +749,35 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const PackedAttnArgs 
   }
 }
 
+// dV | dK = sum over the splits, in their order: one thread per eight columns.
+template <int D>
+__global__ void __launch_bounds__(256) packed_join_kernel(const PackedAttnArgs p) {
+  constexpr int kChunks = D / 8;
+  const int64_t per = static_cast<int64_t>(p.used) * p.kv_heads * kChunks;      // chunks of one tensor
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (at >= 2 * per) return;
+  const int which = at >= per;                                                 // 0: dV, 1: dK
+  const int64_t i = at - which * per;
+  float sum[8] = {};
+  for (int sp = 0; sp < p.splits; ++sp) {
+    const float4* src = reinterpret_cast<const float4*>(p.parts + ((sp * 2 + which) * per + i) * 8);
+    const float4 a = src[0], b = src[1];
+    sum[0] += a.x; sum[1] += a.y; sum[2] += a.z; sum[3] += a.w;
+    sum[4] += b.x; sum[5] += b.y; sum[6] += b.z; sum[7] += b.w;
+  }
+  const int c = static_cast<int>(i % kChunks);
+  const int64_t rh = i / kChunks, row = rh / p.kv_heads, head = rh % p.kv_heads;
+  uint16_t* dst = which == 0 ? reinterpret_cast<uint16_t*>(p.dv) + row * p.dv_strides[0] + head * p.dv_strides[1]
+                             : reinterpret_cast<uint16_t*>(p.dk) + row * p.dk_strides[0] + head * p.dk_strides[1];
+  reinterpret_cast<uint4*>(dst)[c] = make_uint4(pack2(sum[0], sum[1], p.dtype), pack2(sum[2], sum[3], p.dtype),
+                                                pack2(sum[4], sum[5], p.dtype), pack2(sum[6], sum[7], p.dtype));
+}
+
 // ---- dK / dV: persistent CTAs over (key/value tile, key/value head) ------------------------------
-// One CTA per SM walks a static list of tiles, heaviest first (under the causal mask key tile j
-// meets tiles - j query tiles of each head), handed out round by round in alternating CTA order.
+// One CTA per SM takes units of work from a list sorted heaviest first (under the causal mask key tile j
+// meets tiles - j query tiles of each head). Where heads share a key/value head and there are too few
+// units for the SMs, a unit is split by heads (`splits`, see packed_bwd_splits) and packed_join_kernel
+// adds the parts.
 // TMEM, the barriers and the tensor-map prefetch are set up once per CTA; barrier parities therefore
 // run on counters that persist across tiles (`it`: tiles done by this CTA, `g`: query tiles streamed).
 // No CTA-wide barrier separates the tiles: the loads and first score MMAs of the next tile overlap the
@@ -734,24 +799,26 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
   uint8_t* sRing = sV + C::kTileBytes;          // Q_0 dO_0 Q_1 dO_1 ...
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = p.heads / p.kv_heads;
-  const int total_tiles = p.num_k_tiles * p.kv_heads;
+  const int group = p.heads / p.kv_heads, share = group / p.splits;
+  const int units = p.num_k_tiles * p.kv_heads * p.splits;
   if (!bwd_setup(smem, bars, warp, tq, tk, tv, tdo, p.status)) return;
   const uint32_t tmem_base = bars->tmem_base;
   RingPos pos;               // producer and MMA issuer: slot of the next Q tile
   uint32_t cuts = 0;         // producer: tile pairs at a document's end so far
   int g = 0;                 // query tiles streamed by this CTA before the current tile
 
-  for (int round = 0, it = 0; round * static_cast<int>(gridDim.x) < total_tiles; ++round) {
-    const int tile = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-    if (tile >= total_tiles) continue;             // only in the last round
-    const PackedTile w = p.k_tiles[tile / p.kv_heads];
-    const int kv_head = tile % p.kv_heads;
+  for (int it = 0;; ++it) {
+    int unit = next_unit(bars, it, units, p.counters, warp, lane, p.status);
+    if (warp >= 2) unit = wg_min((warp - 2) >> 2, unit);
+    if (unit < 0) break;
+    const PackedTile w = p.k_tiles[unit / (p.kv_heads * p.splits)];
+    const int kv_head = unit % (p.kv_heads * p.splits) / p.splits, split = unit % p.splits;
+    const int head0 = kv_head * group + split * share;
     const int j = w.tile;                          // key/value tile inside the document
     const int q_tiles = (w.len + kTile - 1) / kTile;
     const int i0 = p.causal ? j : 0;
     const int nd = q_tiles - i0;                   // query tiles of the document that see these keys
-    const int nq = nd * group;                     // streamed: all of them for every head of the group
+    const int nq = nd * share;                     // streamed: all of them for every head of this split
     const int last_rows = w.len - (q_tiles - 1) * kTile;   // rows of the document's last tile
     if (warp == 0) {
       // the resident K / V buffers are free once every MMA of the previous tile has completed; the
@@ -766,7 +833,7 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
         }
       }
       __syncwarp();
-      for (int t = 0, i = i0, head = kv_head * group; t < nq && ok; ++t) {
+      for (int t = 0, i = i0, head = head0; t < nq && ok; ++t) {
         ok = stream_pair<D>(bars, sRing, pos, cuts, &tq, &tdo, w.start + i * kTile, head,
                             i == q_tiles - 1 ? last_rows : kTile, lane, p.status);
         if (++i == q_tiles) { i = i0; ++head; }
@@ -856,8 +923,7 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
       bool ok = true;
       // lse / delta of this warpgroup's 64 queries, staged one query tile ahead: the global loads for
       // tile t + 1 are issued before tile t is processed and parked in shared memory after it, so their
-      // latency is never waited for. Streamed tile t is query tile i0 + t % nd of head
-      // kv_head * group + t / nd.
+      // latency is never waited for. Streamed tile t is query tile i0 + t % nd of head head0 + t / nd.
       auto aux_load = [&](int i, int head, float& lse, float& delta) {
         const int qi = i * kTile + wg * 64 + wg_tid;
         const bool in = qi < w.len;
@@ -868,11 +934,11 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
       auto aux_slot = [&](int t) { return sAux + ((wg * 2 + (t & 1)) * 2) * 64; };   // [lse 64 | delta 64]
       if (wg_tid < 64) {
         float lse, delta;
-        aux_load(i0, kv_head * group, lse, delta);
+        aux_load(i0, head0, lse, delta);
         aux_slot(0)[wg_tid] = lse;
         aux_slot(0)[64 + wg_tid] = delta;
       }
-      int i = i0, head = kv_head * group;
+      int i = i0, head = head0;
       for (int t = 0; t < nq; ++t) {
         const int i_next = i + 1 == q_tiles ? i0 : i + 1, head_next = i + 1 == q_tiles ? head + 1 : head;
         ok = wg_and(wg, ok);             // tile t's values are staged; everyone has left tile t - 1
@@ -956,13 +1022,31 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
       if (ok) {
         tc_fence_after();
         const int kv_row = j * kTile + r_local;
-        const int64_t* st = wg == 0 ? p.dv_strides : p.dk_strides;
-        uint16_t* orow = reinterpret_cast<uint16_t*>(wg == 0 ? p.dv : p.dk) +
-                         (static_cast<int64_t>(w.start) + kv_row) * st[0] + kv_head * st[1];
+        const bool row_ok = kv_row < w.len;
+        const int64_t row = static_cast<int64_t>(w.start) + kv_row;
+        const uint32_t acc = tmem_base + 256 + wg * 128 + lane_bits;
+        const float mul = wg == 0 ? 1.0f : p.scale;
+        if (p.splits == 1) {
+          const int64_t* st = wg == 0 ? p.dv_strides : p.dk_strides;
+          uint16_t* orow = reinterpret_cast<uint16_t*>(wg == 0 ? p.dv : p.dk) + row * st[0] + kv_head * st[1];
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c)
-          store_columns<DT>(tmem_base + 256 + wg * 128 + lane_bits + c * 32, orow + c * 32, wg == 0 ? 1.0f : p.scale,
-                            kv_row < w.len);
+          for (int c = 0; c < D / 32; ++c) store_columns<DT>(acc + c * 32, orow + c * 32, mul, row_ok);
+        } else {   // [split, dV | dK, row, kv_head, D] in fp32, summed by packed_join_kernel
+          float* orow = p.parts + (((split * 2 + wg) * static_cast<int64_t>(p.used) + row) * p.kv_heads + kv_head) * D;
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t r[32];
+            __syncwarp();
+            tmem_ld_32x32b_x32(acc + c * 32, r);
+            tmem_ld_wait();
+            if (!row_ok) continue;
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              reinterpret_cast<float4*>(orow + c * 32)[q] =
+                  make_float4(__uint_as_float(r[4 * q]) * mul, __uint_as_float(r[4 * q + 1]) * mul,
+                              __uint_as_float(r[4 * q + 2]) * mul, __uint_as_float(r[4 * q + 3]) * mul);
+          }
+        }
       }
     }
     // End of tile, without a CTA-wide barrier: the roles meet again only through the mbarriers. The
@@ -970,7 +1054,6 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
     // (which overwrite the accumulators) wait for that tile's first P, and a softmax warp writes that
     // only after it has stored its part of these accumulators.
     g += nq;
-    ++it;
     if (!go_on(warp, p.status)) break;
   }
   tc_fence_before();
@@ -983,8 +1066,7 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
 
 // ---- dQ: persistent CTAs over (query tile, head) -------------------------------------------------
 // Like the dK / dV kernel: one CTA per SM, tiles heaviest first (query tile i meets i + 1 key tiles
-// under the causal mask) handed out round by round in alternating CTA order, TMEM and barriers set
-// up once, parities on counters that persist across tiles (`it`, `g`), and no CTA-wide barrier
+// under the causal mask), TMEM and barriers set up once, parities on counters that persist across tiles (`it`, `g`), and no CTA-wide barrier
 // between tiles: the Q / dO loads and first score MMAs of the next tile overlap the dQ store.
 //
 // S = Q K^T and dP = dO V^T read Q and dO as A operands from TMEM (columns [384, 448) and [448, 512)),
@@ -1005,18 +1087,19 @@ packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_consta
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = p.heads / p.kv_heads;
-  const int total_tiles = p.num_q_tiles * p.heads;
+  const int units = p.num_q_tiles * p.heads;
   if (!bwd_setup(smem, bars, warp, tq, tk, tv, tdo, p.status)) return;
   const uint32_t tmem_base = bars->tmem_base;
   RingPos pos;               // producer and MMA issuer: slot of the next K tile
   uint32_t cuts = 0;         // producer: tile pairs at a document's end so far
   int g = 0;                 // key/value tiles streamed by this CTA before the current tile
 
-  for (int round = 0, it = 0; round * static_cast<int>(gridDim.x) < total_tiles; ++round) {
-    const int tile = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-    if (tile >= total_tiles) continue;             // only in the last round
-    const PackedTile w = p.q_tiles[tile / p.heads];
-    const int head = tile % p.heads, kv_head = head / group;
+  for (int it = 0;; ++it) {
+    int unit = next_unit(bars, it, units, p.counters + 1, warp, lane, p.status);
+    if (warp >= 2) unit = wg_min((warp - 2) >> 2, unit);
+    if (unit < 0) break;
+    const PackedTile w = p.q_tiles[unit / p.heads];
+    const int head = unit % p.heads, kv_head = head / group;
     const int i = w.tile;                          // query tile inside the document
     const int kv_tiles = (w.len + kTile - 1) / kTile;
     const int n = p.causal ? i + 1 : kv_tiles;
@@ -1211,7 +1294,6 @@ packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_consta
     // the first dQ MMAs of the next tile (which overwrite the accumulator) wait for that tile's first
     // dS, and a softmax warp writes that only after it has stored its part of this accumulator.
     g += n;
-    ++it;
     if (!go_on(warp, p.status)) break;
   }
   tc_fence_before();
@@ -1233,7 +1315,7 @@ cudaError_t launch_bwd(const PackedAttnArgs& a, cudaStream_t st) {
   static std::atomic<uint64_t> done_kv{0}, done_q{0};
   ETHB_TRY(allow_smem(packed_bwd_dkdv_kernel<D, DT>, C::kSmemBytes, done_kv), "packed backward: shared memory");
   ETHB_TRY(allow_smem(packed_bwd_dq_kernel<D, DT>, C::kSmemBytes, done_q), "packed backward: shared memory");
-  const int64_t k_work = static_cast<int64_t>(a.num_k_tiles) * a.kv_heads;
+  const int64_t k_work = static_cast<int64_t>(a.num_k_tiles) * a.kv_heads * a.splits;
   const int64_t q_work = static_cast<int64_t>(a.num_q_tiles) * a.heads;
   ETHB_RETURN_IF(k_work > 0x3fffffff || q_work > 0x3fffffff, cudaErrorInvalidValue, "packed backward: too many tiles");
   const int sms = sm_count();
@@ -1247,6 +1329,11 @@ cudaError_t launch_bwd(const PackedAttnArgs& a, cudaStream_t st) {
     packed_bwd_dq_kernel<D, DT><<<static_cast<unsigned>(q_work < sms ? q_work : sms), C::kThreads, C::kSmemBytes,
                                   st>>>(tq, tk, tv, tdo, a);
     count_launch(2);
+    if (a.splits > 1) {
+      const int64_t chunks = 2 * static_cast<int64_t>(a.used) * a.kv_heads * (D / 8);
+      packed_join_kernel<D><<<static_cast<unsigned>((chunks + 255) / 256), 256, 0, st>>>(a);
+      count_launch();
+    }
   }
   return cudaGetLastError();
 }
@@ -1273,6 +1360,16 @@ cudaError_t launch_fwd_for(const PackedAttnArgs& a, cudaStream_t st) {
 
 }  // namespace
 
+int attention_packed_splits(int num_k_tiles, int heads, int kv_heads) {
+  const int group = heads / kv_heads;
+  const int64_t units = static_cast<int64_t>(num_k_tiles) * kv_heads;
+  int splits = 1;
+  while (units > 0 && splits < group && units * splits * 2 < 5 * 148) {
+    do ++splits; while (group % splits != 0);
+  }
+  return splits;
+}
+
 bool attention_packed_pairs_heads(int heads, int kv_heads) { return (heads / kv_heads) % 2 == 0; }
 
 cudaError_t attention_packed_fwd(const PackedAttnArgs& a, cudaStream_t st) {
@@ -1287,6 +1384,8 @@ cudaError_t attention_packed_fwd(const PackedAttnArgs& a, cudaStream_t st) {
 cudaError_t attention_packed_bwd(const PackedAttnArgs& a, cudaStream_t st) {
   ETHB_TRY(check_common(a), "packed backward");
   ETHB_TRY(check_out(a.o, a.o_strides), "packed backward: out");
+  ETHB_RETURN_IF(a.counters == nullptr || a.splits < 1 || (a.heads / a.kv_heads) % a.splits != 0 ||
+                     (a.splits > 1 && a.parts == nullptr), cudaErrorInvalidValue, "packed backward: workspace");
   ETHB_TRY(check_out(a.dq, a.dq_strides), "packed backward: dq");
   ETHB_TRY(check_out(a.dk, a.dk_strides), "packed backward: dk");
   ETHB_TRY(check_out(a.dv, a.dv_strides), "packed backward: dv");

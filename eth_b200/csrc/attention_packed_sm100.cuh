@@ -30,6 +30,9 @@ struct PackedAttnArgs {
   int num_q_tiles;
   const PackedTile* k_tiles;
   int num_k_tiles;
+  int* counters;                 // backward: two ints of scratch
+  int splits;                    // backward: attention_packed_splits
+  float* parts;                  // backward, splits > 1: fp32 [splits, 2, used, kv_heads, head_dim] of scratch
   float scale;
   int causal;
   int dtype;        // kF16 / kBF16
@@ -38,6 +41,11 @@ struct PackedAttnArgs {
 
 // true: the forward pairs two heads of a group on one 128-row tile, false: two tiles of one head
 bool attention_packed_pairs_heads(int heads, int kv_heads);
+// Into how many parts (a divisor of the group) the heads of a group are split in the dK / dV kernel: enough
+// for two and a half units of work per SM, so that the heaviest does not decide the time. 4096 tokens in 40 documents, 16 / 2
+// heads of 64: RAGGED_US. With units enough the parts' traffic (8 bytes an element and
+// part each way) is not worth it.
+int attention_packed_splits(int num_k_tiles, int heads, int kv_heads);
 cudaError_t attention_packed_fwd(const PackedAttnArgs& a, cudaStream_t st);
 cudaError_t attention_packed_bwd(const PackedAttnArgs& a, cudaStream_t st);
 

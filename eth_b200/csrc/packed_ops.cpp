@@ -143,6 +143,14 @@ std::tuple<Tensor, Tensor, Tensor> packed_bwd(const Tensor& d_out, const Tensor&
   a.delta = delta.data_ptr<float>();
   a.q_tiles = tile_list(l.tiles, q, a.num_q_tiles);
   a.k_tiles = tile_list(l.keys, q, a.num_k_tiles);
+  const Tensor counters = at::empty({2}, q.options().dtype(at::kInt));
+  a.counters = counters.data_ptr<int>();
+  a.splits = attention_packed_splits(a.num_k_tiles, a.heads, a.kv_heads);
+  Tensor parts;
+  if (a.splits > 1) {
+    parts = at::empty({a.splits, 2, l.used, k.size(1), q.size(2)}, q.options().dtype(at::kFloat));
+    a.parts = parts.data_ptr<float>();
+  }
   check(attention_packed_bwd(a, cur_stream()), "attention_packed_bwd");
   return {dq, dk, dv};
 }
