@@ -529,6 +529,7 @@ struct BwdBarriers {
   uint64_t ds_half;       // dQ: the first 32 of each warpgroup's 64 dS columns are written
   uint64_t ds_full;       // dS is written
   uint64_t done;
+  uint64_t kv_free;       // dK / dV: the last score MMAs of a unit have read K and V
   uint64_t qdo_full;      // dQ: the Q and dO rows of the tile sit in TMEM
   uint64_t unit_full[2];  // the next unit of work is known
   uint64_t unit_empty[2];
@@ -572,6 +573,7 @@ __device__ __forceinline__ bool bwd_setup(uint8_t* smem, BwdBarriers* bars, int 
     mbar_init(&bars->ds_half, 8);
     mbar_init(&bars->ds_full, 8);
     mbar_init(&bars->done, 1);
+    mbar_init(&bars->kv_free, 1);
     mbar_init(&bars->qdo_full, 8);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bars->unit_full[s], 1);
@@ -807,11 +809,17 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
   uint32_t cuts = 0;         // producer: tile pairs at a document's end so far
   int g = 0;                 // query tiles streamed by this CTA before the current tile
 
-  for (int it = 0;; ++it) {
-    int unit = next_unit(bars, it, units, p.counters, warp, lane, p.status);
-    if (warp >= 2) unit = wg_min((warp - 2) >> 2, unit);
-    if (unit < 0) break;
-    const PackedTile w = p.k_tiles[unit / (p.kv_heads * p.splits)];
+  const auto next = [&](int it) {
+    const int unit = next_unit(bars, it, units, p.counters, warp, lane, p.status);
+    return warp < 2 ? unit : wg_min((warp - 2) >> 2, unit);
+  };
+  const auto tile_of = [&](int unit) { return p.k_tiles[unit / (p.kv_heads * p.splits)]; };
+  int unit = next(0), unit_next = -1;
+  PackedTile w_next{};
+  float next_lse = INFINITY, next_delta = 0.f;   // softmax: of the next query tile, requested ahead
+  if (unit >= 0) w_next = tile_of(unit);
+  for (int it = 0; unit >= 0; ++it, unit = unit_next) {
+    const PackedTile w = w_next;
     const int kv_head = unit % (p.kv_heads * p.splits) / p.splits, split = unit % p.splits;
     const int head0 = kv_head * group + split * share;
     const int j = w.tile;                          // key/value tile inside the document
@@ -821,23 +829,27 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
     const int nq = nd * share;                     // streamed: all of them for every head of this split
     const int last_rows = w.len - (q_tiles - 1) * kTile;   // rows of the document's last tile
     if (warp == 0) {
-      // the resident K / V buffers are free once every MMA of the previous tile has completed; the
-      // loads of this tile then run while the other warps still store the previous accumulators
-      bool ok = it == 0 || warp_wait(&bars->done, (it - 1) & 1, p.status, kStatusTimeoutTmemFull);
-      if (ok && elect_one()) {
-        mbar_expect_tx(&bars->res_full, 2 * C::kTileBytes);
-#pragma unroll
-        for (int h = 0; h < C::kHalves; ++h) {
-          tma_load_3d(sK + h * 16384, &tk, &bars->res_full, h * 64, w.start + j * kTile, kv_head);
-          tma_load_3d(sV + h * 16384, &tv, &bars->res_full, h * 64, w.start + j * kTile, kv_head);
-        }
-      }
-      __syncwarp();
+      bool ok = true;
       for (int t = 0, i = i0, head = head0; t < nq && ok; ++t) {
         ok = stream_pair<D>(bars, sRing, pos, cuts, &tq, &tdo, w.start + i * kTile, head,
                             i == q_tiles - 1 ? last_rows : kTile, lane, p.status);
         if (++i == q_tiles) { i = i0; ++head; }
+        if (t > 0) continue;
+        // the resident K / V buffers are free once the last score MMAs of the previous unit are through;
+        // its last softmax, gradient MMAs and stores then overlap these loads
+        ok = ok && (it == 0 || warp_wait(&bars->kv_free, (it - 1) & 1, p.status, kStatusTimeoutTmemFull));
+        if (ok && elect_one()) {
+          mbar_expect_tx(&bars->res_full, 2 * C::kTileBytes);
+#pragma unroll
+          for (int h = 0; h < C::kHalves; ++h) {
+            tma_load_3d(sK + h * 16384, &tk, &bars->res_full, h * 64, w.start + j * kTile, kv_head);
+            tma_load_3d(sV + h * 16384, &tv, &bars->res_full, h * 64, w.start + j * kTile, kv_head);
+          }
+        }
+        __syncwarp();
       }
+      unit_next = next(it + 1);
+      if (unit_next >= 0) w_next = tile_of(unit_next);
     } else if (warp == 1) {
       if (elect_one()) {
         const int fmt = DT == kBF16 ? 1 : 0;
@@ -884,6 +896,7 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
           issue_scores(dK0, at.slot, 0, &bars->s_full);
           ok = wait_full(at.next(1));
           if (ok) issue_scores(dV0, at.next(1).slot, 128, &bars->dp_full);
+          if (nq == 1) tc_commit(&bars->kv_free);
         }
         for (int t = 0; t < nq && ok; ++t) {
           const RingPos qi = at, doi = at.next(1), qn = at.next(2), don = at.next(3);
@@ -902,6 +915,7 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
             ok = wait_full(don);
             if (!ok) break;
             issue_scores(dV0, don.slot, 128, &bars->dp_full);
+            if (t + 2 == nq) tc_commit(&bars->kv_free);
           }
           at = qn;
         }
@@ -912,6 +926,8 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
       const int items = 2 * nq;
       pos.phase ^= static_cast<uint32_t>(((pos.slot + items) / 5) & 1);
       pos.slot = (pos.slot + items) % 5;
+      unit_next = next(it + 1);
+      if (unit_next >= 0) w_next = tile_of(unit_next);
     } else {
       const int wg = (warp - 2) >> 2;      // columns [64 wg, 64 wg + 64) of every tile
       const int quarter = warp & 3;
@@ -924,27 +940,25 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
       // lse / delta of this warpgroup's 64 queries, staged one query tile ahead: the global loads for
       // tile t + 1 are issued before tile t is processed and parked in shared memory after it, so their
       // latency is never waited for. Streamed tile t is query tile i0 + t % nd of head head0 + t / nd.
-      auto aux_load = [&](int i, int head, float& lse, float& delta) {
+      auto aux_load = [&](const PackedTile& doc, int i, int head, float& lse, float& delta) {
         const int qi = i * kTile + wg * 64 + wg_tid;
-        const bool in = qi < w.len;
-        const int64_t at = static_cast<int64_t>(head) * p.rows + w.start + qi;
+        const bool in = qi < doc.len;
+        const int64_t at = static_cast<int64_t>(head) * p.rows + doc.start + qi;
         lse = in ? p.lse[at] * kLog2e : INFINITY;
         delta = in ? p.delta[at] : 0.f;
       };
       auto aux_slot = [&](int t) { return sAux + ((wg * 2 + (t & 1)) * 2) * 64; };   // [lse 64 | delta 64]
-      if (wg_tid < 64) {
-        float lse, delta;
-        aux_load(i0, head0, lse, delta);
-        aux_slot(0)[wg_tid] = lse;
-        aux_slot(0)[64 + wg_tid] = delta;
+      if (it == 0 && wg_tid < 64) aux_load(w, i0, head0, next_lse, next_delta);
+      if (wg_tid < 64) {   // everyone has left the previous unit's tiles: `next` has a barrier
+        aux_slot(0)[wg_tid] = next_lse;
+        aux_slot(0)[64 + wg_tid] = next_delta;
       }
       int i = i0, head = head0;
       for (int t = 0; t < nq; ++t) {
         const int i_next = i + 1 == q_tiles ? i0 : i + 1, head_next = i + 1 == q_tiles ? head + 1 : head;
         ok = wg_and(wg, ok);             // tile t's values are staged; everyone has left tile t - 1
         if (!ok) break;
-        float next_lse = INFINITY, next_delta = 0.f;
-        if (wg_tid < 64 && t + 1 < nq) aux_load(i_next, head_next, next_lse, next_delta);
+        if (wg_tid < 64 && t + 1 < nq) aux_load(w, i_next, head_next, next_lse, next_delta);
         const bool diag = p.causal && (i == j);
         const float* a_lse = aux_slot(t);
         const float* a_del = a_lse + 64;
@@ -1017,6 +1031,15 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
         i = i_next;
         head = head_next;
       }
+      // what the next unit starts with is requested before this one's results are waited for and stored
+      unit_next = next(it + 1);
+      if (unit_next >= 0) {
+        w_next = tile_of(unit_next);
+        const int kv_split = unit_next % (p.kv_heads * p.splits);
+        if (wg_tid < 64)
+          aux_load(w_next, p.causal ? w_next.tile : 0,
+                   kv_split / p.splits * group + kv_split % p.splits * share, next_lse, next_delta);
+      }
       // epilogue: warpgroup 0 stores dV, warpgroup 1 stores dK * scale
       if (ok) ok = warp_wait(&bars->done, it & 1, p.status, kStatusTimeoutTmemFull);
       if (ok) {
@@ -1049,9 +1072,9 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
         }
       }
     }
-    // End of tile, without a CTA-wide barrier: the roles meet again only through the mbarriers. The
-    // producer waits for `done` before it refills K / V; the first dV / dK MMAs of the next tile
-    // (which overwrite the accumulators) wait for that tile's first P, and a softmax warp writes that
+    // End of the unit, without a CTA-wide barrier: the roles meet again only through the mbarriers. The
+    // producer waits for `kv_free` before it refills K / V; the first dV / dK MMAs of the next unit
+    // (which overwrite the accumulators) wait for that unit's first P, and a softmax warp writes that
     // only after it has stored its part of these accumulators.
     g += nq;
     if (!go_on(warp, p.status)) break;
@@ -1094,19 +1117,66 @@ packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_consta
   uint32_t cuts = 0;         // producer: tile pairs at a document's end so far
   int g = 0;                 // key/value tiles streamed by this CTA before the current tile
 
-  for (int it = 0;; ++it) {
-    int unit = next_unit(bars, it, units, p.counters + 1, warp, lane, p.status);
-    if (warp >= 2) unit = wg_min((warp - 2) >> 2, unit);
-    if (unit < 0) break;
-    const PackedTile w = p.q_tiles[unit / p.heads];
+  const auto next = [&](int it) {
+    const int unit = next_unit(bars, it, units, p.counters + 1, warp, lane, p.status);
+    return warp < 2 ? unit : wg_min((warp - 2) >> 2, unit);
+  };
+  // Stages the rows of unit `it` as TMEM operands: warpgroup 0 copies the Q rows, warpgroup 1 the dO rows,
+  // one thread per row, out of the 128-byte-swizzled tiles the TMA wrote (16-byte chunk c of row r
+  // sits at chunk c ^ (r & 7)); element d of a row lands in TMEM column d / 2 of the operand. The score
+  // MMAs of the unit before have been waited for.
+  const auto stage_rows = [&](int it) {
+    const int wg = (warp - 2) >> 2, r_local = (warp & 3) * 32 + lane;
+    if (!warp_wait(&bars->res_full, it & 1, p.status, kStatusTimeoutFull)) return false;
+    const uint8_t* src = (wg == 0 ? sQ : sDO) + r_local * 128;
+    const uint32_t dst = tmem_base + 384 + wg * 64 + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+#pragma unroll
+    for (int h = 0; h < C::kHalves; ++h)
+#pragma unroll
+      for (int gq = 0; gq < 2; ++gq) {
+        uint32_t v[16];
+#pragma unroll
+        for (int c4 = 0; c4 < 4; ++c4) {
+          const int c = gq * 4 + c4;
+          const uint4 x = *reinterpret_cast<const uint4*>(src + h * 16384 + ((c ^ (r_local & 7)) << 4));
+          v[c4 * 4 + 0] = x.x; v[c4 * 4 + 1] = x.y; v[c4 * 4 + 2] = x.z; v[c4 * 4 + 3] = x.w;
+        }
+        tmem_st_32x32b_x16(dst + h * 32 + gq * 16, v);
+      }
+    tmem_st_wait();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars->qdo_full);
+    return true;
+  };
+  int unit = next(0), unit_next = -1;
+  PackedTile w_next{};
+  float lse_next = 0.f, delta_next = 0.f;        // softmax: of this thread's row of the next unit
+  const auto row_stats = [&](const PackedTile& doc, int head) {
+    const int q_local = doc.tile * kTile + (warp & 3) * 32 + lane;
+    const bool in = q_local < doc.len;
+    const int64_t at = static_cast<int64_t>(head) * p.rows + doc.start + q_local;
+    lse_next = in ? p.lse[at] : INFINITY;
+    delta_next = in ? p.delta[at] : 0.f;
+  };
+  bool ok = true;
+  if (unit >= 0) {
+    w_next = p.q_tiles[unit / p.heads];
+    if (warp >= 2) {
+      row_stats(w_next, unit % p.heads);
+      ok = stage_rows(0);
+    }
+  }
+  for (int it = 0; unit >= 0; ++it, unit = unit_next) {
+    const PackedTile w = w_next;
     const int head = unit % p.heads, kv_head = head / group;
     const int i = w.tile;                          // query tile inside the document
     const int kv_tiles = (w.len + kTile - 1) / kTile;
     const int n = p.causal ? i + 1 : kv_tiles;
     const int last_rows = w.len - (kv_tiles - 1) * kTile;   // rows of the document's last tile
     if (warp == 0) {
-      // Q / dO are free once every MMA of the previous tile has completed
-      bool ok = it == 0 || warp_wait(&bars->done, (it - 1) & 1, p.status, kStatusTimeoutTmemFull);
+      // Q / dO are free once the softmax warps have copied the previous unit's rows
+      ok = it == 0 || warp_wait(&bars->qdo_full, (it - 1) & 1, p.status, kStatusTimeoutTmemFull);
       if (ok && elect_one()) {
         mbar_expect_tx(&bars->res_full, 2 * C::kTileBytes);
 #pragma unroll
@@ -1119,6 +1189,8 @@ packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_consta
       for (int t = 0; t < n && ok; ++t)
         ok = stream_pair<D>(bars, sRing, pos, cuts, &tk, &tv, w.start + t * kTile, kv_head,
                             t == kv_tiles - 1 ? last_rows : kTile, lane, p.status);
+      unit_next = next(it + 1);
+      if (unit_next >= 0) w_next = p.q_tiles[unit_next / p.heads];
     } else if (warp == 1) {
       if (elect_one()) {
         const int fmt = DT == kBF16 ? 1 : 0;
@@ -1198,6 +1270,8 @@ packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_consta
       const int items = 2 * n;
       pos.phase ^= static_cast<uint32_t>(((pos.slot + items) / 5) & 1);
       pos.slot = (pos.slot + items) % 5;
+      unit_next = next(it + 1);
+      if (unit_next >= 0) w_next = p.q_tiles[unit_next / p.heads];
     } else {
       const int wg = (warp - 2) >> 2;      // columns [64 wg, 64 wg + 64) of every tile
       const int quarter = warp & 3;
@@ -1208,34 +1282,7 @@ packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_consta
       const uint32_t lane_bits = static_cast<uint32_t>(quarter * 32) << 16;
       const uint32_t s_addr = tmem_base + wg * 64 + lane_bits, dp_addr = s_addr + 128;
       const float sl2 = p.scale * kLog2e;
-      const int64_t at = static_cast<int64_t>(head) * p.rows + q_row;
-      const float neg_lse = row_ok ? -p.lse[at] * kLog2e : -INFINITY;
-      const float delta = row_ok ? p.delta[at] : 0.f;
-      // Stage the tile's rows as TMEM operands: warpgroup 0 copies the Q rows, warpgroup 1 the dO rows,
-      // one thread per row, out of the 128-byte-swizzled tiles the TMA wrote (16-byte chunk c of row r
-      // sits at chunk c ^ (r & 7)); element d of a row lands in TMEM column d / 2 of the operand.
-      bool ok = warp_wait(&bars->res_full, it & 1, p.status, kStatusTimeoutFull);
-      if (ok) {
-        const uint8_t* src = (wg == 0 ? sQ : sDO) + r_local * 128;
-        const uint32_t dst = tmem_base + 384 + wg * 64 + lane_bits;
-#pragma unroll
-        for (int h = 0; h < C::kHalves; ++h)
-#pragma unroll
-          for (int gq = 0; gq < 2; ++gq) {
-            uint32_t v[16];
-#pragma unroll
-            for (int c4 = 0; c4 < 4; ++c4) {
-              const int c = gq * 4 + c4;
-              const uint4 x = *reinterpret_cast<const uint4*>(src + h * 16384 + ((c ^ (r_local & 7)) << 4));
-              v[c4 * 4 + 0] = x.x; v[c4 * 4 + 1] = x.y; v[c4 * 4 + 2] = x.z; v[c4 * 4 + 3] = x.w;
-            }
-            tmem_st_32x32b_x16(dst + h * 32 + gq * 16, v);
-          }
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->qdo_full);
-      }
+      const float neg_lse = -lse_next * kLog2e, delta = delta_next;
       for (int t = 0; t < n && ok; ++t) {
         ok = warp_wait(&bars->s_full, (g + t) & 1, p.status, kStatusTimeoutTmemFull);
         if (!ok) break;
@@ -1280,8 +1327,16 @@ packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_consta
           if (lane == 0) mbar_arrive(half == 0 ? &bars->ds_half : &bars->ds_full);
         }
       }
-      if (ok) ok = warp_wait(&bars->done, it & 1, p.status, kStatusTimeoutTmemFull);
-      if (ok) {
+      // the next unit's rows go into TMEM before this one's result is waited for and stored, so that its
+      // first score MMAs follow the last ones of this unit
+      unit_next = next(it + 1);
+      if (unit_next >= 0) {
+        w_next = p.q_tiles[unit_next / p.heads];
+        row_stats(w_next, unit_next % p.heads);
+        ok = ok && stage_rows(it + 1);
+      }
+      const bool here = ok && warp_wait(&bars->done, it & 1, p.status, kStatusTimeoutTmemFull);
+      if (here) {
         tc_fence_after();
         // each warpgroup stores half of the head dimension
         uint16_t* orow = reinterpret_cast<uint16_t*>(p.dq) + q_row * p.dq_strides[0] + head * p.dq_strides[1];
@@ -1290,9 +1345,9 @@ packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_consta
           store_columns<DT>(tmem_base + 256 + lane_bits + c * 32, orow + c * 32, p.scale, row_ok);
       }
     }
-    // End of tile, without a CTA-wide barrier: the producer waits for `done` before it reloads Q / dO;
-    // the first dQ MMAs of the next tile (which overwrite the accumulator) wait for that tile's first
-    // dS, and a softmax warp writes that only after it has stored its part of this accumulator.
+    // End of the unit, without a CTA-wide barrier: the first dQ MMAs of the next unit (which overwrite the
+    // accumulator) wait for that unit's first dS, and a softmax warp writes that only after it has
+    // stored its part of this accumulator.
     g += n;
     if (!go_on(warp, p.status)) break;
   }
