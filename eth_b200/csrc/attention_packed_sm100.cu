@@ -86,6 +86,55 @@ __device__ __forceinline__ uint32_t pack_pair(float a, float b, int dtype) {
   return pack2(a, b, dtype);
 }
 
+// 2^x on the FMA pipe: x = i + f with i the nearest whole number, 2^f on [-1/2, 1/2] by a polynomial
+// (minimax in relative error, found by Remez exchange), 2^i built in the exponent field. The softmax
+// warps take part of their exponentials this way: 16 special-function results per clock and SM are the
+// longest step of a score tile, the FMA pipe is idle then. Degree 3 is off by 7.5e-5, a fiftieth of a
+// bf16 step; fp16 takes degree 4, 2.7e-6. Below x = -126 the result stays at 2^-126; NaN stays NaN.
+template <int DT>
+__device__ __forceinline__ Pair exp2_poly(Pair x) {
+  float a, b;
+  split(x, a, b);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.f));
+  x = pair(a, b);
+  const float magic = 12582912.f;   // 1.5 * 2^23: the sum's low mantissa bits hold the rounded x
+  const Pair r = x + pair(magic, magic);
+  const Pair f = x + (pair(magic, magic) + r * pair(-1.f, -1.f));
+  Pair y;
+  if constexpr (DT == kBF16) {
+    y = pair(0.05517167f, 0.05517167f);
+    y = fma2(y, f, pair(0.24261112f, 0.24261112f));
+    y = fma2(y, f, pair(0.69326099f, 0.69326099f));
+    y = fma2(y, f, pair(0.99992807f, 0.99992807f));
+  } else {
+    y = pair(0.0095701f, 0.0095701f);
+    y = fma2(y, f, pair(0.05591786f, 0.05591786f));
+    y = fma2(y, f, pair(0.24024745f, 0.24024745f));
+    y = fma2(y, f, pair(0.69312181f, 0.69312181f));
+    y = fma2(y, f, pair(0.99999926f, 0.99999926f));
+  }
+  split(r, a, b);
+  return y * pair(__int_as_float((__float_as_int(a) << 23) + 0x3f800000),
+                  __int_as_float((__float_as_int(b) << 23) + 0x3f800000));
+}
+__device__ __forceinline__ Pair exp2_sfu(Pair x) {
+  float a, b;
+  split(x, a, b);
+  return pair(exp2f(a), exp2f(b));
+}
+// Pair `i` of a row of scores: kPolyPairs out of four take the FMA pipe.
+template <int DT, int kPolyPairs>
+__device__ __forceinline__ Pair exp2_mixed(int i, Pair x) {
+  return (i & 3) < kPolyPairs ? exp2_poly<DT>(x) : exp2_sfu(x);
+}
+__device__ __forceinline__ uint32_t pack_pair(Pair p, int dtype) {
+  float a, b;
+  split(p, a, b);
+  return pack2(a, b, dtype);
+}
+constexpr int kBwdPoly = 2;
+
 // Clears rows [first, 128) of a tile that a TMA load has written (kHalves blocks of 128 rows x 128
 // bytes; the swizzle permutes inside a row only) and makes that visible to the tensor core's reads.
 // Executed by one warp; the caller signals the tile afterwards.
@@ -110,6 +159,75 @@ __device__ __forceinline__ void clear_rows(void* base, int64_t row_stride, int64
     const int64_t rh = i / kChunks;
     uint16_t* at = reinterpret_cast<uint16_t*>(base) + (first + rh / heads) * row_stride + (rh % heads) * head_stride;
     reinterpret_cast<uint4*>(at)[c] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// Four lanes hold four 16-byte chunks of a row each; afterwards lane l of them holds chunk l of the
+// four rows.
+__device__ __forceinline__ void transpose4(uint4 (&c)[4], int lane) {
+  const auto swap = [&](uint4& lo, uint4& hi, int bit) {   // the off-diagonal chunk of a 2 x 2 block
+    const bool up = lane & bit;
+    uint4 x = up ? lo : hi;
+    x.x = __shfl_xor_sync(0xffffffffu, x.x, bit);
+    x.y = __shfl_xor_sync(0xffffffffu, x.y, bit);
+    x.z = __shfl_xor_sync(0xffffffffu, x.z, bit);
+    x.w = __shfl_xor_sync(0xffffffffu, x.w, bit);
+    if (up) lo = x; else hi = x;
+  };
+  swap(c[0], c[1], 1);
+  swap(c[2], c[3], 1);
+  swap(c[0], c[2], 2);
+  swap(c[1], c[3], 2);
+}
+
+// Columns [col, col + 32) of this warp's 32 accumulator rows to a 16-bit output whose row r begins at
+// rows + r * stride; row r is written where r < valid. A thread reads one row from TMEM; stored like
+// that, every 16-byte store of a warp would touch 32 lines (4000 cycles for a 128 x 128 pair of
+// accumulators). Four lanes exchange their chunks first and write 64 bytes of a row together.
+template <int DT>
+__device__ __forceinline__ void store_columns(uint32_t acc, int col, uint16_t* rows, int64_t stride, int first, int valid,
+                                              float mul, int lane) {
+  uint32_t r[32];
+  __syncwarp();
+  tmem_ld_32x32b_x32(acc + col, r);
+  tmem_ld_wait();
+  uint4 c[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    c[q].x = pack_pair(__uint_as_float(r[q * 8 + 0]) * mul, __uint_as_float(r[q * 8 + 1]) * mul, DT);
+    c[q].y = pack_pair(__uint_as_float(r[q * 8 + 2]) * mul, __uint_as_float(r[q * 8 + 3]) * mul, DT);
+    c[q].z = pack_pair(__uint_as_float(r[q * 8 + 4]) * mul, __uint_as_float(r[q * 8 + 5]) * mul, DT);
+    c[q].w = pack_pair(__uint_as_float(r[q * 8 + 6]) * mul, __uint_as_float(r[q * 8 + 7]) * mul, DT);
+  }
+  transpose4(c, lane);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int row = first + (lane & ~3) + k;
+    if (row < valid) reinterpret_cast<uint4*>(rows + row * stride + col)[lane & 3] = c[k];
+  }
+}
+// The same in fp32 (128 bytes of a row, two halves of 16 columns).
+__device__ __forceinline__ void store_columns_f32(uint32_t acc, int col, float* rows, int64_t stride, int first, int valid,
+                                                  float mul, int lane) {
+  uint32_t r[32];
+  __syncwarp();
+  tmem_ld_32x32b_x32(acc + col, r);
+  tmem_ld_wait();
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    uint4 c[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int e = half * 16 + q * 4;
+      c[q] = make_uint4(__float_as_uint(__uint_as_float(r[e]) * mul), __float_as_uint(__uint_as_float(r[e + 1]) * mul),
+                        __float_as_uint(__uint_as_float(r[e + 2]) * mul), __float_as_uint(__uint_as_float(r[e + 3]) * mul));
+    }
+    transpose4(c, lane);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int row = first + (lane & ~3) + k;
+      if (row < valid) reinterpret_cast<uint4*>(rows + row * stride + col + half * 16)[lane & 3] = c[k];
+    }
   }
 }
 
@@ -436,26 +554,11 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
       const float inv_l = 1.0f / l_run;
       const bool row_ok = q_local < w.len;
       const int64_t q_row = static_cast<int64_t>(w.start) + q_local;
-      uint16_t* orow = reinterpret_cast<uint16_t*>(p.o) + q_row * p.o_strides[0] + head * p.o_strides[1];
+      uint16_t* rows = reinterpret_cast<uint16_t*>(p.o) + (static_cast<int64_t>(w.start) + qt * kTile) * p.o_strides[0] +
+                       head * p.o_strides[1];
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t r[32];
-        __syncwarp();
-        tmem_ld_32x32b_x32(o_addr + c * 32, r);
-        tmem_ld_wait();
-        if (row_ok) {
-          uint4* dst = reinterpret_cast<uint4*>(orow + c * 32);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint4 o;
-            o.x = pack_pair(__uint_as_float(r[q * 8 + 0]) * inv_l, __uint_as_float(r[q * 8 + 1]) * inv_l, DT);
-            o.y = pack_pair(__uint_as_float(r[q * 8 + 2]) * inv_l, __uint_as_float(r[q * 8 + 3]) * inv_l, DT);
-            o.z = pack_pair(__uint_as_float(r[q * 8 + 4]) * inv_l, __uint_as_float(r[q * 8 + 5]) * inv_l, DT);
-            o.w = pack_pair(__uint_as_float(r[q * 8 + 6]) * inv_l, __uint_as_float(r[q * 8 + 7]) * inv_l, DT);
-            dst[q] = o;
-          }
-        }
-      }
+      for (int c = 0; c < D; c += 32)
+        store_columns<DT>(o_addr, c, rows, p.o_strides[0], quarter * 32, w.len - qt * kTile, inv_l, lane);
       if (row_ok)
         p.lse[static_cast<int64_t>(head) * p.rows + q_row] = (m_run + log2f(l_run)) * kLn2;
     }
@@ -655,25 +758,6 @@ __device__ __forceinline__ bool stream_pair(BwdBarriers* bars, uint8_t* ring, Ri
   return true;
 }
 
-// 32 fp32 accumulator columns of one row -> 64 bytes of a 16-bit output row.
-template <int DT>
-__device__ __forceinline__ void store_columns(uint32_t acc, uint16_t* dst, float mul, bool row_ok) {
-  uint32_t r[32];
-  __syncwarp();
-  tmem_ld_32x32b_x32(acc, r);
-  tmem_ld_wait();
-  if (!row_ok) return;
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    uint4 o;
-    o.x = pack_pair(__uint_as_float(r[q * 8 + 0]) * mul, __uint_as_float(r[q * 8 + 1]) * mul, DT);
-    o.y = pack_pair(__uint_as_float(r[q * 8 + 2]) * mul, __uint_as_float(r[q * 8 + 3]) * mul, DT);
-    o.z = pack_pair(__uint_as_float(r[q * 8 + 4]) * mul, __uint_as_float(r[q * 8 + 5]) * mul, DT);
-    o.w = pack_pair(__uint_as_float(r[q * 8 + 6]) * mul, __uint_as_float(r[q * 8 + 7]) * mul, DT);
-    reinterpret_cast<uint4*>(dst)[q] = o;
-  }
-}
-
 // Barrier of a warpgroup that also tells all of it whether everybody is still `ok`.
 __device__ __forceinline__ bool wg_and(int wg, bool ok) {
   uint32_t all;
@@ -820,8 +904,8 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
   if (unit >= 0) w_next = tile_of(unit);
   for (int it = 0; unit >= 0; ++it, unit = unit_next) {
     const PackedTile w = w_next;
-    const int kv_head = unit % (p.kv_heads * p.splits) / p.splits, split = unit % p.splits;
-    const int head0 = kv_head * group + split * share;
+    const int kv_head = unit % (p.kv_heads * p.splits) / p.splits, part = unit % p.splits;
+    const int head0 = kv_head * group + part * share;
     const int j = w.tile;                          // key/value tile inside the document
     const int q_tiles = (w.len + kTile - 1) / kTile;
     const int i0 = p.causal ? j : 0;
@@ -937,15 +1021,15 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
       const uint32_t s_addr = tmem_base + wg * 64 + lane_bits, dp_addr = s_addr + 128;
       const float sl2 = p.scale * kLog2e;
       bool ok = true;
-      // lse / delta of this warpgroup's 64 queries, staged one query tile ahead: the global loads for
+      // -lse / -delta of this warpgroup's 64 queries, staged one query tile ahead: the global loads for
       // tile t + 1 are issued before tile t is processed and parked in shared memory after it, so their
       // latency is never waited for. Streamed tile t is query tile i0 + t % nd of head head0 + t / nd.
       auto aux_load = [&](const PackedTile& doc, int i, int head, float& lse, float& delta) {
         const int qi = i * kTile + wg * 64 + wg_tid;
         const bool in = qi < doc.len;
         const int64_t at = static_cast<int64_t>(head) * p.rows + doc.start + qi;
-        lse = in ? p.lse[at] * kLog2e : INFINITY;
-        delta = in ? p.delta[at] : 0.f;
+        lse = in ? -p.lse[at] * kLog2e : -INFINITY;
+        delta = in ? -p.delta[at] : 0.f;
       };
       auto aux_slot = [&](int t) { return sAux + ((wg * 2 + (t & 1)) * 2) * 64; };   // [lse 64 | delta 64]
       if (it == 0 && wg_tid < 64) aux_load(w, i0, head0, next_lse, next_delta);
@@ -962,7 +1046,7 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
         const bool diag = p.causal && (i == j);
         const float* a_lse = aux_slot(t);
         const float* a_del = a_lse + 64;
-        float pv[64];
+        Pair pv[32];
         ok = warp_wait(&bars->s_full, (g + t) & 1, p.status, kStatusTimeoutTmemFull);
         if (!ok) continue;
         tc_fence_after();
@@ -971,29 +1055,32 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
           tmem_ld_32x32b_x32(s_addr, rs[0]);
           tmem_ld_32x32b_x32(s_addr + 32, rs[1]);
           tmem_ld_wait();
-          // lse comes as 16-byte broadcast loads (four query columns each); only the tile on the
+          const Pair scale = pair(sl2, sl2);
+          // -lse comes as 16-byte broadcast loads (four query columns each); only the tile on the
           // diagonal pays for the causal mask
 #pragma unroll
           for (int y = 0; y < 16; ++y) {
             const float4 l4 = *reinterpret_cast<const float4*>(a_lse + 4 * y);
-            const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const int e = 4 * y + c;
-              pv[e] = exp2f(fmaf(__uint_as_float(rs[e >> 5][e & 31]), sl2, -lv[c]));
-            }
+            const uint32_t* r4 = &rs[y >> 3][(4 * y) & 31];
+            pv[2 * y] = exp2_mixed<DT, kBwdPoly>(
+                2 * y, fma2(pair(__uint_as_float(r4[0]), __uint_as_float(r4[1])), scale, pair(l4.x, l4.y)));
+            pv[2 * y + 1] = exp2_mixed<DT, kBwdPoly>(
+                2 * y + 1, fma2(pair(__uint_as_float(r4[2]), __uint_as_float(r4[3])), scale, pair(l4.z, l4.w)));
           }
         }
         if (diag) {
 #pragma unroll
-          for (int e = 0; e < 64; ++e)
-            if (r_local > wg * 64 + e) pv[e] = 0.f;
+          for (int e = 0; e < 32; ++e) {
+            float a, b;
+            split(pv[e], a, b);
+            pv[e] = pair(r_local > wg * 64 + 2 * e ? 0.f : a, r_local > wg * 64 + 2 * e + 1 ? 0.f : b);
+          }
         }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           uint32_t pk[16];
 #pragma unroll
-          for (int x = 0; x < 16; ++x) pk[x] = pack_pair(pv[half * 32 + 2 * x], pv[half * 32 + 2 * x + 1], DT);
+          for (int x = 0; x < 16; ++x) pk[x] = pack_pair(pv[half * 16 + x], DT);
           tmem_st_32x32b_x16(s_addr + half * 16, pk);
         }
         tmem_st_wait();
@@ -1011,12 +1098,11 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
 #pragma unroll
           for (int y = 0; y < 8; ++y) {
             const float4 e4 = *reinterpret_cast<const float4*>(a_del + half * 32 + 4 * y);
-            const float ev[4] = {e4.x, e4.y, e4.z, e4.w};
-            float dv[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) dv[c] = pv[half * 32 + 4 * y + c] * (__uint_as_float(rd[4 * y + c]) - ev[c]);
-            dk[2 * y] = pack_pair(dv[0], dv[1], DT);
-            dk[2 * y + 1] = pack_pair(dv[2], dv[3], DT);
+            dk[2 * y] = pack_pair(pv[half * 16 + 2 * y] * (pair(__uint_as_float(rd[4 * y]), __uint_as_float(rd[4 * y + 1])) +
+                                                           pair(e4.x, e4.y)), DT);
+            dk[2 * y + 1] = pack_pair(pv[half * 16 + 2 * y + 1] *
+                                          (pair(__uint_as_float(rd[4 * y + 2]), __uint_as_float(rd[4 * y + 3])) +
+                                           pair(e4.z, e4.w)), DT);
           }
           tmem_st_32x32b_x16(dp_addr + half * 16, dk);
         }
@@ -1044,31 +1130,21 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
       if (ok) ok = warp_wait(&bars->done, it & 1, p.status, kStatusTimeoutTmemFull);
       if (ok) {
         tc_fence_after();
-        const int kv_row = j * kTile + r_local;
-        const bool row_ok = kv_row < w.len;
-        const int64_t row = static_cast<int64_t>(w.start) + kv_row;
+        // rows of the tile that exist, from its first row on
+        const int valid = w.len - j * kTile, first = quarter * 32;
+        const int64_t row = static_cast<int64_t>(w.start) + j * kTile;
         const uint32_t acc = tmem_base + 256 + wg * 128 + lane_bits;
         const float mul = wg == 0 ? 1.0f : p.scale;
         if (p.splits == 1) {
           const int64_t* st = wg == 0 ? p.dv_strides : p.dk_strides;
-          uint16_t* orow = reinterpret_cast<uint16_t*>(wg == 0 ? p.dv : p.dk) + row * st[0] + kv_head * st[1];
+          uint16_t* rows = reinterpret_cast<uint16_t*>(wg == 0 ? p.dv : p.dk) + row * st[0] + kv_head * st[1];
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) store_columns<DT>(acc + c * 32, orow + c * 32, mul, row_ok);
+          for (int c = 0; c < D; c += 32) store_columns<DT>(acc, c, rows, st[0], first, valid, mul, lane);
         } else {   // [split, dV | dK, row, kv_head, D] in fp32, summed by packed_join_kernel
-          float* orow = p.parts + (((split * 2 + wg) * static_cast<int64_t>(p.used) + row) * p.kv_heads + kv_head) * D;
+          float* rows = p.parts + (((part * 2 + wg) * static_cast<int64_t>(p.used) + row) * p.kv_heads + kv_head) * D;
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t r[32];
-            __syncwarp();
-            tmem_ld_32x32b_x32(acc + c * 32, r);
-            tmem_ld_wait();
-            if (!row_ok) continue;
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-              reinterpret_cast<float4*>(orow + c * 32)[q] =
-                  make_float4(__uint_as_float(r[4 * q]) * mul, __uint_as_float(r[4 * q + 1]) * mul,
-                              __uint_as_float(r[4 * q + 2]) * mul, __uint_as_float(r[4 * q + 3]) * mul);
-          }
+          for (int c = 0; c < D; c += 32)
+            store_columns_f32(acc, c, rows, static_cast<int64_t>(p.kv_heads) * D, first, valid, mul, lane);
         }
       }
     }
@@ -1282,14 +1358,14 @@ packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_consta
       const uint32_t lane_bits = static_cast<uint32_t>(quarter * 32) << 16;
       const uint32_t s_addr = tmem_base + wg * 64 + lane_bits, dp_addr = s_addr + 128;
       const float sl2 = p.scale * kLog2e;
-      const float neg_lse = -lse_next * kLog2e, delta = delta_next;
+      const float neg_lse = -lse_next * kLog2e, neg_delta = -delta_next;
       for (int t = 0; t < n && ok; ++t) {
         ok = warp_wait(&bars->s_full, (g + t) & 1, p.status, kStatusTimeoutTmemFull);
         if (!ok) break;
         tc_fence_after();
         const int kv0 = t * kTile + wg * 64;              // first key of this warpgroup's columns
         const bool masked = (p.causal && t == i) || kv0 + 64 > w.len;
-        float pv[64];
+        Pair pv[32];
         {
           uint32_t rs[2][32];
           tmem_ld_32x32b_x32(s_addr, rs[0]);
@@ -1298,15 +1374,21 @@ packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_consta
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars->s_read);
+          const Pair scale = pair(sl2, sl2), bias = pair(neg_lse, neg_lse);
 #pragma unroll
-          for (int e = 0; e < 64; ++e) pv[e] = exp2f(fmaf(__uint_as_float(rs[e >> 5][e & 31]), sl2, neg_lse));
+          for (int e = 0; e < 32; ++e)
+            pv[e] = exp2_mixed<DT, kBwdPoly>(e, fma2(pair(__uint_as_float(rs[e >> 4][(2 * e) & 31]),
+                                                          __uint_as_float(rs[e >> 4][(2 * e + 1) & 31])), scale, bias));
         }
         if (masked) {   // the common case carries no mask
           // keys this row sees: up to itself on the diagonal tile, up to the document's end on the last
           const int seen = min(p.causal && t == i ? q_local + 1 : w.len, w.len) - kv0;
 #pragma unroll
-          for (int e = 0; e < 64; ++e)
-            if (e >= seen) pv[e] = 0.f;
+          for (int e = 0; e < 32; ++e) {
+            float a, b;
+            split(pv[e], a, b);
+            pv[e] = pair(2 * e >= seen ? 0.f : a, 2 * e + 1 >= seen ? 0.f : b);
+          }
         }
         ok = warp_wait(&bars->dp_full, (g + t) & 1, p.status, kStatusTimeoutTmemFull);
         if (!ok) break;
@@ -1318,8 +1400,8 @@ packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_consta
           tmem_ld_wait();
 #pragma unroll
           for (int x = 0; x < 16; ++x)
-            dk[x] = pack_pair(pv[half * 32 + 2 * x] * (__uint_as_float(rd[2 * x]) - delta),
-                              pv[half * 32 + 2 * x + 1] * (__uint_as_float(rd[2 * x + 1]) - delta), DT);
+            dk[x] = pack_pair(pv[half * 16 + x] * (pair(__uint_as_float(rd[2 * x]), __uint_as_float(rd[2 * x + 1])) +
+                                                   pair(neg_delta, neg_delta)), DT);
           tmem_st_32x32b_x16(dp_addr + half * 16, dk);
           tmem_st_wait();
           tc_fence_before();
@@ -1339,10 +1421,12 @@ packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_consta
       if (here) {
         tc_fence_after();
         // each warpgroup stores half of the head dimension
-        uint16_t* orow = reinterpret_cast<uint16_t*>(p.dq) + q_row * p.dq_strides[0] + head * p.dq_strides[1];
+        uint16_t* rows = reinterpret_cast<uint16_t*>(p.dq) + (static_cast<int64_t>(w.start) + i * kTile) * p.dq_strides[0] +
+                         head * p.dq_strides[1];
 #pragma unroll 1
-        for (int c = wg * (D / 64); c < (wg + 1) * (D / 64); ++c)
-          store_columns<DT>(tmem_base + 256 + lane_bits + c * 32, orow + c * 32, p.scale, row_ok);
+        for (int c = wg * (D / 2); c < (wg + 1) * (D / 2); c += 32)
+          store_columns<DT>(tmem_base + 256 + lane_bits, c, rows, p.dq_strides[0], quarter * 32, w.len - i * kTile, p.scale,
+                            lane);
       }
     }
     // End of the unit, without a CTA-wide barrier: the first dQ MMAs of the next unit (which overwrite the

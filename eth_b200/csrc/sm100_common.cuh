@@ -422,6 +422,34 @@ __device__ __forceinline__ float2 unpack2(uint32_t u, int dtype) {
   }
 }
 
+// ---- two fp32 lanes per instruction --------------------------------------------------------------
+struct Pair {
+  unsigned long long v;
+};
+__device__ __forceinline__ Pair pair(float x, float y) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void split(Pair p, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p.v));
+}
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
 // ---- dropout masks ---------------------------------------------------------------------------
 // The mask of a [rows, cols] tensor is a pure function of (seed, offset, vector index), the vector
 // index being (row * cols + col) / 8: every kernel that applies or re-applies a dropout (the

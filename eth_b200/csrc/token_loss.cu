@@ -94,34 +94,8 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-// Two fp32 lanes per instruction: the kernels below issue four to five instructions per logit, and
-// these pairs are what keeps that below the time DRAM needs.
-struct Pair {
-  unsigned long long v;
-};
-__device__ __forceinline__ Pair pair(float x, float y) {
-  Pair r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ void split(Pair p, float& x, float& y) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p.v));
-}
-__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
-  Pair r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
-  Pair r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-  Pair r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
+// The kernels below issue four to five instructions per logit; the Pair arithmetic (two fp32 lanes per
+// instruction) is what keeps that below the time DRAM needs.
 __device__ __forceinline__ Pair exp2_pair(Pair t) {
   float x, y;
   split(t, x, y);
