@@ -133,7 +133,7 @@ __device__ __forceinline__ uint32_t pack_pair(Pair p, int dtype) {
   split(p, a, b);
   return pack2(a, b, dtype);
 }
-constexpr int kBwdPoly = 2;
+constexpr int kBwdPoly = 1;
 
 // Clears rows [first, 128) of a tile that a TMA load has written (kHalves blocks of 128 rows x 128
 // bytes; the swizzle permutes inside a row only) and makes that visible to the tensor core's reads.
@@ -789,9 +789,10 @@ __device__ __forceinline__ bool go_on(int warp, const int* status) {
 // arithmetic, so 2 * kDeltaRows requests are in flight per thread. The gradients of rows that belong
 // to no document are cleared here as well.
 constexpr int kDeltaRows = 4;
-template <int D>
+template <int D, typename Index>   // Index: 32 bits where they hold rows x heads, the divisions are the work here
 __global__ void __launch_bounds__(256) packed_delta_kernel(const PackedAttnArgs p) {
   constexpr int lanes = D / 8;
+  const Index heads = static_cast<Index>(p.heads);
   constexpr int rows_per_block = 256 / lanes;
   const int64_t total = static_cast<int64_t>(p.used) * p.heads;
   const int sub = threadIdx.x / lanes, vec = threadIdx.x % lanes;
@@ -802,8 +803,9 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const PackedAttnArgs 
   for (int u = 0; u < kDeltaRows; ++u) {
     const int64_t i = row0 + u * stride;
     if (i < total) {
-      const int h = static_cast<int>(i % p.heads);
-      const int64_t s = i / p.heads;
+      const Index n = static_cast<Index>(i);
+      const int h = static_cast<int>(n % heads);
+      const int64_t s = n / heads;
       ov[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.o) + s * p.o_strides[0] +
                                               h * p.o_strides[1] + vec * 8);
       gv[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.d_o) + s * p.do_strides[0] +
@@ -825,7 +827,10 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const PackedAttnArgs 
 #pragma unroll
     for (int off = lanes >> 1; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
     const int64_t i = row0 + u * stride;
-    if (vec == 0 && i < total) p.delta[(i % p.heads) * p.rows + i / p.heads] = acc;
+    if (vec == 0 && i < total) {
+      const Index n = static_cast<Index>(i);
+      p.delta[static_cast<int64_t>(n % heads) * p.rows + static_cast<int64_t>(n / heads)] = acc;
+    }
   }
   if (blockIdx.x == 0 && threadIdx.x < 2) p.counters[threadIdx.x] = 0;   // of the two kernels that follow
   if (p.used < p.rows) {
@@ -1353,8 +1358,6 @@ packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_consta
       const int quarter = warp & 3;
       const int r_local = quarter * 32 + lane;     // query row inside the tile
       const int q_local = i * kTile + r_local;     // row inside the document
-      const bool row_ok = q_local < w.len;
-      const int64_t q_row = static_cast<int64_t>(w.start) + q_local;
       const uint32_t lane_bits = static_cast<uint32_t>(quarter * 32) << 16;
       const uint32_t s_addr = tmem_base + wg * 64 + lane_bits, dp_addr = s_addr + 128;
       const float sl2 = p.scale * kLog2e;
@@ -1460,7 +1463,9 @@ cudaError_t launch_bwd(const PackedAttnArgs& a, cudaStream_t st) {
   const int sms = sm_count();
   const int64_t vectors = static_cast<int64_t>(a.rows) * a.heads;
   constexpr int per_block = 256 / (D / 8) * kDeltaRows;
-  packed_delta_kernel<D><<<static_cast<unsigned>((vectors + per_block - 1) / per_block), 256, 0, st>>>(a);
+  const unsigned delta_grid = static_cast<unsigned>((vectors + per_block - 1) / per_block);
+  if (vectors < (int64_t{1} << 32)) packed_delta_kernel<D, uint32_t><<<delta_grid, 256, 0, st>>>(a);
+  else packed_delta_kernel<D, uint64_t><<<delta_grid, 256, 0, st>>>(a);
   count_launch();
   if (a.used > 0) {
     packed_bwd_dkdv_kernel<D, DT><<<static_cast<unsigned>(k_work < sms ? k_work : sms), C::kThreads, C::kSmemBytes,
