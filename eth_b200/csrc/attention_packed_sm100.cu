@@ -147,14 +147,13 @@ __device__ __forceinline__ void clear_tail(uint8_t* tile, int first, int lane) {
   fence_proxy_async();
 }
 
-// Clears rows [first, rows) of a [rows, heads, D] 16-bit output: block `part` of `parts`.
+// Clears rows [first, rows) of a [rows, heads, D] 16-bit output: part `part` of `parts`, thread `tid` of `threads`.
 template <int D>
 __device__ __forceinline__ void clear_rows(void* base, int64_t row_stride, int64_t head_stride, int first, int rows, int heads,
-                                           int part, int parts) {
+                                           int part, int parts, int tid, int threads) {
   constexpr int kChunks = D / 8;
   const int64_t total = static_cast<int64_t>(rows - first) * heads * kChunks;
-  for (int64_t i = static_cast<int64_t>(part) * blockDim.x + threadIdx.x; i < total;
-       i += static_cast<int64_t>(parts) * blockDim.x) {
+  for (int64_t i = static_cast<int64_t>(part) * threads + tid; i < total; i += static_cast<int64_t>(parts) * threads) {
     const int c = static_cast<int>(i % kChunks);
     const int64_t rh = i / kChunks;
     uint16_t* at = reinterpret_cast<uint16_t*>(base) + (first + rh / heads) * row_stride + (rh % heads) * head_stride;
@@ -262,12 +261,16 @@ template <int D> struct FwdCfg {
   // the V slot of the same tile, so five slots keep the loads a full iteration ahead of their use.
   static constexpr int kSlotBytes = kHalves * 16384;
   static constexpr int kSlots = (D == 128) ? 5 : 8;
-  static constexpr int kSmemBytes = kQBytes + kSlots * kSlotBytes + 1024 + 256;
+  static constexpr int kSmemBytes = kQBytes + kSlots * kSlotBytes + 1024 + 512;
   static constexpr int kThreads = 320;
 };
 
 struct FwdBarriers {
+  uint4 answer[2];        // of the launch control, see NextBlock
+  uint64_t answer_full[2];
+  uint64_t answer_read[2];
   uint64_t q_full;
+  uint64_t q_free;        // the unit's last score MMAs have read Q
   uint64_t tail_full;     // the last V tile of a document has landed, rows behind its end not yet cleared
   uint64_t kv_full[8];
   uint64_t kv_empty[8];
@@ -278,10 +281,74 @@ struct FwdBarriers {
   uint32_t pad;
 };
 
+// A CTA that is done with its block of the grid takes over blocks that have not been launched yet (cluster
+// launch control): the hardware's dispatch in index order, heaviest first, stays as it is, and the set-up
+// of TMEM, barriers and descriptors is paid once per SM. One thread asks for the next block while the
+// current one is worked on; the answer lands in shared memory like a TMA load.
+__device__ __forceinline__ void ask_next_block(FwdBarriers* bars, int it) {
+  mbar_expect_tx(&bars->answer_full[it & 1], 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+               ::"r"(smem_u32(&bars->answer[it & 1])), "r"(smem_u32(&bars->answer_full[it & 1]))
+               : "memory");
+}
+// All lanes of a warp: the block that follows the `it`-th of this CTA, -1 if there is none.
+__device__ __forceinline__ int next_block(FwdBarriers* bars, int it, int lane, int* status) {
+  if (!warp_wait(&bars->answer_full[it & 1], static_cast<uint32_t>(it >> 1) & 1, status, kStatusTimeoutFull)) return -1;
+  uint32_t taken = 0, x = 0;
+  asm volatile(
+      "{\n"
+      ".reg .b128 r;\n"
+      ".reg .pred p;\n"
+      "ld.shared.b128 r, [%2];\n"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n"
+      "selp.u32 %0, 1, 0, p;\n"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n"
+      "}\n"
+      : "=r"(taken), "+r"(x)
+      : "r"(smem_u32(&bars->answer[it & 1]))
+      : "memory");
+  fence_proxy_async();   // the answer has been read before the next one may be written over it
+  __syncwarp();
+  if (lane == 0) mbar_arrive(&bars->answer_read[it & 1]);
+  return taken != 0 ? static_cast<int>(x) : -1;
+}
+
+template <int kSlots> struct FwdRing {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void advance() {
+    if (++slot == kSlots) { slot = 0; phase ^= 1; }
+  }
+};
+
+// What a block of the grid stands for.
+template <bool kPair> struct FwdUnit {
+  PackedTile w;
+  int head0, kv_head, kv_tiles;
+  int qt0, qt1, n0, n1;      // query tiles inside the document and the key tiles they meet
+  int n, tail_rows;
+  __device__ __forceinline__ FwdUnit(const PackedAttnArgs& p, int block) {
+    const int units = kPair ? p.heads / 2 : p.heads;
+    w = p.tiles[block / units];
+    const int unit = block % units;
+    head0 = kPair ? 2 * unit : unit;                 // head of tile t: head0 + t when heads are paired
+    kv_head = head0 / (p.heads / p.kv_heads);
+    kv_tiles = (w.len + kTile - 1) / kTile;
+    qt0 = kPair ? w.tile : 2 * w.tile;
+    qt1 = kPair ? w.tile : 2 * w.tile + 1;
+    n0 = p.causal ? qt0 + 1 : kv_tiles;
+    n1 = qt1 >= kv_tiles ? 0 : p.causal ? qt1 + 1 : kv_tiles;
+    n = max(n0, n1);
+    // rows of the last key tile that belong to the document, if that tile is met: V rows behind them are
+    // cleared, since a probability of 0 times whatever stands there would still be NaN for an infinity
+    tail_rows = n == kv_tiles ? w.len - (kv_tiles - 1) * kTile : kTile;
+  }
+};
+
 template <int D, int DT, bool kPair>
 __global__ void __launch_bounds__(320, 1)
 packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                const __grid_constant__ CUtensorMap tv, const PackedAttnArgs p) {
+                  const __grid_constant__ CUtensorMap tv, const PackedAttnArgs p) {
   using C = FwdCfg<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -292,34 +359,16 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  // 1-D grid, dispatched in index order: the work list is sorted heaviest first, every entry is taken
-  // by all its head units before the next one, so the last CTAs to start are the short ones
-  const int units = kPair ? p.heads / 2 : p.heads;
-  if (static_cast<int>(blockIdx.x) >= p.num_tiles * units) {
-    clear_rows<D>(p.o, p.o_strides[0], p.o_strides[1], p.used, p.rows, p.heads, blockIdx.x - p.num_tiles * units,
-                  gridDim.x - p.num_tiles * units);
-    return;
-  }
-  const PackedTile w = p.tiles[blockIdx.x / units];
-  const int unit = blockIdx.x % units;
-  const int group = p.heads / p.kv_heads;
-  const int head0 = kPair ? 2 * unit : unit;         // head of tile t: head0 + t when heads are paired
-  const int kv_head = head0 / group;
-  const int kv_tiles = (w.len + kTile - 1) / kTile;
-  int n_t[2], qt_t[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    qt_t[t] = kPair ? w.tile : 2 * w.tile + t;       // query tile inside the document
-    if (qt_t[t] * kTile >= w.len) n_t[t] = 0;
-    else n_t[t] = p.causal ? qt_t[t] + 1 : kv_tiles;
-  }
-  const int n = max(n_t[0], n_t[1]);
-  // keys of the last tile that lie behind the document's end (0: none): their V rows are cleared,
-  // since a probability of 0 times whatever stands there would still be NaN for an infinity
-  const int tail_rows = n == kv_tiles ? w.len - (kv_tiles - 1) * kTile : kTile;
+  // blocks of the grid: [work units, heaviest first][rows behind the last document to clear]
+  const int work = p.num_tiles * (kPair ? p.heads / 2 : p.heads);
 
   if (threadIdx.x == 0) {
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&bars->answer_full[b], 1);
+      mbar_init(&bars->answer_read[b], 10);   // every warp
+    }
     mbar_init(&bars->q_full, 1);
+    mbar_init(&bars->q_free, 1);
     mbar_init(&bars->tail_full, 1);
     for (int s = 0; s < C::kSlots; ++s) {
       mbar_init(&bars->kv_full[s], 1);
@@ -341,227 +390,296 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
   tc_fence_after();
   const uint32_t tmem_base = bars->tmem_base;
 
+  // Every role walks over the CTA's blocks on its own; barrier parities run on what it has counted so far.
+  const auto each_block = [&](auto one) {
+    for (int it = 0, block = blockIdx.x; block >= 0; ++it) {
+      one(it, block);
+      block = next_block(bars, it, lane, p.status);
+      if (!__all_sync(0xffffffffu, p.status == nullptr || *reinterpret_cast<volatile int*>(p.status) == 0)) break;
+    }
+  };
   if (warp == 0) {
-    // ---------------------------------------------------------------- producer
-    const bool cut = tail_rows < kTile;
-    if (elect_one()) {
-      mbar_expect_tx(&bars->q_full, C::kQBytes);
+    FwdRing<C::kSlots> ring;
+    uint32_t units = 0, cuts = 0;
+    each_block([&](int it, int block) {
+      // Asked for when this block's last loads are on their way: early enough for the answer to be there
+      // when the others need it, late enough that a CTA with a long block does not take another one
+      // that a CTA about to finish could start on.
+      const auto ask = [&] {
+        if (warp_wait(&bars->answer_read[it & 1], (static_cast<uint32_t>(it >> 1) & 1) ^ 1, p.status,
+                      kStatusTimeoutEmpty) && elect_one())
+          ask_next_block(bars, it);
+        __syncwarp();
+      };
+      if (block >= work) return ask();
+      const FwdUnit<kPair> u(p, block);
+      const PackedTile& w = u.w;
+      const int n = u.n;
+      // ---------------------------------------------------------------- producer
+      const bool cut = u.tail_rows < kTile;
+      bool ok = warp_wait(&bars->q_free, (units & 1) ^ 1, p.status, kStatusTimeoutEmpty);
+      if (ok && elect_one()) {
+        mbar_expect_tx(&bars->q_full, C::kQBytes);
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int h = 0; h < C::kHalves; ++h)
-          tma_load_3d(sQ + (t * C::kHalves + h) * 16384, &tq, &bars->q_full, h * 64, w.start + qt_t[t] * kTile,
-                      kPair ? head0 + t : head0);
-      int slot = 0;
-      uint32_t phase = 0;
-      for (int i = 0; i < 2 * n; ++i) {   // item 2j is K_j, item 2j + 1 is V_j
-        if (!mbar_wait(&bars->kv_empty[slot], phase ^ 1, p.status, kStatusTimeoutEmpty)) break;
-        uint8_t* dst = sKV + slot * C::kSlotBytes;
-        uint64_t* full = cut && i == 2 * n - 1 ? &bars->tail_full : &bars->kv_full[slot];
-        mbar_expect_tx(full, C::kSlotBytes);
-#pragma unroll
-        for (int h = 0; h < C::kHalves; ++h)
-          tma_load_3d(dst + h * 16384, (i & 1) ? &tv : &tk, full, h * 64, w.start + (i >> 1) * kTile, kv_head);
-        if (++slot == C::kSlots) { slot = 0; phase ^= 1; }
+          for (int h = 0; h < C::kHalves; ++h)
+            tma_load_3d(sQ + (t * C::kHalves + h) * 16384, &tq, &bars->q_full, h * 64,
+                        w.start + (t == 0 ? u.qt0 : u.qt1) * kTile, kPair ? u.head0 + t : u.head0);
       }
-    }
-    __syncwarp();
-    if (cut && warp_wait(&bars->tail_full, 0, p.status, kStatusTimeoutFull)) {
-      const int slot = (2 * n - 1) % C::kSlots;
-      clear_tail<C::kHalves>(sKV + slot * C::kSlotBytes, tail_rows, lane);
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->kv_full[slot]);
-    }
-  } else if (warp == 1) {
-    // ---------------------------------------------------------------- MMA issuer
-    if (elect_one()) {
-      const int fmt = DT == kBF16 ? 1 : 0;
-      const uint32_t idesc_qk = make_idesc_f16(fmt, 0, 0, 128, 128);
-      const uint32_t idesc_pv = make_idesc_f16(fmt, 0, 1, 128, D);
-      bool ok = mbar_wait(&bars->q_full, 0, p.status, kStatusTimeoutFull);
-      // One thread issues every MMA, so the issue path is kept short: descriptors of the tile
-      // origins are built once, each MMA only adds a constant to them.
-      const uint64_t dq0 = make_smem_desc_sw128(smem_u32(sQ), 16, 1024);
-      const uint64_t dk0 = make_smem_desc_sw128(smem_u32(sKV), 16, 1024);
-      const uint64_t dv0 = make_smem_desc_sw128(smem_u32(sKV), 16384, 1024);
-      auto issue_qk = [&](int t, int slot) {
-        const uint64_t dq = desc_advance(dq0, t * C::kHalves * 16384);
-        const uint64_t dk = desc_advance(dk0, slot * C::kSlotBytes);
-#pragma unroll
-        for (int h = 0; h < C::kHalves; ++h)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            tc_mma_f16(tmem_base + t * 128, desc_advance(dq, h * 16384 + k * 32),
-                       desc_advance(dk, h * 16384 + k * 32), idesc_qk, (h | k) != 0 ? 1u : 0u);
-        tc_commit(&bars->s_full[t]);
-      };
-      // O_t += P_t V_j in two halves of the key range: the first four MMAs start as soon as the
-      // softmax warps have written P columns 0-63, while they still compute columns 64-127.
-      auto issue_pv = [&](int t, int slot, int j) {
-        const uint64_t dv = desc_advance(dv0, slot * C::kSlotBytes);
-        bool got = true;
-#pragma unroll
-        for (int half = 0; half < 4 && got; ++half) {
-          got = mbar_wait(&bars->p_half[4 * t + half], j & 1, p.status, kStatusTimeoutTmemFull);
-          tc_fence_after();
-          if (!got) break;
-#pragma unroll
-          for (int k = half * 2; k < half * 2 + 2; ++k)
-            tc_mma_f16_ts(tmem_base + 256 + t * 128, tmem_base + t * 128 + k * 8,
-                          desc_advance(dv, k * 2048), idesc_pv, (j | k) != 0 ? 1u : 0u);
-        }
-        if (got) tc_commit(&bars->o_done[t]);
-        return got;
-      };
-      // ring position of item i (K_j is item 2j, V_j item 2j + 1)
-      auto wait_item = [&](int i) {
-        const bool got = mbar_wait(&bars->kv_full[i % C::kSlots], (i / C::kSlots) & 1, p.status, kStatusTimeoutFull);
-        tc_fence_after();
-        return got;
-      };
-      if (ok && n > 0) {
-        ok = wait_item(0);
-        if (ok) {
-          if (n_t[0] > 0) issue_qk(0, 0);
-          if (n_t[1] > 0) issue_qk(1, 0);
-          tc_commit(&bars->kv_empty[0]);
-        }
-      }
-      for (int j = 0; j < n && ok; ++j) {
-        const int vslot = (2 * j + 1) % C::kSlots, kslot = (2 * j + 2) % C::kSlots;
-        ok = wait_item(2 * j + 1);
+      int last_slot = 0;
+      for (int i = 0; i < 2 * n && ok; ++i) {   // item 2j is K_j, item 2j + 1 is V_j
+        ok = warp_wait(&bars->kv_empty[ring.slot], ring.phase ^ 1, p.status, kStatusTimeoutEmpty);
         if (!ok) break;
-        if (j < n_t[0]) {
-          ok = issue_pv(0, vslot, j);
-          if (!ok) break;
+        if (elect_one()) {
+          uint8_t* dst = sKV + ring.slot * C::kSlotBytes;
+          uint64_t* full = cut && i == 2 * n - 1 ? &bars->tail_full : &bars->kv_full[ring.slot];
+          mbar_expect_tx(full, C::kSlotBytes);
+#pragma unroll
+          for (int h = 0; h < C::kHalves; ++h)
+            tma_load_3d(dst + h * 16384, (i & 1) ? &tv : &tk, full, h * 64, w.start + (i >> 1) * kTile, u.kv_head);
         }
-        if (j + 1 < n) {
-          ok = wait_item(2 * j + 2);
-          if (!ok) break;
-        }
-        if (j + 1 < n_t[0]) issue_qk(0, kslot);
-        if (j < n_t[1]) {
-          ok = issue_pv(1, vslot, j);
-          if (!ok) break;
-        }
-        tc_commit(&bars->kv_empty[vslot]);
-        if (j + 1 < n_t[1]) issue_qk(1, kslot);
-        if (j + 1 < n) tc_commit(&bars->kv_empty[kslot]);
+        __syncwarp();
+        last_slot = ring.slot;
+        ring.advance();
       }
-    }
-  } else {
-    // ---------------------------------------------------------------- softmax + epilogue
-    const int t = (warp - 2) >> 2;       // query tile of this warpgroup
-    const int quarter = warp & 3;        // TMEM lane quarter
-    const int r_local = quarter * 32 + lane;
-    const int qt = t == 0 ? qt_t[0] : qt_t[1];
-    const int q_local = qt * kTile + r_local;      // row inside the document
-    const int head = kPair ? head0 + t : head0;
-    const uint32_t lane_bits = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t s_addr = tmem_base + t * 128 + lane_bits;
-    const uint32_t o_addr = tmem_base + 256 + t * 128 + lane_bits;
-    const float sl2 = p.scale * kLog2e;
-    float m_run = -INFINITY, l_run = 0.f;
-    bool ok = true;
-    const int nt = t == 0 ? n_t[0] : n_t[1];
-    for (int j = 0; j < nt && ok; ++j) {
-      ok = warp_wait(&bars->s_full[t], j & 1, p.status, kStatusTimeoutTmemFull);
-      if (!ok) break;
-      tc_fence_after();
-      const bool diag = p.causal && (j == qt);
-      const bool tail = (j + 1) * kTile > w.len;
-      const int col_limit_tail = w.len - j * kTile;  // valid columns in a tail tile
-      // One TMEM read of the whole 128-column score row: the four loads are issued back to back
-      // and waited for once, so their latency overlaps.
-      uint32_t r[4][32];
-      __syncwarp();
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_addr + c * 32, r[c]);
-      tmem_ld_wait();
-      if (diag || tail) {   // rare: the diagonal tile of a causal row block, or a ragged last tile
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int col = c * 32 + i;
-            if ((diag && col > r_local) || (tail && col >= col_limit_tail)) r[c][i] = 0xff800000u;  // -inf
-          }
-      }
-      float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        mx0 = fmaxf(mx0, __uint_as_float(r[0][i]));
-        mx1 = fmaxf(mx1, __uint_as_float(r[1][i]));
-        mx2 = fmaxf(mx2, __uint_as_float(r[2][i]));
-        mx3 = fmaxf(mx3, __uint_as_float(r[3][i]));
-      }
-      const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
-      const float m_new = fmaxf(m_run, mx * sl2);
-      if (j == 0) {
-        m_run = m_new;
-      } else {
-        const bool need = m_new > m_run + kRescaleThreshold;
-        if (__any_sync(0xffffffffu, need)) {
-          const float m_upd = need ? m_new : m_run;
-          const float alpha = exp2f(m_run - m_upd);
-          l_run *= alpha;
-          m_run = m_upd;
-          // PV_{j-1} must have landed before O is touched
-          ok = warp_wait(&bars->o_done[t], (j - 1) & 1, p.status, kStatusTimeoutTmemFull);
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll 1
-          for (int c = 0; c < D / 16; ++c) {
-            uint32_t o16[16];
-            tmem_ld_32x32b_x16(o_addr + c * 16, o16);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o16[i] = __float_as_uint(__uint_as_float(o16[i]) * alpha);
-            tmem_st_32x32b_x16(o_addr + c * 16, o16);
-          }
-          tmem_st_wait();
-        }
-      }
-      // P = exp2(s * scale_log2 - m), packed to 16 bit into the first 64 score columns
-      float ls0 = 0.f, ls1 = 0.f;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float p0 = exp2f(fmaf(__uint_as_float(r[c][2 * i]), sl2, -m_run));
-          const float p1 = exp2f(fmaf(__uint_as_float(r[c][2 * i + 1]), sl2, -m_run));
-          ls0 += p0;
-          ls1 += p1;
-          pk[i] = pack_pair(p0, p1, DT);
-        }
-        tmem_st_32x32b_x16(s_addr + c * 16, pk);
-        {   // a quarter of the key range is complete: hand it to the MMA warp
-          tmem_st_wait();
-          tc_fence_before();
+      ask();
+      if (cut && ok) {
+        ok = warp_wait(&bars->tail_full, cuts & 1, p.status, kStatusTimeoutFull);
+        ++cuts;
+        if (ok) {
+          clear_tail<C::kHalves>(sKV + last_slot * C::kSlotBytes, u.tail_rows, lane);
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->p_half[4 * t + c]);
+          if (lane == 0) mbar_arrive(&bars->kv_full[last_slot]);
         }
       }
-      const float lsum = ls0 + ls1;
-      l_run += lsum;
-    }
-    if (ok && nt > 0) {
-      ok = warp_wait(&bars->o_done[t], (nt - 1) & 1, p.status, kStatusTimeoutTmemFull);
-      tc_fence_after();
-    }
-    if (ok && nt > 0) {
-      const float inv_l = 1.0f / l_run;
-      const bool row_ok = q_local < w.len;
-      const int64_t q_row = static_cast<int64_t>(w.start) + q_local;
-      uint16_t* rows = reinterpret_cast<uint16_t*>(p.o) + (static_cast<int64_t>(w.start) + qt * kTile) * p.o_strides[0] +
-                       head * p.o_strides[1];
+      ++units;
+    });
+  } else if (warp == 1) {
+    FwdRing<C::kSlots> ring;
+    uint32_t units = 0;
+    int base0 = 0, base1 = 0;            // key tiles that the two query tiles have met
+    each_block([&](int, int block) {
+      if (block >= work) return;
+      const FwdUnit<kPair> u(p, block);
+      const PackedTile& w = u.w;
+      const int n = u.n;
+      // ---------------------------------------------------------------- MMA issuer
+      if (elect_one()) {
+        const int fmt = DT == kBF16 ? 1 : 0;
+        const uint32_t idesc_qk = make_idesc_f16(fmt, 0, 0, 128, 128);
+        const uint32_t idesc_pv = make_idesc_f16(fmt, 0, 1, 128, D);
+        // One thread issues every MMA, so the issue path is kept short: descriptors of the tile
+        // origins are built once, each MMA only adds a constant to them.
+        const uint64_t dq0 = make_smem_desc_sw128(smem_u32(sQ), 16, 1024);
+        const uint64_t dk0 = make_smem_desc_sw128(smem_u32(sKV), 16, 1024);
+        const uint64_t dv0 = make_smem_desc_sw128(smem_u32(sKV), 16384, 1024);
+        auto issue_qk = [&](int t, int slot) {
+          const uint64_t dq = desc_advance(dq0, t * C::kHalves * 16384);
+          const uint64_t dk = desc_advance(dk0, slot * C::kSlotBytes);
+#pragma unroll
+          for (int h = 0; h < C::kHalves; ++h)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              tc_mma_f16(tmem_base + t * 128, desc_advance(dq, h * 16384 + k * 32),
+                         desc_advance(dk, h * 16384 + k * 32), idesc_qk, (h | k) != 0 ? 1u : 0u);
+          tc_commit(&bars->s_full[t]);
+        };
+        // O_t += P_t V_j in four quarters of the key range: the first MMAs start as soon as the
+        // softmax warps have written P columns 0-31, while they still compute the others.
+        auto issue_pv = [&](int t, int slot, int j) {
+          const uint64_t dv = desc_advance(dv0, slot * C::kSlotBytes);
+          const uint32_t parity = ((t == 0 ? base0 : base1) + j) & 1;
+          bool got = true;
+#pragma unroll
+          for (int part = 0; part < 4 && got; ++part) {
+            got = mbar_wait(&bars->p_half[4 * t + part], parity, p.status, kStatusTimeoutTmemFull);
+            tc_fence_after();
+            if (!got) break;
+#pragma unroll
+            for (int k = part * 2; k < part * 2 + 2; ++k)
+              tc_mma_f16_ts(tmem_base + 256 + t * 128, tmem_base + t * 128 + k * 8,
+                            desc_advance(dv, k * 2048), idesc_pv, (j | k) != 0 ? 1u : 0u);
+          }
+          if (got) tc_commit(&bars->o_done[t]);
+          return got;
+        };
+        FwdRing<C::kSlots> at = ring;     // of the next item: K_0 V_0 K_1 V_1 ...
+        auto wait_item = [&] {
+          const bool got = mbar_wait(&bars->kv_full[at.slot], at.phase, p.status, kStatusTimeoutFull);
+          tc_fence_after();
+          return got;
+        };
+        bool ok = mbar_wait(&bars->q_full, units & 1, p.status, kStatusTimeoutFull) && wait_item();
+        if (ok) {
+          issue_qk(0, at.slot);
+          if (u.n1 > 0) issue_qk(1, at.slot);
+          tc_commit(&bars->kv_empty[at.slot]);
+          if (n == 1) tc_commit(&bars->q_free);
+          at.advance();
+        }
+        for (int j = 0; j < n && ok; ++j) {
+          const int vslot = at.slot;
+          ok = wait_item();
+          if (!ok) break;
+          at.advance();
+          if (j < u.n0) {
+            ok = issue_pv(0, vslot, j);
+            if (!ok) break;
+          }
+          const int kslot = at.slot;
+          if (j + 1 < n) {
+            ok = wait_item();
+            if (!ok) break;
+            at.advance();
+          }
+          if (j + 1 < u.n0) issue_qk(0, kslot);
+          if (j < u.n1) {
+            ok = issue_pv(1, vslot, j);
+            if (!ok) break;
+          }
+          tc_commit(&bars->kv_empty[vslot]);
+          if (j + 1 < u.n1) issue_qk(1, kslot);
+          if (j + 1 < n) tc_commit(&bars->kv_empty[kslot]);
+          if (j + 2 == n) tc_commit(&bars->q_free);
+        }
+      }
+      __syncwarp();
+      // every lane tracks the ring position, whichever lane is elected next time
+      ring.phase ^= static_cast<uint32_t>(((ring.slot + 2 * n) / C::kSlots) & 1);
+      ring.slot = (ring.slot + 2 * n) % C::kSlots;
+      ++units;
+      base0 += u.n0;
+      base1 += u.n1;
+    });
+  } else {
+    int base = 0;                        // key tiles that this warpgroup's query tile has met
+    each_block([&](int, int block) {
+      if (block >= work) {
+        clear_rows<D>(p.o, p.o_strides[0], p.o_strides[1], p.used, p.rows, p.heads, block - work, gridDim.x - work,
+                      threadIdx.x - 64, 256);
+        return;
+      }
+      const FwdUnit<kPair> u(p, block);
+      const PackedTile& w = u.w;
+      // ---------------------------------------------------------------- softmax + epilogue
+      const int t = (warp - 2) >> 2;       // query tile of this warpgroup
+      const int quarter = warp & 3;        // TMEM lane quarter
+      const int r_local = quarter * 32 + lane;
+      const int qt = t == 0 ? u.qt0 : u.qt1;
+      const int q_local = qt * kTile + r_local;      // row inside the document
+      const int head = kPair ? u.head0 + t : u.head0;
+      const uint32_t lane_bits = static_cast<uint32_t>(quarter * 32) << 16;
+      const uint32_t s_addr = tmem_base + t * 128 + lane_bits;
+      const uint32_t o_addr = tmem_base + 256 + t * 128 + lane_bits;
+      const float sl2 = p.scale * kLog2e;
+      float m_run = -INFINITY, l_run = 0.f;
+      bool ok = true;
+      const int nt = t == 0 ? u.n0 : u.n1;
+      for (int j = 0; j < nt && ok; ++j) {
+        ok = warp_wait(&bars->s_full[t], (base + j) & 1, p.status, kStatusTimeoutTmemFull);
+        if (!ok) break;
+        tc_fence_after();
+        const bool diag = p.causal && (j == qt);
+        const bool tail = (j + 1) * kTile > w.len;
+        const int col_limit_tail = w.len - j * kTile;  // valid columns in a tail tile
+        // One TMEM read of the whole 128-column score row: the four loads are issued back to back
+        // and waited for once, so their latency overlaps.
+        uint32_t r[4][32];
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_addr + c * 32, r[c]);
+        tmem_ld_wait();
+        if (diag || tail) {   // rare: the diagonal tile of a causal row block, or a ragged last tile
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const int col = c * 32 + i;
+              if ((diag && col > r_local) || (tail && col >= col_limit_tail)) r[c][i] = 0xff800000u;  // -inf
+            }
+        }
+        float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          mx0 = fmaxf(mx0, __uint_as_float(r[0][i]));
+          mx1 = fmaxf(mx1, __uint_as_float(r[1][i]));
+          mx2 = fmaxf(mx2, __uint_as_float(r[2][i]));
+          mx3 = fmaxf(mx3, __uint_as_float(r[3][i]));
+        }
+        const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
+        const float m_new = fmaxf(m_run, mx * sl2);
+        if (j == 0) {
+          m_run = m_new;
+        } else {
+          const bool need = m_new > m_run + kRescaleThreshold;
+          if (__any_sync(0xffffffffu, need)) {
+            const float m_upd = need ? m_new : m_run;
+            const float alpha = exp2f(m_run - m_upd);
+            l_run *= alpha;
+            m_run = m_upd;
+            // PV_{j-1} must have landed before O is touched
+            ok = warp_wait(&bars->o_done[t], (base + j - 1) & 1, p.status, kStatusTimeoutTmemFull);
+            if (!ok) break;
+            tc_fence_after();
 #pragma unroll 1
-      for (int c = 0; c < D; c += 32)
-        store_columns<DT>(o_addr, c, rows, p.o_strides[0], quarter * 32, w.len - qt * kTile, inv_l, lane);
-      if (row_ok)
-        p.lse[static_cast<int64_t>(head) * p.rows + q_row] = (m_run + log2f(l_run)) * kLn2;
-    }
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o16[16];
+              tmem_ld_32x32b_x16(o_addr + c * 16, o16);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o16[i] = __float_as_uint(__uint_as_float(o16[i]) * alpha);
+              tmem_st_32x32b_x16(o_addr + c * 16, o16);
+            }
+            tmem_st_wait();
+          }
+        }
+        // P = exp2(s * scale_log2 - m), packed to 16 bit into the first 64 score columns
+        float ls0 = 0.f, ls1 = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float p0 = exp2f(fmaf(__uint_as_float(r[c][2 * i]), sl2, -m_run));
+            const float p1 = exp2f(fmaf(__uint_as_float(r[c][2 * i + 1]), sl2, -m_run));
+            ls0 += p0;
+            ls1 += p1;
+            pk[i] = pack_pair(p0, p1, DT);
+          }
+          tmem_st_32x32b_x16(s_addr + c * 16, pk);
+          {   // a quarter of the key range is complete: hand it to the MMA warp
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->p_half[4 * t + c]);
+          }
+        }
+        const float lsum = ls0 + ls1;
+        l_run += lsum;
+      }
+      if (ok && nt > 0) {
+        ok = warp_wait(&bars->o_done[t], (base + nt - 1) & 1, p.status, kStatusTimeoutTmemFull);
+        tc_fence_after();
+      }
+      if (ok && nt > 0) {
+        const float inv_l = 1.0f / l_run;
+        const bool row_ok = q_local < w.len;
+        const int64_t q_row = static_cast<int64_t>(w.start) + q_local;
+        uint16_t* rows = reinterpret_cast<uint16_t*>(p.o) + (static_cast<int64_t>(w.start) + qt * kTile) * p.o_strides[0] +
+                         head * p.o_strides[1];
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32)
+          store_columns<DT>(o_addr, c, rows, p.o_strides[0], quarter * 32, w.len - qt * kTile, inv_l, lane);
+        if (row_ok)
+          p.lse[static_cast<int64_t>(head) * p.rows + q_row] = (m_run + log2f(l_run)) * kLn2;
+      }
+      base += nt;
+    });
+    // A unit ends without a CTA-wide barrier: the next unit's loads and first score MMAs overlap the
+    // stores of this one. Its first O += P V MMAs, which overwrite the accumulators, wait for its first P,
+    // and a softmax warp writes that only after it has read its part of these accumulators.
   }
 
   tc_fence_before();
@@ -834,9 +952,9 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const PackedAttnArgs 
   }
   if (blockIdx.x == 0 && threadIdx.x < 2) p.counters[threadIdx.x] = 0;   // of the two kernels that follow
   if (p.used < p.rows) {
-    clear_rows<D>(p.dq, p.dq_strides[0], p.dq_strides[1], p.used, p.rows, p.heads, blockIdx.x, gridDim.x);
-    clear_rows<D>(p.dk, p.dk_strides[0], p.dk_strides[1], p.used, p.rows, p.kv_heads, blockIdx.x, gridDim.x);
-    clear_rows<D>(p.dv, p.dv_strides[0], p.dv_strides[1], p.used, p.rows, p.kv_heads, blockIdx.x, gridDim.x);
+    clear_rows<D>(p.dq, p.dq_strides[0], p.dq_strides[1], p.used, p.rows, p.heads, blockIdx.x, gridDim.x, threadIdx.x, 256);
+    clear_rows<D>(p.dk, p.dk_strides[0], p.dk_strides[1], p.used, p.rows, p.kv_heads, blockIdx.x, gridDim.x, threadIdx.x, 256);
+    clear_rows<D>(p.dv, p.dv_strides[0], p.dv_strides[1], p.used, p.rows, p.kv_heads, blockIdx.x, gridDim.x, threadIdx.x, 256);
   }
 }
 
