@@ -561,29 +561,30 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
                       threadIdx.x - 64, 256);
         return;
       }
-      const FwdUnit<kPair> u(p, block);
-      const PackedTile& w = u.w;
       // ---------------------------------------------------------------- softmax + epilogue
       const int t = (warp - 2) >> 2;       // query tile of this warpgroup
       const int quarter = warp & 3;        // TMEM lane quarter
       const int r_local = quarter * 32 + lane;
-      const int qt = t == 0 ? u.qt0 : u.qt1;
-      const int q_local = qt * kTile + r_local;      // row inside the document
-      const int head = kPair ? u.head0 + t : u.head0;
+      int qt, nt, len;
+      {   // only this lives through the loop; the rest is worked out again for the stores
+        const FwdUnit<kPair> u(p, block);
+        qt = t == 0 ? u.qt0 : u.qt1;
+        nt = t == 0 ? u.n0 : u.n1;
+        len = u.w.len;
+      }
       const uint32_t lane_bits = static_cast<uint32_t>(quarter * 32) << 16;
       const uint32_t s_addr = tmem_base + t * 128 + lane_bits;
       const uint32_t o_addr = tmem_base + 256 + t * 128 + lane_bits;
       const float sl2 = p.scale * kLog2e;
       float m_run = -INFINITY, l_run = 0.f;
       bool ok = true;
-      const int nt = t == 0 ? u.n0 : u.n1;
       for (int j = 0; j < nt && ok; ++j) {
         ok = warp_wait(&bars->s_full[t], (base + j) & 1, p.status, kStatusTimeoutTmemFull);
         if (!ok) break;
         tc_fence_after();
         const bool diag = p.causal && (j == qt);
-        const bool tail = (j + 1) * kTile > w.len;
-        const int col_limit_tail = w.len - j * kTile;  // valid columns in a tail tile
+        const bool tail = (j + 1) * kTile > len;
+        const int col_limit_tail = len - j * kTile;  // valid columns in a tail tile
         // One TMEM read of the whole 128-column score row: the four loads are issued back to back
         // and waited for once, so their latency overlaps.
         uint32_t r[4][32];
@@ -664,7 +665,12 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
         tc_fence_after();
       }
       if (ok && nt > 0) {
+        asm volatile("" : "+r"(block));
+        const FwdUnit<kPair> u(p, block);
+        const PackedTile& w = u.w;
+        const int head = kPair ? u.head0 + t : u.head0;
         const float inv_l = 1.0f / l_run;
+        const int q_local = qt * kTile + r_local;      // row inside the document
         const bool row_ok = q_local < w.len;
         const int64_t q_row = static_cast<int64_t>(w.start) + q_local;
         uint16_t* rows = reinterpret_cast<uint16_t*>(p.o) + (static_cast<int64_t>(w.start) + qt * kTile) * p.o_strides[0] +
