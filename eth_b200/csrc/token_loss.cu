@@ -507,11 +507,14 @@ constexpr int kScanGroup = 8;   // loads in flight per thread of the kernels tha
 // most of an SM loading, with eight loads in flight per thread so that a few of them suffice when the
 // last rows run out. Without the entropy, GB/s for 128 threads x 8 per SM, 256 x 4, 512 x 2 and 1024 x 1:
 // 8192 x 50304 bf16 6590, 6230, 4715, 2452; 2048 x 128000 5928, 6055, 5556, 3933; 250 x 50304 fp32
-// 3816, 4203, 3920, 2938.
+// 3816, 4203, 3920, 2938. With alternatives there are loads behind the row (select_top) that queue behind
+// all that the SM's other rows have requested: 5.8 us with eight loads a thread, so four are in flight
+// there and more CTAs wait beside each other (32 alternatives: 199 us with 4 x 12 CTAs, 215 with 8 x 8).
 template <typename T, bool kTop, int kThreads, int kPerSm>
 __global__ void __launch_bounds__(kThreads, kPerSm)
 token_scores_kernel(const T* __restrict__ z, int64_t ld, int vocab, int64_t v0, const int64_t* __restrict__ tokens,
                     int top_k, float inv_t, TokenScoresOut out, float* __restrict__ partial) {
+  constexpr int kGroup = kTop && kThreads < 512 ? 4 : kScanGroup;
   __shared__ float red[96];
   __shared__ SelectSmem<kThreads> sel;
   const int64_t row = blockIdx.x;
@@ -519,12 +522,12 @@ token_scores_kernel(const T* __restrict__ z, int64_t ld, int vocab, int64_t v0, 
   const float s2 = inv_t * kLog2e;
   using Seg = std::conditional_t<kTop, Segments, NoSegments>;
   Seg seg = [&] {
-    if constexpr (kTop) return Segments(sel.segment_max, r.nvec, kScanGroup);
+    if constexpr (kTop) return Segments(sel.segment_max, r.nvec, kGroup);
     else return NoSegments{};
   }();
   int64_t t = -1;
   float zt = CUDART_NAN_F;
-  const Running<true> own = scan_row<T, true, kScanGroup>(r, s2, seg, [&] {
+  const Running<true> own = scan_row<T, true, kGroup>(r, s2, seg, [&] {
     if (threadIdx.x != 0) return;
     t = tokens[row];
     const int64_t local = t - v0;
@@ -546,7 +549,7 @@ token_scores_kernel(const T* __restrict__ z, int64_t ld, int vocab, int64_t v0, 
     }
   }
   if constexpr (kTop) {
-    select_top<T, kScanGroup>(r, top_k, own.mx, own.l != own.l, seg, sel);
+    select_top<T, kGroup>(r, top_k, own.mx, own.l != own.l, seg, sel);
     for (int i = threadIdx.x; i < top_k; i += blockDim.x) {
       const int id = static_cast<int>(0xffffffffu - static_cast<uint32_t>(sel.best[i]));
       const float zi = value_of(static_cast<uint32_t>(sel.best[i] >> 32));
@@ -998,9 +1001,9 @@ void launch_scores_for(const LogitsView& a, const int64_t* tokens, int top_k, co
   if (few_rows(a.rows, a.vocab))
     top_k > 0 ? go(token_scores_kernel<T, true, 512, 2>, 512) : go(token_scores_kernel<T, false, 512, 2>, 512);
   else if (top_k > 64)
-    go(token_scores_kernel<T, true, 256, 4>, 256);
+    go(token_scores_kernel<T, true, 256, 6>, 256);
   else
-    top_k > 0 ? go(token_scores_kernel<T, true, 128, 8>, 128) : go(token_scores_kernel<T, false, 128, 8>, 128);
+    top_k > 0 ? go(token_scores_kernel<T, true, 128, 12>, 128) : go(token_scores_kernel<T, false, 128, 8>, 128);
 }
 cudaError_t launch_scores(const LogitsView& a, const int64_t* tokens, int top_k, const TokenScoresOut& out,
                           float* partial, cudaStream_t st) {
