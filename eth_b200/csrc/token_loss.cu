@@ -304,7 +304,7 @@ __device__ __forceinline__ Running<kEntropy> scan_row(const Row<T>& r, float s2,
       const uint4 single[1] = {u[k]};
       m = fmaxf(m, run.template add_group<T>(single, s2));
     }
-  seg.add(m);
+  if (c < r.nvec) seg.add(m);   // (not an empty rest: a row of exactly kSegments full segments has no more)
   seg.close();
   return run;
 }

@@ -149,6 +149,71 @@ def test_captured_forward_and_backward():
             assert all(torch.equal(a, b) for a, b in zip(out, eager))
 
 
+def test_two_calls_at_once():
+    """Forward and backward on two streams that run side by side, with few and with many units of work."""
+    lengths = [1000, 3, 257, 700, 128]
+    sets = [_inputs(lengths, 16, kv, 128, torch.bfloat16, seed=s) for s, kv in ((11, 16), (12, 2))]
+    layout = ops.PackedLayout(lengths, device=DEV)
+    alone = [_check(lengths, *x, True, layout=layout) for x in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        outs = []
+        for s, (q, k, v, do) in zip(streams, sets):
+            with torch.cuda.stream(s):
+                out, lse = raw.attention_packed_fwd(q, k, v, layout)
+                outs.append([out, *raw.attention_packed_bwd(do, q, k, v, out, lse, layout)])
+        torch.cuda.synchronize()
+        native.check_status()
+        for got, want in zip(outs, alone):
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_captured_autograd():
+    lengths = [200, 70]
+    q, k, v, do = (t.contiguous() for t in _inputs(lengths, 4, 2, 64, torch.float16, seed=13))
+    layout = ops.PackedLayout(lengths, device=DEV)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+
+    def work():
+        out = ops.flash_attention_packed(*leaves, layout)
+        return [out.detach(), *torch.autograd.grad(out, leaves, do)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work()
+    with torch.no_grad():
+        for t in leaves:
+            t.copy_(torch.randn_like(t))
+    graph.replay()
+    torch.cuda.synchronize()
+    native.check_status()
+    want = oracle.attention(*leaves, lengths, True, d_out=do)
+    for name, t in zip(("out", "dq", "dk", "dv"), got):
+        assert oracle.excess(t, want[name]) <= 1, name
+
+
+def test_offsets_beyond_32_bits():
+    """Rows 2^24 elements apart: the last documents lie behind 2^31 elements of the buffer."""
+    lengths, h, hk, d, pitch = [40, 100], 2, 1, 64, 1 << 24
+    rows = sum(lengths)
+    flat = torch.empty((rows - 1) * pitch + 1024, dtype=torch.bfloat16, device=DEV)
+    parts = []
+    for i, n in enumerate((h, hk, hk, h)):
+        parts.append(flat[i * 128:].as_strided((rows, n, d), (pitch, d, 1)))
+    packed = _inputs(lengths, h, hk, d, torch.bfloat16, seed=14)
+    for dst, src in zip(parts, packed):
+        dst.copy_(src)
+    got = _check(lengths, *parts, True)
+    want = _check(lengths, *packed, True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_no_documents():
     q, k, v, do = _inputs([0, 0], 4, 2, 64, torch.bfloat16, spare=9)
     got = _check([0, 0], q, k, v, do, True)

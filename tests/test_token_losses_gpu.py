@@ -84,6 +84,22 @@ def test_ties_and_masks(dtype, vocab, top_k):
     _same_scores(ops.token_logprobs(z, tokens, top_k), z, tokens, top_k, 1.0)
 
 
+@pytest.mark.parametrize("rows,vocab,top_k,dtype", [(150, 32768, 64, torch.bfloat16), (150, 32768, 64, torch.float16),
+                                                    (150, 16384, 64, torch.float32), (150, 65536, 100, torch.bfloat16),
+                                                    (3, 262144, 128, torch.bfloat16), (3, 131072, 128, torch.float32)])
+def test_rows_of_whole_segments(rows, vocab, top_k, dtype):
+    """Vocabularies that fill every thread's segments exactly, in rows where all of them hold candidates."""
+    z, g = _logits(rows, vocab, 0, 0, dtype, seed=12)
+    z[0] = -math.inf
+    z[1] = 2.0
+    z[2] = torch.finfo(dtype).min
+    tokens = torch.randint(vocab, (rows,), generator=g, device=DEV)
+    r = ops.token_logprobs(z, tokens, top_k)
+    order = torch.sort(z.double(), dim=1, descending=True, stable=True).indices[:, :top_k]
+    assert torch.equal(r.top_index, order)
+    _same_scores(ops.token_logprobs(z[1:], tokens[1:], top_k), z[1:], tokens[1:], top_k, 1.0)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_undefined_rows_and_tokens(dtype):
     z, g = _logits(7, 6000, 0, 0, dtype, seed=2)
