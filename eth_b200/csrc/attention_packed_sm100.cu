@@ -740,7 +740,7 @@ template <int D> struct BwdCfg {
   static constexpr int kSlots = 5;
   // [lse | delta of two query tiles, 2 KB][barriers, 1 KB][two resident tiles][ring]: with D = 128 all
   // 227 KB that a block may have, so the tiles rely on the 1024-byte alignment of dynamic shared memory
-  static constexpr int kFrontBytes = 3072;
+  static constexpr int kFrontBytes = 3 * 1024;
   static constexpr int kSmemBytes = kFrontBytes + (2 + kSlots) * kTileBytes;
   static constexpr int kThreads = 320;
 };

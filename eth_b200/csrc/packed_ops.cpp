@@ -194,7 +194,7 @@ Tensor unit_rows(const Tensor& z, double temperature) {
   TORCH_CHECK_VALUE(z.scalar_type() == at::kFloat || z.scalar_type() == at::kHalf || z.scalar_type() == at::kBFloat16,
                     "logits of type ", z.scalar_type(), " are not supported");
   TORCH_CHECK_VALUE(z.size(0) < 0x7fffffff && z.size(1) < (int64_t{1} << 30), "logits are too large: ", z.sizes());
-  TORCH_CHECK_VALUE(std::isfinite(temperature) && temperature > 0, "temperature must be positive and finite, got ",
+  TORCH_CHECK_VALUE(temperature >= 1e-30 && temperature <= 1e30, "temperature must be between 1e-30 and 1e30, got ",
                     temperature);
   const bool bad = (z.size(1) > 1 && z.stride(1) != 1) || (z.size(0) > 1 && z.stride(0) < z.size(1));
   return bad ? z.contiguous() : z;
@@ -355,14 +355,14 @@ Tensor distill_part(const Tensor& logits, const Tensor& index, const Tensor& log
   const Tensor z = unit_rows(logits, temperature);
   const Teacher t(index, logit, z, z.size(0));
   c10::cuda::CUDAGuard guard(z.device());
-  Tensor part = at::empty({z.size(0), 4}, z.options().dtype(at::kFloat));
+  Tensor part = at::empty({z.size(0), kDistillParts}, z.options().dtype(at::kFloat));
   check(distill_partial(logits_view(z, vocab_start, temperature), t.view(), fptr(part), cur_stream()),
         "distill_partial");
   return part;
 }
 std::tuple<Tensor, Tensor> distill_join(const Tensor& parts, const Tensor& index, const Tensor& logit,
                                         double temperature) {
-  const int64_t rows = index.size(0), world = check_parts(parts, rows, 4);
+  const int64_t rows = index.size(0), world = check_parts(parts, rows, kDistillParts);
   const Teacher t(index, logit, parts, rows);
   c10::cuda::CUDAGuard guard(parts.device());
   Tensor loss = at::empty({rows}, parts.options()), stats = at::empty({rows, 2}, parts.options());

@@ -106,7 +106,7 @@ __device__ __forceinline__ Pair exp2_pair(Pair t) {
 // needs 2^t * t, logits below kFloor are raised to it, which leaves 2^t at 0 (it is 0 in fp32 below
 // t = -150) and t finite. Rows that lie so low themselves, or a temperature so high, that this does
 // not hold take a clamp per element instead.
-constexpr float kFloor = -60000.f;   // exact enough in every type, fp16 included
+constexpr float kFloor = -57344.f;   // -7 * 2^13: exact in every type
 __device__ __forceinline__ bool has_floor(float mu, float s2) { return (mu - kFloor) * s2 > 200.f; }
 __device__ __forceinline__ uint32_t max_nan(uint32_t x, float low) {
   uint32_t r;
@@ -816,8 +816,8 @@ __device__ __forceinline__ float log_weight(const TeacherRow& t, float logit, fl
   return (logit - t.tmax) * inv_t - t.log_sum;
 }
 
-// One warp: the loss of a staged row whose listed logits are all on this shard; NaN where an entry with
-// weight is not, 0 where there are no entries.
+// One warp: the loss of a staged row whose listed logits are all on this shard; NaN where a used entry
+// is not, 0 where there are no entries.
 __device__ __forceinline__ float listed_loss(const Listed& li, int k, const TeacherRow& tr, float inv_t, float mu,
                                              float log_l) {
   float part = 0.f;
@@ -825,6 +825,7 @@ __device__ __forceinline__ float listed_loss(const Listed& li, int k, const Teac
   for (int i = threadIdx.x & 31; i < k; i += 32) {
     const float log_q = log_weight(tr, li.w[i], inv_t), q = exp2f(log_q * kLog2e);
     if (q != 0.f) part += q * (log_q - ((li.z[i] - mu) * inv_t - log_l));
+    if (li.id[i] < 0 && li.w[i] != -INFINITY) part = CUDART_NAN_F;
   }
   return warp_sum(part);
 }
@@ -846,19 +847,20 @@ distill_fwd_kernel(const T* __restrict__ z, int64_t ld, int vocab, int64_t v0, T
   const float mu = all.mu();
   const TeacherRow tr = teacher_row(li, t.k, inv_t);
   if (partial != nullptr) {
-    float found = 0.f, weight = 0.f;
+    float found = 0.f, weight = 0.f, count = 0.f;
     for (int i = threadIdx.x; i < t.k && tr.mass != 0.f; i += 32) {
+      if (li.id[i] < 0) continue;
       const float q = exp2f(log_weight(tr, li.w[i], inv_t) * kLog2e);
-      if (li.id[i] >= 0 && q != 0.f) {
-        found += q * ((li.z[i] - mu) * inv_t);
-        weight += q;
-      }
+      if (q != 0.f) found += q * ((li.z[i] - mu) * inv_t);
+      weight += q;
+      count += 1.f;
     }
     found = warp_sum(found);
     weight = warp_sum(weight);
+    count = warp_sum(count);
     if (threadIdx.x == 0) {
-      float* q = partial + row * 4;
-      q[0] = all.mx; q[1] = all.l; q[2] = found; q[3] = weight;
+      float* q = partial + row * kDistillParts;
+      q[0] = all.mx; q[1] = all.l; q[2] = found; q[3] = weight; q[4] = count;
     }
     return;
   }
@@ -878,28 +880,30 @@ __global__ void distill_combine_kernel(const float* __restrict__ parts, int worl
   if (row >= rows) return;
   const float s2 = inv_t * kLog2e;
   float mx = -INFINITY;
-  for (int w = 0; w < world; ++w) mx = fmaxf(mx, parts[(w * rows + row) * 4]);
+  for (int w = 0; w < world; ++w) mx = fmaxf(mx, parts[(w * rows + row) * kDistillParts]);
   Running<false> all;
   all.mx = mx;
   const float mu = all.mu();
-  float found = 0.f, weight = 0.f;
+  float found = 0.f, count = 0.f;
   for (int w = 0; w < world; ++w) {
-    const float* q = parts + (w * rows + row) * 4;
+    const float* q = parts + (w * rows + row) * kDistillParts;
     Running<false> x;
     x.mx = q[0]; x.l = q[1];
     if (q[3] != 0.f) found += q[2] + q[3] * ((x.mu() - mu) * inv_t);
-    weight += q[3];
+    count += q[4];
     x.rebase(mx, s2);
     all.l += x.l;
   }
   const float* tl = t.logit + row * t.k;
-  float tmax = -INFINITY, sum = 0.f, self = 0.f;
+  float tmax = -INFINITY, sum = 0.f, self = 0.f, used = 0.f;
   bool nan = false;
   for (int i = lane; i < t.k; i += 32) {
     tmax = fmaxf(tmax, tl[i]);
     nan |= tl[i] != tl[i];
+    used += tl[i] != -INFINITY;
   }
   tmax = warp_max(tmax);
+  used = warp_sum(used);
   nan = __any_sync(0xffffffffu, nan);
   const bool empty = tmax == -INFINITY && !nan;
   for (int i = lane; i < t.k; i += 32) sum += empty ? 0.f : exp2f((tl[i] - tmax) * inv_t * kLog2e);
@@ -911,8 +915,7 @@ __global__ void distill_combine_kernel(const float* __restrict__ parts, int worl
   }
   self = warp_sum(self);
   if (lane == 0) {
-    // the weights found over all shards add up to 1 unless an entry lies outside the vocabulary
-    const bool whole = fabsf(weight - 1.f) < 1e-4f;
+    const bool whole = count == used;   // else an entry lies outside the vocabulary
     loss[row] = empty ? 0.f : whole ? self - found + kLn2 * log2f(all.l) : CUDART_NAN_F;
     stats[2 * row] = empty ? 0.f : mu;
     stats[2 * row + 1] = empty ? 1.f : all.l;

@@ -46,7 +46,9 @@ struct TeacherView {
   int k;
 };
 cudaError_t distill_fwd(const LogitsView& a, const TeacherView& t, float* loss, float* stats, cudaStream_t st);
-// one shard's part: [rows, 4] = max, sum, weighted sum of the listed logits found here, their weight
+// one shard's part: [rows, kDistillParts] = max, sum, weighted sum of the listed logits found here, their
+// weight, their number
+constexpr int kDistillParts = 5;
 cudaError_t distill_partial(const LogitsView& a, const TeacherView& t, float* partial, cudaStream_t st);
 cudaError_t distill_combine(const float* partials, int world, int64_t rows, const TeacherView& t,
                             float inv_temperature, float* loss, float* stats, cudaStream_t st);

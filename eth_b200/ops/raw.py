@@ -557,8 +557,8 @@ def _check_logits(logits, temperature, what):
         raise ValueError(f"{what}: logits must be [tokens, vocab], got {tuple(logits.shape)}")
     if logits.dtype not in (torch.float32, torch.float16, torch.bfloat16, torch.float64):
         raise ValueError(f"{what}: logits of type {logits.dtype} are not supported")
-    if not (math.isfinite(temperature) and temperature > 0):
-        raise ValueError(f"{what}: temperature must be positive and finite, got {temperature}")
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError(f"{what}: temperature must be between 1e-30 and 1e30, got {temperature}")
 
 
 def _check_rows(t, logits, dtypes, shape, what):
@@ -697,17 +697,18 @@ def distill_fwd(logits, teacher_index, teacher_logit, temperature=1.0, vocab_sta
     mx = z.amax(1)
     mu = torch.where(mx == -math.inf, 0.0, mx)
     local = index - vocab_start
-    here = (q != 0) & (local >= 0) & (local < vocab)
+    used = logit != -math.inf
+    here = used & (local >= 0) & (local < vocab)
     picked = (z.gather(1, local.clamp(0, vocab - 1)) - mu[:, None]) / temperature
-    part = torch.stack([mx, torch.exp((z - mu[:, None]) / temperature).sum(1), torch.where(here, q * picked, 0.0).sum(1),
-                        torch.where(here, q, 0.0).sum(1)], 1)
+    part = torch.stack([mx, torch.exp((z - mu[:, None]) / temperature).sum(1), torch.where(here & (q != 0), q * picked, 0.0).sum(1),
+                        torch.where(here, q, 0.0).sum(1), here.sum(1).to(z.dtype)], 1)
     parts = gather_fn(part) if gather_fn is not None else part.unsqueeze(0)
     top = parts[:, :, 0].amax(0)
     mu = torch.where(top == -math.inf, 0.0, top)
     d = (torch.where(parts[:, :, 0] == -math.inf, 0.0, parts[:, :, 0]) - mu) / temperature
     total = torch.where(parts[:, :, 1] == 0, 0.0, torch.exp(d) * parts[:, :, 1]).sum(0)
     found = torch.where(parts[:, :, 3] == 0, 0.0, parts[:, :, 2] + parts[:, :, 3] * d).sum(0)
-    whole = (parts[:, :, 3].sum(0) - 1).abs() < 1e-4
+    whole = parts[:, :, 4].sum(0) == used.sum(1)
     loss = torch.where(q != 0, q * log_q, 0.0).sum(1) - found + torch.log(total)
     loss = torch.where(some, torch.where(whole, loss, math.nan), 0.0)
     return loss, torch.stack([torch.where(some, mu, 0.0), torch.where(some, total, 1.0)], 1)

@@ -166,6 +166,23 @@ def test_distillation(dtype, shape, k):
     assert oracle.grad_error(buf[:, :vocab].contiguous(), want, noise) <= 1 and (buf[:, vocab:] == 7).all()
 
 
+def test_low_rows_and_extreme_temperatures():
+    """Rows around the floor that keeps masked logits finite, and temperatures that stretch or flatten it."""
+    z, g = _logits(8, 3001, 0, 0, torch.bfloat16, seed=15)
+    z -= torch.tensor([0.0, 57000.0, 57344.0, 57600.0, 59900.0, 1e6, 1e30, 1e38], device=DEV)[:, None].to(z.dtype)
+    z[:, ::7] = -math.inf
+    tokens = torch.full((8,), 3, device=DEV)
+    for temperature in (0.01, 1.0, 1e4, 1e30):
+        zr = z.clone().requires_grad_(True)
+        r = ops.token_logprobs(zr, tokens, 5, temperature)
+        _same_scores(r, z, tokens, 5, temperature)
+        d = [torch.randn(8, generator=g, device=DEV) for _ in range(2)]
+        got, = torch.autograd.grad(r[:2], zr, d)
+        want = oracle.scores_grad(z, tokens, None, *d, None, temperature)
+        noise = sum(x.abs() for x in d) * (2.0 ** -17 / temperature)
+        assert oracle.grad_error(got, want, noise) <= 1
+
+
 def test_unused_entries_and_strangers():
     z, g = _logits(4, 3000, 0, 0, torch.bfloat16)
     z.requires_grad_(True)
