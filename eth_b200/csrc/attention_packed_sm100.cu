@@ -205,6 +205,33 @@ __device__ __forceinline__ void store_columns(uint32_t acc, int col, uint16_t* r
     if (row < valid) reinterpret_cast<uint4*>(rows + row * stride + col)[lane & 3] = c[k];
   }
 }
+// What the rounding of store_columns takes off, in the same type, to rows that are laid out alike.
+template <int DT>
+__device__ __noinline__ void store_residue(uint32_t acc, int col, uint16_t* rows, int64_t stride, int first, int valid,
+                                           float mul, int lane) {
+  uint32_t r[32];
+  __syncwarp();
+  tmem_ld_32x32b_x32(acc + col, r);
+  tmem_ld_wait();
+  uint4 c[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint32_t lo[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x = __uint_as_float(r[q * 8 + 2 * e]), y = __uint_as_float(r[q * 8 + 2 * e + 1]);
+      const float2 h = unpack2(pack_pair(x * mul, y * mul, DT), DT);
+      lo[e] = pack_pair(fmaf(x, mul, -h.x), fmaf(y, mul, -h.y), DT);
+    }
+    c[q] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+  }
+  transpose4(c, lane);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int row = first + (lane & ~3) + k;
+    if (row < valid) reinterpret_cast<uint4*>(rows + row * stride + col)[lane & 3] = c[k];
+  }
+}
 // The same in fp32 (128 bytes of a row, two halves of 16 columns).
 __device__ __forceinline__ void store_columns_f32(uint32_t acc, int col, float* rows, int64_t stride, int first, int valid,
                                                   float mul, int lane) {
@@ -678,6 +705,14 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
 #pragma unroll 1
         for (int c = 0; c < D; c += 32)
           store_columns<DT>(o_addr, c, rows, p.o_strides[0], quarter * 32, w.len - qt * kTile, inv_l, lane);
+        if (p.residue != nullptr) {   // a training step: its backward takes rowsum(dO * O) from the unrounded O
+          uint16_t* left = reinterpret_cast<uint16_t*>(p.residue) +
+                           ((static_cast<int64_t>(w.start) + qt * kTile) * p.heads + head) * D;
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32)
+            store_residue<DT>(o_addr, c, left, static_cast<int64_t>(p.heads) * D, quarter * 32, w.len - qt * kTile, inv_l,
+                              lane);
+        }
         if (row_ok)
           p.lse[static_cast<int64_t>(head) * p.rows + q_row] = (m_run + log2f(l_run)) * kLn2;
       }
@@ -907,7 +942,9 @@ __device__ __forceinline__ bool go_on(int warp, const int* status) {
   return warp < 2 ? __all_sync(0xffffffffu, go) : wg_and((warp - 2) >> 2, go);
 }
 
-// delta[h, row] = sum_d dO * O. A (row, head) vector of head_dim elements is covered by head_dim / 8
+// delta[h, row] = sum_d dO * O, with the residue of O where the forward left one: the rounding of O to 16
+// bits would otherwise be a common error of a row's whole dS (dQ and dK of 8192 rows in nine documents: 1.5
+// times the error of the formula with only its results rounded, against 1.45). A (row, head) vector of head_dim elements is covered by head_dim / 8
 // adjacent lanes with one 16-byte load each per tensor (head_dim is 64 or 128: 8 or 16 lanes); a
 // thread takes kDeltaRows of them, strided by the grid, and issues all their loads before any
 // arithmetic, so 2 * kDeltaRows requests are in flight per thread. The gradients of rows that belong
@@ -922,7 +959,7 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const PackedAttnArgs 
   const int sub = threadIdx.x / lanes, vec = threadIdx.x % lanes;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * rows_per_block;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * rows_per_block + sub;
-  uint4 ov[kDeltaRows], gv[kDeltaRows];
+  uint4 ov[kDeltaRows], lv[kDeltaRows], gv[kDeltaRows];
 #pragma unroll
   for (int u = 0; u < kDeltaRows; ++u) {
     const int64_t i = row0 + u * stride;
@@ -934,19 +971,24 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const PackedAttnArgs 
                                               h * p.o_strides[1] + vec * 8);
       gv[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.d_o) + s * p.do_strides[0] +
                                               h * p.do_strides[1] + vec * 8);
+      lv[u] = p.residue == nullptr
+                  ? make_uint4(0, 0, 0, 0)
+                  : reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.residue) + i * D)[vec];
     } else {
       ov[u] = make_uint4(0, 0, 0, 0);
+      lv[u] = make_uint4(0, 0, 0, 0);
       gv[u] = make_uint4(0, 0, 0, 0);
     }
   }
 #pragma unroll
   for (int u = 0; u < kDeltaRows; ++u) {
     const uint32_t ow[4] = {ov[u].x, ov[u].y, ov[u].z, ov[u].w}, gw[4] = {gv[u].x, gv[u].y, gv[u].z, gv[u].w};
+    const uint32_t lw[4] = {lv[u].x, lv[u].y, lv[u].z, lv[u].w};
     float acc = 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float2 a = unpack2(ow[e], p.dtype), d = unpack2(gw[e], p.dtype);
-      acc += a.x * d.x + a.y * d.y;
+      const float2 a = unpack2(ow[e], p.dtype), l = unpack2(lw[e], p.dtype), d = unpack2(gw[e], p.dtype);
+      acc += (a.x + l.x) * d.x + (a.y + l.y) * d.y;
     }
 #pragma unroll
     for (int off = lanes >> 1; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);

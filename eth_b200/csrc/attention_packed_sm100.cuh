@@ -24,6 +24,7 @@ struct PackedAttnArgs {
   int64_t do_strides[2], dq_strides[2], dk_strides[2], dv_strides[2];
   float* lse;       // [heads, rows]  log-sum-exp of the scaled scores (natural log)
   float* delta;     // [heads, rows]  rowsum(dO * O), written by the backward
+  void* residue;    // [rows, heads, head_dim] contiguous, type of q, or null: what rounding took off `o`
   const PackedTile* tiles;       // forward: work list, heaviest first
   int num_tiles;
   const PackedTile* q_tiles;     // backward: query tiles / key tiles, heaviest first

@@ -110,23 +110,34 @@ PackedAttnArgs packed_args(const Tensor& q, const Tensor& k, const Tensor& v, co
   return a;
 }
 
-std::tuple<Tensor, Tensor> packed_fwd(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Lists& l,
-                                      double scale, bool causal, const Tensor& status) {
+// out, lse and, if asked for, what the rounding of out to 16 bits took off (the backward's rowsum(dO * O)
+// takes the sum of both).
+std::tuple<Tensor, Tensor, Tensor> packed_fwd(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Lists& l,
+                                              double scale, bool causal, const Tensor& status, bool with_residue) {
   check_packed(q0, k0, v0, l, scale);
   c10::cuda::CUDAGuard guard(q0.device());
   const Tensor q = tma_view(q0), k = tma_view(k0), v = tma_view(v0);
   Tensor out = at::empty(q.sizes(), q.options());
   Tensor lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
+  Tensor residue;
   auto a = packed_args(q, k, v, out, lse, l, scale, causal, status);
+  if (with_residue) {
+    residue = at::empty(q.sizes(), q.options());
+    a.residue = residue.data_ptr();
+  }
   a.tiles = tile_list(attention_packed_pairs_heads(a.heads, a.kv_heads) ? l.tiles : l.blocks, q, a.num_tiles);
   check(attention_packed_fwd(a, cur_stream()), "attention_packed_fwd");
-  return {out, lse};
+  return {out, lse, residue};
 }
 
 std::tuple<Tensor, Tensor, Tensor> packed_bwd(const Tensor& d_out, const Tensor& q0, const Tensor& k0,
                                               const Tensor& v0, const Tensor& out, const Tensor& lse, const Lists& l,
-                                              double scale, bool causal, const Tensor& status) {
+                                              double scale, bool causal, const Tensor& status,
+                                              const Tensor& residue) {
   check_packed(q0, k0, v0, l, scale);
+  TORCH_CHECK_VALUE(!residue.defined() || (residue.device() == q0.device() && residue.scalar_type() == q0.scalar_type() &&
+                                           residue.sizes() == q0.sizes() && residue.is_contiguous()),
+                    "packed attention: the residue is a contiguous tensor like out");
   for (const Tensor& t : {d_out, out})
     TORCH_CHECK_VALUE(t.device() == q0.device() && t.scalar_type() == q0.scalar_type() && t.sizes() == q0.sizes(),
                       "packed attention: out and its gradient must match q");
@@ -141,6 +152,7 @@ std::tuple<Tensor, Tensor, Tensor> packed_bwd(const Tensor& d_out, const Tensor&
   rhd_strides(d_o, a.do_strides); rhd_strides(dq, a.dq_strides);
   rhd_strides(dk, a.dk_strides); rhd_strides(dv, a.dv_strides);
   a.delta = delta.data_ptr<float>();
+  a.residue = residue.defined() ? residue.data_ptr() : nullptr;
   a.q_tiles = tile_list(l.tiles, q, a.num_q_tiles);
   a.k_tiles = tile_list(l.keys, q, a.num_k_tiles);
   const Tensor counters = at::empty({2}, q.options().dtype(at::kInt));
@@ -158,9 +170,10 @@ std::tuple<Tensor, Tensor, Tensor> packed_bwd(const Tensor& d_out, const Tensor&
 struct PackedAttention : torch::autograd::Function<PackedAttention> {
   static Variable forward(AutogradContext* ctx, const Variable& q, const Variable& k, const Variable& v,
                           const Tensor& tiles, const Tensor& blocks, const Tensor& keys, int64_t used, int64_t total,
-                          double scale, bool causal, const Tensor& status) {
-    auto [out, lse] = packed_fwd(q, k, v, Lists{tiles, blocks, keys, used, total}, scale, causal, status);
-    ctx->save_for_backward({q, k, v, out, lse, tiles, blocks, keys, status});
+                          double scale, bool causal, const Tensor& status, bool needs_grad) {
+    auto [out, lse, residue] =
+        packed_fwd(q, k, v, Lists{tiles, blocks, keys, used, total}, scale, causal, status, needs_grad);
+    ctx->save_for_backward({q, k, v, out, lse, tiles, blocks, keys, status, residue});
     ctx->saved_data["used"] = used;
     ctx->saved_data["total"] = total;
     ctx->saved_data["scale"] = scale;
@@ -172,8 +185,8 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
     const auto s = ctx->get_saved_variables();
     const Lists l{s[5], s[6], s[7], ctx->saved_data["used"].toInt(), ctx->saved_data["total"].toInt()};
     auto [dq, dk, dv] = packed_bwd(grads[0], s[0], s[1], s[2], s[3], s[4], l, ctx->saved_data["scale"].toDouble(),
-                                   ctx->saved_data["causal"].toBool(), s[8]);
-    return {dq, dk, dv, Variable(), Variable(), Variable(), Variable(), Variable(), Variable(), Variable(), Variable()};
+                                   ctx->saved_data["causal"].toBool(), s[8], s[9]);
+    return {dq, dk, dv, Variable(), Variable(), Variable(), Variable(), Variable(), Variable(), Variable(), Variable(), Variable()};
   }
 };
 
@@ -432,19 +445,24 @@ void bind_packed_ops(pybind11::module_& m) {
   m.def("flash_attention_packed",
         [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& tiles, const Tensor& blocks,
            const Tensor& keys, int64_t used, int64_t total, c10::optional<double> scale, bool causal, const Tensor& status) {
-          return PackedAttention::apply(q, k, v, tiles, blocks, keys, used, total, scale_of(q, scale), causal, status);
+          const bool needs_grad = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
+          return PackedAttention::apply(q, k, v, tiles, blocks, keys, used, total, scale_of(q, scale), causal, status,
+                                        needs_grad);
         }, unlocked());
   m.def("attention_packed_fwd",
         [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& tiles, const Tensor& blocks,
-           const Tensor& keys, int64_t used, int64_t total, c10::optional<double> scale, bool causal, const Tensor& status) {
-          return packed_fwd(q, k, v, Lists{tiles, blocks, keys, used, total}, scale_of(q, scale), causal, status);
+           const Tensor& keys, int64_t used, int64_t total, c10::optional<double> scale, bool causal, const Tensor& status,
+           bool with_residue) {
+          auto [out, lse, residue] = packed_fwd(q, k, v, Lists{tiles, blocks, keys, used, total}, scale_of(q, scale), causal,
+                                                status, with_residue);
+          return std::make_tuple(out, lse, residue.defined() ? OptTensor(residue) : OptTensor());
         }, unlocked());
   m.def("attention_packed_bwd",
         [](const Tensor& d_out, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out, const Tensor& lse,
            const Tensor& tiles, const Tensor& blocks, const Tensor& keys, int64_t used, int64_t total,
-           c10::optional<double> scale, bool causal, const Tensor& status) {
+           c10::optional<double> scale, bool causal, const Tensor& status, const OptTensor& residue) {
           return packed_bwd(d_out, q, k, v, out, lse, Lists{tiles, blocks, keys, used, total}, scale_of(q, scale), causal,
-                            status);
+                            status, residue.value_or(Tensor()));
         }, unlocked());
   m.def("token_logprobs",
         [](const Tensor& logits, const Tensor& tokens, int64_t top_k, double temperature, int64_t vocab_start) {

@@ -374,14 +374,16 @@ def attention_bwd(d_out, qkv, out, lse, batch, seq, heads, head_dim, scale=None,
 
 
 # ---------------------------------------------------------------------------------- attention over packed documents
-def attention_packed_fwd(q, k, v, layout, scale=None, causal=True):
+def attention_packed_fwd(q, k, v, layout, scale=None, causal=True, with_residue=False):
     """Attention inside each document of `layout` (a `PackedLayout`). q: [total, heads, head_dim], k / v:
     [total, kv_heads, head_dim] (head h reads key/value head h // (heads / kv_heads)). Returns (out like
-    q, contiguous; lse [heads, total]). Rows behind the last document are 0 in `out`."""
+    q, contiguous; lse [heads, total]). Rows behind the last document are 0 in `out`. `with_residue` adds
+    what rounding took off `out` (None on the CPU): handed to `attention_packed_bwd` it keeps the rounding
+    out of rowsum(d_out * out)."""
     if native.use_native(q):
-        return native.lib().attention_packed_fwd(q, k, v, *layout.work_lists(causal), layout.used, layout.total,
-                                                 scale, bool(causal),
-                                                 native.status(q.device))
+        r = native.lib().attention_packed_fwd(q, k, v, *layout.work_lists(causal), layout.used, layout.total, scale,
+                                              bool(causal), native.status(q.device), with_residue)
+        return r if with_residue else r[:2]
     scale = _check_packed(q, k, v, layout, scale)
     out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.zeros((q.shape[1], q.shape[0]), dtype=_wide(q).dtype, device=q.device)
@@ -389,15 +391,14 @@ def attention_packed_fwd(q, k, v, layout, scale=None, causal=True):
         rows = slice(start, start + n)
         o, l = _document_ref(*(_wide(t[rows]) for t in (q, k, v)), scale, causal)
         out[rows], lse[:, rows] = o.to(q.dtype), l
-    return out, lse
+    return (out, lse, None) if with_residue else (out, lse)
 
 
-def attention_packed_bwd(d_out, q, k, v, out, lse, layout, scale=None, causal=True):
+def attention_packed_bwd(d_out, q, k, v, out, lse, layout, scale=None, causal=True, residue=None):
     """(dq, dk, dv), contiguous; gradients of a shared key/value head are summed over its group."""
     if native.use_native(q):
         return native.lib().attention_packed_bwd(d_out, q, k, v, out, lse, *layout.work_lists(causal), layout.used,
-                                                 layout.total, scale,
-                                                 bool(causal), native.status(q.device))
+                                                 layout.total, scale, bool(causal), native.status(q.device), residue)
     scale = _check_packed(q, k, v, layout, scale)
     if d_out.shape != q.shape or d_out.dtype != q.dtype or d_out.device != q.device:
         raise ValueError("attention_packed_bwd: d_out must match q")

@@ -124,6 +124,30 @@ def test_same_bits_every_time_and_on_another_stream():
         assert all(torch.equal(a, b) for a, b in zip(first, again))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_residue_holds_what_rounding_took(dtype):
+    """out + residue is the fp32 accumulator to twice the type's precision, and the gradients come closer."""
+    lengths = [40, 300, 7, 128]
+    q, k, v, do = _inputs(lengths, 8, 2, 64, dtype, spare=3, seed=16)
+    layout = ops.PackedLayout(lengths, device=DEV, total=q.shape[0])
+    out, lse, residue = raw.attention_packed_fwd(q, k, v, layout, with_residue=True)
+    plain, _ = raw.attention_packed_fwd(q, k, v, layout)
+    rows = slice(0, layout.used)
+    assert torch.equal(out, plain)
+    half = torch.finfo(dtype).eps / 2
+    assert (residue[rows].float().abs() <= half * out[rows].float().abs() * 1.01 + 2.0 ** -25).all()
+    both = (out[rows].double() + residue[rows].double())
+    assert torch.equal(both.to(dtype), out[rows])        # it rounds back to out
+    want = oracle.attention(q, k, v, lengths, True, d_out=do)
+    errors = []
+    for r in (residue, None):
+        grads = raw.attention_packed_bwd(do, q, k, v, out, lse, layout, residue=r)
+        errors.append([((g.double() - want[n][0]).norm() / want[n][0].norm()).item()
+                       for n, g in zip(("dq", "dk", "dv"), grads)])
+    native.check_status()
+    assert errors[0][0] < errors[1][0] and errors[0][1] < errors[1][1] and errors[0][2] == errors[1][2]
+
+
 def test_captured_forward_and_backward():
     lengths = [300, 1, 130]
     q, k, v, do = (t.contiguous() for t in _inputs(lengths, 4, 2, 64, torch.bfloat16, spare=5, seed=6))
@@ -162,8 +186,8 @@ def test_two_calls_at_once():
         outs = []
         for s, (q, k, v, do) in zip(streams, sets):
             with torch.cuda.stream(s):
-                out, lse = raw.attention_packed_fwd(q, k, v, layout)
-                outs.append([out, *raw.attention_packed_bwd(do, q, k, v, out, lse, layout)])
+                out, lse, residue = raw.attention_packed_fwd(q, k, v, layout, with_residue=True)
+                outs.append([out, *raw.attention_packed_bwd(do, q, k, v, out, lse, layout, residue=residue)])
         torch.cuda.synchronize()
         native.check_status()
         for got, want in zip(outs, alone):
@@ -245,6 +269,7 @@ def test_refusals_on_the_device():
                 lambda: ops.flash_attention_packed(q, k, v, layout, scale=0.0),
                 lambda: ops.flash_attention_packed(q, k, v, layout, scale=math.nan),
                 lambda: raw.attention_packed_bwd(q[:, :2], q, k, v, q, None, layout),
+                lambda: raw.attention_packed_bwd(q, q, k, v, q, torch.zeros(4, 5, device=DEV), layout, residue=q[:, :2]),
                 lambda: raw.attention_packed_bwd(q[:, :2], q, k, v, q, torch.zeros(4, 5, device=DEV), layout)):
         with pytest.raises((ValueError, TypeError)):
             bad()
