@@ -205,31 +205,40 @@ __device__ __forceinline__ void store_columns(uint32_t acc, int col, uint16_t* r
     if (row < valid) reinterpret_cast<uint4*>(rows + row * stride + col)[lane & 3] = c[k];
   }
 }
-// What the rounding of store_columns takes off, in the same type, to rows that are laid out alike.
-template <int DT>
-__device__ __noinline__ void store_residue(uint32_t acc, int col, uint16_t* rows, int64_t stride, int first, int valid,
-                                           float mul, int lane) {
-  uint32_t r[32];
-  __syncwarp();
-  tmem_ld_32x32b_x32(acc + col, r);
-  tmem_ld_wait();
-  uint4 c[4];
+// All D columns, and what their rounding took off to a second output that is laid out alike. A call of its
+// own: inlined, it costs the forward's softmax loop registers that it does not have.
+template <int D, int DT>
+__device__ __noinline__ void store_with_residue(uint32_t acc, uint16_t* rows, int64_t stride, uint16_t* left,
+                                                int64_t left_stride, int first, int valid, float mul, int lane) {
+#pragma unroll 1
+  for (int col = 0; col < D; col += 32) {
+    uint32_t r[32];
+    __syncwarp();
+    tmem_ld_32x32b_x32(acc + col, r);
+    tmem_ld_wait();
+    uint4 c[4], d[4];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    uint32_t lo[4];
+    for (int q = 0; q < 4; ++q) {
+      uint32_t hi[4], lo[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float x = __uint_as_float(r[q * 8 + 2 * e]), y = __uint_as_float(r[q * 8 + 2 * e + 1]);
-      const float2 h = unpack2(pack_pair(x * mul, y * mul, DT), DT);
-      lo[e] = pack_pair(fmaf(x, mul, -h.x), fmaf(y, mul, -h.y), DT);
+      for (int e = 0; e < 4; ++e) {
+        const float x = __uint_as_float(r[q * 8 + 2 * e]) * mul, y = __uint_as_float(r[q * 8 + 2 * e + 1]) * mul;
+        hi[e] = pack_pair(x, y, DT);
+        const float2 h = unpack2(hi[e], DT);
+        lo[e] = pack_pair(x - h.x, y - h.y, DT);
+      }
+      c[q] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      d[q] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
-    c[q] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-  }
-  transpose4(c, lane);
+    transpose4(c, lane);
+    transpose4(d, lane);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int row = first + (lane & ~3) + k;
-    if (row < valid) reinterpret_cast<uint4*>(rows + row * stride + col)[lane & 3] = c[k];
+    for (int k = 0; k < 4; ++k) {
+      const int row = first + (lane & ~3) + k;
+      if (row >= valid) continue;
+      reinterpret_cast<uint4*>(rows + row * stride + col)[lane & 3] = c[k];
+      reinterpret_cast<uint4*>(left + row * left_stride + col)[lane & 3] = d[k];
+    }
   }
 }
 // The same in fp32 (128 bytes of a row, two halves of 16 columns).
@@ -702,16 +711,15 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
         const int64_t q_row = static_cast<int64_t>(w.start) + q_local;
         uint16_t* rows = reinterpret_cast<uint16_t*>(p.o) + (static_cast<int64_t>(w.start) + qt * kTile) * p.o_strides[0] +
                          head * p.o_strides[1];
-#pragma unroll 1
-        for (int c = 0; c < D; c += 32)
-          store_columns<DT>(o_addr, c, rows, p.o_strides[0], quarter * 32, w.len - qt * kTile, inv_l, lane);
-        if (p.residue != nullptr) {   // a training step: its backward takes rowsum(dO * O) from the unrounded O
-          uint16_t* left = reinterpret_cast<uint16_t*>(p.residue) +
-                           ((static_cast<int64_t>(w.start) + qt * kTile) * p.heads + head) * D;
+        if (p.residue == nullptr) {
 #pragma unroll 1
           for (int c = 0; c < D; c += 32)
-            store_residue<DT>(o_addr, c, left, static_cast<int64_t>(p.heads) * D, quarter * 32, w.len - qt * kTile, inv_l,
-                              lane);
+            store_columns<DT>(o_addr, c, rows, p.o_strides[0], quarter * 32, w.len - qt * kTile, inv_l, lane);
+        } else {   // a training step: its backward takes rowsum(dO * O) from the unrounded O
+          uint16_t* left = reinterpret_cast<uint16_t*>(p.residue) +
+                           ((static_cast<int64_t>(w.start) + qt * kTile) * p.heads + head) * D;
+          store_with_residue<D, DT>(o_addr, rows, p.o_strides[0], left, static_cast<int64_t>(p.heads) * D, quarter * 32,
+                                    w.len - qt * kTile, inv_l, lane);
         }
         if (row_ok)
           p.lse[static_cast<int64_t>(head) * p.rows + q_row] = (m_run + log2f(l_run)) * kLn2;
