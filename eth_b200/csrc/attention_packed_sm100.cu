@@ -133,6 +133,9 @@ __device__ __forceinline__ uint32_t pack_pair(Pair p, int dtype) {
   split(p, a, b);
   return pack2(a, b, dtype);
 }
+// Measured: dK / dV of 8192 rows in five documents, 32 / 8 heads of 128, 297 us with none, 287 with a quarter, 294
+// with a half, 311 with three quarters. (In the forward, whose registers are full, a quarter took 93 us in place
+// of 74 at nine documents, 8192 rows, 16 heads of 128.)
 constexpr int kBwdPoly = 1;
 
 // Clears rows [first, 128) of a tile that a TMA load has written (kHalves blocks of 128 rows x 128
@@ -593,8 +596,11 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
     int base = 0;                        // key tiles that this warpgroup's query tile has met
     each_block([&](int, int block) {
       if (block >= work) {
-        clear_rows<D>(p.o, p.o_strides[0], p.o_strides[1], p.used, p.rows, p.heads, block - work, gridDim.x - work,
-                      threadIdx.x - 64, 256);
+        const int part = block - work, parts = gridDim.x - work, tid = threadIdx.x - 64;
+        clear_rows<D>(p.o, p.o_strides[0], p.o_strides[1], p.used, p.rows, p.heads, part, parts, tid, 256);
+        const int64_t spare = p.rows - p.used;
+        for (int64_t i = part * 256 + tid; i < spare * p.heads; i += parts * 256)
+          p.lse[i / spare * p.rows + p.used + i % spare] = 0.f;
         return;
       }
       // ---------------------------------------------------------------- softmax + epilogue
@@ -775,8 +781,10 @@ cudaError_t launch_fwd(const PackedAttnArgs& a, cudaStream_t st) {
 // what overlaps is the two halves of an iteration: while the exponentials of S are taken the tensor
 // core works on the dP side, and the other way round. (64-column tiles with two buffers of S and dP,
 // as in attention_sm100.cu, need 1.25 times the shared-memory reads per MMA and leave the tensor core
-// waiting for the softmax of a buffer: dK / dV 133 -> DKDV_US us, dQ 107 -> DQ_US us at 8192 rows of nine documents,
-// 16 heads of 128.)
+// waiting for the softmax of a buffer: 133 and 107 us for dK / dV and dQ at 8192 rows of nine documents, 16
+// heads of 128; now 109 and 78 us = 47 and 51 % of the tensor pipe's cycles. What bounds them is the chain
+// "P written -> dV += P^T dO -> next S -> its exponentials"; a second S buffer does not fit beside two
+// accumulators of 128 columns in 512 TMEM columns.)
 template <int D> struct BwdCfg {
   static constexpr int kHalves = D / 64;
   static constexpr int kTileBytes = kHalves * 16384;        // one 128-row tile
@@ -941,8 +949,8 @@ __device__ __forceinline__ bool wg_and(int wg, bool ok) {
   return all != 0;
 }
 
-// The smallest value of a warpgroup: all of it has the same unit of work, or, after a timeout, none.
-__device__ __forceinline__ int wg_min(int wg, int v) { return wg_and(wg, v >= 0) ? v : -1; }
+// All of a warpgroup has the same unit of work, or, where a wait gave up in one of its warps, none.
+__device__ __forceinline__ int wg_unit(int wg, int v) { return wg_and(wg, v >= 0) ? v : -1; }
 
 // A wait gave up somewhere: stop after this tile. A warpgroup decides together, its barrier needs all of it.
 __device__ __forceinline__ bool go_on(int warp, const int* status) {
@@ -952,8 +960,9 @@ __device__ __forceinline__ bool go_on(int warp, const int* status) {
 
 // delta[h, row] = sum_d dO * O, with the residue of O where the forward left one: the rounding of O to 16
 // bits would otherwise be a common error of a row's whole dS (dQ and dK of 8192 rows in nine documents: 1.5
-// times the error of the formula with only its results rounded, against 1.45). A (row, head) vector of head_dim elements is covered by head_dim / 8
-// adjacent lanes with one 16-byte load each per tensor (head_dim is 64 or 128: 8 or 16 lanes); a
+// times the error of the formula with only its results rounded, against 1.45). A (row, head) vector of
+// head_dim elements is covered by head_dim / 8 adjacent lanes with one 16-byte load each per tensor (head_dim
+// is 64 or 128: 8 or 16 lanes); a
 // thread takes kDeltaRows of them, strided by the grid, and issues all their loads before any
 // arithmetic, so 2 * kDeltaRows requests are in flight per thread. The gradients of rows that belong
 // to no document are cleared here as well.
@@ -1041,10 +1050,10 @@ __global__ void __launch_bounds__(256) packed_join_kernel(const PackedAttnArgs p
 // ---- dK / dV: persistent CTAs over (key/value tile, key/value head) ------------------------------
 // One CTA per SM takes units of work from a list sorted heaviest first (under the causal mask key tile j
 // meets tiles - j query tiles of each head). Where heads share a key/value head and there are too few
-// units for the SMs, a unit is split by heads (`splits`, see packed_bwd_splits) and packed_join_kernel
+// units for the SMs, a unit is split by heads (`splits`, see attention_packed_splits) and packed_join_kernel
 // adds the parts.
 // TMEM, the barriers and the tensor-map prefetch are set up once per CTA; barrier parities therefore
-// run on counters that persist across tiles (`it`: tiles done by this CTA, `g`: query tiles streamed).
+// run on counters that persist across tiles (`it`: units done by this CTA, `g`: query tiles streamed).
 // No CTA-wide barrier separates the tiles: the loads and first score MMAs of the next tile overlap the
 // accumulator stores of the current one.
 //
@@ -1074,7 +1083,7 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
 
   const auto next = [&](int it) {
     const int unit = next_unit(bars, it, units, p.counters, warp, lane, p.status);
-    return warp < 2 ? unit : wg_min((warp - 2) >> 2, unit);
+    return warp < 2 ? unit : wg_unit((warp - 2) >> 2, unit);
   };
   const auto tile_of = [&](int unit) { return p.k_tiles[unit / (p.kv_heads * p.splits)]; };
   int unit = next(0), unit_next = -1;
@@ -1343,9 +1352,10 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
 }
 
 // ---- dQ: persistent CTAs over (query tile, head) -------------------------------------------------
-// Like the dK / dV kernel: one CTA per SM, tiles heaviest first (query tile i meets i + 1 key tiles
-// under the causal mask), TMEM and barriers set up once, parities on counters that persist across tiles (`it`, `g`), and no CTA-wide barrier
-// between tiles: the Q / dO loads and first score MMAs of the next tile overlap the dQ store.
+// Like the dK / dV kernel: one CTA per SM, units heaviest first (query tile i meets i + 1 key tiles
+// under the causal mask), TMEM and barriers set up once, parities on counters that persist across units
+// (`it`, `g`), and no CTA-wide barrier between them: the Q / dO loads and first score MMAs of the next
+// unit overlap the dQ store.
 //
 // S = Q K^T and dP = dO V^T read Q and dO as A operands from TMEM (columns [384, 448) and [448, 512)),
 // where the softmax warps put them once per tile: an MMA then fetches only its B operand from shared
@@ -1374,7 +1384,7 @@ packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_consta
 
   const auto next = [&](int it) {
     const int unit = next_unit(bars, it, units, p.counters + 1, warp, lane, p.status);
-    return warp < 2 ? unit : wg_min((warp - 2) >> 2, unit);
+    return warp < 2 ? unit : wg_unit((warp - 2) >> 2, unit);
   };
   // Stages the rows of unit `it` as TMEM operands: warpgroup 0 copies the Q rows, warpgroup 1 the dO rows,
   // one thread per row, out of the 128-byte-swizzled tiles the TMA wrote (16-byte chunk c of row r

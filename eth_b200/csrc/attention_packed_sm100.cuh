@@ -13,7 +13,7 @@ struct PackedTile {
 
 // q/o (and their gradients) are [rows, heads, head_dim] views, k/v [rows, kv_heads, head_dim], with
 // head_dim contiguous; strides[] = element strides of (row, head). head_dim is 64 or 128, heads a
-// multiple of kv_heads. Rows from `used` on belong to no document: outputs and gradients there are 0.
+// multiple of kv_heads. Rows from `used` on belong to no document: outputs, lse and gradients there are 0.
 struct PackedAttnArgs {
   int rows, used, heads, kv_heads, head_dim;
   const void *q, *k, *v;
@@ -43,9 +43,9 @@ struct PackedAttnArgs {
 // true: the forward pairs two heads of a group on one 128-row tile, false: two tiles of one head
 bool attention_packed_pairs_heads(int heads, int kv_heads);
 // Into how many parts (a divisor of the group) the heads of a group are split in the dK / dV kernel: enough
-// for two and a half units of work per SM, so that the heaviest does not decide the time. 4096 tokens in 40 documents, 16 / 2
-// heads of 64: RAGGED_US. With units enough the parts' traffic (8 bytes an element and
-// part each way) is not worth it.
+// for two and a half units of work per SM, so that the heaviest does not decide the time. About 4000 tokens in 40
+// documents, 16 / 2 heads of 64: 44 us without splitting, 30 and 4 us for the join with it (26 and 4 by now). With
+// units enough the parts' traffic (8 bytes an element and part each way) is not worth it.
 int attention_packed_splits(int num_k_tiles, int heads, int kv_heads);
 cudaError_t attention_packed_fwd(const PackedAttnArgs& a, cudaStream_t st);
 cudaError_t attention_packed_bwd(const PackedAttnArgs& a, cudaStream_t st);

@@ -5,6 +5,7 @@
 // host time with Python nodes).
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <cmath>
@@ -63,12 +64,16 @@ void rhd_strides(const Tensor& t, int64_t out[2]) {
   out[1] = t.size(1) == 1 ? t.size(2) : t.stride(1);
   out[0] = t.size(0) <= 1 ? t.size(1) * t.size(2) : t.stride(0);
 }
+// A layout may be let go of while a call on another stream than its own still runs: the allocator is told
+// (it returns at once on the layout's own stream), as a kernel that met other data in its list would
+// address memory by it.
 const PackedTile* tile_list(const Tensor& t, const Tensor& like, int& n) {
   TORCH_CHECK_VALUE(t.is_cuda() && t.get_device() == like.get_device(), "packed attention: layout on ", t.device(),
                     ", tensors on ", like.device());
   TORCH_CHECK_VALUE(t.scalar_type() == at::kInt && t.dim() == 2 && t.size(1) == 4 && t.is_contiguous(),
                     "packed attention: work lists are int32 [n, 4]");
   n = static_cast<int>(t.size(0));
+  c10::cuda::CUDACachingAllocator::recordStream(t.storage().data_ptr(), at::cuda::getCurrentCUDAStream());
   return reinterpret_cast<const PackedTile*>(t.data_ptr());
 }
 
@@ -87,7 +92,7 @@ void check_packed(const Tensor& q, const Tensor& k, const Tensor& v, const Lists
                     "packed attention: fp16 / bf16 with head_dim 64 or 128 only, got ", q.scalar_type(), ", ", q.size(2));
   TORCH_CHECK_VALUE(l.total == q.size(0), "packed attention: layout of ", l.total, " rows, tensors of ", q.size(0));
   TORCH_CHECK_VALUE(l.used >= 0 && l.used <= l.total && l.total < 0x7fffff00, "packed attention: rows of the layout");
-  TORCH_CHECK_VALUE(std::isfinite(scale) && scale > 0, "packed attention: scale must be positive and finite, got ", scale);
+  TORCH_CHECK_VALUE(scale >= 1e-30 && scale <= 1e30, "packed attention: scale must be between 1e-30 and 1e30, got ", scale);
 }
 
 double scale_of(const Tensor& q, c10::optional<double> scale) {

@@ -377,7 +377,7 @@ def attention_bwd(d_out, qkv, out, lse, batch, seq, heads, head_dim, scale=None,
 def attention_packed_fwd(q, k, v, layout, scale=None, causal=True, with_residue=False):
     """Attention inside each document of `layout` (a `PackedLayout`). q: [total, heads, head_dim], k / v:
     [total, kv_heads, head_dim] (head h reads key/value head h // (heads / kv_heads)). Returns (out like
-    q, contiguous; lse [heads, total]). Rows behind the last document are 0 in `out`. `with_residue` adds
+    q, contiguous; lse [heads, total]). Rows behind the last document are 0 in both. `with_residue` adds
     what rounding took off `out` (None on the CPU): handed to `attention_packed_bwd` it keeps the rounding
     out of rowsum(d_out * out)."""
     if native.use_native(q):
@@ -433,8 +433,8 @@ def _check_packed(q, k, v, layout, scale):
     if layout.total != q.shape[0]:
         raise ValueError(f"packed attention: layout of {layout.total} rows, tensors of {q.shape[0]}")
     scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
-    if not (math.isfinite(scale) and scale > 0):
-        raise ValueError(f"packed attention: scale must be positive and finite, got {scale}")
+    if not 1e-30 <= scale <= 1e30:
+        raise ValueError(f"packed attention: scale must be between 1e-30 and 1e30, got {scale}")
     return scale
 
 

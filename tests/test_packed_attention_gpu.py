@@ -244,6 +244,46 @@ def test_no_documents():
     assert _check([], *empty, True)[0].shape == (0, 4, 64)
 
 
+@pytest.mark.parametrize("heads,kv_heads,spare", [(4, 2, 9), (3, 1, 700), (1, 1, 1)])
+def test_lse_of_rows_behind_the_last_document(heads, kv_heads, spare):
+    q, k, v, _ = _inputs([130, 5], heads, kv_heads, 64, torch.bfloat16, spare=spare)
+    torch.full((heads, q.shape[0]), math.nan, device=DEV)      # what the allocator hands out next
+    _, lse = raw.attention_packed_fwd(q, k, v, ops.PackedLayout([130, 5], device=DEV, total=q.shape[0]))
+    assert (lse[:, 135:] == 0).all() and lse[:, :135].isfinite().all()
+
+
+def test_layout_outlives_a_call_on_another_stream():
+    lengths = [300, 1, 513, 64]
+    q, k, v, do = _inputs(lengths, 8, 2, 128, torch.bfloat16, seed=5)
+    layout = ops.PackedLayout(lengths, device=DEV)
+    lists = layout.work_lists(True)[0]
+    at, size = lists.untyped_storage().data_ptr(), lists.untyped_storage().nbytes()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)
+        out = ops.flash_attention_packed(q, k, v, layout)
+    del layout, lists
+    again = [torch.empty(size, dtype=torch.uint8, device=DEV) for _ in range(64)]
+    assert not side.query() and all(t.data_ptr() != at for t in again)
+    side.synchronize()
+    want = oracle.attention(q, k, v, lengths, True, None, do)
+    assert oracle.excess(out, want["out"]) <= 1
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-4, 1.0])
+def test_scales(scale):
+    lengths = [130, 1, 257]
+    _check(lengths, *_inputs(lengths, 4, 2, 64, torch.bfloat16, seed=9), True, scale=scale)
+
+
+@pytest.mark.parametrize("scale", [0.0, -1.0, 1e-31, 1e31, math.inf, math.nan])
+def test_scales_out_of_range(scale):
+    q, k, v, _ = _inputs([5], 4, 2, 64, torch.bfloat16)
+    with pytest.raises(ValueError, match="scale"):
+        ops.flash_attention_packed(q, k, v, ops.PackedLayout([5], device=DEV), scale=scale)
+
+
 def test_no_second_derivative():
     q, k, v, do = (t.contiguous().requires_grad_(True) for t in _inputs([5], 4, 2, 64, torch.bfloat16))
     out = ops.flash_attention_packed(q, k, v, ops.PackedLayout([5], device=DEV))
