@@ -165,26 +165,19 @@ template <bool kEntropy> struct Running {
   __device__ __forceinline__ float add_group(const uint4 (&u)[N], float s2);
 };
 
-template <typename T, bool kNan = false>
+template <typename T>
 __device__ __forceinline__ float max_of(const uint4& u) {
   if constexpr (std::is_same<T, __nv_bfloat16>::value) {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
-    const __nv_bfloat162 m = kNan ? __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]))
-                                  : __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-    const __nv_bfloat16 r = kNan ? __hmax_nan(__low2bfloat16(m), __high2bfloat16(m))
-                                 : __hmax(__low2bfloat16(m), __high2bfloat16(m));
-    return __bfloat162float(r);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return __bfloat162float(__hmax(__low2bfloat16(m), __high2bfloat16(m)));
   } else if constexpr (std::is_same<T, __half>::value) {
     const __half2* h = reinterpret_cast<const __half2*>(&u);
-    const __half2 m = kNan ? __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]))
-                           : __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-    const __half r = kNan ? __hmax_nan(__low2half(m), __high2half(m)) : __hmax(__low2half(m), __high2half(m));
-    return __half2float(r);
+    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return __half2float(__hmax(__low2half(m), __high2half(m)));
   } else {
-    const float m = fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)),
-                          fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
-    static_assert(!kNan, "fp32 elements are looked at one by one where NaN counts");
-    return m;
+    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)),
+                 fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
   }
 }
 
@@ -430,32 +423,43 @@ __device__ void select_top(const Row<T>& r, int k, float thread_max, bool thread
     for (int i = r.tail() + tid; i < r.n; i += kThreads) take(HalfTraits<T>::to_f(r.p[i]), i);
   }
   __syncthreads();
-  // the block reads the segments' vectors together, four loads at a time
-  const int per = seg.length * kGroup, items = s.owners * per;
-  for (int i0 = tid; i0 < items; i0 += 4 * kThreads) {
-    uint4 u[4];
-    int at[4];
+  // The block reads the segments' vectors together, eight lanes a segment and four loads a thread at a time.
+  // What cannot be a candidate is sorted out by float comparisons (they flush below kTiny, where all pass; NaN
+  // passes), the rest by its key.
+  const float least = fabsf(value_of(bound)) < kTiny ? -INFINITY : value_of(bound);
+  const int per = seg.length * kGroup, owners = s.owners;
+  constexpr int kLanes = 8, kTeams = kThreads / kLanes;
+  for (int o = tid / kLanes; o < owners; o += 4 * kTeams)
+    for (int i = tid % kLanes; i < per; i += kLanes) {
+      uint4 u[4];
+      int at[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int i = i0 + q * kThreads;
-      at[q] = -1;
-      if (i < items) {
-        const int own_seg = s.owner[i / per];
-        const int c = (own_seg / kThreads * per + i % per) * kThreads + own_seg % kThreads;
-        if (c < r.nvec) at[q] = c;
+      for (int q = 0; q < 4; ++q) {
+        at[q] = -1;
+        if (o + q * kTeams < owners) {
+          const int own_seg = s.owner[o + q * kTeams];
+          const int c = (own_seg / kThreads * per + i) * kThreads + own_seg % kThreads;
+          if (c < r.nvec) at[q] = c;
+        }
+        if (at[q] >= 0) u[q] = r.vec()[at[q]];
       }
-      if (at[q] >= 0) u[q] = r.vec()[at[q]];
-    }
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      if (at[q] < 0) continue;
-      if (sizeof(T) == 2 && order_key(max_of<T, sizeof(T) == 2>(u[q])) < bound) continue;   // (fp32 maxima flush)
-      float x[kVec<T>];
-      unpack<T>(u[q], x);
+      for (int q = 0; q < 4; ++q) {
+        if (at[q] < 0) continue;
+        float x[kVec<T>];
+        unpack<T>(u[q], x);
+        uint32_t in = 0;
 #pragma unroll
-      for (int j = 0; j < kVec<T>; ++j) take(x[j], r.head + at[q] * kVec<T> + j);
+        for (int j = 0; j < kVec<T>; ++j) in |= !(x[j] < least) ? 1u << j : 0u;
+        for (; in != 0; in &= in - 1) {
+          const int j = __ffs(in) - 1;
+          float z = x[0];
+#pragma unroll
+          for (int e = 1; e < kVec<T>; ++e) z = j == e ? x[e] : z;
+          take(z, r.head + at[q] * kVec<T> + j);
+        }
+      }
     }
-  }
   __syncthreads();
   int found = s.count;
   if (found > kCandidates || found < k) {   // (fewer than k cannot be; the exact way needs no such argument)
