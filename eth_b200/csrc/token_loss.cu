@@ -512,13 +512,14 @@ constexpr int kScanGroup = 8;   // loads in flight per thread of the kernels tha
 // last rows run out. Without the entropy, GB/s for 128 threads x 8 per SM, 256 x 4, 512 x 2 and 1024 x 1:
 // 8192 x 50304 bf16 6590, 6230, 4715, 2452; 2048 x 128000 5928, 6055, 5556, 3933; 250 x 50304 fp32
 // 3816, 4203, 3920, 2938. With alternatives there are loads behind the row (select_top) that queue behind
-// all that the SM's other rows have requested: 5.8 us with eight loads a thread, so four are in flight
-// there and more CTAs wait beside each other (32 alternatives: 199 us with 4 x 12 CTAs, 215 with 8 x 8).
+// all that the SM's other rows have requested. 8192 x 50304 bf16 with 32 of them, back to back: eight loads a
+// thread and 8 CTAs per SM 187 us, 7 and 9 CTAs 192 and 195, four loads and 10 or 12 CTAs 190 and 194. With
+// 256 threads (100 of them) four loads and 6 CTAs 255, eight and 4 262.
 template <typename T, bool kTop, int kThreads, int kPerSm>
 __global__ void __launch_bounds__(kThreads, kPerSm)
 token_scores_kernel(const T* __restrict__ z, int64_t ld, int vocab, int64_t v0, const int64_t* __restrict__ tokens,
                     int top_k, float inv_t, TokenScoresOut out, float* __restrict__ partial) {
-  constexpr int kGroup = kTop && kThreads < 512 ? 4 : kScanGroup;
+  constexpr int kGroup = kTop && kThreads == 256 ? 4 : kScanGroup;
   __shared__ float red[96];
   __shared__ SelectSmem<kThreads> sel;
   const int64_t row = blockIdx.x;
@@ -997,7 +998,8 @@ cudaError_t check_view(const LogitsView& a) {
 }
 
 // With 128 threads the bound on the k-th alternative (the k-th largest of as many maxima) is loose for k
-// near 128: about 620 elements would reach it. 256 threads leave about 180.
+// near 128: about 620 elements would reach it. 256 threads leave about 180. 8192 x 50304 bf16: 235 us with
+// 128 threads against 238 at k = 72, 264 against 249 at 88, 344 against 274 at 112.
 template <typename T>
 void launch_scores_for(const LogitsView& a, const int64_t* tokens, int top_k, const TokenScoresOut& out, float* partial,
                        cudaStream_t st) {
@@ -1010,7 +1012,7 @@ void launch_scores_for(const LogitsView& a, const int64_t* tokens, int top_k, co
   else if (top_k > 64)
     go(token_scores_kernel<T, true, 256, 6>, 256);
   else
-    top_k > 0 ? go(token_scores_kernel<T, true, 128, 12>, 128) : go(token_scores_kernel<T, false, 128, 8>, 128);
+    top_k > 0 ? go(token_scores_kernel<T, true, 128, 8>, 128) : go(token_scores_kernel<T, false, 128, 8>, 128);
 }
 cudaError_t launch_scores(const LogitsView& a, const int64_t* tokens, int top_k, const TokenScoresOut& out,
                           float* partial, cudaStream_t st) {
