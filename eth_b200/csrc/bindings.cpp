@@ -365,12 +365,17 @@ void ce_combine(const Tensor& stats_all, Tensor& loss, Tensor& gmax, Tensor& gsu
                          gmax.data_ptr<float>(), gsum.data_ptr<float>(), loss.numel(),
                          static_cast<int>(world), cur_stream()), "ce_combine");
 }
-void ce_bwd(Tensor& logits, const Tensor& targets, const Tensor& gmax, const Tensor& gsum,
-            const Tensor& dloss, int64_t vocab_start) {
+// `grad` may be the logits themselves. A write over them counts as a change in place, so that a node that
+// has saved them and runs later raises and does not read a gradient as logits.
+void ce_bwd(const Tensor& logits, Tensor& grad, const Tensor& targets, const Tensor& gmax,
+            const Tensor& gsum, const Tensor& dloss, int64_t vocab_start) {
   c10::cuda::CUDAGuard guard(logits.device());
-  check(ethb::ce_bwd(logits.data_ptr(), targets.data_ptr<int64_t>(), gmax.data_ptr<float>(),
+  TORCH_CHECK(grad.sizes() == logits.sizes() && grad.scalar_type() == logits.scalar_type() &&
+              grad.device() == logits.device() && grad.stride(1) == 1, "ce_bwd: grad must match the logits");
+  grad.unsafeGetTensorImpl()->bump_version();
+  check(ethb::ce_bwd(logits.data_ptr(), grad.data_ptr(), targets.data_ptr<int64_t>(), gmax.data_ptr<float>(),
                      gsum.data_ptr<float>(), dloss.data_ptr<float>(), logits.size(0),
-                     static_cast<int>(logits.size(1)), logits.stride(0),
+                     static_cast<int>(logits.size(1)), logits.stride(0), grad.stride(0),
                      static_cast<int>(vocab_start), dtype_code(logits), cur_stream()), "ce_bwd");
 }
 

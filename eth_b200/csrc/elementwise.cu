@@ -816,13 +816,14 @@ __global__ void ce_combine_kernel(const float* __restrict__ all, float* __restri
   loss[r] = __logf(s) + m - t;
 }
 template <typename T>
-__global__ void ce_bwd_kernel(T* __restrict__ logits, const int64_t* __restrict__ targets,
+__global__ void ce_bwd_kernel(const T* logits, T* grad, const int64_t* __restrict__ targets,
                               const float* __restrict__ gmax, const float* __restrict__ gsum,
                               const float* __restrict__ dloss, int64_t rows, int vl, int64_t ld,
-                              int v0) {
+                              int64_t ldg, int v0) {   // grad may be the logits themselves
   const int nvec = vl >> 3;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    T* lr = logits + row * ld;
+    const T* lr = logits + row * ld;
+    T* gr = grad + row * ldg;
     const float m = gmax[row], inv = 1.0f / gsum[row], g = dloss[row];
     const int64_t t = targets[row] - v0;
     for (int c = threadIdx.x; c < nvec; c += blockDim.x) {
@@ -834,7 +835,7 @@ __global__ void ce_bwd_kernel(T* __restrict__ logits, const int64_t* __restrict_
         if (c * 8 + j == t) sm -= 1.0f;
         v[j] = sm * g;
       }
-      store8(lr + c * 8, v);
+      store8(gr + c * 8, v);
     }
   }
 }
@@ -1245,14 +1246,15 @@ cudaError_t ce_combine(const float* stats_all, float* loss, float* gmax, float* 
   count_launch();
   return cudaGetLastError();
 }
-cudaError_t ce_bwd(void* logits, const int64_t* targets, const float* gmax, const float* gsum,
-                   const float* dloss, int64_t rows, int vocab_local, int64_t ld, int vocab_start,
-                   int dtype, cudaStream_t st) {
-  if (vocab_local % 8 || ld % 8) return cudaErrorInvalidValue;
+cudaError_t ce_bwd(const void* logits, void* grad, const int64_t* targets, const float* gmax,
+                   const float* gsum, const float* dloss, int64_t rows, int vocab_local, int64_t ld,
+                   int64_t ldg, int vocab_start, int dtype, cudaStream_t st) {
+  if (vocab_local % 8 || ld % 8 || ldg % 8) return cudaErrorInvalidValue;
   const int grid = rows < kSMs * 8 ? static_cast<int>(rows) : kSMs * 8;
   ETHB_DISPATCH(dtype, T,
-                (ce_bwd_kernel<T><<<grid, 256, 0, st>>>((T*)logits, targets, gmax, gsum, dloss, rows,
-                                                        vocab_local, ld, vocab_start)));
+                (ce_bwd_kernel<T><<<grid, 256, 0, st>>>((const T*)logits, (T*)grad, targets, gmax, gsum,
+                                                        dloss, rows, vocab_local, ld, ldg,
+                                                        vocab_start)));
   count_launch();
   return cudaGetLastError();
 }

@@ -86,10 +86,10 @@ cudaError_t ce_local_stats(const void* logits, const int64_t* targets, float* st
 // Combine `world` stats blocks ([world, rows, 3]) into loss[row], and keep gmax/gsum for backward.
 cudaError_t ce_combine(const float* stats_all, float* loss, float* gmax, float* gsum, int64_t rows,
                        int world, cudaStream_t st);
-// logits <- (softmax - onehot) * dloss[row]   (in place, 16-bit or fp32)
-cudaError_t ce_bwd(void* logits, const int64_t* targets, const float* gmax, const float* gsum,
-                   const float* dloss, int64_t rows, int vocab_local, int64_t ld, int vocab_start,
-                   int dtype, cudaStream_t st);
+// grad <- (softmax - onehot) * dloss[row]   (16-bit or fp32); grad may be the logits themselves
+cudaError_t ce_bwd(const void* logits, void* grad, const int64_t* targets, const float* gmax,
+                   const float* gsum, const float* dloss, int64_t rows, int vocab_local, int64_t ld,
+                   int64_t ldg, int vocab_start, int dtype, cudaStream_t st);
 
 // ---- optimizer -----------------------------------------------------------------------------------
 // acc[0] += sum((g * inv_scale)^2), acc[1] = 1 if any non-finite value was seen.

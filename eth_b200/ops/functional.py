@@ -477,11 +477,10 @@ def embedding(tokens, word, pos, seq, vocab_start=0, add_pos=True):
 # ------------------------------------------------------------------------------------------
 class _VocabParallelCEFn(torch.autograd.Function):
     """Per-token loss from vocab-sharded logits. One exchange of (max, sum-exp, target-logit)
-    triples replaces the three all-reduces of eth/runtime/megatron/mpu/cross_entropy.py:33-118.
-    Backward overwrites the logits buffer with the gradient."""
+    triples replaces the three all-reduces of eth/runtime/megatron/mpu/cross_entropy.py:33-118."""
 
     @staticmethod
-    def forward(ctx, logits, targets, vocab_start, gather_fn):
+    def forward(ctx, logits, targets, vocab_start, gather_fn, overwrite_logits):
         rows = logits.shape[0]
         targets = targets.reshape(-1).contiguous()
         if native.use_native(logits):
@@ -506,7 +505,7 @@ class _VocabParallelCEFn(torch.autograd.Function):
             gsum = (all_stats[:, :, 1] * torch.exp(all_stats[:, :, 0] - gmax)).sum(0)
             loss = torch.log(gsum) + gmax - all_stats[:, :, 2].sum(0)
         ctx.save_for_backward(logits, targets, gmax, gsum)
-        ctx.vocab_start = vocab_start
+        ctx.vocab_start, ctx.overwrite_logits = vocab_start, overwrite_logits
         return loss
 
     @staticmethod
@@ -514,8 +513,9 @@ class _VocabParallelCEFn(torch.autograd.Function):
         logits, targets, gmax, gsum = ctx.saved_tensors
         dloss = dloss.float().contiguous()
         if native.use_native(logits):
-            native.lib().ce_bwd(logits, targets, gmax, gsum, dloss, ctx.vocab_start)
-            return logits, None, None, None
+            grad = logits if ctx.overwrite_logits else torch.empty_like(logits, memory_format=torch.contiguous_format)
+            native.lib().ce_bwd(logits, grad, targets, gmax, gsum, dloss, ctx.vocab_start)
+            return grad, None, None, None, None
         lf = logits.float()
         sm = torch.exp(lf - gmax[:, None]) / gsum[:, None]
         t = targets - ctx.vocab_start
@@ -523,13 +523,20 @@ class _VocabParallelCEFn(torch.autograd.Function):
         onehot = torch.zeros_like(sm)
         onehot[mine, t[mine]] = 1.0
         g = ((sm - onehot) * dloss[:, None]).to(logits.dtype)
-        return g, None, None, None
+        if ctx.overwrite_logits:
+            g = logits.copy_(g)
+        return g, None, None, None, None
 
 
-def vocab_parallel_cross_entropy(logits, targets, vocab_start=0, gather_fn=None):
+def vocab_parallel_cross_entropy(logits, targets, vocab_start=0, gather_fn=None, overwrite_logits=False):
     """logits: [tokens, vocab_local]; targets: [tokens] global ids. `gather_fn(stats[rows,3])`
-    returns the `[tp, rows, 3]` stack over the tensor-parallel group (None for TP=1)."""
-    return _VocabParallelCEFn.apply(logits, targets, int(vocab_start), gather_fn)
+    returns the `[tp, rows, 3]` stack over the tensor-parallel group (None for TP=1).
+
+    The gradient has memory of its own, so other losses may share the logits, built before or after this
+    one. `overwrite_logits` saves that memory: the backward then leaves the gradient in the logits
+    themselves, and a backward that runs later and needs the logits raises (autograd runs the loss that was
+    built last first)."""
+    return _VocabParallelCEFn.apply(logits, targets, int(vocab_start), gather_fn, bool(overwrite_logits))
 
 
 # ------------------------------------------------------------------------------------------

@@ -324,7 +324,7 @@ def ce_bwd_(logits, targets, gmax, gsum, dloss, vocab_start):
     """Overwrites `logits` with d loss / d logits scaled by dloss[row]; returns it."""
     targets = targets.reshape(-1).contiguous()
     if native.use_native(logits):
-        native.lib().ce_bwd(logits, targets, gmax, gsum, dloss.float().contiguous(), vocab_start)
+        native.lib().ce_bwd(logits, logits, targets, gmax, gsum, dloss.float().contiguous(), vocab_start)
         return logits
     sm = torch.exp(logits.float() - gmax[:, None]) / gsum[:, None]
     t = targets - vocab_start

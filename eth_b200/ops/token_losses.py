@@ -2,8 +2,9 @@
 alternatives, and the loss against a teacher's top logits.
 
 Both stand beside `vocab_parallel_cross_entropy` and take the same `vocab_start` / `gather_fn` for
-vocabulary-sharded logits: one exchange of per-token statistics per call. Unlike it they leave the
-logits as they are and allocate the gradient, so several of them may share one set of logits.
+vocabulary-sharded logits: one exchange of per-token statistics per call. They leave the
+logits as they are and allocate the gradient. Several of them, and that cross entropy, may share one set
+of logits, built in any order (with `overwrite_logits` the cross entropy has to be built first).
 """
 from __future__ import annotations
 

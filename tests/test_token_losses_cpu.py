@@ -174,3 +174,23 @@ def test_no_rows():
     loss = ops.topk_distillation_loss(z, torch.zeros(0, 2, dtype=torch.long), torch.zeros(0, 2))
     g, = torch.autograd.grad(loss.sum() + r.entropy.sum(), z)
     assert g.shape == (0, 11)
+
+
+@pytest.mark.parametrize("overwrite", [False, True])
+@pytest.mark.parametrize("last", [False, True])
+def test_logits_shared_with_cross_entropy(overwrite, last):
+    """Cross entropy built before or after the teacher's loss; where it may overwrite, autograd must notice."""
+    g = torch.Generator().manual_seed(8)
+    z = torch.randn(5, 24, generator=g, requires_grad=True)
+    index, logit = _teacher(5, 24, 4)
+    build = [lambda: ops.vocab_parallel_cross_entropy(z, index[:, 0], overwrite_logits=overwrite),
+             lambda: ops.topk_distillation_loss(z, index, logit)]
+    ones = torch.ones(5)
+    want = oracle.distill(z, index, logit, ones, 1.0)[1] + oracle.scores_grad(z, index[:, 0], None, -ones, None, None, 1.0)
+    outs = [f() for f in (build[::-1] if last else build)]
+    if overwrite and last:
+        with pytest.raises(RuntimeError, match="inplace"):
+            torch.autograd.grad(outs, z, [ones, ones])
+        return
+    got, = torch.autograd.grad(outs, z, [ones, ones])
+    torch.testing.assert_close(got.double(), want, rtol=0, atol=2e-6)

@@ -1,5 +1,6 @@
 """Vocabulary kernels (token log-probabilities with entropy and alternatives, distillation) against
 their definitions in 64 bits."""
+import itertools
 import math
 
 import pytest
@@ -307,3 +308,56 @@ def test_refusals_on_the_device():
                 lambda: raw.distill_step(z[:, :10], index, logit, torch.ones(3, device=DEV), out=z[:, 1:])):
         with pytest.raises(ValueError):
             bad()
+
+
+def _three_losses(z, order, g, **cross_entropy):
+    """Label loss, teacher loss and scores of the same logits, their nodes built in `order`; with the
+    gradients handed to them and the sum of the three in 64 bits (and of the magnitudes)."""
+    rows, vocab = z.shape
+    targets = torch.randint(vocab, (rows,), generator=g, device=DEV)
+    index, logit = _teacher(rows, vocab, 9, g)
+    build = {"cross entropy": lambda: ops.vocab_parallel_cross_entropy(z, targets, **cross_entropy),
+             "distillation": lambda: ops.topk_distillation_loss(z, index, logit),
+             "scores": lambda: ops.token_logprobs(z, targets)[:2]}
+    outs, d, parts = [], [], []
+    for name in order:
+        out = build[name]()
+        out = list(out) if name == "scores" else [out]
+        dout = [torch.randn(rows, generator=g, device=DEV) for _ in out]
+        outs, d = outs + out, d + dout
+        if name == "distillation":
+            parts.append(oracle.distill(z, index, logit, dout[0], 1.0)[1])
+        elif name == "scores":
+            parts.append(oracle.scores_grad(z, targets, None, *dout, None, 1.0))
+        else:
+            parts.append(oracle.scores_grad(z, targets, None, -dout[0], None, None, 1.0))
+    return outs, d, sum(parts), sum(p.abs() for p in parts)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("order", list(itertools.permutations(("cross entropy", "distillation", "scores"))))
+def test_losses_that_share_logits_with_cross_entropy(dtype, order):
+    """Autograd runs the node that was built last first, so none may write over what the others have saved."""
+    z, g = _logits(37, 4104, 0, 0, dtype, seed=21)
+    before = z.clone()
+    outs, d, want, size = _three_losses(z.requires_grad_(True), order, g)
+    got, = torch.autograd.grad(outs, z, d)
+    # each of the three is rounded once, and so are their two sums, which are at most `size`
+    bound = torch.finfo(dtype).eps / 2 * 3.01 * size + sum(x.abs() for x in d)[:, None] * 2.0 ** -17 + 2.0 ** -23
+    assert ((got.double() - want).abs() <= bound).all()
+    assert torch.equal(z.detach(), before)
+
+
+def test_cross_entropy_that_overwrites_is_noticed():
+    """In the order that autograd can honour the results are right; in the other it raises."""
+    z, g = _logits(37, 4104, 0, 0, torch.bfloat16, seed=27)
+    order = ("cross entropy", "distillation", "scores")
+    outs, d, want, size = _three_losses(z.requires_grad_(True), order, g, overwrite_logits=True)
+    got, = torch.autograd.grad(outs, z, d)
+    bound = torch.finfo(z.dtype).eps / 2 * 3.01 * size + sum(x.abs() for x in d)[:, None] * 2.0 ** -17
+    assert ((got.double() - want).abs() <= bound).all()
+    for order in (("distillation", "cross entropy"), ("scores", "cross entropy")):
+        z = _logits(37, 4104, 0, 0, torch.bfloat16, seed=28)[0].requires_grad_(True)
+        outs, d, _, _ = _three_losses(z, order, g, overwrite_logits=True)
+        with pytest.raises(RuntimeError, match="inplace"):
+            torch.autograd.grad(outs, z, d)
