@@ -415,6 +415,8 @@ std::tuple<Tensor, Tensor> distill_both(const Tensor& logits, const Tensor& inde
     const bool same = dz.data_ptr() == logits.data_ptr() && dz.strides() == logits.strides();
     TORCH_CHECK_VALUE(same || dz.storage().data() != logits.storage().data(),
                       "distill_step: out may be the logits themselves or other memory, not an overlapping view");
+    // a change in place: a node that has saved the logits and runs later raises, it does not read a gradient
+    dz.unsafeGetTensorImpl()->bump_version();
   } else {
     dz = grad_rows(z);
   }

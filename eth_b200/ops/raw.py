@@ -732,7 +732,8 @@ def distill_bwd(logits, teacher_index, teacher_logit, stats, dloss, temperature=
 def distill_step(logits, teacher_index, teacher_logit, dloss, temperature=1.0, out=None):
     """(loss, d logits) of `distill_fwd` and `distill_bwd` in one pass over the logits, for a caller that
     knows the gradient of every row's loss beforehand (the last pipeline stage does: loss scale over
-    token count). Whole vocabulary only. `out` takes the gradient; it may be `logits` itself."""
+    token count). Whole vocabulary only. `out` takes the gradient; it may be `logits` itself, which counts
+    as a change in place: a loss built on the same logits whose backward runs later raises."""
     if native.use_native(logits):
         return native.lib().distill_step(logits, teacher_index, teacher_logit, dloss, temperature, out)
     _check_logits(logits, temperature, "distill_step")

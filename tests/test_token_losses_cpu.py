@@ -194,3 +194,12 @@ def test_logits_shared_with_cross_entropy(overwrite, last):
         return
     got, = torch.autograd.grad(outs, z, [ones, ones])
     torch.testing.assert_close(got.double(), want, rtol=0, atol=2e-6)
+
+
+def test_step_into_saved_logits_is_noticed():
+    z = torch.randn(4, 9, generator=torch.Generator().manual_seed(9), requires_grad=True)
+    index, logit = _teacher(4, 9, 3)
+    loss = ops.topk_distillation_loss(z, index, logit)
+    raw.distill_step(z.detach(), index, logit, torch.ones(4), out=z.detach())
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(loss, z, torch.ones(4))

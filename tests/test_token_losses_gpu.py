@@ -361,3 +361,16 @@ def test_cross_entropy_that_overwrites_is_noticed():
         outs, d, _, _ = _three_losses(z, order, g, overwrite_logits=True)
         with pytest.raises(RuntimeError, match="inplace"):
             torch.autograd.grad(outs, z, d)
+
+
+def test_step_into_saved_logits_is_noticed():
+    """The gradient that replaces the logits must not pass for them in a backward that comes later."""
+    z, g = _logits(5, 1003, 0, 0, torch.bfloat16, seed=22)
+    index, logit = _teacher(5, 1003, 4, g)
+    tokens, ones = torch.zeros(5, dtype=torch.long, device=DEV), torch.ones(5, device=DEV)
+    for build in (lambda x: ops.token_logprobs(x, tokens).logprob, lambda x: ops.topk_distillation_loss(x, index, logit)):
+        leaf = z.clone().requires_grad_(True)
+        loss = build(leaf)
+        raw.distill_step(leaf.detach(), index, logit, ones, out=leaf.detach())
+        with pytest.raises(RuntimeError, match="inplace"):
+            torch.autograd.grad(loss, leaf, ones)
