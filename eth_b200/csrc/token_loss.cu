@@ -502,6 +502,12 @@ __device__ void select_top(const Row<T>& r, int k, float thread_max, bool thread
   __syncthreads();
 }
 
+// The sum of exponentials as the backward gets it: negative where the row's token lies outside the vocabulary
+// (zt is NaN), so that the gradient of its log-probability, which is NaN, is NaN as well.
+__device__ __forceinline__ float marked_sum(float l, int64_t token, float zt) {
+  return token >= 0 && zt != zt ? -l : l;
+}
+
 constexpr int kScanGroup = 8;   // loads in flight per thread of the kernels that read a row once
 
 // ---------------------------------------------------------------------------------------------
@@ -550,7 +556,7 @@ token_scores_kernel(const T* __restrict__ z, int64_t ld, int vocab, int64_t v0, 
       out.logprob[row] = t < 0 ? 0.f : (zt - mu) * inv_t - log_l;
       out.entropy[row] = log_l - kLn2 * (all.a / all.l);
       out.stats[2 * row] = mu;
-      out.stats[2 * row + 1] = all.l;
+      out.stats[2 * row + 1] = marked_sum(all.l, t, zt);
     }
   }
   if constexpr (kTop) {
@@ -598,7 +604,7 @@ __global__ void token_scores_combine_kernel(const float* __restrict__ parts, int
     out.logprob[row] = tokens[row] < 0 ? 0.f : (zt - mu) * inv_t - log_l;
     out.entropy[row] = log_l - kLn2 * (all.a / all.l);
     out.stats[2 * row] = mu;
-    out.stats[2 * row + 1] = all.l;
+    out.stats[2 * row + 1] = marked_sum(all.l, tokens[row], zt);
   }
   auto key = [&](int c) {
     const float* q = parts + ((c / top_k) * rows + row) * width + 4 + c % top_k;
@@ -771,8 +777,9 @@ __global__ void token_scores_bwd_kernel(const T* z, int64_t ld, int vocab, int64
     write_zero(d, vocab);
     return;
   }
-  const float A = -(gr + usum + (kLog ? hr * entropy[row] : 0.f)) * inv_t;
-  const DenseTerm f = DenseTerm::of(stats[2 * row], stats[2 * row + 1], inv_t * kLog2e, A, kLog ? -hr * inv_t : 0.f);
+  const float l = stats[2 * row + 1];   // see marked_sum
+  const float A = l < 0.f && gr != 0.f ? CUDART_NAN_F : -(gr + usum + (kLog ? hr * entropy[row] : 0.f)) * inv_t;
+  const DenseTerm f = DenseTerm::of(stats[2 * row], fabsf(l), inv_t * kLog2e, A, kLog ? -hr * inv_t : 0.f);
   write_grad<T, kLog, false>(r, d, f, li, 1 + extra, [&](int i) { return li.w[i]; });
 }
 

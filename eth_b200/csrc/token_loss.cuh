@@ -20,7 +20,8 @@ struct LogitsView {
   float inv_temperature;
 };
 
-// stats: [rows, 2] (subtracted maximum, sum of exponentials) kept for the backward pass.
+// stats: [rows, 2] (subtracted maximum, sum of exponentials, negative where the token lies outside the vocabulary)
+// kept for the backward pass.
 struct TokenScoresOut {
   float *logprob, *entropy, *top_logprob;   // [rows], [rows], [rows, top_k]
   int64_t* top_index;                       // [rows, top_k] global token ids

@@ -573,11 +573,12 @@ def _check_rows(t, logits, dtypes, shape, what):
 def token_scores_fwd(logits, tokens, top_k=0, temperature=1.0, vocab_start=0, gather_fn=None):
     """Log-probability of `tokens` under softmax(logits / temperature), entropy of that distribution and
     its `top_k` most likely tokens. Returns (logprob, entropy, top_logprob, top_index, stats); `stats`
-    [tokens, 2] (subtracted maximum, sum of exponentials) belongs to `token_scores_bwd`.
+    [tokens, 2] (subtracted maximum, sum of exponentials) belongs to `token_scores_bwd`. The sum is
+    negative where the token lies outside the vocabulary.
 
     logits: [tokens, vocab_local] of a vocabulary shard that starts at `vocab_start`; `gather_fn` as in
     `ce_fwd`. A negative token is none: its log-probability is 0 and has no gradient; one at or beyond
-    the whole vocabulary has NaN. Alternatives fall in log-probability, equal ones go by rising id."""
+    the whole vocabulary has NaN, and so has its gradient. Alternatives fall in log-probability, equal ones go by rising id."""
     if native.use_native(logits):
         if gather_fn is None:
             return native.lib().token_scores_fwd(logits, tokens, top_k, temperature, vocab_start)
@@ -620,6 +621,7 @@ def token_scores_fwd(logits, tokens, top_k=0, temperature=1.0, vocab_start=0, ga
         best = torch.sort(value, dim=1, descending=True, stable=True).indices[:, :top_k]
         top_logprob = (value.gather(1, best) - mu[:, None]) / temperature - log_total[:, None]
         top_index = index.gather(1, best)
+    total = torch.where((tokens >= 0) & zt.isnan(), -total, total)
     return logprob, entropy, top_logprob, top_index, torch.stack([mu, total], 1)
 
 
@@ -639,10 +641,11 @@ def token_scores_bwd(logits, tokens, stats, entropy, top_index, d_logprob=None, 
         grads.append(None if t is None else _check_rows(t, logits, wide, shape, what))
     g, h, u = grads
     z = _wide(logits)
-    logp = (z - stats[:, :1]) / temperature - torch.log(stats[:, 1:])
+    logp = (z - stats[:, :1]) / temperature - torch.log(stats[:, 1:].abs())
     p = torch.exp(logp)
     zero = z.new_zeros(rows)
     g = zero if g is None else torch.where(tokens >= 0, g, 0.0).to(z.dtype)
+    g = torch.where((stats[:, 1] < 0) & (g != 0), math.nan, g)
     h = zero if h is None else h.to(z.dtype)
     total = g if u is None else g + u.sum(1).to(z.dtype)
     dz = -p * total[:, None] - torch.where(p > 0, p * (logp + entropy[:, None]), 0.0) * h[:, None]

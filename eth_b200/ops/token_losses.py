@@ -49,10 +49,10 @@ def token_logprobs(logits, tokens, top_k=0, temperature=1.0, vocab_start=0, gath
     top_logprob, top_index)`, all differentiable but the ids.
 
     logits: [tokens, vocab_local], fp32 / fp16 / bf16, any row pitch; tokens: [tokens] int64 global ids,
-    a negative one marks a token that is not scored (log-probability 0, no gradient). `top_k` (up to
-    128) adds the most likely tokens, equal ones by rising id. `vocab_start` and `gather_fn` as in
-    `vocab_parallel_cross_entropy` (`gather_fn` returns the `[tp, tokens, n]` stack of a `[tokens, n]`
-    tensor over the tensor-parallel group)."""
+    a negative one marks a token that is not scored (log-probability 0, no gradient), one outside the
+    vocabulary has NaN for both. `top_k` (up to 128) adds the most likely tokens, equal ones by rising id.
+    `vocab_start` and `gather_fn` as in `vocab_parallel_cross_entropy` (`gather_fn` returns the `[tp,
+    tokens, n]` stack of a `[tokens, n]` tensor over the tensor-parallel group)."""
     if gather_fn is None and native.use_native(logits):     # the autograd node is native too
         r = native.lib().token_logprobs(logits, tokens, top_k, temperature, vocab_start)
         return TokenScores(*r) if top_k else TokenScores(*r, None, None)

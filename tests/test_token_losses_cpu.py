@@ -203,3 +203,15 @@ def test_step_into_saved_logits_is_noticed():
     raw.distill_step(z.detach(), index, logit, torch.ones(4), out=z.detach())
     with pytest.raises(RuntimeError, match="inplace"):
         torch.autograd.grad(loss, z, torch.ones(4))
+
+
+def test_gradient_of_a_token_outside_the_vocabulary():
+    """NaN where the log-probability is NaN and has a gradient; the entropy's own gradient stays defined."""
+    z = torch.randn(4, 9, generator=torch.Generator().manual_seed(10), requires_grad=True)
+    tokens, ones = torch.tensor([9, 8, -1, 9]), torch.ones(4)
+    r = ops.token_logprobs(z, tokens)
+    got, = torch.autograd.grad(r.logprob, z, torch.tensor([1.0, 1.0, 1.0, 0.0]), retain_graph=True)
+    assert got[0].isnan().all() and got[1].isfinite().all() and (got[2:] == 0).all()
+    got, = torch.autograd.grad(r.entropy, z, ones)
+    want = oracle.scores_grad(z, torch.zeros(4, dtype=torch.long), None, None, ones, None, 1.0)
+    torch.testing.assert_close(got.double(), want, rtol=0, atol=1e-6)

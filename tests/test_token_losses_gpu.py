@@ -374,3 +374,35 @@ def test_step_into_saved_logits_is_noticed():
         raw.distill_step(leaf.detach(), index, logit, ones, out=leaf.detach())
         with pytest.raises(RuntimeError, match="inplace"):
             torch.autograd.grad(loss, leaf, ones)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradient_of_a_token_outside_the_vocabulary(dtype):
+    """NaN where the log-probability is NaN and has a gradient; the entropy's own gradient stays defined."""
+    z, g = _logits(5, 6000, 0, 0, dtype, seed=23)
+    z.requires_grad_(True)
+    tokens = torch.tensor([6000, 1 << 40, 5999, -1, 6000], device=DEV)
+    r = ops.token_logprobs(z, tokens)
+    assert r.logprob[[0, 1, 4]].isnan().all()
+    d = torch.ones(5, device=DEV)
+    d[4] = 0
+    got, = torch.autograd.grad(r.logprob, z, d, retain_graph=True)
+    assert got[:2].isnan().all() and got[2].isfinite().all() and (got[3:] == 0).all()
+    got, = torch.autograd.grad(r.entropy, z, torch.ones(5, device=DEV))
+    want = oracle.scores_grad(z, torch.zeros_like(tokens), None, None, torch.ones(5, device=DEV), None, 1.0)
+    assert oracle.grad_error(got, want, torch.full((5,), 2.0 ** -17, device=DEV)) <= 1
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradient_of_a_token_outside_sharded_vocabularies(dtype):
+    part, world = 3001, 2
+    logits, g = _logits(4, part * world, 0, 0, dtype, seed=24)
+    tokens = torch.tensor([part * world, 17, part, -1], device=DEV)
+    shards, sent = logits.split(part, 1), []
+    for w, z in enumerate(shards):
+        ops.token_logprobs(z, tokens, 0, 1.0, w * part, lambda x: (sent.append(x), x.unsqueeze(0))[1])
+    for w, z in enumerate(shards):
+        z = z.detach().requires_grad_(True)
+        r = ops.token_logprobs(z, tokens, 0, 1.0, w * part, lambda x: torch.stack(sent))
+        got, = torch.autograd.grad(r.logprob.sum(), z)
+        assert got[0].isnan().all() and got[1:3].isfinite().all() and (got[3] == 0).all()
