@@ -842,6 +842,14 @@ __device__ __forceinline__ float listed_loss(const Listed& li, int k, const Teac
   return warp_sum(part);
 }
 
+// All lanes of a warp: whether the used entries of a staged whole-vocabulary list all lie in the vocabulary.
+// Where not, the loss is NaN, and a sum of exponentials of NaN carries that into the gradient.
+__device__ __forceinline__ bool all_known(const Listed& li, int k) {
+  bool known = true;
+  for (int i = threadIdx.x & 31; i < k; i += 32) known &= li.id[i] >= 0 || li.w[i] == -INFINITY;
+  return __all_sync(0xffffffffu, known);
+}
+
 // Same shape as token_scores_kernel, without the entropy (8192 x 50304 bf16: 6.6 TB/s).
 template <typename T, int kThreads, int kPerSm>
 __global__ void __launch_bounds__(kThreads, kPerSm)
@@ -877,11 +885,12 @@ distill_fwd_kernel(const T* __restrict__ z, int64_t ld, int vocab, int64_t v0, T
     return;
   }
   const float l = listed_loss(li, t.k, tr, inv_t, mu, kLn2 * log2f(all.l));
+  const bool known = all_known(li, t.k);
   if (threadIdx.x == 0) {
     const bool empty = tr.mass == 0.f;   // nothing listed: no loss, whatever the logits
     loss[row] = l;
     stats[2 * row] = empty ? 0.f : mu;
-    stats[2 * row + 1] = empty ? 1.f : all.l;
+    stats[2 * row + 1] = empty ? 1.f : known ? all.l : CUDART_NAN_F;
   }
 }
 
@@ -930,7 +939,7 @@ __global__ void distill_combine_kernel(const float* __restrict__ parts, int worl
     const bool whole = count == used;   // else an entry lies outside the vocabulary
     loss[row] = empty ? 0.f : whole ? self - found + kLn2 * log2f(all.l) : CUDART_NAN_F;
     stats[2 * row] = empty ? 0.f : mu;
-    stats[2 * row + 1] = empty ? 1.f : all.l;
+    stats[2 * row + 1] = empty ? 1.f : whole ? all.l : CUDART_NAN_F;   // see all_known
   }
 }
 
@@ -984,7 +993,7 @@ distill_step_kernel(const T* z, int64_t ld, int vocab, int64_t v0, TeacherView t
   if (tr.mass == 0.f || g == 0.f) {
     write_zero(d, vocab);
   } else {
-    const DenseTerm f = DenseTerm::of(mu, all.l, s2, g * tr.mass, 0.f);
+    const DenseTerm f = DenseTerm::of(mu, all_known(li, t.k) ? all.l : CUDART_NAN_F, s2, g * tr.mass, 0.f);
     write_grad<T, false, true>(r, d, f, li, t.k, [&](int i) { return listed_grad(li, tr, inv_t, g, i); });
   }
   if (threadIdx.x < 32) {

@@ -687,7 +687,7 @@ def distill_fwd(logits, teacher_index, teacher_logit, temperature=1.0, vocab_sta
     """Per-token loss sum_k q_k (log q_k - log p[teacher_index_k]), q = softmax of the listed teacher
     logits / temperature, p = softmax(logits / temperature) over the whole vocabulary. Returns (loss,
     stats for `distill_bwd`). An entry at -inf is unused; a row without entries has loss 0; a used
-    entry outside the vocabulary makes the row's loss NaN. An id listed twice counts twice."""
+    entry outside the vocabulary makes the row's loss and gradient NaN. An id listed twice counts twice."""
     if native.use_native(logits):
         if gather_fn is None:
             return native.lib().distill_fwd(logits, teacher_index, teacher_logit, temperature, vocab_start)
@@ -715,6 +715,7 @@ def distill_fwd(logits, teacher_index, teacher_logit, temperature=1.0, vocab_sta
     whole = parts[:, :, 4].sum(0) == used.sum(1)
     loss = torch.where(q != 0, q * log_q, 0.0).sum(1) - found + torch.log(total)
     loss = torch.where(some, torch.where(whole, loss, math.nan), 0.0)
+    total = torch.where(whole, total, math.nan)      # the gradient of a loss that is NaN is NaN
     return loss, torch.stack([torch.where(some, mu, 0.0), torch.where(some, total, 1.0)], 1)
 
 

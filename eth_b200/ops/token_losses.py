@@ -82,8 +82,8 @@ def topk_distillation_loss(logits, teacher_index, teacher_logit, temperature=1.0
     [tokens, k] fp32 logits or log-probabilities (what `token_logprobs(..., top_k=k)` reports), -inf for
     unused entries. The teacher is renormalised over its list at `temperature`, the student is its full
     softmax at the same temperature: loss = sum_k q_k (log q_k - log p_k). The customary factor
-    temperature**2 is left to the caller. A row without entries has loss 0 and no gradient. No gradient
-    flows to the teacher. `vocab_start` / `gather_fn`: see `token_logprobs`."""
+    temperature**2 is left to the caller. A row without entries has loss 0 and no gradient, one with a
+    used entry outside the vocabulary NaN for both. No gradient flows to the teacher. `vocab_start` / `gather_fn`: see `token_logprobs`."""
     if gather_fn is None and native.use_native(logits):
         return native.lib().topk_distillation_loss(logits, teacher_index, teacher_logit, temperature, vocab_start)
     return _DistillFn.apply(logits, teacher_index, teacher_logit, float(temperature), int(vocab_start), gather_fn)

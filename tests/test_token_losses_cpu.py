@@ -215,3 +215,13 @@ def test_gradient_of_a_token_outside_the_vocabulary():
     got, = torch.autograd.grad(r.entropy, z, ones)
     want = oracle.scores_grad(z, torch.zeros(4, dtype=torch.long), None, None, ones, None, 1.0)
     torch.testing.assert_close(got.double(), want, rtol=0, atol=1e-6)
+
+
+def test_gradient_of_a_list_with_an_entry_outside_the_vocabulary():
+    z = torch.randn(3, 9, generator=torch.Generator().manual_seed(11), requires_grad=True)
+    index, logit = torch.tensor([[5, 9], [7, 8], [1, 9]]), torch.tensor([[0.0, -40.0], [0.0, 1.0], [0.0, -math.inf]])
+    loss = ops.topk_distillation_loss(z, index, logit)
+    got, = torch.autograd.grad(loss, z, torch.ones(3))
+    _, step = raw.distill_step(z.detach(), index, logit, torch.ones(3))
+    for t in (got, step):
+        assert t[0].isnan().all() and t[1:].isfinite().all()

@@ -406,3 +406,26 @@ def test_gradient_of_a_token_outside_sharded_vocabularies(dtype):
         r = ops.token_logprobs(z, tokens, 0, 1.0, w * part, lambda x: torch.stack(sent))
         got, = torch.autograd.grad(r.logprob.sum(), z)
         assert got[0].isnan().all() and got[1:3].isfinite().all() and (got[3] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradient_of_a_list_with_an_entry_outside_the_vocabulary(dtype):
+    z, g = _logits(4, 3000, 0, 0, dtype, seed=25)
+    index = torch.tensor([[5, 3000], [2999, -3], [7, 8], [9, 3000]], device=DEV)
+    logit = torch.tensor([[0.0, -40.0], [0.5, 0.0], [0.0, 1.0], [0.0, -math.inf]], device=DEV)
+    leaf = z.clone().requires_grad_(True)
+    ones = torch.ones(4, device=DEV)
+    loss = ops.topk_distillation_loss(leaf, index, logit)
+    assert loss[:2].isnan().all() and loss[2:].isfinite().all()
+    got, = torch.autograd.grad(loss, leaf, ones)
+    _, step = raw.distill_step(z, index, logit, ones)
+    sent, part = [], 1500
+    for w, x in enumerate(z.split(part, 1)):
+        ops.topk_distillation_loss(x, index, logit, 1.0, w * part, lambda s: (sent.append(s), s.unsqueeze(0))[1])
+    shards = []
+    for w, x in enumerate(z.split(part, 1)):
+        x = x.detach().requires_grad_(True)
+        loss = ops.topk_distillation_loss(x, index, logit, 1.0, w * part, lambda s: torch.stack(sent))
+        shards.append(torch.autograd.grad(loss, x, ones)[0])
+    for t in (got, step, torch.cat(shards, 1)):
+        assert t[:2].isnan().all() and t[2:].isfinite().all()
