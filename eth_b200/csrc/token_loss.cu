@@ -105,9 +105,13 @@ __device__ __forceinline__ Pair exp2_pair(Pair t) {
 // A masked (-inf) logit has 2^t = 0 and t = -inf, whose product would be NaN. Where a sum or gradient
 // needs 2^t * t, logits below kFloor are raised to it, which leaves 2^t at 0 (it is 0 in fp32 below
 // t = -150) and t finite. Rows that lie so low themselves, or a temperature so high, that this does
-// not hold take a clamp per element instead.
+// not hold take a clamp per element instead; so do rows so high (a token forced by the type's highest
+// value), or a temperature so low, that t or its product with a gradient's factor would pass fp32's range.
 constexpr float kFloor = -57344.f;   // -7 * 2^13: exact in every type
-__device__ __forceinline__ bool has_floor(float mu, float s2) { return (mu - kFloor) * s2 > 200.f; }
+__device__ __forceinline__ bool has_floor(float mu, float s2, float factor = 1.f) {
+  const float depth = (mu - kFloor) * s2;   // -t of a raised logit
+  return depth > 200.f && depth * fmaxf(fabsf(factor), 1.f) < 1e38f;
+}
 __device__ __forceinline__ uint32_t max_nan(uint32_t x, float low) {
   uint32_t r;
   asm("max.NaN.f32 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(__float_as_uint(low)));
@@ -648,7 +652,7 @@ struct DenseTerm {
     const float inv = 1.0f / l;
     f.a = (B == 0.f ? A : A - B * (kLn2 * log2f(l))) * inv;
     f.b = B * kLn2 * inv;
-    f.floor = has_floor(mu, s2);
+    f.floor = has_floor(mu, s2, f.b);
     return f;
   }
   template <bool kLog> __device__ __forceinline__ float at(float z) const {

@@ -429,3 +429,26 @@ def test_gradient_of_a_list_with_an_entry_outside_the_vocabulary(dtype):
         shards.append(torch.autograd.grad(loss, x, ones)[0])
     for t in (got, step, torch.cat(shards, 1)):
         assert t[:2].isnan().all() and t[2:].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("temperature", [1.0, 1e-20, 1e-30])
+def test_forced_tokens(dtype, temperature):
+    """One logit so far above the others that their distance in units of the temperature passes what fp32
+    holds: probability 1, entropy 0 and no gradient, not NaN."""
+    info = torch.finfo(dtype)
+    z, g = _logits(6, 5003, 0, 0, dtype, seed=26)
+    z[0, 17] = info.max
+    z[1] = info.min
+    z[1, 17] = info.max
+    z[2, 17] = info.max / 4
+    z[3, 17] = 200.0
+    z[4] = -math.inf
+    z[4, 17] = info.max
+    z[5, 17] = 1000.0
+    tokens = torch.full((6,), 17, device=DEV)
+    z.requires_grad_(True)
+    r = ops.token_logprobs(z, tokens, top_k=3, temperature=temperature)
+    assert (r.logprob == 0).all() and (r.entropy == 0).all() and (r.top_index[:, 0] == 17).all()
+    got, = torch.autograd.grad((r.logprob, r.entropy), z, [torch.ones(6, device=DEV)] * 2)
+    assert (got == 0).all()
