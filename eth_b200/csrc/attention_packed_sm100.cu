@@ -89,31 +89,22 @@ __device__ __forceinline__ uint32_t pack_pair(float a, float b, int dtype) {
 // 2^x on the FMA pipe: x = i + f with i the nearest whole number, 2^f on [-1/2, 1/2] by a polynomial
 // (minimax in relative error, found by Remez exchange), 2^i built in the exponent field. The softmax
 // warps take part of their exponentials this way: 16 special-function results per clock and SM are the
-// longest step of a score tile, the FMA pipe is idle then. Degree 3 is off by 7.5e-5, a fiftieth of a
-// bf16 step; fp16 takes degree 4, 2.7e-6. Below x = -126 the result stays at 2^-126; NaN stays NaN.
-template <int DT>
+// longest step of a score tile, the FMA pipe is idle then. Degree 4 is off by 2.7e-6 at most. Below
+// x = -126.5 the result is 0 (the exponent field of i = -127 is that of 0); NaN stays NaN.
 __device__ __forceinline__ Pair exp2_poly(Pair x) {
   float a, b;
   split(x, a, b);
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-127.f));
   x = pair(a, b);
   const float magic = 12582912.f;   // 1.5 * 2^23: the sum's low mantissa bits hold the rounded x
   const Pair r = x + pair(magic, magic);
   const Pair f = x + (pair(magic, magic) + r * pair(-1.f, -1.f));
-  Pair y;
-  if constexpr (DT == kBF16) {
-    y = pair(0.05517167f, 0.05517167f);
-    y = fma2(y, f, pair(0.24261112f, 0.24261112f));
-    y = fma2(y, f, pair(0.69326099f, 0.69326099f));
-    y = fma2(y, f, pair(0.99992807f, 0.99992807f));
-  } else {
-    y = pair(0.0095701f, 0.0095701f);
-    y = fma2(y, f, pair(0.05591786f, 0.05591786f));
-    y = fma2(y, f, pair(0.24024745f, 0.24024745f));
-    y = fma2(y, f, pair(0.69312181f, 0.69312181f));
-    y = fma2(y, f, pair(0.99999926f, 0.99999926f));
-  }
+  Pair y = pair(0.0095701f, 0.0095701f);
+  y = fma2(y, f, pair(0.05591786f, 0.05591786f));
+  y = fma2(y, f, pair(0.24024745f, 0.24024745f));
+  y = fma2(y, f, pair(0.69312181f, 0.69312181f));
+  y = fma2(y, f, pair(0.99999926f, 0.99999926f));
   split(r, a, b);
   return y * pair(__int_as_float((__float_as_int(a) << 23) + 0x3f800000),
                   __int_as_float((__float_as_int(b) << 23) + 0x3f800000));
@@ -124,9 +115,9 @@ __device__ __forceinline__ Pair exp2_sfu(Pair x) {
   return pair(exp2f(a), exp2f(b));
 }
 // Pair `i` of a row of scores: kPolyPairs out of four take the FMA pipe.
-template <int DT, int kPolyPairs>
+template <int kPolyPairs>
 __device__ __forceinline__ Pair exp2_mixed(int i, Pair x) {
-  return (i & 3) < kPolyPairs ? exp2_poly<DT>(x) : exp2_sfu(x);
+  return (i & 3) < kPolyPairs ? exp2_poly(x) : exp2_sfu(x);
 }
 __device__ __forceinline__ uint32_t pack_pair(Pair p, int dtype) {
   float a, b;
@@ -1265,9 +1256,9 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
           for (int y = 0; y < 16; ++y) {
             const float4 l4 = *reinterpret_cast<const float4*>(a_lse + 4 * y);
             const uint32_t* r4 = &rs[y >> 3][(4 * y) & 31];
-            pv[2 * y] = exp2_mixed<DT, kBwdPoly>(
+            pv[2 * y] = exp2_mixed<kBwdPoly>(
                 2 * y, fma2(pair(__uint_as_float(r4[0]), __uint_as_float(r4[1])), scale, pair(l4.x, l4.y)));
-            pv[2 * y + 1] = exp2_mixed<DT, kBwdPoly>(
+            pv[2 * y + 1] = exp2_mixed<kBwdPoly>(
                 2 * y + 1, fma2(pair(__uint_as_float(r4[2]), __uint_as_float(r4[3])), scale, pair(l4.z, l4.w)));
           }
         }
@@ -1579,7 +1570,7 @@ packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_consta
           const Pair scale = pair(sl2, sl2), bias = pair(neg_lse, neg_lse);
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            pv[e] = exp2_mixed<DT, kBwdPoly>(e, fma2(pair(__uint_as_float(rs[e >> 4][(2 * e) & 31]),
+            pv[e] = exp2_mixed<kBwdPoly>(e, fma2(pair(__uint_as_float(rs[e >> 4][(2 * e) & 31]),
                                                           __uint_as_float(rs[e >> 4][(2 * e + 1) & 31])), scale, bias));
         }
         if (masked) {   // the common case carries no mask

@@ -1,5 +1,7 @@
 """Packed-document attention on the CPU path, the work lists of its layout, and its refusals."""
 import math
+import re
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -92,3 +94,26 @@ def test_layout_from_tensors_and_arrays():
         layout = ops.PackedLayout(lengths, total=7)
         assert layout.lengths == (3, 0, 2) and layout.used == 5 and layout.total == 7
         assert list(layout.documents()) == [(0, 3), (3, 2)]
+
+
+def test_exponential_on_the_fma_pipe():
+    """`exp2_poly` of the backward kernels, restated step by step in fp32 with the coefficients of its source:
+    within 2^-17 of 2^x (the oracle grants all fp32 steps together 2^-15), 0 where 2^x is no normal number."""
+    source = Path(raw.__file__).parents[1].joinpath("csrc", "attention_packed_sm100.cu").read_text()
+    body = source[source.index("Pair exp2_poly(Pair x)"):source.index("Pair exp2_sfu")]
+    f32 = np.float32
+    floor = f32(re.search(r'"f"\((-[\d.]+)f\)', body).group(1))
+    coefficients = [f32(c) for c in re.findall(r"pair\((0\.\d+)f, \1f\)", body)]
+    magic = f32(12582912.0)
+    x = np.concatenate([np.linspace(-130, 1, 1 << 20), -np.arange(131), [-126.5, -1e4, -np.inf]]).astype(f32)
+    at = np.maximum(x, floor)
+    r = at + magic
+    f = at + (magic - r)
+    y = np.full_like(f, coefficients[0])
+    for c in coefficients[1:]:
+        y = (y.astype(np.float64) * f + c).astype(f32)          # fused: one rounding
+    field = ((r.view(np.int32).astype(np.int64) << 23) + 0x3f800000).astype(np.uint32).view(f32)
+    got, want = (y * field).astype(np.float64), np.exp2(x.astype(np.float64))
+    normal = x >= -126
+    assert (np.abs(got - want)[normal] <= 2.0 ** -17 * want[normal]).all()
+    assert (np.abs(got - want)[~normal] <= 2.0 ** -126).all() and (got[x <= -127] == 0).all()

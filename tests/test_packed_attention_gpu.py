@@ -363,3 +363,12 @@ def test_teacher_and_student_on_packed_documents():
     assert abs(total.item() - total64.item()) < 0.01 * abs(total64.item())
     for a, b in zip(got, want):
         assert ((a.double() - b).norm() / b.norm()).item() < 0.06
+
+
+def test_keys_far_below_the_maximum():
+    """A probability of 2^-288 is 0 in dV, however large the gradient that comes in."""
+    q, k, v, do = (torch.zeros(2, 1, 64, dtype=torch.bfloat16, device=DEV) for _ in range(4))
+    q[0, 0, 0] = 1.0
+    k[1, 0, 0] = -200.0
+    do[0] = 2.0 ** 125
+    _check([2], q, k, v, do, False, scale=1.0)
