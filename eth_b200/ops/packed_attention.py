@@ -31,9 +31,11 @@ class PackedLayout:
             lengths = lengths.astype(np.int64)
         if lengths.ndim != 1 or lengths.dtype.kind not in "iu":
             raise ValueError("PackedLayout: lengths must be a 1-D sequence of whole numbers")
-        lengths = lengths.astype(np.int64)
         if lengths.size and int(lengths.min()) < 0:
             raise ValueError("PackedLayout: a document cannot have fewer than 0 tokens")
+        if lengths.size and int(lengths.max()) >= 2 ** 31:      # also keeps the 64-bit sum below from wrapping
+            raise ValueError(f"PackedLayout: a document of {int(lengths.max())} tokens is too long")
+        lengths = lengths.astype(np.int64)
         self.used = int(lengths.sum())
         self.total = self.used if total is None else int(total)
         if not self.used <= self.total < 2 ** 31 - 256:

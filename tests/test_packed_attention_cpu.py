@@ -117,3 +117,10 @@ def test_exponential_on_the_fma_pipe():
     normal = x >= -126
     assert (np.abs(got - want)[normal] <= 2.0 ** -17 * want[normal]).all()
     assert (np.abs(got - want)[~normal] <= 2.0 ** -126).all() and (got[x <= -127] == 0).all()
+
+
+@pytest.mark.parametrize("lengths", [[2 ** 62, 2 ** 62], [2 ** 63 - 1, 2], [2 ** 62] * 4,
+                                     np.array([2 ** 64 - 1], dtype=np.uint64), [2 ** 31]])
+def test_lengths_whose_sum_wraps(lengths):
+    with pytest.raises(ValueError):
+        ops.PackedLayout(lengths)
