@@ -38,6 +38,8 @@ class PackedLayout:
         lengths = lengths.astype(np.int64)
         self.used = int(lengths.sum())
         self.total = self.used if total is None else int(total)
+        if total is not None and self.total != total:
+            raise ValueError(f"PackedLayout: total must be a whole number, got {total}")
         if not self.used <= self.total < 2 ** 31 - 256:
             raise ValueError(f"PackedLayout: documents of {self.used} tokens do not fit {self.total} rows")
         self.lengths = tuple(int(n) for n in lengths)

@@ -124,3 +124,11 @@ def test_exponential_on_the_fma_pipe():
 def test_lengths_whose_sum_wraps(lengths):
     with pytest.raises(ValueError):
         ops.PackedLayout(lengths)
+
+
+def test_total_is_a_whole_number():
+    for total in (7, 7.0, np.int32(7), torch.tensor(7)):
+        assert ops.PackedLayout([3, 2], total=total).total == 7
+    for total in (7.5, 5.999, math.nan):
+        with pytest.raises(ValueError):
+            ops.PackedLayout([3, 2], total=total)
