@@ -92,7 +92,7 @@ void check_packed(const Tensor& q, const Tensor& k, const Tensor& v, const Lists
                     "packed attention: fp16 / bf16 with head_dim 64 or 128 only, got ", q.scalar_type(), ", ", q.size(2));
   TORCH_CHECK_VALUE(l.total == q.size(0), "packed attention: layout of ", l.total, " rows, tensors of ", q.size(0));
   TORCH_CHECK_VALUE(l.used >= 0 && l.used <= l.total && l.total < 0x7fffff00, "packed attention: rows of the layout");
-  TORCH_CHECK_VALUE(scale >= 1e-30 && scale <= 1e30, "packed attention: scale must be between 1e-30 and 1e30, got ", scale);
+  TORCH_CHECK_VALUE(scale >= 1e-30 && scale <= 1e3, "packed attention: scale must be between 1e-30 and 1e3, got ", scale);
 }
 
 double scale_of(const Tensor& q, c10::optional<double> scale) {

@@ -433,8 +433,8 @@ def _check_packed(q, k, v, layout, scale):
     if layout.total != q.shape[0]:
         raise ValueError(f"packed attention: layout of {layout.total} rows, tensors of {q.shape[0]}")
     scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
-    if not 1e-30 <= scale <= 1e30:
-        raise ValueError(f"packed attention: scale must be between 1e-30 and 1e30, got {scale}")
+    if not 1e-30 <= scale <= 1e3:
+        raise ValueError(f"packed attention: scale must be between 1e-30 and 1e3, got {scale}")
     return scale
 
 

@@ -372,3 +372,30 @@ def test_keys_far_below_the_maximum():
     k[1, 0, 0] = -200.0
     do[0] = 2.0 ** 125
     _check([2], q, k, v, do, False, scale=1.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_largest_scale(dtype, dim):
+    """Scaled scores of up to x: fp32 sums of the products and an fp32 log-sum-exp are off by 2^-22 of that
+    each at most, so a probability by x 2^-21 of itself, and sums over them by twice that."""
+    lengths = [130, 257]
+    q, k, v, do = (t.contiguous().requires_grad_(True) for t in _inputs(lengths, 4, 2, dim, dtype, seed=17))
+    out = ops.flash_attention_packed(q, k, v, ops.PackedLayout(lengths, device=DEV), scale=1e3)
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), do)
+    want = oracle.attention(q, k, v, lengths, True, 1e3, do.detach())
+    x = 1e3 * max((q[r].double().norm(dim=2).max() * k[r].double().norm(dim=2).max()).item()
+                  for r in oracle.documents(lengths))
+    for name, t in (("out", out), ("dv", dv)):
+        value = want[name][0]
+        assert ((t.double() - value).norm() / value.norm()).item() <= x * 2.0 ** -20 + torch.finfo(dtype).eps
+    assert dq.isfinite().all() and dk.isfinite().all()
+
+
+@pytest.mark.parametrize("scale", [1.1e3, 1e7, 1e30])
+def test_scales_whose_scores_leave_fp32(scale):
+    q, k, v, _ = _inputs([5], 4, 2, 64, torch.bfloat16)
+    with pytest.raises(ValueError, match="scale"):
+        ops.flash_attention_packed(q, k, v, ops.PackedLayout([5], device=DEV), scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        ops.flash_attention_packed(q.cpu(), k.cpu(), v.cpu(), ops.PackedLayout([5]), scale=scale)
