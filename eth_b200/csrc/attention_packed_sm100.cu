@@ -76,10 +76,22 @@ cudaError_t make_tmap_rhd(CUtensorMap* map, const void* base, int dtype, int d, 
   return cudaSuccess;
 }
 
+// Where a wait that gave up leaves its mark: the device's status word, which the host reads, and a flag of
+// the CTA, by which its roles stop. They do not stop for the status word itself, as a mark that an earlier
+// kernel has left there would leave results of this one unwritten.
+struct Marks {
+  int* status;
+  int* gave_up;
+};
+__device__ __forceinline__ bool marked_wait(uint64_t* bar, uint32_t parity, const Marks& marks, int code) {
+  const bool got = mbar_wait(bar, parity, marks.status, code);
+  if (!got) *reinterpret_cast<volatile int*>(marks.gave_up) = 1;
+  return got;
+}
 // A wait whose outcome all lanes of the warp share, so that a timeout cannot split a warp (or, through
 // wg_and, a warpgroup) between leaving and going on to the next warp-wide or group-wide operation.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status, int code) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code));
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const Marks& marks, int code) {
+  return __all_sync(0xffffffffu, marked_wait(bar, parity, marks, code));
 }
 
 __device__ __forceinline__ uint32_t pack_pair(float a, float b, int dtype) {
@@ -308,7 +320,7 @@ struct FwdBarriers {
   uint64_t p_half[8];     // [tile * 4 + quarter]: 32 more P columns of a tile are written
   uint64_t o_done[2];
   uint32_t tmem_base;
-  uint32_t pad;
+  int gave_up;            // see Marks
 };
 
 // A CTA that is done with its block of the grid takes over blocks that have not been launched yet (cluster
@@ -322,8 +334,8 @@ __device__ __forceinline__ void ask_next_block(FwdBarriers* bars, int it) {
                : "memory");
 }
 // All lanes of a warp: the block that follows the `it`-th of this CTA, -1 if there is none.
-__device__ __forceinline__ int next_block(FwdBarriers* bars, int it, int lane, int* status) {
-  if (!warp_wait(&bars->answer_full[it & 1], static_cast<uint32_t>(it >> 1) & 1, status, kStatusTimeoutFull)) return -1;
+__device__ __forceinline__ int next_block(FwdBarriers* bars, int it, int lane, const Marks& marks) {
+  if (!warp_wait(&bars->answer_full[it & 1], static_cast<uint32_t>(it >> 1) & 1, marks, kStatusTimeoutFull)) return -1;
   uint32_t taken = 0, x = 0;
   asm volatile(
       "{\n"
@@ -392,7 +404,9 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
   // blocks of the grid: [work units, heaviest first][rows behind the last document to clear]
   const int work = p.num_tiles * (kPair ? p.heads / 2 : p.heads);
 
+  const Marks marks{p.status, &bars->gave_up};
   if (threadIdx.x == 0) {
+    bars->gave_up = 0;
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bars->answer_full[b], 1);
       mbar_init(&bars->answer_read[b], 10);   // every warp
@@ -424,8 +438,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
   const auto each_block = [&](auto one) {
     for (int it = 0, block = blockIdx.x; block >= 0; ++it) {
       one(it, block);
-      block = next_block(bars, it, lane, p.status);
-      if (!__all_sync(0xffffffffu, p.status == nullptr || *reinterpret_cast<volatile int*>(p.status) == 0)) break;
+      block = next_block(bars, it, lane, marks);
+      if (__any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&bars->gave_up) != 0)) break;
     }
   };
   if (warp == 0) {
@@ -436,7 +450,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
       // when the others need it, late enough that a CTA with a long block does not take another one
       // that a CTA about to finish could start on.
       const auto ask = [&] {
-        if (warp_wait(&bars->answer_read[it & 1], (static_cast<uint32_t>(it >> 1) & 1) ^ 1, p.status,
+        if (warp_wait(&bars->answer_read[it & 1], (static_cast<uint32_t>(it >> 1) & 1) ^ 1, marks,
                       kStatusTimeoutEmpty) && elect_one())
           ask_next_block(bars, it);
         __syncwarp();
@@ -447,7 +461,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
       const int n = u.n;
       // ---------------------------------------------------------------- producer
       const bool cut = u.tail_rows < kTile;
-      bool ok = warp_wait(&bars->q_free, (units & 1) ^ 1, p.status, kStatusTimeoutEmpty);
+      bool ok = warp_wait(&bars->q_free, (units & 1) ^ 1, marks, kStatusTimeoutEmpty);
       if (ok && elect_one()) {
         mbar_expect_tx(&bars->q_full, C::kQBytes);
 #pragma unroll
@@ -460,7 +474,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
       __syncwarp();
       int last_slot = 0;
       for (int i = 0; i < 2 * n && ok; ++i) {   // item 2j is K_j, item 2j + 1 is V_j
-        ok = warp_wait(&bars->kv_empty[ring.slot], ring.phase ^ 1, p.status, kStatusTimeoutEmpty);
+        ok = warp_wait(&bars->kv_empty[ring.slot], ring.phase ^ 1, marks, kStatusTimeoutEmpty);
         if (!ok) break;
         if (elect_one()) {
           uint8_t* dst = sKV + ring.slot * C::kSlotBytes;
@@ -476,7 +490,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
       }
       ask();
       if (cut && ok) {
-        ok = warp_wait(&bars->tail_full, cuts & 1, p.status, kStatusTimeoutFull);
+        ok = warp_wait(&bars->tail_full, cuts & 1, marks, kStatusTimeoutFull);
         ++cuts;
         if (ok) {
           clear_tail<C::kHalves>(sKV + last_slot * C::kSlotBytes, u.tail_rows, lane);
@@ -524,7 +538,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
           bool got = true;
 #pragma unroll
           for (int part = 0; part < 4 && got; ++part) {
-            got = mbar_wait(&bars->p_half[4 * t + part], parity, p.status, kStatusTimeoutTmemFull);
+            got = marked_wait(&bars->p_half[4 * t + part], parity, marks, kStatusTimeoutTmemFull);
             tc_fence_after();
             if (!got) break;
 #pragma unroll
@@ -537,11 +551,11 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
         };
         FwdRing<C::kSlots> at = ring;     // of the next item: K_0 V_0 K_1 V_1 ...
         auto wait_item = [&] {
-          const bool got = mbar_wait(&bars->kv_full[at.slot], at.phase, p.status, kStatusTimeoutFull);
+          const bool got = marked_wait(&bars->kv_full[at.slot], at.phase, marks, kStatusTimeoutFull);
           tc_fence_after();
           return got;
         };
-        bool ok = mbar_wait(&bars->q_full, units & 1, p.status, kStatusTimeoutFull) && wait_item();
+        bool ok = marked_wait(&bars->q_full, units & 1, marks, kStatusTimeoutFull) && wait_item();
         if (ok) {
           issue_qk(0, at.slot);
           if (u.n1 > 0) issue_qk(1, at.slot);
@@ -612,7 +626,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
       float m_run = -INFINITY, l_run = 0.f;
       bool ok = true;
       for (int j = 0; j < nt && ok; ++j) {
-        ok = warp_wait(&bars->s_full[t], (base + j) & 1, p.status, kStatusTimeoutTmemFull);
+        ok = warp_wait(&bars->s_full[t], (base + j) & 1, marks, kStatusTimeoutTmemFull);
         if (!ok) break;
         tc_fence_after();
         const bool diag = p.causal && (j == qt);
@@ -654,7 +668,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
             l_run *= alpha;
             m_run = m_upd;
             // PV_{j-1} must have landed before O is touched
-            ok = warp_wait(&bars->o_done[t], (base + j - 1) & 1, p.status, kStatusTimeoutTmemFull);
+            ok = warp_wait(&bars->o_done[t], (base + j - 1) & 1, marks, kStatusTimeoutTmemFull);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll 1
@@ -694,7 +708,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
         l_run += lsum;
       }
       if (ok && nt > 0) {
-        ok = warp_wait(&bars->o_done[t], (base + nt - 1) & 1, p.status, kStatusTimeoutTmemFull);
+        ok = warp_wait(&bars->o_done[t], (base + nt - 1) & 1, marks, kStatusTimeoutTmemFull);
         tc_fence_after();
       }
       if (ok && nt > 0) {
@@ -804,6 +818,7 @@ struct BwdBarriers {
   uint64_t unit_empty[2];
   int unit[2];
   uint32_t tmem_base;
+  int gave_up;            // see Marks
 };
 
 // Position in the ring of slots.
@@ -830,6 +845,7 @@ __device__ __forceinline__ bool bwd_setup(uint8_t* smem, BwdBarriers* bars, int 
     return false;
   }
   if (threadIdx.x == 0) {
+    bars->gave_up = 0;
     mbar_init(&bars->res_full, 1);
     mbar_init(&bars->tail_full, 2);
     for (int s = 0; s < 5; ++s) {
@@ -872,7 +888,7 @@ __device__ __forceinline__ void allow_dependents() { asm volatile("griddepcontro
 // works on a unit depends on timing, its result does not. The producer warp asks (its loads run ahead,
 // so the answer is there before the others need it) and passes the number on.
 __device__ __forceinline__ int next_unit(BwdBarriers* bars, int it, int units, int* counter, int warp, int lane,
-                                         int* status) {
+                                         const Marks& marks) {
   const int b = it & 1;
   const uint32_t phase = static_cast<uint32_t>(it >> 1) & 1;
   int unit = -1;
@@ -880,7 +896,7 @@ __device__ __forceinline__ int next_unit(BwdBarriers* bars, int it, int units, i
     if (lane == 0) unit = it == 0 ? static_cast<int>(blockIdx.x) : static_cast<int>(gridDim.x) + atomicAdd(counter, 1);
     unit = __shfl_sync(0xffffffffu, unit, 0);
     if (unit >= units) unit = -1;
-    if (!warp_wait(&bars->unit_empty[b], phase ^ 1, status, kStatusTimeoutEmpty)) unit = -1;
+    if (!warp_wait(&bars->unit_empty[b], phase ^ 1, marks, kStatusTimeoutEmpty)) unit = -1;
     if (lane == 0) {
       bars->unit[b] = unit;
       mbar_arrive(&bars->unit_full[b]);
@@ -888,7 +904,7 @@ __device__ __forceinline__ int next_unit(BwdBarriers* bars, int it, int units, i
     __syncwarp();
     return unit;
   }
-  if (!warp_wait(&bars->unit_full[b], phase, status, kStatusTimeoutFull)) return -1;
+  if (!warp_wait(&bars->unit_full[b], phase, marks, kStatusTimeoutFull)) return -1;
   unit = *reinterpret_cast<volatile int*>(&bars->unit[b]);
   __syncwarp();
   if (lane == 0) mbar_arrive(&bars->unit_empty[b]);
@@ -901,13 +917,13 @@ __device__ __forceinline__ int next_unit(BwdBarriers* bars, int it, int units, i
 template <int D>
 __device__ __forceinline__ bool stream_pair(BwdBarriers* bars, uint8_t* ring, RingPos& pos, uint32_t& cuts,
                                             const CUtensorMap* ma, const CUtensorMap* mb, int row, int head,
-                                            int tail_rows, int lane, int* status) {
+                                            int tail_rows, int lane, const Marks& marks) {
   using C = BwdCfg<D>;
   const bool cut = tail_rows < kTile;
   const int first = pos.slot;
 #pragma unroll
   for (int a = 0; a < 2; ++a) {
-    if (!warp_wait(&bars->empty[pos.slot], pos.phase ^ 1, status, kStatusTimeoutEmpty)) return false;
+    if (!warp_wait(&bars->empty[pos.slot], pos.phase ^ 1, marks, kStatusTimeoutEmpty)) return false;
     if (elect_one()) {
       uint64_t* full = cut ? &bars->tail_full : &bars->full[pos.slot];
       mbar_expect_tx(full, C::kTileBytes);
@@ -920,7 +936,7 @@ __device__ __forceinline__ bool stream_pair(BwdBarriers* bars, uint8_t* ring, Ri
   }
   if (cut) {
     const int second = first == 4 ? 0 : first + 1;
-    if (!warp_wait(&bars->tail_full, cuts & 1, status, kStatusTimeoutFull)) return false;
+    if (!warp_wait(&bars->tail_full, cuts & 1, marks, kStatusTimeoutFull)) return false;
     ++cuts;
     clear_tail<C::kHalves>(ring + first * C::kTileBytes, tail_rows, lane);
     clear_tail<C::kHalves>(ring + second * C::kTileBytes, tail_rows, lane);
@@ -952,9 +968,9 @@ __device__ __forceinline__ bool wg_and(int wg, bool ok) {
 // All of a warpgroup has the same unit of work, or, where a wait gave up in one of its warps, none.
 __device__ __forceinline__ int wg_unit(int wg, int v) { return wg_and(wg, v >= 0) ? v : -1; }
 
-// A wait gave up somewhere: stop after this tile. A warpgroup decides together, its barrier needs all of it.
-__device__ __forceinline__ bool go_on(int warp, const int* status) {
-  const bool go = status == nullptr || *reinterpret_cast<const volatile int*>(status) == 0;
+// A wait of this CTA gave up: stop after this tile. A warpgroup decides together, its barrier needs all of it.
+__device__ __forceinline__ bool go_on(int warp, const Marks& marks) {
+  const bool go = *reinterpret_cast<const volatile int*>(marks.gave_up) == 0;
   return warp < 2 ? __all_sync(0xffffffffu, go) : wg_and((warp - 2) >> 2, go);
 }
 
@@ -1077,13 +1093,14 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
   const int group = p.heads / p.kv_heads, share = group / p.splits;
   const int units = p.num_k_tiles * p.kv_heads * p.splits;
   if (!bwd_setup(smem, bars, warp, tq, tk, tv, tdo, p.status)) return;
+  const Marks marks{p.status, &bars->gave_up};
   const uint32_t tmem_base = bars->tmem_base;
   RingPos pos;               // producer and MMA issuer: slot of the next Q tile
   uint32_t cuts = 0;         // producer: tile pairs at a document's end so far
   int g = 0;                 // query tiles streamed by this CTA before the current tile
 
   const auto next = [&](int it) {
-    const int unit = next_unit(bars, it, units, p.counters, warp, lane, p.status);
+    const int unit = next_unit(bars, it, units, p.counters, warp, lane, marks);
     return warp < 2 ? unit : wg_unit((warp - 2) >> 2, unit);
   };
   const auto tile_of = [&](int unit) { return p.k_tiles[unit / (p.kv_heads * p.splits)]; };
@@ -1109,12 +1126,12 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
       bool ok = true;
       for (int t = 0, i = i0, head = head0; t < nq && ok; ++t) {
         ok = stream_pair<D>(bars, sRing, pos, cuts, &tq, &tdo, w.start + i * kTile, head,
-                            i == q_tiles - 1 ? last_rows : kTile, lane, p.status);
+                            i == q_tiles - 1 ? last_rows : kTile, lane, marks);
         if (++i == q_tiles) { i = i0; ++head; }
         if (t > 0) continue;
         // the resident K / V buffers are free once the last score MMAs of the previous unit are through;
         // its last softmax, gradient MMAs and stores then overlap these loads
-        ok = ok && (it == 0 || warp_wait(&bars->kv_free, (it - 1) & 1, p.status, kStatusTimeoutTmemFull));
+        ok = ok && (it == 0 || warp_wait(&bars->kv_free, (it - 1) & 1, marks, kStatusTimeoutTmemFull));
         if (ok && elect_one()) {
           mbar_expect_tx(&bars->res_full, 2 * C::kTileBytes);
 #pragma unroll
@@ -1159,17 +1176,17 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
           tc_commit(&bars->empty[slot]);
         };
         auto wait_full = [&](const RingPos& at) {
-          const bool got = mbar_wait(&bars->full[at.slot], at.phase, p.status, kStatusTimeoutFull);
+          const bool got = marked_wait(&bars->full[at.slot], at.phase, marks, kStatusTimeoutFull);
           tc_fence_after();
           return got;
         };
         auto wait_softmax = [&](uint64_t* bar, int iter) {
-          const bool got = mbar_wait(bar, iter & 1, p.status, kStatusTimeoutTmemFull);
+          const bool got = marked_wait(bar, iter & 1, marks, kStatusTimeoutTmemFull);
           tc_fence_after();
           return got;
         };
         RingPos at = pos;
-        bool ok = mbar_wait(&bars->res_full, it & 1, p.status, kStatusTimeoutFull) && wait_full(at);
+        bool ok = marked_wait(&bars->res_full, it & 1, marks, kStatusTimeoutFull) && wait_full(at);
         if (ok) {
           issue_scores(dK0, at.slot, 0, &bars->s_full);
           ok = wait_full(at.next(1));
@@ -1241,7 +1258,7 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
         const float* a_lse = aux_slot(t);
         const float* a_del = a_lse + 64;
         Pair pv[32];
-        ok = warp_wait(&bars->s_full, (g + t) & 1, p.status, kStatusTimeoutTmemFull);
+        ok = warp_wait(&bars->s_full, (g + t) & 1, marks, kStatusTimeoutTmemFull);
         if (!ok) continue;
         tc_fence_after();
         {
@@ -1281,7 +1298,7 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->s_read);
-        ok = warp_wait(&bars->dp_full, (g + t) & 1, p.status, kStatusTimeoutTmemFull);
+        ok = warp_wait(&bars->dp_full, (g + t) & 1, marks, kStatusTimeoutTmemFull);
         if (!ok) continue;
         tc_fence_after();
 #pragma unroll
@@ -1321,7 +1338,7 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
                    kv_split / p.splits * group + kv_split % p.splits * share, next_lse, next_delta);
       }
       // epilogue: warpgroup 0 stores dV, warpgroup 1 stores dK * scale
-      if (ok) ok = warp_wait(&bars->done, it & 1, p.status, kStatusTimeoutTmemFull);
+      if (ok) ok = warp_wait(&bars->done, it & 1, marks, kStatusTimeoutTmemFull);
       if (ok) {
         tc_fence_after();
         // rows of the tile that exist, from its first row on
@@ -1347,7 +1364,7 @@ packed_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_cons
     // (which overwrite the accumulators) wait for that unit's first P, and a softmax warp writes that
     // only after it has stored its part of these accumulators.
     g += nq;
-    if (!go_on(warp, p.status)) break;
+    if (!go_on(warp, marks)) break;
   }
   tc_fence_before();
   __syncthreads();
@@ -1383,13 +1400,14 @@ packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_consta
   const int group = p.heads / p.kv_heads;
   const int units = p.num_q_tiles * p.heads;
   if (!bwd_setup(smem, bars, warp, tq, tk, tv, tdo, p.status)) return;
+  const Marks marks{p.status, &bars->gave_up};
   const uint32_t tmem_base = bars->tmem_base;
   RingPos pos;               // producer and MMA issuer: slot of the next K tile
   uint32_t cuts = 0;         // producer: tile pairs at a document's end so far
   int g = 0;                 // key/value tiles streamed by this CTA before the current tile
 
   const auto next = [&](int it) {
-    const int unit = next_unit(bars, it, units, p.counters + 1, warp, lane, p.status);
+    const int unit = next_unit(bars, it, units, p.counters + 1, warp, lane, marks);
     return warp < 2 ? unit : wg_unit((warp - 2) >> 2, unit);
   };
   // Stages the rows of unit `it` as TMEM operands: warpgroup 0 copies the Q rows, warpgroup 1 the dO rows,
@@ -1398,7 +1416,7 @@ packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_consta
   // MMAs of the unit before have been waited for.
   const auto stage_rows = [&](int it) {
     const int wg = (warp - 2) >> 2, r_local = (warp & 3) * 32 + lane;
-    if (!warp_wait(&bars->res_full, it & 1, p.status, kStatusTimeoutFull)) return false;
+    if (!warp_wait(&bars->res_full, it & 1, marks, kStatusTimeoutFull)) return false;
     const uint8_t* src = (wg == 0 ? sQ : sDO) + r_local * 128;
     const uint32_t dst = tmem_base + 384 + wg * 64 + (static_cast<uint32_t>((warp & 3) * 32) << 16);
 #pragma unroll
@@ -1447,7 +1465,7 @@ packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_consta
     const int last_rows = w.len - (kv_tiles - 1) * kTile;   // rows of the document's last tile
     if (warp == 0) {
       // Q / dO are free once the softmax warps have copied the previous unit's rows
-      ok = it == 0 || warp_wait(&bars->qdo_full, (it - 1) & 1, p.status, kStatusTimeoutTmemFull);
+      ok = it == 0 || warp_wait(&bars->qdo_full, (it - 1) & 1, marks, kStatusTimeoutTmemFull);
       if (ok && elect_one()) {
         mbar_expect_tx(&bars->res_full, 2 * C::kTileBytes);
 #pragma unroll
@@ -1459,7 +1477,7 @@ packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_consta
       __syncwarp();
       for (int t = 0; t < n && ok; ++t)
         ok = stream_pair<D>(bars, sRing, pos, cuts, &tk, &tv, w.start + t * kTile, kv_head,
-                            t == kv_tiles - 1 ? last_rows : kTile, lane, p.status);
+                            t == kv_tiles - 1 ? last_rows : kTile, lane, marks);
       unit_next = next(it + 1);
       if (unit_next >= 0) w_next = p.q_tiles[unit_next / p.heads];
     } else if (warp == 1) {
@@ -1492,17 +1510,17 @@ packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_consta
           }
         };
         auto wait_full = [&](const RingPos& at) {
-          const bool got = mbar_wait(&bars->full[at.slot], at.phase, p.status, kStatusTimeoutFull);
+          const bool got = marked_wait(&bars->full[at.slot], at.phase, marks, kStatusTimeoutFull);
           tc_fence_after();
           return got;
         };
         auto wait_softmax = [&](uint64_t* bar, int iter) {
-          const bool got = mbar_wait(bar, iter & 1, p.status, kStatusTimeoutTmemFull);
+          const bool got = marked_wait(bar, iter & 1, marks, kStatusTimeoutTmemFull);
           tc_fence_after();
           return got;
         };
         RingPos at = pos;
-        bool ok = mbar_wait(&bars->qdo_full, it & 1, p.status, kStatusTimeoutFull) && wait_full(at);
+        bool ok = marked_wait(&bars->qdo_full, it & 1, marks, kStatusTimeoutFull) && wait_full(at);
         if (ok) {
           tc_fence_after();
           issue_scores(384, at.slot, 0, &bars->s_full);
@@ -1553,7 +1571,7 @@ packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_consta
       const float sl2 = p.scale * kLog2e;
       const float neg_lse = -lse_next * kLog2e, neg_delta = -delta_next;
       for (int t = 0; t < n && ok; ++t) {
-        ok = warp_wait(&bars->s_full, (g + t) & 1, p.status, kStatusTimeoutTmemFull);
+        ok = warp_wait(&bars->s_full, (g + t) & 1, marks, kStatusTimeoutTmemFull);
         if (!ok) break;
         tc_fence_after();
         const int kv0 = t * kTile + wg * 64;              // first key of this warpgroup's columns
@@ -1583,7 +1601,7 @@ packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_consta
             pv[e] = pair(2 * e >= seen ? 0.f : a, 2 * e + 1 >= seen ? 0.f : b);
           }
         }
-        ok = warp_wait(&bars->dp_full, (g + t) & 1, p.status, kStatusTimeoutTmemFull);
+        ok = warp_wait(&bars->dp_full, (g + t) & 1, marks, kStatusTimeoutTmemFull);
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
@@ -1610,7 +1628,7 @@ packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_consta
         row_stats(w_next, unit_next % p.heads);
         ok = ok && stage_rows(it + 1);
       }
-      const bool here = ok && warp_wait(&bars->done, it & 1, p.status, kStatusTimeoutTmemFull);
+      const bool here = ok && warp_wait(&bars->done, it & 1, marks, kStatusTimeoutTmemFull);
       if (here) {
         tc_fence_after();
         // each warpgroup stores half of the head dimension
@@ -1626,7 +1644,7 @@ packed_bwd_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_consta
     // accumulator) wait for that unit's first dS, and a softmax warp writes that only after it has
     // stored its part of this accumulator.
     g += n;
-    if (!go_on(warp, p.status)) break;
+    if (!go_on(warp, marks)) break;
   }
   if (threadIdx.x == 0) after_prerequisite();   // whatever follows in the stream may rely on dK / dV as well
   tc_fence_before();

@@ -114,6 +114,8 @@ def flash_attention_packed(q, k, v, layout, scale=None, causal=True):
     On CUDA: fp16 / bf16, head_dim 64 or 128; views such as the q, k and v slices of one projection are
     read in place, what a tensor map cannot address is copied. A document attends to itself only: what
     stands in other documents or behind the last one, infinities and NaN included, does not reach it.
+    Waits inside the kernels are bounded: one that gave up leaves results unwritten and a mark that
+    `native.check_status` raises on, which a training loop calls once per step.
     `scale` (1e-30 to 1e3) defaults to 1 / sqrt(head_dim). Scores and their log-sum-exp are fp32: a scaled
     score of magnitude x is off by about x 2^-22, its probability by that part of itself (from x = 10^8 on,
     results would not be finite)."""

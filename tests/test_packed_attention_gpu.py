@@ -399,3 +399,23 @@ def test_scales_whose_scores_leave_fp32(scale):
         ops.flash_attention_packed(q, k, v, ops.PackedLayout([5], device=DEV), scale=scale)
     with pytest.raises(ValueError, match="scale"):
         ops.flash_attention_packed(q.cpu(), k.cpu(), v.cpu(), ops.PackedLayout([5]), scale=scale)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(16, 2), (8, 8)])
+def test_mark_of_an_earlier_kernel_does_not_cost_results(heads, kv_heads):
+    """The status word tells of a wait that gave up, here or in any kernel before; only the former may leave
+    results unwritten. More units of work than SMs, so that CTAs take a second one."""
+    lengths = [1024, 700, 256, 1500, 77, 129, 1024]
+    inputs = _inputs(lengths, heads, kv_heads, 128, torch.bfloat16, seed=18)
+    q, k, v, do = inputs
+    layout = ops.PackedLayout(lengths, device=DEV)
+    want = _check(lengths, *inputs, True, layout=layout)
+    word = native.status(q.device)
+    word.fill_(7)
+    try:
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        out = ops.flash_attention_packed(*leaves, layout)
+        got = [out.detach(), *torch.autograd.grad(out, leaves, do)]
+        assert word.item() == 7 and all(torch.equal(a, b) for a, b in zip(got, want))
+    finally:
+        word.zero_()
