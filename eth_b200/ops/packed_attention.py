@@ -48,6 +48,7 @@ class PackedLayout:
             self.device = torch.device("cuda", torch.cuda.current_device())
         self._lists = None
         if self.device.type == "cuda":
+            native.status(self.device)      # a call inside a graph capture must not be the one that makes it
             parts = list(self._work_lists(lengths))
             host = torch.from_numpy(np.concatenate([x for _, x in parts]))
             flat = host.to(self.device)

@@ -419,3 +419,20 @@ def test_mark_of_an_earlier_kernel_does_not_cost_results(heads, kv_heads):
         assert word.item() == 7 and all(torch.equal(a, b) for a, b in zip(got, want))
     finally:
         word.zero_()
+
+
+def test_first_call_of_a_process_inside_a_capture(monkeypatch):
+    """The status word is made, and cleared, with the layout: made inside the capture it would live in the
+    graph's memory and be cleared by replays only."""
+    lengths = [130, 3]
+    q, k, v, do = (t.contiguous() for t in _inputs(lengths, 4, 2, 64, torch.bfloat16, seed=19))
+    monkeypatch.setattr(native, "_status", {})
+    layout = ops.PackedLayout(lengths, device=DEV)
+    assert len(native._status) == 1
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, _ = raw.attention_packed_fwd(q, k, v, layout)
+    assert len(native._status) == 1
+    _check(lengths, q, k, v, do, True, layout=layout)       # before any replay
+    graph.replay()
+    assert oracle.excess(out, oracle.attention(q, k, v, lengths, True)["out"]) <= 1
