@@ -119,7 +119,7 @@ def build_parser() -> argparse.ArgumentParser:
     g.add_argument("--eod-mask-loss", action="store_true", help="No loss on end-of-document tokens.")
     g.add_argument("--reset-position-ids", action="store_true", help="Not supported (positions run over the sequence).")
     g.add_argument("--reset-attention-mask", action="store_true",
-                   help="Not supported (attention is causal over the whole sequence).")
+                   help="Not supported (the model's attention is causal over the whole sequence).")
     g.add_argument("--data-impl", type=str, default="mmap", choices=["lazy", "cached", "mmap", "infer"],
                    help="Indexed dataset implementation.")
     g.add_argument("--reference-zero-labels", action="store_true",
@@ -218,7 +218,7 @@ def finalize_args(args, config=None):
                                  f"divisible by the number of stages (pipeline {i}: {p['num_stages']} stages, "
                                  f"{n_mb} micro-batches)")
     if args.reset_position_ids or args.reset_attention_mask:
-        raise ValueError("--reset-position-ids / --reset-attention-mask are not supported: the attention kernels are "
+        raise ValueError("--reset-position-ids / --reset-attention-mask are not supported: the model's attention is "
                          "causal over the whole sequence and positions are not restarted at document boundaries")
     args.eod_token = None
     if bool(args.vocab_file) != bool(args.merge_file):
