@@ -178,7 +178,13 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
                           double scale, bool causal, const Tensor& status, bool needs_grad) {
     auto [out, lse, residue] =
         packed_fwd(q, k, v, Lists{tiles, blocks, keys, used, total}, scale, causal, status, needs_grad);
-    ctx->save_for_backward({q, k, v, out, lse, tiles, blocks, keys, status, residue});
+    ctx->save_for_backward({q, k, v, out, lse, residue});
+    // the kernels' own data, no values of the graph: neither hooks on saved tensors nor their version checks
+    // apply (the status word is cleared in place between steps)
+    ctx->saved_data["tiles"] = tiles;
+    ctx->saved_data["blocks"] = blocks;
+    ctx->saved_data["keys"] = keys;
+    ctx->saved_data["status"] = status;
     ctx->saved_data["used"] = used;
     ctx->saved_data["total"] = total;
     ctx->saved_data["scale"] = scale;
@@ -188,9 +194,10 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     refuse_double_backward();
     const auto s = ctx->get_saved_variables();
-    const Lists l{s[5], s[6], s[7], ctx->saved_data["used"].toInt(), ctx->saved_data["total"].toInt()};
+    const Lists l{ctx->saved_data["tiles"].toTensor(), ctx->saved_data["blocks"].toTensor(),
+                  ctx->saved_data["keys"].toTensor(), ctx->saved_data["used"].toInt(), ctx->saved_data["total"].toInt()};
     auto [dq, dk, dv] = packed_bwd(grads[0], s[0], s[1], s[2], s[3], s[4], l, ctx->saved_data["scale"].toDouble(),
-                                   ctx->saved_data["causal"].toBool(), s[8], s[9]);
+                                   ctx->saved_data["causal"].toBool(), ctx->saved_data["status"].toTensor(), s[5]);
     return {dq, dk, dv, Variable(), Variable(), Variable(), Variable(), Variable(), Variable(), Variable(), Variable(), Variable()};
   }
 };

@@ -1,4 +1,5 @@
 """Packed-document attention kernels against the definition in 64 bits, element by element."""
+import contextlib
 import math
 
 import pytest
@@ -436,3 +437,16 @@ def test_first_call_of_a_process_inside_a_capture(monkeypatch):
     _check(lengths, q, k, v, do, True, layout=layout)       # before any replay
     graph.replay()
     assert oracle.excess(out, oracle.attention(q, k, v, lengths, True)["out"]) <= 1
+
+
+@pytest.mark.parametrize("hooks", [contextlib.nullcontext, torch.autograd.graph.save_on_cpu])
+def test_status_cleared_between_forward_and_backward(hooks):
+    lengths = [130, 3]
+    q, k, v, do = (t.contiguous().requires_grad_(True) for t in _inputs(lengths, 4, 2, 64, torch.bfloat16, seed=20))
+    with hooks():
+        out = ops.flash_attention_packed(q, k, v, ops.PackedLayout(lengths, device=DEV))
+    native.status(q.device).zero_()
+    grads = torch.autograd.grad(out, (q, k, v), do)
+    want = oracle.attention(q, k, v, lengths, True, d_out=do.detach())
+    for name, t in zip(("dq", "dk", "dv"), grads):
+        assert oracle.excess(t, want[name]) <= 1, name
