@@ -108,9 +108,10 @@ __device__ __forceinline__ Pair exp2_pair(Pair t) {
 // not hold take a clamp per element instead; so do rows so high (a token forced by the type's highest
 // value), or a temperature so low, that t or its product with a gradient's factor would pass fp32's range.
 constexpr float kFloor = -57344.f;   // -7 * 2^13: exact in every type
-__device__ __forceinline__ bool has_floor(float mu, float s2, float factor = 1.f) {
-  const float depth = (mu - kFloor) * s2;   // -t of a raised logit
-  return depth > 200.f && depth * fmaxf(fabsf(factor), 1.f) < 1e38f;
+__device__ __forceinline__ bool has_floor(float mu, float s2) {
+  const float depth = (mu - kFloor) * s2;   // -t of a raised logit: above 200 and finite, in one comparison
+  constexpr uint32_t kLow = 0x43480000u, kInf = 0x7f800000u;   // 200, infinity
+  return __float_as_uint(depth) - kLow < kInf - kLow;
 }
 __device__ __forceinline__ uint32_t max_nan(uint32_t x, float low) {
   uint32_t r;
@@ -508,8 +509,8 @@ __device__ void select_top(const Row<T>& r, int k, float thread_max, bool thread
 
 // The sum of exponentials as the backward gets it: negative where the row's token lies outside the vocabulary
 // (zt is NaN), so that the gradient of its log-probability, which is NaN, is NaN as well.
-__device__ __forceinline__ float marked_sum(float l, int64_t token, float zt) {
-  return token >= 0 && zt != zt ? -l : l;
+__device__ __forceinline__ float marked_sum(float l, bool scored, float zt) {
+  return scored && zt != zt ? -l : l;
 }
 
 constexpr int kScanGroup = 8;   // loads in flight per thread of the kernels that read a row once
@@ -540,12 +541,12 @@ token_scores_kernel(const T* __restrict__ z, int64_t ld, int vocab, int64_t v0, 
     if constexpr (kTop) return Segments(sel.segment_max, r.nvec, kGroup);
     else return NoSegments{};
   }();
-  int64_t t = -1;
+  bool scored = false;
   float zt = CUDART_NAN_F;
   const Running<true> own = scan_row<T, true, kGroup>(r, s2, seg, [&] {
     if (threadIdx.x != 0) return;
-    t = tokens[row];
-    const int64_t local = t - v0;
+    const int64_t t = tokens[row], local = t - v0;
+    scored = t >= 0;
     if (t >= 0 && local >= 0 && local < vocab) zt = HalfTraits<T>::to_f(r.p[local]);
   });
   const Running<true> all = block_merge<true>(own, s2, red);
@@ -557,10 +558,10 @@ token_scores_kernel(const T* __restrict__ z, int64_t ld, int vocab, int64_t v0, 
       float* q = partial + row * width;
       q[0] = all.mx; q[1] = all.l; q[2] = all.a; q[3] = zt;
     } else {
-      out.logprob[row] = t < 0 ? 0.f : (zt - mu) * inv_t - log_l;
+      out.logprob[row] = scored ? (zt - mu) * inv_t - log_l : 0.f;
       out.entropy[row] = log_l - kLn2 * (all.a / all.l);
       out.stats[2 * row] = mu;
-      out.stats[2 * row + 1] = marked_sum(all.l, t, zt);
+      out.stats[2 * row + 1] = marked_sum(all.l, scored, zt);
     }
   }
   if constexpr (kTop) {
@@ -608,7 +609,7 @@ __global__ void token_scores_combine_kernel(const float* __restrict__ parts, int
     out.logprob[row] = tokens[row] < 0 ? 0.f : (zt - mu) * inv_t - log_l;
     out.entropy[row] = log_l - kLn2 * (all.a / all.l);
     out.stats[2 * row] = mu;
-    out.stats[2 * row + 1] = marked_sum(all.l, tokens[row], zt);
+    out.stats[2 * row + 1] = marked_sum(all.l, tokens[row] >= 0, zt);
   }
   auto key = [&](int c) {
     const float* q = parts + ((c / top_k) * rows + row) * width + 4 + c % top_k;
@@ -652,7 +653,7 @@ struct DenseTerm {
     const float inv = 1.0f / l;
     f.a = (B == 0.f ? A : A - B * (kLn2 * log2f(l))) * inv;
     f.b = B * kLn2 * inv;
-    f.floor = has_floor(mu, s2, f.b);
+    f.floor = has_floor(mu, s2) && (mu - kFloor) * s2 * fabsf(f.b) < 1e38f;
     return f;
   }
   template <bool kLog> __device__ __forceinline__ float at(float z) const {
@@ -798,14 +799,16 @@ struct TeacherRow {
 
 // The row's list in shared memory: local ids (-1: not on this shard or unused), teacher logits, student
 // logits. Staged while the row is read (scan_row's `first`), so only the few warps that hold entries wait
-// for the two dependent loads, the others read on; a barrier follows.
+// for the two dependent loads, the others read on; a barrier follows. `whole`: the row is the whole vocabulary,
+// where a used entry that lies outside turns its teacher logit, and so the row's loss and gradient, into NaN.
 template <typename T>
-__device__ __forceinline__ void stage_list(const TeacherView& t, int64_t row, const Row<T>& r, int64_t v0, Listed& li) {
+__device__ __forceinline__ void stage_list(const TeacherView& t, int64_t row, const Row<T>& r, int64_t v0, bool whole,
+                                           Listed& li) {
   for (int i = threadIdx.x; i < t.k; i += blockDim.x) {
     const float logit = t.logit[row * t.k + i];
     const int64_t id = t.index[row * t.k + i] - v0;
-    const bool here = logit != -INFINITY && id >= 0 && id < r.n;
-    li.w[i] = logit;
+    const bool used = logit != -INFINITY, here = used && id >= 0 && id < r.n;
+    li.w[i] = whole && used && !here ? CUDART_NAN_F : logit;
     li.id[i] = here ? static_cast<int>(id) : -1;
     li.z[i] = here ? HalfTraits<T>::to_f(r.p[id]) : CUDART_NAN_F;
   }
@@ -832,8 +835,7 @@ __device__ __forceinline__ float log_weight(const TeacherRow& t, float logit, fl
   return (logit - t.tmax) * inv_t - t.log_sum;
 }
 
-// One warp: the loss of a staged row whose listed logits are all on this shard; NaN where a used entry
-// is not, 0 where there are no entries.
+// One warp: the loss of a staged row of the whole vocabulary; 0 where there are no entries.
 __device__ __forceinline__ float listed_loss(const Listed& li, int k, const TeacherRow& tr, float inv_t, float mu,
                                              float log_l) {
   float part = 0.f;
@@ -841,17 +843,8 @@ __device__ __forceinline__ float listed_loss(const Listed& li, int k, const Teac
   for (int i = threadIdx.x & 31; i < k; i += 32) {
     const float log_q = log_weight(tr, li.w[i], inv_t), q = exp2f(log_q * kLog2e);
     if (q != 0.f) part += q * (log_q - ((li.z[i] - mu) * inv_t - log_l));
-    if (li.id[i] < 0 && li.w[i] != -INFINITY) part = CUDART_NAN_F;
   }
   return warp_sum(part);
-}
-
-// All lanes of a warp: whether the used entries of a staged whole-vocabulary list all lie in the vocabulary.
-// Where not, the loss is NaN, and a sum of exponentials of NaN carries that into the gradient.
-__device__ __forceinline__ bool all_known(const Listed& li, int k) {
-  bool known = true;
-  for (int i = threadIdx.x & 31; i < k; i += 32) known &= li.id[i] >= 0 || li.w[i] == -INFINITY;
-  return __all_sync(0xffffffffu, known);
 }
 
 // Same shape as token_scores_kernel, without the entropy (8192 x 50304 bf16: 6.6 TB/s).
@@ -865,7 +858,9 @@ distill_fwd_kernel(const T* __restrict__ z, int64_t ld, int vocab, int64_t v0, T
   const Row<T> r(z + row * ld, vocab);
   const float s2 = inv_t * kLog2e;
   NoSegments none;
-  const Running<false> own = scan_row<T, false, kScanGroup>(r, s2, none, [&] { stage_list(t, row, r, v0, li); });
+  const Running<false> own = scan_row<T, false, kScanGroup>(r, s2, none, [&] {
+    stage_list(t, row, r, v0, partial == nullptr, li);
+  });
   const Running<false> all = block_merge<false>(own, s2, red);   // its barrier publishes the list, too
   if (threadIdx.x >= 32) return;
   const float mu = all.mu();
@@ -889,12 +884,11 @@ distill_fwd_kernel(const T* __restrict__ z, int64_t ld, int vocab, int64_t v0, T
     return;
   }
   const float l = listed_loss(li, t.k, tr, inv_t, mu, kLn2 * log2f(all.l));
-  const bool known = all_known(li, t.k);
   if (threadIdx.x == 0) {
     const bool empty = tr.mass == 0.f;   // nothing listed: no loss, whatever the logits
     loss[row] = l;
     stats[2 * row] = empty ? 0.f : mu;
-    stats[2 * row + 1] = empty ? 1.f : known ? all.l : CUDART_NAN_F;
+    stats[2 * row + 1] = empty ? 1.f : all.l * tr.mass;   // NaN like the loss where the list is bad
   }
 }
 
@@ -943,7 +937,7 @@ __global__ void distill_combine_kernel(const float* __restrict__ parts, int worl
     const bool whole = count == used;   // else an entry lies outside the vocabulary
     loss[row] = empty ? 0.f : whole ? self - found + kLn2 * log2f(all.l) : CUDART_NAN_F;
     stats[2 * row] = empty ? 0.f : mu;
-    stats[2 * row + 1] = empty ? 1.f : whole ? all.l : CUDART_NAN_F;   // see all_known
+    stats[2 * row + 1] = empty ? 1.f : whole ? all.l : CUDART_NAN_F;   // the gradient is NaN as well
   }
 }
 
@@ -961,7 +955,7 @@ __global__ void distill_bwd_kernel(const T* z, int64_t ld, int vocab, int64_t v0
   const Row<T> r(z + row * ld, vocab);
   T* d = dz + row * ldd;
   const float g = dloss[row] * inv_t;
-  stage_list(t, row, r, v0, li);
+  stage_list(t, row, r, v0, false, li);
   __syncthreads();
   const TeacherRow tr = teacher_row(li, t.k, inv_t);
   if (tr.mass == 0.f || g == 0.f) {
@@ -990,14 +984,14 @@ distill_step_kernel(const T* z, int64_t ld, int vocab, int64_t v0, TeacherView t
   const float s2 = inv_t * kLog2e;
   const float g = dloss[row] * inv_t;
   NoSegments none;
-  const Running<false> own = scan_row<T, false, kUnroll>(r, s2, none, [&] { stage_list(t, row, r, v0, li); });
+  const Running<false> own = scan_row<T, false, kUnroll>(r, s2, none, [&] { stage_list(t, row, r, v0, true, li); });
   const Running<false> all = block_merge<false>(own, s2, red);
   const float mu = all.mu();
   const TeacherRow tr = teacher_row(li, t.k, inv_t);
   if (tr.mass == 0.f || g == 0.f) {
     write_zero(d, vocab);
   } else {
-    const DenseTerm f = DenseTerm::of(mu, all_known(li, t.k) ? all.l : CUDART_NAN_F, s2, g * tr.mass, 0.f);
+    const DenseTerm f = DenseTerm::of(mu, all.l, s2, g * tr.mass, 0.f);
     write_grad<T, false, true>(r, d, f, li, t.k, [&](int i) { return listed_grad(li, tr, inv_t, g, i); });
   }
   if (threadIdx.x < 32) {
