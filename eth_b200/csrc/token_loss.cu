@@ -751,6 +751,8 @@ __global__ void token_scores_bwd_kernel(const T* z, int64_t ld, int vocab, int64
   const int64_t t = tokens[row];
   const float gr = g != nullptr && t >= 0 ? g[row] : 0.f;
   const float hr = kLog ? h[row] : 0.f;
+  // requested before the list's barrier: the sum of exponentials (see marked_sum), the maximum, the entropy
+  const float l = stats[2 * row + 1], mu = stats[2 * row], ent = kLog ? entropy[row] : 0.f;
   const int extra = u != nullptr ? top_k : 0;
   if (threadIdx.x < 32) {
     float sum = 0.f;
@@ -782,9 +784,8 @@ __global__ void token_scores_bwd_kernel(const T* z, int64_t ld, int vocab, int64
     write_zero(d, vocab);
     return;
   }
-  const float l = stats[2 * row + 1];   // see marked_sum
-  const float A = l < 0.f && gr != 0.f ? CUDART_NAN_F : -(gr + usum + (kLog ? hr * entropy[row] : 0.f)) * inv_t;
-  const DenseTerm f = DenseTerm::of(stats[2 * row], fabsf(l), inv_t * kLog2e, A, kLog ? -hr * inv_t : 0.f);
+  const float A = l < 0.f && gr != 0.f ? CUDART_NAN_F : -(gr + usum + (kLog ? hr * ent : 0.f)) * inv_t;
+  const DenseTerm f = DenseTerm::of(mu, fabsf(l), inv_t * kLog2e, A, kLog ? -hr * inv_t : 0.f);
   write_grad<T, kLog, false>(r, d, f, li, 1 + extra, [&](int i) { return li.w[i]; });
 }
 
