@@ -142,9 +142,10 @@ __device__ __forceinline__ uint32_t pack_pair(Pair p, int dtype) {
   split(p, a, b);
   return pack2(a, b, dtype);
 }
-// Measured: dK / dV of 8192 rows in five documents, 32 / 8 heads of 128, 297 us with none, 287 with a quarter, 294
-// with a half, 311 with three quarters. (In the forward, whose registers are full, a quarter took 93 us in place
-// of 74 at nine documents, 8192 rows, 16 heads of 128.)
+// Measured: dK / dV and dQ of 8192 rows in five documents, 32 / 8 heads of 128: 295 and 226 us with none, 290 and
+// 227 with a quarter, 289 and 236 with a half, 313 and 245 with three quarters; nine documents, 16 heads of 128: 112
+// and 80, 109 and 80, 110 and 83, 116 and 85. (In the forward, whose registers are full, a quarter took 93 us in
+// place of 74 at nine documents.)
 constexpr int kBwdPoly = 1;
 
 // Clears rows [first, 128) of a tile that a TMA load has written (kHalves blocks of 128 rows x 128
@@ -795,9 +796,9 @@ cudaError_t launch_fwd(const PackedAttnArgs& a, cudaStream_t st) {
 // core works on the dP side, and the other way round. (64-column tiles with two buffers of S and dP,
 // as in attention_sm100.cu, need 1.25 times the shared-memory reads per MMA and leave the tensor core
 // waiting for the softmax of a buffer: 133 and 107 us for dK / dV and dQ at 8192 rows of nine documents, 16
-// heads of 128; now 109 and 78 us = 47 and 51 % of the tensor pipe's cycles. What bounds them is the chain
+// heads of 128; now 109 and 80 us = 47 and 51 % of the tensor pipe's cycles. What bounds them is the chain
 // "P written -> dV += P^T dO -> next S -> its exponentials"; a second S buffer does not fit beside two
-// accumulators of 128 columns in 512 TMEM columns.)
+// accumulators of 128 columns in 512 TMEM columns. With D = 64 it would; that has not been tried.)
 template <int D> struct BwdCfg {
   static constexpr int kHalves = D / 64;
   static constexpr int kTileBytes = kHalves * 16384;        // one 128-row tile

@@ -1057,7 +1057,8 @@ cudaError_t launch_distill(const LogitsView& a, const TeacherView& t, float* los
 
 // Rows in flight take SMs x rows per SM x row bytes of L2 (126 MB, which also passes the gradients on):
 // four a SM up to 150 KB (89 MB), two beyond. Back to back at the power limit, with 4 x 320, 2 x 512, 3 x
-// 512, 1 x 1024 threads: 8192 x 50304 bf16 343, 393, 388, - us; 2048 x 128000 245, 225, 243, 278 us.
+// 512, 1 x 1024 threads: 8192 x 50304 bf16 343, 393, 388, - us; 2048 x 128000 245, 225, 243, 278 us. Between
+// them, fp32: 4096 x 50304 349 us with the first, 324 with the second; 1500 x 65536 186 and 179.
 template <typename T>
 void launch_step(const LogitsView& a, const TeacherView& t, const float* dloss, float* loss, T* dz, int64_t ldd,
                  cudaStream_t st) {

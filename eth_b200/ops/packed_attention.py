@@ -21,7 +21,8 @@ class PackedLayout:
 
     `lengths` are whole numbers >= 0 known on the host: a sequence, an array or a CPU tensor (a CUDA
     tensor is copied back, which waits for its stream). On a CUDA `device` the kernels' work lists are
-    built and copied there once, so a layout is made per batch, outside CUDA graph capture, and kept."""
+    built and copied there once (about 0.1 ms of host time for tens of documents), so a layout is made per
+    batch, outside CUDA graph capture, and kept."""
 
     def __init__(self, lengths, device="cpu", total=None):
         if isinstance(lengths, torch.Tensor):
@@ -115,6 +116,8 @@ def flash_attention_packed(q, k, v, layout, scale=None, causal=True):
     On CUDA: fp16 / bf16, head_dim 64 or 128; views such as the q, k and v slices of one projection are
     read in place, what a tensor map cannot address is copied. A document attends to itself only: what
     stands in other documents or behind the last one, infinities and NaN included, does not reach it.
+    P and dS are rounded to the input type for the tensor cores, sums are fp32. Where a gradient is needed,
+    the forward also keeps what rounding took off its result (one more tensor like it) for the backward.
     Waits inside the kernels are bounded: one that gave up leaves results unwritten and a mark that
     `native.check_status` raises on, which a training loop calls once per step.
     `scale` (1e-30 to 1e3) defaults to 1 / sqrt(head_dim). Scores and their log-sum-exp are fp32: a scaled
